@@ -355,6 +355,119 @@ int mmr_prefill_qkv_rows(const float* qkv, const float* q_norm, const float* k_n
 int mmr_prefill_attention(const float* query, const mmr_kv_cache* cache, int64_t start_position, int64_t seq_len,
                           int64_t q_heads, int64_t kv_heads, int64_t head_dim, float* out, mmr_stream_t stream);
 
+/* ---- 8-bit paged KV cache (no counterpart in the reference, whose cache is
+ * fp16 and one sequence long: ascend_custom_ops.cpp:59-65) ------------------
+ * A page holds 64 tokens of every KV head in four blocks of 16 tokens.  A
+ * cached value is code * 2^e: an int8 code and the int8 exponent that its
+ * (block, KV head) has for keys and another for values.  The caller owns the
+ * memory (device buffers, nothing in them needs to be set before the first
+ * append) and passes its layout in this struct:
+ *   keys        int8 [pages][kv_heads][64][head_dim]
+ *   values      int8 [pages][kv_heads][head_dim][64]   (tokens contiguous)
+ *   key_exps, value_exps  int8 [pages][kv_heads][4]
+ *   table       int32 [seqs][pages_per_seq]: page p of sequence s holds its
+ *               positions 64 p .. 64 p + 63; entries past a sequence's last
+ *               page are not read.
+ * keys and values are 16-byte aligned, the rest 4-byte aligned; head_dim is
+ * 32, 64, 96 or 128, kv_heads at most 64, seqs at most 65535.  Sequences may
+ * share pages that neither of them appends to.
+ *
+ * Both calls take the new rows of all sequences together: sequence s brings
+ * rows offsets[s] .. offsets[s + 1] - 1 (none where they are equal), which
+ * take its positions context[s] .. context[s] + n - 1.  offsets [seqs + 1]
+ * and context [seqs] are int32 on the device, so a recorded graph serves
+ * every step; rows is what the row buffers hold, max_rows the most that one
+ * sequence brings (both size the launch).  Rows outside [offsets[0],
+ * offsets[seqs]) are left as they are.  rows or max_rows of 0 is no work.
+ *
+ * *error (device int32, never cleared here) gets bits: 1 if a sequence's
+ * offsets fall or leave [0, rows], it brings more than max_rows rows, reaches
+ * past its table row, the rotation table or max_tokens, or a page number is
+ * outside [0, pages).  Nothing is appended for such a sequence, or for the
+ * blocks of such a page, and its output rows are left as they are; attention
+ * takes the keys of such a page as absent.  2 if a key or value that was
+ * appended is not finite. */
+#define MMR_KV8_PAGE 64
+#define MMR_KV8_BLOCK 16
+#define MMR_KV8_ERROR_ROWS 1
+#define MMR_KV8_ERROR_NOT_FINITE 2
+typedef struct mmr_kv8_pages {
+  int8_t* keys;
+  int8_t* values;
+  int8_t* key_exps;
+  int8_t* value_exps;
+  const int32_t* table;
+  int64_t pages;
+  int64_t seqs;
+  int64_t pages_per_seq;
+  int64_t kv_heads;
+  int64_t head_dim;
+} mmr_kv8_pages;
+/* The 8-bit counterpart of mmr_prefill_qkv_rows / mmr_decode_qkv_postprocess:
+ * qkv fp32 [rows][(q_heads + 2 kv_heads) d], per-head RMSNorm of q and k
+ * (q_norm, k_norm fp32 [d], each may be NULL for none), RoPE at the row's position,
+ * rotated queries to query fp32 [rows][q_heads d], keys and values to the
+ * cache.  A block's exponent e is the least in [-126, 122] with max |x| <=
+ * 127 * 2^e over the rows that the call adds to it, or the one it has if that
+ * is larger and it holds earlier rows (those before the call's first
+ * position); where it grows, the earlier codes become rint(code * 2^(old -
+ * e)).  A code is rint(x * 2^-e), ties to even.  Keys are normalised and
+ * rotated in 64 bits by the angle position * theta^(-2 i / d) itself (not its
+ * fp32 product), so codes do not depend on how the work is laid out; splitting
+ * a block's rows over several calls rounds its earlier rows again.
+ * Values that are not finite don't count in e and are stored as +-127 (an
+ * infinity) or 0 (NaN), with the error bit.  qkv and query are 16-byte
+ * aligned.  No allocation, no synchronisation, graph-capturable. */
+int mmr_kv8_append(const float* qkv, const float* q_norm, const float* k_norm, float eps, const mmr_rope_table* rope,
+                   const mmr_kv8_pages* cache, const int32_t* offsets, const int32_t* context, int64_t rows,
+                   int64_t max_rows, int64_t q_heads, float* query, int32_t* error, mmr_stream_t stream);
+/* The 8-bit counterpart of mmr_attention_from_cache / mmr_prefill_attention:
+ * row i of sequence s attends its keys 0 .. context[s] + i (appended before),
+ * softmax(q.k / sqrt(d)) v per head, GQA mapping kv = h / (Hq/Hkv).  query
+ * and out fp32 [rows][q_heads d], 16-byte aligned, q_heads a multiple of
+ * kv_heads.  max_tokens bounds context[s] + n over all sequences and sizes
+ * the split along the context.  A query row that is not finite gives a row of
+ * NaN and no other.  The workspace
+ * (mmr_kv8_attention_workspace_size bytes of the same sizes, possibly 0;
+ * 16-byte aligned) holds the split partials and is the call's own until it
+ * has run; it keeps nothing between calls.  No allocation, no
+ * synchronisation, graph-capturable. */
+size_t mmr_kv8_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
+                                        int64_t rows, int64_t max_rows, int64_t max_tokens);
+int mmr_kv8_attention(const float* query, const mmr_kv8_pages* cache, const int32_t* offsets, const int32_t* context,
+                      int64_t rows, int64_t max_rows, int64_t max_tokens, int64_t q_heads, float* out,
+                      void* workspace, size_t workspace_bytes, int32_t* error, mmr_stream_t stream);
+
+/* ---- products with 4-bit weights (no counterpart in the reference, whose
+ * projections are fp16: ascend_matmul.cpp:385-410) ---------------------------
+ * w[r][c] = scale[r][c / group] * q[r][c], q a whole number in [-8, 7], scale
+ * fp16 [rows][ceil(cols / group)], group 32, 64 or 128, cols a multiple of
+ * 32.  Codes [rows][ceil(cols / 128)][64 bytes]: of a run of 128 columns,
+ * 4-byte word 4 p + j holds columns 32 j + 8 p + 0 .. 7, its byte i column
+ * 2 i in the low nibble and 2 i + 1 in the high one, in two's complement;
+ * columns past cols are 0.
+ * mmr_q4_quantize / mmr_q4_dequantize (host memory) lay fp32 weights
+ * [rows][cols] out this way and back: scale = fp16(max |w| / 7) over the
+ * group (at most the largest fp16), q = rint(w / scale) within [-8, 7] (0
+ * where the scale is 0); weights must be finite.  mmr_q4_code_bytes is the
+ * size of the codes. */
+size_t mmr_q4_code_bytes(int64_t rows, int64_t cols);
+int mmr_q4_quantize(const float* w, int64_t rows, int64_t cols, int64_t group, uint8_t* codes, uint16_t* scales);
+int mmr_q4_dequantize(const uint8_t* codes, const uint16_t* scales, int64_t rows, int64_t cols, int64_t group,
+                      float* w);
+/* mmr_matvec_f16_ex with such weights, for `batch` rows of x at once:
+ * y[b][r] = sum_c w[r][c] x[b][c], x fp32 [batch][cols], the same prologues
+ * (of each row of x) and epilogues: y and residual fp32 [batch][rows],
+ * residual may alias y; MMR_EPI_SWIGLU takes an even number of rows,
+ * interleaved gate_0, up_0, ..., and gives y [batch][rows / 2].  codes are 16-byte
+ * aligned.  The workspace (mmr_matvec_q4_workspace_size bytes, 0 for few
+ * rows of x; 16-byte aligned) is the call's own until it has run.  No
+ * allocation, no synchronisation, graph-capturable. */
+size_t mmr_matvec_q4_workspace_size(int64_t cols, int64_t batch);
+int mmr_matvec_q4(const uint8_t* codes, const uint16_t* scales, int64_t group, int64_t rows, int64_t cols,
+                  const float* x, int64_t batch, const float* norm_w, float eps, int prologue, int epilogue,
+                  const float* residual, float* y, void* workspace, size_t workspace_bytes, mmr_stream_t stream);
+
 /* ---- support ops (ascend_custom_ops.h:70-79,109-120) ----------------------- */
 int mmr_rms_norm_rows(const float* in, const float* w, float eps, int64_t rows, int64_t cols, float* out,
                       mmr_stream_t stream);

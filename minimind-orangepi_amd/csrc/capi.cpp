@@ -37,6 +37,7 @@ struct mmr_batch_state {
 };
 struct mmr_rope_table {
   DeviceBuffer inv_freq;  // [d/2]: 1 / powf(theta, 2i / d); cos/sin(pos * inv_freq) on the device
+  DeviceBuffer turns;     // [d/2]: theta^(-2i / d) / 2 pi turns in units of 2^-64 (the 8-bit cache's append)
   int64_t max_positions = 0;
   int64_t head_dim = 0;
   const float* data() const { return static_cast<const float*>(inv_freq.data()); }
@@ -492,6 +493,18 @@ int mmr_rope_table_create(int64_t max_positions, int64_t head_dim, float theta, 
           1.0F / std::pow(theta, static_cast<float>(i * 2) / static_cast<float>(head_dim));
     t->inv_freq.reset(inv.size() * sizeof(float));
     hip(hipMemcpy(t->inv_freq.data(), inv.data(), inv.size() * sizeof(float), hipMemcpyHostToDevice), "hipMemcpy");
+    // Modulo 2^64: whole turns drop out (theta < 1 has frequencies above one turn).
+    std::vector<uint64_t> turns(static_cast<size_t>(half));
+    for (int64_t i = 0; i < half; ++i) {
+      const long double f = std::pow(static_cast<long double>(theta),
+                                     -static_cast<long double>(2 * i) / static_cast<long double>(head_dim)) /
+                            6.283185307179586476925286766559005768L;
+      const long double part = std::fmod(f, 1.0L) * 18446744073709551616.0L;
+      turns[static_cast<size_t>(i)] = part < 18446744073709551615.0L ? static_cast<uint64_t>(part + 0.5L) : 0;
+    }
+    t->turns.reset(turns.size() * sizeof(uint64_t));
+    hip(hipMemcpy(t->turns.data(), turns.data(), turns.size() * sizeof(uint64_t), hipMemcpyHostToDevice),
+        "hipMemcpy");
     t->max_positions = max_positions;
     t->head_dim = head_dim;
     *out = t.release();
@@ -989,6 +1002,220 @@ int mmr_prefill_attention(const float* query, const mmr_kv_cache* cache, int64_t
     a.out = out;
     a.out_stride = static_cast<int>(q_heads * head_dim);
     hip(mmr::launch_prefill_attention(a, cache->kv(), as_stream(stream)), "prefill attention launch");
+  });
+}
+
+namespace {
+
+bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+void check_kv8_sizes(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs, int64_t rows,
+                     int64_t max_rows) {
+  require(head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128,
+          "head_dim must be 32, 64, 96 or 128");
+  require(kv_heads >= 1 && kv_heads <= 64, "kv_heads must be in [1, 64]");
+  require(q_heads >= kv_heads && q_heads <= 4096 && q_heads % kv_heads == 0,
+          "q_heads must be a multiple of kv_heads, at most 4096");
+  require(seqs >= 1 && seqs <= 65535, "seqs must be in [1, 65535]");
+  require(rows >= 0 && max_rows >= 0 && max_rows <= rows, "need 0 <= max_rows <= rows");
+  require(rows <= (int64_t{1} << 24) && rows * (q_heads + 2 * kv_heads) <= (int64_t{1} << 27), "too many rows");
+}
+
+mmr::Kv8Pages kv8_pages(const mmr_kv8_pages* c) {
+  require(c, "null cache");
+  require(c->keys && c->values && c->key_exps && c->value_exps && c->table, "null cache buffer");
+  require(aligned(c->keys, 16) && aligned(c->values, 16), "keys and values must be 16-byte aligned");
+  require(aligned(c->key_exps, 4) && aligned(c->value_exps, 4) && aligned(c->table, 4),
+          "exponents and table must be 4-byte aligned");
+  require(c->pages >= 1 && c->pages <= INT32_MAX, "pages out of range");
+  require(c->pages_per_seq >= 1 && c->pages_per_seq <= (int64_t{1} << 24), "pages_per_seq must be in [1, 2^24]");
+  mmr::Kv8Pages p;
+  p.keys = c->keys;
+  p.values = c->values;
+  p.key_exps = c->key_exps;
+  p.value_exps = c->value_exps;
+  p.table = c->table;
+  p.pages = static_cast<int>(c->pages);
+  p.seqs = static_cast<int>(c->seqs);
+  p.per_seq = static_cast<int>(c->pages_per_seq);
+  p.hkv = static_cast<int>(c->kv_heads);
+  p.d = static_cast<int>(c->head_dim);
+  return p;
+}
+
+mmr::Kv8AttnPlan kv8_plan(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs, int64_t rows,
+                          int64_t max_rows, int64_t max_tokens) {
+  return mmr::kv8_attention_plan(static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(head_dim),
+                                 static_cast<int>(seqs), static_cast<int>(rows), static_cast<int>(max_rows),
+                                 max_tokens);
+}
+
+void check_q4_shape(int64_t rows, int64_t cols, int64_t group) {
+  require(rows > 0 && cols > 0 && rows <= (1 << 24) && cols <= (1 << 20), "rows or cols out of range");
+  require(cols % 32 == 0, "cols must be a multiple of 32");
+  require(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128");
+}
+
+// Byte of a row's codes that holds column c.
+int64_t q4_byte(int64_t c) {
+  const int64_t u = c % mmr::kQ4Cols;
+  return c / mmr::kQ4Cols * 64 + (u % 32 / 8 * 4 + u / 32) * 4 + u % 8 / 2;
+}
+
+int64_t q4_row_bytes(int64_t cols) { return (cols + mmr::kQ4Cols - 1) / mmr::kQ4Cols * 64; }
+
+}  // namespace
+
+int mmr_kv8_append(const float* qkv, const float* q_norm, const float* k_norm, float eps, const mmr_rope_table* rope,
+                   const mmr_kv8_pages* cache, const int32_t* offsets, const int32_t* context, int64_t rows,
+                   int64_t max_rows, int64_t q_heads, float* query, int32_t* error, mmr_stream_t stream) {
+  return guarded([&] {
+    mmr::Kv8AppendArgs a;
+    a.cache = kv8_pages(cache);
+    check_kv8_sizes(q_heads, cache->kv_heads, cache->head_dim, cache->seqs, rows, max_rows);
+    require(qkv && rope && offsets && context && query && error, "null argument");
+    require(aligned(qkv, 16) && aligned(query, 16), "qkv and query must be 16-byte aligned");
+    require(rope->head_dim == cache->head_dim, "rope table head_dim mismatch");
+    require(eps >= 0.0f, "eps must not be negative");
+    if (max_rows == 0) return;
+    a.qkv = qkv;
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.eps = eps;
+    a.turns = static_cast<const uint64_t*>(rope->turns.data());
+    a.max_positions = rope->max_positions;
+    a.offsets = offsets;
+    a.context = context;
+    a.rows = static_cast<int>(rows);
+    a.max_rows = static_cast<int>(max_rows);
+    a.hq = static_cast<int>(q_heads);
+    a.query = query;
+    a.error = error;
+    hip(mmr::launch_kv8_append(a, as_stream(stream)), "8-bit cache append launch");
+  });
+}
+
+size_t mmr_kv8_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
+                                        int64_t rows, int64_t max_rows, int64_t max_tokens) {
+  if (guarded([&] { check_kv8_sizes(q_heads, kv_heads, head_dim, seqs, rows, max_rows); }) != MMR_OK) return 0;
+  if (max_rows == 0 || max_tokens < 1) return 0;
+  return static_cast<size_t>(
+             kv8_plan(q_heads, kv_heads, head_dim, seqs, rows, max_rows, max_tokens).partial_floats) *
+         sizeof(float);
+}
+
+int mmr_kv8_attention(const float* query, const mmr_kv8_pages* cache, const int32_t* offsets, const int32_t* context,
+                      int64_t rows, int64_t max_rows, int64_t max_tokens, int64_t q_heads, float* out,
+                      void* workspace, size_t workspace_bytes, int32_t* error, mmr_stream_t stream) {
+  return guarded([&] {
+    mmr::Kv8AttnArgs a;
+    a.cache = kv8_pages(cache);
+    check_kv8_sizes(q_heads, cache->kv_heads, cache->head_dim, cache->seqs, rows, max_rows);
+    require(query && offsets && context && out && error, "null argument");
+    require(aligned(query, 16) && aligned(out, 16) && aligned(workspace, 16),
+            "query, out and workspace must be 16-byte aligned");
+    require(max_tokens >= 1 && max_tokens <= cache->pages_per_seq * mmr::kKv8Page,
+            "max_tokens must be in [1, 64 pages_per_seq]");
+    if (max_rows == 0) return;
+    const mmr::Kv8AttnPlan p =
+        kv8_plan(q_heads, cache->kv_heads, cache->head_dim, cache->seqs, rows, max_rows, max_tokens);
+    const size_t need = static_cast<size_t>(p.partial_floats) * sizeof(float);
+    require(need == 0 || workspace, "null workspace");
+    require(workspace_bytes >= need, "workspace too small");
+    a.query = query;
+    a.offsets = offsets;
+    a.context = context;
+    a.rows = static_cast<int>(rows);
+    a.max_rows = static_cast<int>(max_rows);
+    a.hq = static_cast<int>(q_heads);
+    a.max_tokens = max_tokens;
+    a.out = out;
+    a.part = static_cast<float*>(workspace);
+    a.error = error;
+    hip(mmr::launch_kv8_attention(a, as_stream(stream)), "8-bit cache attention launch");
+  });
+}
+
+size_t mmr_q4_code_bytes(int64_t rows, int64_t cols) {
+  return rows > 0 && cols > 0 ? static_cast<size_t>(rows) * static_cast<size_t>(q4_row_bytes(cols)) : 0;
+}
+
+int mmr_q4_quantize(const float* w, int64_t rows, int64_t cols, int64_t group, uint8_t* codes, uint16_t* scales) {
+  return guarded([&] {
+    require(w && codes && scales, "null buffer");
+    check_q4_shape(rows, cols, group);
+    const int64_t groups = (cols + group - 1) / group, bytes = q4_row_bytes(cols);
+    for (int64_t i = 0; i < rows * cols; ++i) require(std::isfinite(w[i]), "weights must be finite");
+    std::memset(codes, 0, static_cast<size_t>(rows * bytes));
+    for (int64_t r = 0; r < rows; ++r) {
+      for (int64_t g = 0; g < groups; ++g) {
+        const int64_t first = g * group, last = std::min(first + group, cols);
+        float top = 0.0f;
+        for (int64_t c = first; c < last; ++c) top = std::max(top, std::fabs(w[r * cols + c]));
+        const uint16_t half = float_to_half(std::min(top / 7.0f, 65504.0f));
+        const float scale = half_to_float(half);
+        scales[r * groups + g] = half;
+        for (int64_t c = first; c < last && scale > 0.0f; ++c) {
+          const float q = std::nearbyint(w[r * cols + c] / scale);
+          const int n = static_cast<int>(std::min(7.0f, std::max(-8.0f, q)));
+          codes[r * bytes + q4_byte(c)] |= static_cast<uint8_t>((n & 15) << (c % 2 * 4));
+        }
+      }
+    }
+  });
+}
+
+int mmr_q4_dequantize(const uint8_t* codes, const uint16_t* scales, int64_t rows, int64_t cols, int64_t group,
+                      float* w) {
+  return guarded([&] {
+    require(w && codes && scales, "null buffer");
+    check_q4_shape(rows, cols, group);
+    const int64_t groups = (cols + group - 1) / group, bytes = q4_row_bytes(cols);
+    for (int64_t r = 0; r < rows; ++r)
+      for (int64_t c = 0; c < cols; ++c) {
+        const int n = codes[r * bytes + q4_byte(c)] >> (c % 2 * 4) & 15;
+        w[r * cols + c] = static_cast<float>((n ^ 8) - 8) * half_to_float(scales[r * groups + c / group]);
+      }
+  });
+}
+
+size_t mmr_matvec_q4_workspace_size(int64_t cols, int64_t batch) {
+  if (cols <= 0 || batch <= 0 || cols > (1 << 20) || batch > (1 << 16)) return 0;
+  return static_cast<size_t>(mmr::matvec_q4_workspace(static_cast<int>(cols), static_cast<int>(batch)));
+}
+
+int mmr_matvec_q4(const uint8_t* codes, const uint16_t* scales, int64_t group, int64_t rows, int64_t cols,
+                  const float* x, int64_t batch, const float* norm_w, float eps, int prologue, int epilogue,
+                  const float* residual, float* y, void* workspace, size_t workspace_bytes, mmr_stream_t stream) {
+  return guarded([&] {
+    require(codes && scales && x && y, "null buffer");
+    check_q4_shape(rows, cols, group);
+    require(batch > 0 && batch <= (1 << 16), "batch must be in [1, 65536]");
+    require(aligned(codes, 16) && aligned(workspace, 16), "codes and workspace must be 16-byte aligned");
+    require(prologue >= MMR_PRO_PLAIN && prologue <= MMR_PRO_RMSNORM_FINAL, "unknown prologue");
+    require(epilogue >= MMR_EPI_STORE && epilogue <= MMR_EPI_SWIGLU, "unknown epilogue");
+    require(prologue == MMR_PRO_PLAIN || norm_w, "the RMSNorm prologue needs norm_w");
+    require(epilogue != MMR_EPI_RESIDUAL || residual, "the residual epilogue needs residual");
+    require(epilogue != MMR_EPI_SWIGLU || rows % 2 == 0, "SwiGLU needs an even number of rows");
+    const size_t need = mmr_matvec_q4_workspace_size(cols, batch);
+    require(need == 0 || workspace, "null workspace");
+    require(workspace_bytes >= need, "workspace too small");
+    mmr::MatvecQ4Args a;
+    a.codes = codes;
+    a.scales = reinterpret_cast<const __half*>(scales);
+    a.group = static_cast<int>(group);
+    a.rows = static_cast<int>(rows);
+    a.cols = static_cast<int>(cols);
+    a.batch = static_cast<int>(batch);
+    a.x = x;
+    a.norm_w = norm_w;
+    a.eps = eps;
+    a.residual = residual;
+    a.y = y;
+    a.workspace = workspace;
+    hip(mmr::launch_matvec_q4(a, static_cast<mmr::GemvPrologue>(prologue), static_cast<mmr::GemvEpilogue>(epilogue),
+                              as_stream(stream)),
+        "4-bit matvec launch");
   });
 }
 

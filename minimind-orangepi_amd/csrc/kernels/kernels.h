@@ -557,4 +557,78 @@ hipError_t launch_embedding_gather(const __half* table, const int32_t* ids, int 
 // `reps` times on a private stream (probe.hip).
 hipError_t measure_launch_floor(int kernels, int blocks, bool load_store, int reps, float* us_per_kernel);
 
+// ------------------------------------------------- 8-bit paged cache ----
+// Layout and the meaning of the codes: kv8_common.h.
+constexpr int kKv8Page = 64;   // tokens of a page
+constexpr int kKv8Block = 16;  // tokens of a block under one exponent
+constexpr int kKv8MinExp = -126, kKv8MaxExp = 122;
+enum Kv8Error : int { kKv8BadRows = 1, kKv8NotFinite = 2 };  // bits of *error
+
+struct Kv8Pages {
+  int8_t* keys = nullptr;
+  int8_t* values = nullptr;
+  int8_t* key_exps = nullptr;
+  int8_t* value_exps = nullptr;
+  const int32_t* table = nullptr;  // [seqs][per_seq] page numbers
+  int pages = 0, seqs = 0, per_seq = 0, hkv = 0, d = 0;
+};
+
+// Normalises (norms nullable), rotates and appends rows offsets[s] ..
+// offsets[s + 1] - 1 of qkv at positions context[s] + i of sequence s; the
+// rotated queries go to query.
+struct Kv8AppendArgs {
+  Kv8Pages cache;
+  const float* qkv = nullptr;
+  const float* q_norm = nullptr;
+  const float* k_norm = nullptr;
+  float eps = 0.0f;
+  const uint64_t* turns = nullptr;  // [d/2]: turns per position, in 2^-64
+  int64_t max_positions = 0;
+  const int32_t* offsets = nullptr;
+  const int32_t* context = nullptr;
+  int rows = 0, max_rows = 0, hq = 0;
+  float* query = nullptr;
+  int32_t* error = nullptr;
+};
+hipError_t launch_kv8_append(const Kv8AppendArgs& a, hipStream_t stream);
+
+// Causal attention of the same rows over the cache.
+struct Kv8AttnArgs {
+  Kv8Pages cache;
+  const float* query = nullptr;
+  const int32_t* offsets = nullptr;
+  const int32_t* context = nullptr;
+  int rows = 0, max_rows = 0, hq = 0;
+  int64_t max_tokens = 0;  // most keys a sequence has with its new rows
+  float* out = nullptr;
+  float* part = nullptr;  // kv8_attention_plan(...).partial_floats floats
+  int32_t* error = nullptr;
+};
+struct Kv8AttnPlan {
+  int tile_rows = 0;    // (token, head) rows of one KV group that a block takes
+  int chunk_pages = 0;  // pages of a split
+  int splits = 0;
+  int64_t partial_floats = 0;  // 0 when one split covers every context
+};
+Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens);
+hipError_t launch_kv8_attention(const Kv8AttnArgs& a, hipStream_t stream);
+
+// ------------------------------------------- 4-bit matrix-vector product ----
+// y[b][r] = sum_c scale[r][c / group] * q[r][c] * x[b][c], the prologues and
+// epilogues of the fp16 GEMV (no combine, embedding or argmax forms).
+constexpr int kQ4Cols = 128;  // columns of a packed run of 64 bytes
+struct MatvecQ4Args {
+  const uint8_t* codes = nullptr;  // [rows][ceil(cols / 128)][64]
+  const __half* scales = nullptr;  // [rows][ceil(cols / group)]
+  int group = 0, rows = 0, cols = 0, batch = 0;
+  const float* x = nullptr;
+  const float* norm_w = nullptr;
+  float eps = 0.0f;
+  const float* residual = nullptr;
+  float* y = nullptr;
+  void* workspace = nullptr;  // matvec_q4_workspace(cols, batch) bytes
+};
+int64_t matvec_q4_workspace(int cols, int batch);
+hipError_t launch_matvec_q4(const MatvecQ4Args& a, GemvPrologue pro, GemvEpilogue epi, hipStream_t stream);
+
 }  // namespace mmr

@@ -74,6 +74,11 @@ class Config(C.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class _Kv8PagesStruct(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("keys", "values", "key_exps", "value_exps", "table")] + \
+               [(n, C.c_int64) for n in ("pages", "seqs", "pages_per_seq", "kv_heads", "head_dim")]
+
+
 VP, I64, I32, U64, F32, SZ = C.c_void_p, C.c_int64, C.c_int32, C.c_uint64, C.c_float, C.c_size_t
 P_I32 = C.POINTER(C.c_int32)
 P_F32 = C.POINTER(C.c_float)
@@ -152,6 +157,14 @@ _SIGS = {
     "mmr_matmul_f16": ([VP, I64, I64, VP, I64, VP, VP, VP], C.c_int),
     "mmr_prefill_qkv_rows": ([VP, VP, VP, F32, VP, VP, I64, I64, I64, I64, I64, VP, VP], C.c_int),
     "mmr_prefill_attention": ([VP, VP, I64, I64, I64, I64, I64, VP, VP], C.c_int),
+    "mmr_kv8_append": ([VP, VP, VP, F32, VP, C.POINTER(_Kv8PagesStruct), VP, VP, I64, I64, I64, VP, VP, VP], C.c_int),
+    "mmr_kv8_attention_workspace_size": ([I64] * 7, SZ),
+    "mmr_kv8_attention": ([VP, C.POINTER(_Kv8PagesStruct), VP, VP, I64, I64, I64, I64, VP, VP, SZ, VP, VP], C.c_int),
+    "mmr_q4_code_bytes": ([I64, I64], SZ),
+    "mmr_q4_quantize": ([VP, I64, I64, I64, VP, VP], C.c_int),
+    "mmr_q4_dequantize": ([VP, VP, I64, I64, I64, VP], C.c_int),
+    "mmr_matvec_q4_workspace_size": ([I64, I64], SZ),
+    "mmr_matvec_q4": ([VP, VP, I64, I64, I64, VP, I64, VP, F32, C.c_int, C.c_int, VP, VP, VP, SZ, VP], C.c_int),
     "mmr_rms_norm_rows": ([VP, VP, F32, I64, I64, VP, VP], C.c_int),
     "mmr_add": ([VP, VP, I64, VP, VP], C.c_int),
     "mmr_swiglu_rows": ([VP, I64, I64, VP, VP], C.c_int),
@@ -601,6 +614,84 @@ def prefill_attention(query, cache: KvCache, start_position, seq_len, q_heads, k
                       stream=None) -> None:
     check(_lib.mmr_prefill_attention(query.ptr, cache.handle, start_position, seq_len, q_heads, kv_heads, head_dim,
                                      out.ptr, _s(stream)))
+
+
+KV8_PAGE, KV8_BLOCK = 64, 16
+KV8_ERROR_ROWS, KV8_ERROR_NOT_FINITE = 1, 2
+
+
+class Kv8Pages:
+    """The memory of an 8-bit paged cache (mmr_kv8_pages): int8 codes and
+    exponents and an int32 page table [seqs][pages_per_seq], in buffers that
+    the caller owns (anything with .ptr; kept alive by this object)."""
+
+    def __init__(self, keys, values, key_exps, value_exps, table, pages: int, seqs: int, pages_per_seq: int,
+                 kv_heads: int, head_dim: int):
+        self.buffers = (keys, values, key_exps, value_exps, table)
+        self.pages, self.seqs, self.pages_per_seq = pages, seqs, pages_per_seq
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+        self.struct = _Kv8PagesStruct(*(b.ptr for b in self.buffers), pages, seqs, pages_per_seq, kv_heads, head_dim)
+        self.ref = C.byref(self.struct)
+
+    @classmethod
+    def allocate(cls, table: np.ndarray, pages: int, kv_heads: int, head_dim: int) -> "Kv8Pages":
+        """Pages of the library's own allocation under a host table [seqs][pages_per_seq]."""
+        table = np.ascontiguousarray(table, dtype=np.int32)
+        codes, exps = (pages, kv_heads, KV8_PAGE, head_dim), (pages, kv_heads, KV8_PAGE // KV8_BLOCK)
+        return cls(DeviceArray(codes, np.int8, zero=True),
+                   DeviceArray((pages, kv_heads, head_dim, KV8_PAGE), np.int8, zero=True),
+                   DeviceArray(exps, np.int8, zero=True), DeviceArray(exps, np.int8, zero=True),
+                   DeviceArray.from_numpy(table), pages, *table.shape, kv_heads, head_dim)
+
+
+def kv8_append(qkv, q_norm, k_norm, eps, rope: RopeTable, cache: Kv8Pages, offsets, context, rows: int, max_rows: int,
+               q_heads: int, query, error, stream=None) -> None:
+    check(_lib.mmr_kv8_append(qkv.ptr, q_norm.ptr if q_norm else None, k_norm.ptr if k_norm else None, eps,
+                              rope.handle, cache.ref, offsets.ptr, context.ptr, rows, max_rows, q_heads, query.ptr,
+                              error.ptr, _s(stream)))
+
+
+def kv8_attention_workspace_size(q_heads: int, kv_heads: int, head_dim: int, seqs: int, rows: int, max_rows: int,
+                                 max_tokens: int) -> int:
+    return int(_lib.mmr_kv8_attention_workspace_size(q_heads, kv_heads, head_dim, seqs, rows, max_rows, max_tokens))
+
+
+def kv8_attention(query, cache: Kv8Pages, offsets, context, rows: int, max_rows: int, max_tokens: int, q_heads: int,
+                  out, workspace, error, stream=None) -> None:
+    check(_lib.mmr_kv8_attention(query.ptr, cache.ref, offsets.ptr, context.ptr, rows, max_rows, max_tokens, q_heads,
+                                 out.ptr, workspace.ptr if workspace else None, workspace.nbytes if workspace else 0,
+                                 error.ptr, _s(stream)))
+
+
+def q4_quantize(w: np.ndarray, group: int) -> tuple[np.ndarray, np.ndarray]:
+    """Host weights fp32 [rows][cols] -> (codes uint8 [rows][bytes], scales fp16 [rows][groups])."""
+    w = np.ascontiguousarray(w, dtype=np.float32)
+    rows, cols = w.shape
+    codes = np.empty((rows, int(_lib.mmr_q4_code_bytes(rows, cols)) // max(rows, 1)), np.uint8)
+    scales = np.empty((rows, -(-cols // group) if group > 0 else 0), np.uint16)
+    check(_lib.mmr_q4_quantize(_ptr(w), rows, cols, group, _ptr(codes), _ptr(scales)))
+    return codes, scales.view(np.float16)
+
+
+def q4_dequantize(codes: np.ndarray, scales: np.ndarray, cols: int, group: int) -> np.ndarray:
+    """The fp32 weights [rows][cols] that q4_quantize's result stands for."""
+    codes, scales = np.ascontiguousarray(codes, np.uint8), np.ascontiguousarray(scales, np.float16)
+    rows = codes.shape[0]
+    assert codes.nbytes == int(_lib.mmr_q4_code_bytes(rows, cols)) and scales.shape == (rows, -(-cols // group))
+    w = np.empty((rows, cols), np.float32)
+    check(_lib.mmr_q4_dequantize(_ptr(codes), _ptr(scales), rows, cols, group, _ptr(w)))
+    return w
+
+
+def matvec_q4_workspace_size(cols: int, batch: int) -> int:
+    return int(_lib.mmr_matvec_q4_workspace_size(cols, batch))
+
+
+def matvec_q4(codes, scales, group: int, rows: int, cols: int, x, batch: int, y, *, norm_w=None, eps=0.0,
+              prologue=PRO_PLAIN, epilogue=EPI_STORE, residual=None, workspace=None, stream=None) -> None:
+    check(_lib.mmr_matvec_q4(codes.ptr, scales.ptr, group, rows, cols, x.ptr, batch, norm_w.ptr if norm_w else None,
+                             eps, prologue, epilogue, residual.ptr if residual else None, y.ptr,
+                             workspace.ptr if workspace else None, workspace.nbytes if workspace else 0, _s(stream)))
 
 
 def rms_norm_rows(x, w, eps, rows, cols, out, stream=None) -> None:

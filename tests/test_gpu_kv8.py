@@ -1,0 +1,358 @@
+"""The 8-bit paged cache on the GPU against its definition in 64 bits: codes and
+exponents bit for bit, queries to half a step, attention within the bound that
+low_bit_reference.attention derives for each row."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import low_bit_reference as ref
+
+pytestmark = pytest.mark.gpu
+THETA, EPS = 1e6, 1e-5
+HALF_STEP = 2.0 ** -24
+
+
+def ints(mmr, values):
+    return mmr.DeviceArray.from_numpy(np.asarray(values, np.int32))
+
+
+def pages_for(rows, context):
+    return max(1, max(-(-(n + c) // ref.PAGE) for n, c in zip(rows, context)))
+
+
+def offsets_of(rows):
+    return np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+
+
+class Append:
+    """One append on the device and the same in 64 bits."""
+
+    def __init__(self, mmr, cache, hq, norms=True, positions=32768, rng=None):
+        self.mmr, self.cache, self.hq, d = mmr, cache, hq, cache.d
+        self.rope = mmr.RopeTable(positions, d, THETA)
+        self.norms = [(1 + 0.1 * rng.standard_normal(d)).astype(np.float32) if norms else None for _ in range(2)]
+        self.dnorms = [mmr.DeviceArray.from_numpy(n) if norms else None for n in self.norms]
+        self.device = cache.upload(mmr)
+        self.error = ints(mmr, [0])
+
+    def __call__(self, qkv, rows, context, stream=None, max_rows=None):
+        mmr, offsets = self.mmr, offsets_of(rows)
+        fill = np.full((len(qkv), self.hq * self.cache.d), 7.5, np.float32)
+        query = mmr.DeviceArray.from_numpy(fill)
+        mmr.kv8_append(mmr.DeviceArray.from_numpy(qkv), *self.dnorms, EPS, self.rope, self.device,
+                       ints(mmr, offsets), ints(mmr, context), len(qkv), max_rows or max(rows), self.hq, query,
+                       self.error, stream=stream)
+        mmr.synchronize()
+        want = ref.append(self.cache, qkv, offsets, context, self.hq, THETA, *self.norms, EPS, fill)
+        return query.numpy(), want
+
+    def check(self, qkv, rows, context, error=0):
+        got, want = self(qkv, rows, context)
+        self.cache.assert_equals(self.device)
+        # Computed in 64 bits and rounded once.
+        assert (np.abs(got - want) <= HALF_STEP * np.abs(want) + 1e-12).all()
+        assert int(self.error.numpy()[0]) == error
+
+
+def qkv_rows(rng, n, hq, hkv, d, std=0.6):
+    return (rng.standard_normal((n, (hq + 2 * hkv) * d)) * std).astype(np.float32)
+
+
+HEADS = [(8, 2, 96), (4, 4, 64), (8, 1, 128), (6, 2, 32)]
+
+
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+@pytest.mark.parametrize("rows,context", [([1], [0]), ([1], [777]), ([1, 1, 1], [15, 16, 63]), ([5, 0, 17, 64], [3, 9, 60, 0]),
+                                          ([130], [1]), ([16, 16], [16, 8])])
+def test_append(gpu, hq, hkv, d, rows, context):
+    print(f"[case] append {hq},{hkv},{d} rows {rows} context {context}", flush=True)
+    rng = np.random.default_rng(sum(rows) * 31 + d)
+    per = pages_for(rows, context)
+    cache = ref.Cache(rng, len(rows) * per + 2, len(rows), per, hkv, d)
+    cache.fill(rng, context)
+    # Two rows behind the last sequence, whose queries stay as they are.
+    Append(gpu, cache, hq, rng=rng).check(qkv_rows(rng, sum(rows) + 2, hq, hkv, d), rows, context)
+
+
+def test_append_token_by_token_moves_blocks(gpu):
+    """Every token larger than the ones before: the block's codes move to a larger exponent again and again."""
+    rng = np.random.default_rng(5)
+    cache = ref.Cache(rng, 3, 1, 2, 2, 96)
+    step = Append(gpu, cache, 8, norms=False, rng=rng)
+    for t in range(70):
+        step.check(qkv_rows(rng, 1, 8, 2, 96, 1e-3 * 1.3 ** (t % 37)), [1], [t])
+
+
+def test_append_sizes_at_both_ends(gpu):
+    rng = np.random.default_rng(6)
+    cache = ref.Cache(rng, 4, 1, 2, 2, 64)
+    step = Append(gpu, cache, 4, norms=False, rng=rng)
+    qkv = qkv_rows(rng, 80, 4, 2, 64)
+    qkv[0:16] = 0.0
+    qkv[16:32] *= 2.0 ** -130  # subnormal: the least exponent
+    qkv[32:48] *= 2.0 ** 126
+    qkv[48] = 127.0  # exactly on the border, and just past it
+    qkv[49:64] = np.nextafter(np.float32(127.0), np.float32(200.0))
+    qkv[64:80, ::3] = 0.5  # ties to even
+    with np.errstate(over="ignore"):
+        got, want = step(qkv, [80], [0])
+    cache.assert_equals(step.device)
+    assert int(step.error.numpy()[0]) == 0
+
+
+def test_append_keeps_and_flags_what_is_not_finite(gpu):
+    rng = np.random.default_rng(7)
+    hq, hkv, d = 4, 2, 64
+    cache = ref.Cache(rng, 4, 2, 2, hkv, d)
+    step = Append(gpu, cache, hq, norms=False, rng=rng)
+    qkv = qkv_rows(rng, 40, hq, hkv, d)
+    v = (hq + hkv) * d
+    qkv[3, v + 5], qkv[4, v + 6], qkv[5, v + d + 7] = np.inf, -np.inf, np.nan
+    got, want = step(qkv, [20, 20], [0, 30])
+    cache.assert_equals(step.device)
+    assert int(step.error.numpy()[0]) == gpu.KV8_ERROR_NOT_FINITE
+    assert np.isfinite(got).all()
+
+
+def test_append_refuses_on_the_device(gpu):
+    """Bad rows and pages are flagged; the other sequences are appended."""
+    mmr, rng = gpu, np.random.default_rng(8)
+    hq, hkv, d = 8, 2, 96
+    cache = ref.Cache(rng, 12, 3, 3, hkv, d)
+    cache.table[1, 1] = 12  # page past the pool
+    step = Append(mmr, cache, hq, positions=150, rng=rng)
+    before = [b.numpy() for b in step.device.buffers]
+    qkv = qkv_rows(rng, 30, hq, hkv, d)
+    offsets, context = [0, 10, 20, 30], [0, 64, 145]  # the last reaches past the rotation table
+    query = mmr.DeviceArray.from_numpy(np.full((30, hq * d), 7.5, np.float32))
+    mmr.kv8_append(mmr.DeviceArray.from_numpy(qkv), *step.dnorms, EPS, step.rope, step.device, ints(mmr, offsets),
+                   ints(mmr, context), 30, 10, hq, query, step.error)
+    assert int(step.error.numpy()[0]) == mmr.KV8_ERROR_ROWS
+    got = query.numpy()
+    assert (got[10:] == 7.5).all() and (got[:10] != 7.5).any(-1).all()
+    for name, buffer, old in zip(("keys", "values", "key_exps", "value_exps"), step.device.buffers, before):
+        now = buffer.numpy()
+        now[cache.table[0, 0]] = old[cache.table[0, 0]]
+        np.testing.assert_array_equal(now, old, err_msg=name)
+    # Rows up to `fine` belong to a sequence that is in order.
+    for offsets, rows, most, fine in (([0, 10, 5, 5], 30, 10, 10), ([0, 31, 31, 31], 30, 30, 0),
+                                      ([0, 10, 10, 10], 30, 9, 0), ([-1, 0, 0, 0], 30, 9, 0)):
+        step.error.zero()
+        query.upload(np.full((30, hq * d), 7.5, np.float32))
+        mmr.kv8_append(mmr.DeviceArray.from_numpy(qkv), *step.dnorms, EPS, step.rope, step.device,
+                       ints(mmr, offsets), ints(mmr, [0, 0, 0]), rows, most, hq, query, step.error)
+        assert int(step.error.numpy()[0]) == mmr.KV8_ERROR_ROWS, offsets
+        got = query.numpy()
+        assert (got[fine:] == 7.5).all() and (got[:fine] != 7.5).any(-1).all()
+
+
+def test_append_at_far_positions(gpu):
+    """Angles at positions near 2^24, on a table row of a quarter million pages that shares a few."""
+    rng = np.random.default_rng(9)
+    per, hq, hkv, d = 2 ** 18, 4, 2, 64
+    cache = ref.Cache(rng, 5, 1, 1, hkv, d)
+    cache.table = np.resize(cache.table, (1, per)).astype(np.int32)
+    cache.table[0, -2:] = [3, 4]
+    cache.per_seq = per
+    context = [2 ** 24 - 70]
+    Append(gpu, cache, hq, positions=2 ** 24, rng=rng).check(qkv_rows(rng, 70, hq, hkv, d), [70], context)
+
+
+def attend(mmr, device, cache, query, offsets, context, hq, *, max_rows, max_tokens=None, stream=None, out=None):
+    max_tokens = max_tokens or cache.per_seq * ref.PAGE
+    size = mmr.kv8_attention_workspace_size(hq, cache.kv_heads, cache.d, cache.seqs, len(query), max_rows, max_tokens)
+    out = out if out is not None else mmr.DeviceArray.from_numpy(np.full(query.shape, 7.5, np.float32))
+    error = ints(mmr, [0])
+    workspace = mmr.DeviceArray(size, np.uint8) if size else None
+    mmr.kv8_attention(mmr.DeviceArray.from_numpy(query), device, ints(mmr, offsets), ints(mmr, context), len(query),
+                      max_rows, max_tokens, hq, out, workspace, error, stream=stream)
+    mmr.synchronize()
+    return out.numpy(), int(error.numpy()[0])
+
+
+def check_attention(mmr, cache, query, rows, context, hq):
+    offsets = offsets_of(rows)
+    got, error = attend(mmr, cache.upload(mmr), cache, query, offsets, context, hq, max_rows=max(rows))
+    want, bound = ref.attention(cache, query, offsets, context, hq, np.full(query.shape, 7.5, np.float32))
+    assert error == 0
+    assert (np.abs(got - want) <= bound).all(), float((np.abs(got - want) / np.maximum(bound, 1e-300)).max())
+    inside = slice(0, int(offsets[-1]))
+    # Rounding errors of either sign: sums over n pages are off by about sqrt(n), not n, half steps.
+    norm = np.linalg.norm(got[inside] - want[inside]) / np.linalg.norm(want[inside])
+    assert norm <= 4e-6, norm
+
+
+@pytest.mark.parametrize("hq,hkv,d", HEADS + [(12, 4, 96), (16, 1, 64), (3, 3, 128)])
+@pytest.mark.parametrize("rows,context", [
+    ([1], [0]), ([1], [1]), ([1], [63]), ([1], [64]), ([1, 1, 1], [15, 777, 200]), ([1], [5000]),
+    ([3, 0, 5], [100, 7, 511]), ([17, 2], [0, 130]), ([64], [0]), ([150], [77])])
+def test_attention(gpu, hq, hkv, d, rows, context):
+    print(f"[case] attention {hq},{hkv},{d} rows {rows} context {context}", flush=True)
+    rng = np.random.default_rng(sum(rows) * 17 + sum(context) + d)
+    per = pages_for(rows, context)
+    cache = ref.Cache(rng, len(rows) * per + 1, len(rows), per, hkv, d)
+    cache.fill(rng, [a + b for a, b in zip(rows, context)])
+    query = rng.standard_normal((sum(rows) + 2, hq * d)).astype(np.float32)
+    check_attention(gpu, cache, query, rows, context, hq)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_attention_over_many_rows_of_blocks(gpu, rows):
+    """Enough (sequence, tile) pairs that no split along the context is taken, and prompts of several waves a block."""
+    rng = np.random.default_rng(rows)
+    hq, hkv, d, seqs = 8, 8, 32, 130 if rows < 40 else 70
+    context = [int(c) for c in rng.integers(0, 60 if rows == 40 else 200, seqs)]
+    per = pages_for([rows] * seqs, context)
+    cache = ref.Cache(rng, seqs * per, seqs, per, hkv, d)
+    cache.fill(rng, [c + rows for c in context])
+    check_attention(gpu, cache, rng.standard_normal((rows * seqs, hq * d)).astype(np.float32), [rows] * seqs, context,
+                    hq)
+
+
+@pytest.mark.parametrize("rows", [1, 9])
+def test_attention_over_values_of_any_size(gpu, rows):
+    """Blocks whose values are 2^40 apart, all zero, or at the ends of the exponents; peaked and flat rows."""
+    rng = np.random.default_rng(rows + 20)
+    hq, hkv, d, n = 8, 2, 96, 700
+    cache = ref.Cache(rng, 12, 1, 12, hkv, d)
+    cache.fill(rng, [n + rows])
+    cache.value_exps[cache.table[0, 2:4]] += 40
+    cache.value_exps[cache.table[0, 5]] = -126
+    cache.values[cache.table[0, 6]] = 0
+    cache.key_exps[cache.table[0, 7]] -= 30
+    query = rng.standard_normal((rows, hq * d)).astype(np.float32)
+    query[:, :d] *= 30.0   # one key takes nearly all
+    query[:, d:2 * d] = 0  # all keys alike
+    query[:, 2 * d:3 * d] *= 1e-30
+    check_attention(gpu, cache, query, [rows], [n], hq)
+    # Without the large blocks the small ones must come out as exactly.
+    cache.value_exps[:] = -60
+    check_attention(gpu, cache, query, [rows], [n], hq)
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+def test_attention_rows_that_are_not_finite(gpu, rows):
+    rng = np.random.default_rng(31)
+    hq, hkv, d = 8, 2, 64
+    cache = ref.Cache(rng, 8, 2, 4, hkv, d)
+    cache.fill(rng, [100 + rows, 130 + rows])
+    query = rng.standard_normal((2 * rows, hq * d)).astype(np.float32)
+    device, offsets = cache.upload(gpu), offsets_of([rows, rows])
+    want, bound = ref.attention(cache, query, offsets, [100, 130], hq, query)
+    bad = query.copy()
+    bad[0, 3], bad[rows, d + 5], bad[-1, 5 * d] = np.nan, np.inf, -np.inf
+    got, error = attend(gpu, device, cache, bad, offsets, [100, 130], hq, max_rows=rows)
+    assert error == 0
+    mask = np.zeros(want.shape, bool)
+    mask[0, :d] = mask[rows, d:2 * d] = mask[-1, 5 * d:6 * d] = True
+    assert np.isnan(got[mask]).all()
+    assert (np.abs(got - want) <= bound)[~mask].all()
+
+
+def test_attention_takes_keys_of_bad_pages_as_absent(gpu):
+    rng = np.random.default_rng(33)
+    hq, hkv, d = 8, 2, 96
+    cache = ref.Cache(rng, 12, 2, 4, hkv, d)
+    cache.fill(rng, [200, 64])
+    query = rng.standard_normal((2, hq * d)).astype(np.float32)
+    good = cache.upload(gpu)
+    table = cache.table.copy()
+    table[0, 1], table[1, 0] = -1, 12  # of the second sequence nothing is left: a row of zeros
+    bad = gpu.Kv8Pages(*good.buffers[:4], ints(gpu, table), 12, 2, 4, hkv, d)
+    got, error = attend(gpu, bad, cache, query, [0, 1, 2], [199, 63], hq, max_rows=1)
+    assert error == gpu.KV8_ERROR_ROWS and (got[1] == 0).all()
+    short = ref.Cache(rng, 12, 1, 4, hkv, d)  # the same keys without that page
+    short.keys, short.values, short.key_exps, short.value_exps = (
+        cache.keys, cache.values, cache.key_exps, cache.value_exps)
+    short.table = cache.table[:1, [0, 2, 3, 1]].copy()
+    want, bound = ref.attention(short, query[:1], [0, 1], [199 - 64], hq, query[:1])
+    assert (np.abs(got[0] - want[0]) <= bound[0]).all()
+    # More keys than the launch was sized for, and offsets that fall: nothing is written.
+    for offsets, context, tokens in (([0, 1, 2], [199, 63], 150), ([1, 0, 2], [199, 63], 256)):
+        got, error = attend(gpu, good, cache, query, offsets, context, hq, max_rows=1, max_tokens=tokens)
+        assert error == gpu.KV8_ERROR_ROWS and (got[0] == 7.5).all()
+
+
+def test_pages_past_four_gigabytes(gpu):
+    mmr, rng = gpu, np.random.default_rng(35)
+    hq, hkv, d, pages = 8, 2, 128, 300_000  # 4.9 GB of codes each
+    small = ref.Cache(rng, 3, 1, 3, hkv, d)
+    at = np.array([[pages - 1, 7, pages - 9]], np.int32)
+    big = mmr.Kv8Pages(mmr.DeviceArray((pages, hkv, 64, d), np.int8), mmr.DeviceArray((pages, hkv, d, 64), np.int8),
+                       mmr.DeviceArray((pages, hkv, 4), np.int8), mmr.DeviceArray((pages, hkv, 4), np.int8),
+                       ints(mmr, at), pages, 1, 3, hkv, d)
+    step = Append(mmr, small, hq, rng=rng)
+    twin = step.device
+    step.device = big
+    query, want = step(qkv_rows(rng, 140, hq, hkv, d), [140], [0])
+    assert (np.abs(query - want) <= HALF_STEP * np.abs(want) + 1e-12).all()
+    got, error = attend(mmr, big, small, query, [0, 140], [0], hq, max_rows=140)
+    want, bound = ref.attention(small, query, [0, 140], [0], hq, query)
+    assert error == 0 and (np.abs(got - want) <= bound).all()
+    del twin
+
+
+def test_recorded_steps_follow_the_device_arrays(gpu):
+    """Append and attention in one graph, replayed with contexts and pages advanced in device memory, against the same
+    calls made eagerly on another stream; two graphs with workspaces of their own, replayed in turn."""
+    mmr, rng = gpu, np.random.default_rng(37)
+    hq, hkv, d, seqs, per = 8, 2, 96, 3, 8
+    twins = []
+    for stream in (mmr.Stream(), mmr.Stream(), mmr.Stream()):
+        r = np.random.default_rng(39)
+        cache = ref.Cache(r, seqs * per, seqs, per, hkv, d)
+        cache.fill(r, [40, 15, 300])
+        step = Append(mmr, cache, hq, rng=r)
+        size = mmr.kv8_attention_workspace_size(hq, hkv, d, seqs, seqs, 1, per * 64)
+        t = dict(step=step, stream=stream, qkv=mmr.DeviceArray((seqs, (hq + 2 * hkv) * d), np.float32),
+                 offsets=ints(mmr, [0, 1, 2, 3]), context=ints(mmr, [0, 0, 0]),
+                 query=mmr.DeviceArray((seqs, hq * d), np.float32), out=mmr.DeviceArray((seqs, hq * d), np.float32),
+                 workspace=mmr.DeviceArray(max(size, 1), np.uint8))
+        twins.append(t)
+
+    def calls(t):
+        s = t["step"]
+        mmr.kv8_append(t["qkv"], *s.dnorms, EPS, s.rope, s.device, t["offsets"], t["context"], seqs, 1, hq, t["query"],
+                       s.error, stream=t["stream"])
+        mmr.kv8_attention(t["query"], s.device, t["offsets"], t["context"], seqs, 1, per * 64, hq, t["out"],
+                          t["workspace"], s.error, stream=t["stream"])
+
+    graphs = []
+    for t in twins[:2]:
+        with mmr.Graph(t["stream"]) as g:
+            calls(t)
+        graphs.append(g)
+    for step in range(20):
+        qkv = qkv_rows(rng, seqs, hq, hkv, d)
+        for t in twins:
+            t["qkv"].upload(qkv)
+            t["context"].upload(np.array([40 + step, 15 + step, 300 + step], np.int32))
+        calls(twins[2])
+        for t, g in zip(twins, graphs):
+            g.launch(t["stream"])
+        mmr.synchronize()
+        for t in twins[:2]:
+            for name in ("query", "out"):
+                np.testing.assert_array_equal(t[name].numpy(), twins[2][name].numpy(), err_msg=f"{name} step {step}")
+            for a, b in zip(t["step"].device.buffers, twins[2]["step"].device.buffers):
+                np.testing.assert_array_equal(a.numpy(), b.numpy())
+
+
+def test_no_rows_is_no_work(gpu):
+    mmr, rng = gpu, np.random.default_rng(41)
+    cache = ref.Cache(rng, 2, 1, 2, 2, 96)
+    step = Append(mmr, cache, 8, rng=rng)
+    one = mmr.DeviceArray.from_numpy(np.full((1, 1152), 7.5, np.float32))
+    for rows in (0, 1):
+        mmr.kv8_append(one, *step.dnorms, EPS, step.rope, step.device, ints(mmr, [0, 0]), ints(mmr, [128]), rows, 0, 8,
+                       one, step.error)
+        mmr.kv8_attention(one, step.device, ints(mmr, [0, 0]), ints(mmr, [128]), rows, 0, 128, 8, one, None,
+                          step.error)
+    # A sequence without rows in a launch that could have brought one; its context may be the whole table.
+    mmr.kv8_append(one, *step.dnorms, EPS, step.rope, step.device, ints(mmr, [0, 0]), ints(mmr, [128]), 1, 1, 8, one,
+                   step.error)
+    got, error = attend(mmr, step.device, cache, np.zeros((1, 768), np.float32), [0, 0], [128], 8, max_rows=1)
+    mmr.synchronize()
+    assert error == 0 and (got == 7.5).all() and (one.numpy() == 7.5).all() and int(step.error.numpy()[0]) == 0
+    cache.assert_equals(step.device)
