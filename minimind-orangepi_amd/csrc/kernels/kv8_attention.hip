@@ -4,28 +4,32 @@
 //   s_mj = (q_m . k_j) log2(e) / sqrt(d)     for keys j <= context + token(m)
 //
 // with one pass over the keys and a running reference r_m in place of the row
-// maximum.  Both products run on the int8 matrix cores with the cache's codes
-// as they are stored.  The fp32 operand goes in as fixed-point digits: an
-// integer n is the sum of d_k 256^k with d_k in [-128, 127], and the bytes of
-// n + 0x808080 are those digits, the lower three with their top bit flipped.
-// Products and sums of digits and codes are exact in int32, so the only
-// roundings are those of q (2^-30 or 2^-23 of its row's largest value), of p
-// (2^-26) and of the fp32 sums over pages; nothing is converted to fp16.
+// maximum: a score may pass it by kLead before everything is scaled down to a
+// new one.  Two kernels, by the rows (token, head) that a sequence brings to a
+// group of heads that share their keys:
 //
-// S^T = K Q^T has keys as rows and query rows as columns, O^T = V^T P^T
-// dimensions as rows.  In the result layout (lane l: column l % 16, rows
-// 4 (l / 16) + i) and in the operand layout (lane l: row or column l % 16, 16
-// bytes of K from part l / 16) a lane therefore keeps its column, and if key
-// row 4 g + i of the t-th of a page's four products is key 16 g + 4 t + i, the
-// 16 scores that a lane gets are those of the 16 keys whose digits it has to
-// supply: P goes from one product to the next in registers.
+// Steps, up to 4 rows (a decode step of four heads): int8 matrix cores on the
+// codes as they are stored.  The fp32 operand goes in as fixed-point digits:
+// an integer n is the sum of d_k 256^k with d_k in [-128, 127], and the bytes
+// of n + 0x808080 are those digits, the lower three with their top bit
+// flipped.  Products and sums of digits and codes are exact in int32; rounded
+// are q (to 2^-30 of its row's largest value), p (2^-26) and the fp32 sums
+// over pages.  The 16 columns of a product are 4 rows x 4 digits, so K and V
+// are each the operand of one product, and a score is the sum over four lanes.
 //
-// Two forms of a tile:
-//   4 rows:  the 16 columns are 4 rows x 4 digits: the K and V operands are
-//            read by one product each, and a score is the sum over four lanes.
-//            A decode step of a group of four heads is one tile.
-//   16 rows: a column is a row, digits are products of their own (3 of q, 4
-//            of p) that a lane adds up itself.
+// More rows: fp16 matrix cores on codes widened to fp16 (exactly) once per
+// block, with the fp32 operand as two fp16 planes (22 bits).  Per 16 rows this
+// takes as many matrix cycles as digits would (a digit operand multiplies
+// twice the columns, but takes three digits of q and four of p), but none of
+// the adding up and taking apart of digits, which was most of that form's
+// time, and a quarter of its accumulators.
+//
+// In both, S^T = K Q^T has keys as rows and query rows as columns, O^T = V^T
+// P^T dimensions as rows.  In the result layout (lane l: column l % 16, rows
+// 4 (l / 16) + i) and in the operand layout (lane l: row or column l % 16, a
+// run of K from part l / 16) a lane keeps its column, and the keys are dealt
+// to the rows of S^T so that the scores that a lane gets are those of the keys
+// whose weights it has to supply: P never leaves the lane.
 #include "device_common.h"
 #include "kv8_common.h"
 
@@ -38,9 +42,18 @@ namespace {
 
 constexpr int kAttnWaves = 4;
 constexpr int kAttnThreads = kAttnWaves * kWave;
+constexpr int kWideWaves = 8;  // of a block that takes a short context without a split
 constexpr float kNoRow = -FLT_MAX / 2;  // reference of a row that has met no key
 constexpr float kLead = 5.0f;           // a score may pass the reference by 2^kLead
+constexpr int kRowsThreads = 256;
+constexpr int kFewSplits = 8;
+constexpr int kRowsTile = 128;          // rows of a block of the kernel for many
+constexpr int kRowsPBits = 10;          // its p in units of 2^-10: at most 2^15 with the lead
 constexpr int kPBits = 25;              // p in units of 2^-25: at most 2^30 with the lead
+constexpr int kWidePages = 16, kStepBlocks = 256, kRowsBlocks = 512;  // see kv8_attention_plan
+constexpr int kMostSplits = 64;  // at most one a thread of the combine
+using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
+using f32x4 = float __attribute__((ext_vector_type(4)));
 constexpr int kMostPages = 1024;        // int32 sums: 64 keys x 128 x 127 < 2^20 a page
 
 // D columns of an operand, 64 to a product; of 32 left over, each part's 8
@@ -92,20 +105,29 @@ __device__ __forceinline__ int gather_digits(const int u[4], uint32_t sel, uint3
   return static_cast<int>(__builtin_amdgcn_perm(hi, lo, 0x05040100u) ^ flip);
 }
 __device__ __forceinline__ uint32_t digit_select(int k) { return k | (4 + k) << 8; }
-__device__ __forceinline__ uint32_t digit_flip(int k, int top) { return k < top ? 0x80808080u : 0u; }
+__device__ __forceinline__ uint32_t digit_flip(int k) { return k < 3 ? 0x80808080u : 0u; }
 
-template <int D, int kRows, bool kKeySplit>
-__global__ __launch_bounds__(kAttnThreads) void kv8_attention_kernel(Kv8AttnArgs a, int chunk, int splits) {
-  constexpr int kTiles = D / 16;                  // of the output's dimensions
-  constexpr int kQ = kRows == 4 ? 1 : 3;          // digit operands of q
-  constexpr int kP = kRows == 4 ? 1 : 4;          // and of p
-  constexpr int kQTop = kRows == 4 ? 3 : 2;       // the signed digit
-  constexpr int kQBits = kRows == 4 ? 29 : 22;
+// Reference and sum of a row's split, after all the splits' outputs.
+__device__ __forceinline__ void store_ml(const Kv8AttnArgs& a, int64_t row, int splits, int split, int d, float ref,
+                                         float l) {
+  float* ml = a.part + static_cast<int64_t>(a.rows) * a.hq * splits * d + (row * splits + split) * 2;
+  ml[0] = ref;
+  ml[1] = l;
+}
+
+// Waves take the pages of a split in turn and join their results at the end.
+template <int D, int kWaves>
+__global__ __launch_bounds__(kWaves* kWave, 2) void kv8_step_kernel(Kv8AttnArgs a, int chunk, int splits) {
+  constexpr int kRows = 4, kTiles = D / 16;  // tiles of the output's dimensions
   const int s = blockIdx.y, hkv = a.cache.hkv, group = a.hq / hkv;
-  const int split = blockIdx.x % splits, unit_of_grid = blockIdx.x / splits;  // (tile, head), a tile's heads together
-  const int h = unit_of_grid % hkv;
+  const int split = blockIdx.x % splits, h = blockIdx.x / splits;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int g = lane / 16, col = lane % 16;
+  // Page numbers of this wave's first 64 steps, one a lane: read along with the
+  // offsets, not after them.
+  const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
+  const int from = split * chunk + wave;
+  int numbers = table[min(from + kWaves * lane, a.cache.per_seq - 1)];
   Kv8Span span;
   const bool fine = kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span);
   if (!fine || (span.n > 0 && static_cast<int64_t>(span.context) + span.n > a.max_tokens)) {
@@ -113,38 +135,74 @@ __global__ __launch_bounds__(kAttnThreads) void kv8_attention_kernel(Kv8AttnArgs
     return;
   }
   const int total = span.n * group;  // rows of this group of heads
-  const int tile = kKeySplit ? unit_of_grid / hkv : unit_of_grid / hkv * kAttnWaves + wave;
-  const int first = tile * kRows;
-  if (first >= total) return;  // a wave of the form without a key split has no barrier ahead
-  const int last_token = (min(first + kRows, total) - 1) / group;
-  const int pages = (span.context + last_token) / kKv8Page + 1;
+  if (total == 0) return;
+  const int pages = (span.context + span.n - 1) / kKv8Page + 1;
   const int begin = split * chunk, end = min(begin + chunk, pages);
   if (begin >= end) return;
-  const int used = (pages + chunk - 1) / chunk;  // splits of this tile
+  const int used = (pages + chunk - 1) / chunk;
 
-  // This lane's column.
-  const int m = first + (kRows == 4 ? col / 4 : col);
-  const int digit = kRows == 4 ? col % 4 : 0;
+  // This lane's column: digit `digit` of row m.
+  const int m = col / 4, digit = col % 4;
   const bool is_row = m < total;
   const int token = is_row ? m / group : 0, head = h * group + (is_row ? m % group : 0);
   const int limit = is_row ? span.context + token : -1;  // its last key
   const int64_t row = (static_cast<int64_t>(span.first) + token) * a.hq + head;
-  const int all_see = span.context + first / group;  // every row sees keys up to here
 
-  Operand<D> q[kQ];
-  float unit;       // of a score's integer, in log2
-  bool bad = false; // a query that is not finite gives a row of NaN
+  // The operands of the next page, asked for as soon as those of the page at
+  // hand are used.  A page number that is out of range reads page 0, hidden.
+  Operand<D> kf[4];
+  i32x4 vf[kTiles];
+  uint32_t next_key_exps, next_value_exps;
+  bool next_hidden;
+  const int8_t *next_k, *next_v;
+  int ask_at = 0;
+  auto ask = [&]() {  // addresses and exponents of step ask_at, at most the last
+    const int step = min(ask_at, (end - 1 - from) / kWaves);
+    if (ask_at > 0 && step % kWave == 0) numbers = table[min(from + kWaves * (step + lane), a.cache.per_seq - 1)];
+    ++ask_at;
+    const int number = __builtin_amdgcn_readlane(numbers, step % kWave);
+    next_hidden = number < 0 || number >= a.cache.pages;
+    const int page = next_hidden ? 0 : number;
+    const int64_t at = kv8_offset(page, h, hkv, D), exp_at = kv8_exp_offset(page, h, hkv);
+    next_k = a.cache.keys + at;
+    next_v = a.cache.values + at;
+    next_key_exps = *reinterpret_cast<const uint32_t*>(a.cache.key_exps + exp_at);
+    next_value_exps = *reinterpret_cast<const uint32_t*>(a.cache.value_exps + exp_at);
+  };
+  // Row 4 g + i of the t-th product is key 16 g + 4 t + i: a lane's scores are
+  // those of part g's 16 keys of P.
+  auto ask_keys = [&]() {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) load_operand(kf[t], next_k + (16 * (col / 4) + 4 * t + col % 4) * D, g);
+  };
+  auto ask_values = [&]() {
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+      vf[t] = *reinterpret_cast<const i32x4*>(next_v + (16 * t + col) * kKv8Page + 16 * g);
+  };
+  if (from < end) {
+    ask();
+    ask_keys();
+    ask_values();
+  }
+
+  Operand<D> q;
+  float unit;        // of a score's integer, in log2
+  bool bad = false;  // a query that is not finite gives a row of NaN
   {
+    constexpr int kQBits = 29;
     const float* p = a.query + row * D;
     constexpr int kFull = Operand<D>::kFull, kHalf = Operand<D>::kHalf;
     float v[16 * kFull + 8 * kHalf];
 #pragma unroll
     for (int c = 0; c < kFull; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(v + 16 * c + 4 * i) = *reinterpret_cast<const float4*>(p + 64 * c + 16 * g + 4 * i);
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4*>(v + 16 * c + 4 * i) = *reinterpret_cast<const float4*>(p + 64 * c + 16 * g + 4 * i);
 #pragma unroll
     for (int i = 0; i < 2 * kHalf; ++i)
-      *reinterpret_cast<float4*>(v + 16 * kFull + 4 * i) = *reinterpret_cast<const float4*>(p + 64 * kFull + 8 * g + 4 * i);
+      *reinterpret_cast<float4*>(v + 16 * kFull + 4 * i) =
+          *reinterpret_cast<const float4*>(p + 64 * kFull + 8 * g + 4 * i);
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16 * kFull + 8 * kHalf; ++i) {
@@ -156,25 +214,23 @@ __global__ __launch_bounds__(kAttnThreads) void kv8_attention_kernel(Kv8AttnArgs
     int x = 0;
     if (top > 0.0f && !bad) (void)frexpf(top, &x);
     constexpr int kWords = 4 * kFull + 2 * kHalf;
-    int n[4 * kWords];
+    int w[kWords];
 #pragma unroll
-    for (int i = 0; i < 4 * kWords; ++i)
-      n[i] = (bad ? 0 : static_cast<int>(rintf(ldexpf(v[i], kQBits - x)))) + (kRows == 4 ? 0x808080 : 0x8080);
+    for (int i = 0; i < kWords; ++i) {
+      int n[4];
 #pragma unroll
-    for (int k = 0; k < kQ; ++k) {
-      const int which = kRows == 4 ? digit : k;
-      int w[kWords];
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) w[i] = gather_digits(n + 4 * i, digit_select(which), digit_flip(which, kQTop));
-#pragma unroll
-      for (int c = 0; c < kFull; ++c) q[k].word[c] = i32x4{w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]};
-      if constexpr (kHalf) q[k].word[kFull] = i32x4{w[4 * kFull], w[4 * kFull + 1], 0, 0};
+      for (int j = 0; j < 4; ++j)
+        n[j] = (bad ? 0 : static_cast<int>(rintf(ldexpf(v[4 * i + j], kQBits - x)))) + 0x808080;
+      w[i] = gather_digits(n, digit_select(digit), digit_flip(digit));
     }
+#pragma unroll
+    for (int c = 0; c < kFull; ++c) q.word[c] = i32x4{w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]};
+    if constexpr (kHalf) q.word[kFull] = i32x4{w[4 * kFull], w[4 * kFull + 1], 0, 0};
     unit = ldexpf(1.4426950408889634f / sqrtf(static_cast<float>(D)), x - kQBits);
   }
-  const float weight = kRows == 4 ? ldexpf(1.0f, 8 * digit) : 1.0f;
+  const float weight = ldexpf(1.0f, 8 * digit);
 
-  i32x4 sum[kP][kTiles] = {};    // digits of the output since the last move
+  i32x4 sum[kTiles] = {};        // digits of the output since the last move
   float out[kTiles][4] = {};     // and before it
   float ref = kNoRow, l = 0.0f;  // l: of this lane's keys
   int held_exp = kKv8MinExp - 1; // of V in sum
@@ -186,44 +242,18 @@ __global__ __launch_bounds__(kAttnThreads) void kv8_attention_kernel(Kv8AttnArgs
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float f;
-        if constexpr (kRows == 4) {
-          f = static_cast<float>(sum[0][t][i]);
-          sum[0][t][i] = 0;
-        } else {
-          f = static_cast<float>(sum[3][t][i]);
-          f = f * 256.0f + static_cast<float>(sum[2][t][i]);
-          f = f * 256.0f + static_cast<float>(sum[1][t][i]);
-          f = f * 256.0f + static_cast<float>(sum[0][t][i]);
-          sum[0][t][i] = sum[1][t][i] = sum[2][t][i] = sum[3][t][i] = 0;
-        }
-        out[t][i] = (out[t][i] + f * w) * factor;
+        out[t][i] = (out[t][i] + static_cast<float>(sum[t][i]) * w) * factor;
+        sum[t][i] = 0;
       }
     l *= factor;
     since = 0;
   };
 
-  const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
-  for (int p = begin + (kKeySplit ? wave : 0); p < end; p += kKeySplit ? kAttnWaves : 1) {
-    const int page = table[p];
-    if (page < 0 || page >= a.cache.pages) {  // its keys count as hidden
-      if (lane == 0) atomicOr(a.error, kKv8BadRows);
-      continue;
-    }
-    const int64_t at = kv8_offset(page, h, hkv, D), exp_at = kv8_exp_offset(page, h, hkv);
-    const int8_t* k = a.cache.keys + at;
-    const int8_t* v = a.cache.values + at;
-    const uint32_t key_exps = *reinterpret_cast<const uint32_t*>(a.cache.key_exps + exp_at);
-    const uint32_t value_exps = *reinterpret_cast<const uint32_t*>(a.cache.value_exps + exp_at);
-    Operand<D> kf[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) load_operand(kf[t], k + (16 * (col / 4) + 4 * t + col % 4) * D, g);
-    i32x4 vf[kTiles];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) vf[t] = *reinterpret_cast<const i32x4*>(v + (16 * t + col) * kKv8Page + 16 * g);
-
-    // Blocks past the tile's last key hold anything: their exponents don't count.
-    const int blocks = min(kKv8Blocks, (span.context + last_token - p * kKv8Page) / kKv8Block + 1);
+  for (int p = from; p < end; p += kWaves) {
+    const uint32_t key_exps = next_key_exps, value_exps = next_value_exps;
+    const bool hidden = next_hidden;
+    // Blocks past the last key hold anything: their exponents don't count.
+    const int blocks = hidden ? 0 : min(kKv8Blocks, (span.context + span.n - 1 - p * kKv8Page) / kKv8Block + 1);
     int page_exp = kKv8MinExp - 1;
 #pragma unroll
     for (int b = 0; b < kKv8Blocks; ++b)
@@ -232,30 +262,28 @@ __global__ __launch_bounds__(kAttnThreads) void kv8_attention_kernel(Kv8AttnArgs
 
     float score[4][4];
     const float to_log2 = unit * ldexpf(1.0f, static_cast<int8_t>(key_exps >> (8 * g)));
-    float top = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      i32x4 acc[kQ];
+      const i32x4 acc = multiply<D>(kf[t], q);
 #pragma unroll
-      for (int n = 0; n < kQ; ++n) acc[n] = multiply<D>(kf[t], q[n]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float f;
-        if constexpr (kRows == 4) {
-          f = quad_add(static_cast<float>(acc[0][i]) * weight);
-        } else {
-          f = fmaf(static_cast<float>(acc[2][i] * 256 + acc[1][i]), 256.0f, static_cast<float>(acc[0][i]));
-        }
-        score[t][i] = f * to_log2;
-      }
+      for (int i = 0; i < 4; ++i) score[t][i] = quad_add(static_cast<float>(acc[i]) * weight) * to_log2;
     }
-    if (p * kKv8Page + kKv8Page - 1 > all_see) {
+    ask();
+    ask_keys();
+    if (hidden) {
+      if (lane == 0) atomicOr(a.error, kKv8BadRows);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) score[t][i] = -INFINITY;
+    } else if (p * kKv8Page + kKv8Page - 1 > span.context) {  // the first token sees keys up to context
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (p * kKv8Page + 16 * g + 4 * t + i > limit) score[t][i] = -INFINITY;
     }
+    float top = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -270,7 +298,7 @@ __global__ __launch_bounds__(kAttnThreads) void kv8_attention_kernel(Kv8AttnArgs
     ++since;
     // Keys of hidden blocks have p = 0: any finite factor will do.
     const float to_int = ldexpf(1.0f, min(my_exp - held_exp, 0) + kPBits);
-    int digits[kP][4];
+    i32x4 pf;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       int u[4];
@@ -280,130 +308,474 @@ __global__ __launch_bounds__(kAttnThreads) void kv8_attention_kernel(Kv8AttnArgs
         l += e;
         u[i] = static_cast<int>(fmaf(e, to_int, 0.5f)) + 0x808080;
       }
-#pragma unroll
-      for (int n = 0; n < kP; ++n) {
-        const int which = kRows == 4 ? digit : n;
-        digits[n][t] = gather_digits(u, digit_select(which), digit_flip(which, 3));
-      }
+      pf[t] = gather_digits(u, digit_select(digit), digit_flip(digit));
     }
 #pragma unroll
-    for (int n = 0; n < kP; ++n) {
-      const i32x4 pf = {digits[n][0], digits[n][1], digits[n][2], digits[n][3]};
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-        sum[n][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[t], pf, sum[n][t], 0, 0, 0);
-    }
+    for (int t = 0; t < kTiles; ++t)
+      sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[t], pf, sum[t], 0, 0, 0);
+    ask_values();
   }
   move(1.0f);
   l = column_sum(l);
   if (bad) l = __builtin_nanf("");
-  if constexpr (kRows == 4) {
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
+  for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) out[t][i] = quad_add(out[t][i]);
-  }
+    for (int i = 0; i < 4; ++i) out[t][i] = quad_add(out[t][i]);
 
-  float* const part_ml = a.part + static_cast<int64_t>(a.rows) * a.hq * splits * D;
-  if constexpr (!kKeySplit) {
-    if (!is_row) return;
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  __shared__ float sh_ref[kWaves][kRows], sh_l[kWaves][kRows];
+  __shared__ __align__(16) float sh_out[kWaves][kRows][D];
+  if (digit == 0) {
+    if (g == 0) {
+      sh_ref[wave][m] = ref;
+      sh_l[wave][m] = l;
+    }
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
-      *reinterpret_cast<float4*>(a.out + row * D + 16 * t + 4 * g) =
-          make_float4(out[t][0] * inv, out[t][1] * inv, out[t][2] * inv, out[t][3] * inv);
-  } else {
-    __shared__ float sh_ref[kAttnWaves][kRows], sh_l[kAttnWaves][kRows];
-    __shared__ __align__(16) float sh_out[kAttnWaves][kRows][D];
-    const int r = kRows == 4 ? col / 4 : col;
-    if (digit == 0) {
-      if (g == 0) {
-        sh_ref[wave][r] = ref;
-        sh_l[wave][r] = l;
-      }
+      *reinterpret_cast<float4*>(&sh_out[wave][m][16 * t + 4 * g]) =
+          make_float4(out[t][0], out[t][1], out[t][2], out[t][3]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < total * D; i += kWaves * kWave) {
+    const int mr = i / D, dim = i - mr * D;
+    float top = sh_ref[0][mr];
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-        *reinterpret_cast<float4*>(&sh_out[wave][r][16 * t + 4 * g]) =
-            make_float4(out[t][0], out[t][1], out[t][2], out[t][3]);
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sh_ref[w][mr]);
+    float o = 0.0f, ll = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sh_ref[w][mr] - top);
+      o += f * sh_out[w][mr][dim];
+      ll += f * sh_l[w][mr];
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kRows * D; i += kAttnThreads) {
-      const int mr = i / D, dim = i - mr * D, mm = first + mr;
-      if (mm >= total) break;
-      float top = sh_ref[0][mr];
-#pragma unroll
-      for (int w = 1; w < kAttnWaves; ++w) top = fmaxf(top, sh_ref[w][mr]);
-      float o = 0.0f, ll = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kAttnWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(sh_ref[w][mr] - top);
-        o += f * sh_out[w][mr][dim];
-        ll += f * sh_l[w][mr];
-      }
-      const int64_t to = (static_cast<int64_t>(span.first) + mm / group) * a.hq + h * group + mm % group;
-      if (used == 1) {
-        a.out[to * D + dim] = ll != 0.0f ? o / ll : 0.0f;
-      } else {
-        a.part[(to * splits + split) * D + dim] = o;
-        if (dim == 0) {
-          part_ml[(to * splits + split) * 2] = top;
-          part_ml[(to * splits + split) * 2 + 1] = ll;
-        }
-      }
+    const int64_t to = (static_cast<int64_t>(span.first) + mr / group) * a.hq + h * group + mr % group;
+    if (used == 1) {
+      a.out[to * D + dim] = ll != 0.0f ? o / ll : 0.0f;
+    } else {
+      a.part[(to * splits + split) * D + dim] = o;
+      if (dim == 0) store_ml(a, to, splits, split, D, top, ll);
     }
   }
 }
 
-// Joins the splits of the rows that had more than one: a wave per (token, head).
-__global__ __launch_bounds__(kAttnThreads) void kv8_combine_kernel(Kv8AttnArgs a, int chunk, int splits,
-                                                                   int tile_rows) {
-  const int s = blockIdx.y, lane = threadIdx.x % kWave, d = a.cache.d;
+// 16 codes as fp16: a byte with its top bit flipped is code + 128, and below
+// the exponent byte 0x64 it is the fp16 number 1024 + 128 + code.
+__device__ __forceinline__ void widen(const uint4& codes, uint4* lo, uint4* hi) {
+  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t t = w[i] ^ 0x80808080u;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f16x2 v = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, t, j ? 0x04030402u : 0x04010400u));
+      h[2 * i + j] = __builtin_bit_cast(uint32_t, v - f16x2{1152.0f, 1152.0f});
+    }
+  }
+  *lo = make_uint4(h[0], h[1], h[2], h[3]);
+  *hi = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+// x * f = hi + lo in fp16, two at a time (split2 with the product inside).
+__device__ __forceinline__ void split2_scaled(float x0, float x1, float f, uint32_t& hi, uint32_t& lo) {
+  asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(hi) : "v"(x0), "v"(f));
+  asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(hi) : "v"(x1), "v"(f));
+  asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(lo) : "v"(x0), "v"(f), "v"(hi));
+  asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(lo) : "v"(x1), "v"(f), "v"(hi));
+}
+
+// 32 rows a wave, all waves over the same pages, which the block widens into
+// LDS: the operands of every product, 16 bytes a lane in the order of lanes.
+template <int D>
+__global__ __launch_bounds__(kRowsThreads, 2) void kv8_rows_kernel(Kv8AttnArgs a, int chunk, int splits) {
+  constexpr int kTiles = D / 16, kRuns = D / 32;  // tiles of the output, products along D
+  constexpr int kPieces = D / 32;                 // 16-byte pieces of a page that a thread widens
+  constexpr int kOperand = kWave;                 // of uint4
+  constexpr int kSets = 2;                        // of 16 rows of a wave
+  __shared__ uint4 stage[2][(4 * kRuns + 2 * kTiles) * kOperand];  // K [4 t][runs], then V [2 u][tiles]
+  const int s = blockIdx.y, hkv = a.cache.hkv, group = a.hq / hkv;
+  const int split = blockIdx.x % splits, unit_of_grid = blockIdx.x / splits;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  const int g = lane / 16, col = lane % 16;
   Kv8Span span;
-  if (!kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span)) return;
-  if (static_cast<int64_t>(span.context) + span.n > a.max_tokens) return;
-  const int i = blockIdx.x * kAttnWaves + threadIdx.x / kWave;
-  if (i >= span.n * a.hq) return;
+  const bool fine = kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span);
+  if (!fine || (span.n > 0 && static_cast<int64_t>(span.context) + span.n > a.max_tokens)) {
+    if (blockIdx.x == 0 && tid == 0) atomicOr(a.error, kKv8BadRows);
+    return;
+  }
+  const int total = span.n * group, h = unit_of_grid % hkv;
+  const int tiles = (total + kRowsTile - 1) / kRowsTile, tile = tiles - 1 - unit_of_grid / hkv;  // the longest first
+  if (tile < 0) return;
+  const int first = tile * kRowsTile;
+  const int last_token = (min(first + kRowsTile, total) - 1) / group;
+  const int pages = (span.context + last_token) / kKv8Page + 1;
+  const int begin = split * chunk, end = min(begin + chunk, pages);
+  if (begin >= end) return;
+  const int used = (pages + chunk - 1) / chunk;
+
+  // This lane's rows, one a set.
+  const int wave_first = first + 16 * kSets * wave;
+  const bool works = wave_first < total;
+  const int all_see = span.context + min(wave_first, total - 1) / group;
+  const int wave_last = span.context + (min(wave_first + 16 * kSets, total) - 1) / group;  // last key of any row
+  int limit[kSets];
+  int64_t row[kSets];
+#pragma unroll
+  for (int n = 0; n < kSets; ++n) {
+    const int m = wave_first + 16 * n + col, token = m < total ? m / group : 0;
+    limit[n] = m < total ? span.context + token : -1;
+    row[n] = (static_cast<int64_t>(span.first) + token) * a.hq + h * group + (m < total ? m % group : 0);
+  }
+
+  const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
+  int numbers = table[min(begin + lane, a.cache.per_seq - 1)];
+  uint4 piece[kPieces];
+  uint32_t next_key_exps, next_value_exps;
+  bool next_hidden;
+  auto ask = [&](int p) {
+    const int step = p - begin;
+    if (step > 0 && step % kWave == 0) numbers = table[min(p + lane, a.cache.per_seq - 1)];
+    const int number = __builtin_amdgcn_readlane(numbers, step % kWave);
+    next_hidden = number < 0 || number >= a.cache.pages;
+    const int page = next_hidden ? 0 : number;
+    const int64_t at = kv8_offset(page, h, hkv, D), exp_at = kv8_exp_offset(page, h, hkv);
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      const int x = tid + kRowsThreads * j;  // keys are 4 D pieces, values as many: a wave is in one of them
+      piece[j] = *reinterpret_cast<const uint4*>(x < 4 * D ? a.cache.keys + at + 16 * x
+                                                           : a.cache.values + at + 16 * (x - 4 * D));
+    }
+    next_key_exps = *reinterpret_cast<const uint32_t*>(a.cache.key_exps + exp_at);
+    next_value_exps = *reinterpret_cast<const uint32_t*>(a.cache.value_exps + exp_at);
+  };
+  // Key 32 u + 8 g + 4 w + i is row 4 g + i of product t = 2 u + w, so a lane's
+  // scores of products 2 u and 2 u + 1 are of the 8 keys that are its run of
+  // the u-th product with V.  Places of an operand are exchanged within runs
+  // of 8 (128 bytes, all banks): the 16 lanes that write together hold a few
+  // keys' runs of dimensions, or a few dimensions' runs of keys.
+  auto key_place = [](int operand, int part) { return (2 * operand + part / 2) & 7; };
+  auto value_place = [](int u, int part) { return ((part / 2 ^ u) & 1) * 4; };
+  auto put = [&](uint4* to) {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      const int x = tid + kRowsThreads * j;
+      uint4 lo, hi;
+      widen(piece[j], &lo, &hi);
+      uint4* at;
+      int place;
+      if (x < 4 * D) {  // 16 dimensions of a key
+        const int key = x / (D / 16), dims = x % (D / 16);
+        const int t = key / 32 * 2 + key % 8 / 4, r = key % 32 / 8 * 4 + key % 4;
+        at = to + (t * kRuns + dims / 2) * kOperand + dims % 2 * 32;
+        place = r ^ key_place(t * kRuns + dims / 2, dims % 2 * 2);
+      } else {  // 16 keys of a dimension
+        const int dim = (x - 4 * D) / 4, b = x % 4;
+        at = to + (4 * kRuns + b / 2 * kTiles + dim / 16) * kOperand + b % 2 * 32;
+        place = dim % 16 ^ value_place(b / 2, b % 2 * 2);
+      }
+      at[place] = lo;
+      at[16 + place] = hi;
+    }
+  };
+  ask(begin);
+
+  f16x8 q_hi[kSets][kRuns], q_lo[kSets][kRuns];
+  float unit[kSets];
+  bool bad[kSets];
+#pragma unroll
+  for (int n = 0; n < kSets; ++n) {
+    float v[8 * kRuns];
+#pragma unroll
+    for (int c = 0; c < kRuns; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<float4*>(v + 8 * c + 4 * i) =
+            *reinterpret_cast<const float4*>(a.query + row[n] * D + 32 * c + 8 * g + 4 * i);
+    float top = 0.0f;
+    bool broken = false;
+#pragma unroll
+    for (int i = 0; i < 8 * kRuns; ++i) {
+      broken = broken || !(fabsf(v[i]) < __builtin_inff());
+      top = fmaxf(top, fabsf(v[i]));
+    }
+    top = column_max(top);
+    bad[n] = column_max(broken ? 1.0f : 0.0f) > 0.0f;
+    int x = 0;
+    if (top > 0.0f && !bad[n]) (void)frexpf(top, &x);
+    // The largest below 2^15: what is rounded off is under 2^-39 of it.
+#pragma unroll
+    for (int c = 0; c < kRuns; ++c) {
+      uint4 hi, lo;
+      uint32_t *ph = &hi.x, *pl = &lo.x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        split2(bad[n] ? 0.0f : ldexpf(v[8 * c + 2 * i], 15 - x), bad[n] ? 0.0f : ldexpf(v[8 * c + 2 * i + 1], 15 - x),
+               ph[i], pl[i]);
+      q_hi[n][c] = __builtin_bit_cast(f16x8, hi);
+      q_lo[n][c] = __builtin_bit_cast(f16x8, lo);
+    }
+    unit[n] = ldexpf(1.4426950408889634f / sqrtf(static_cast<float>(D)), x - 15);
+  }
+
+  f32x4 out[kSets][kTiles] = {};
+  float ref[kSets], l[kSets];
+#pragma unroll
+  for (int n = 0; n < kSets; ++n) ref[n] = kNoRow, l[n] = 0.0f;
+  int held_exp = kKv8MinExp - 1;
+  put(stage[0]);
+  for (int p = begin; p < end; ++p) {
+    const uint4* now = stage[(p - begin) % 2];
+    const uint32_t key_exps = next_key_exps, value_exps = next_value_exps;
+    const bool hidden = next_hidden;
+    __syncthreads();  // this page is in LDS, and every wave is done with the one before
+    if (p + 1 < end) ask(p + 1);
+    if (works && p * kKv8Page <= wave_last && !hidden) {
+      const int blocks = min(kKv8Blocks, (wave_last - p * kKv8Page) / kKv8Block + 1);
+      int page_exp = kKv8MinExp - 1;
+#pragma unroll
+      for (int b = 0; b < kKv8Blocks; ++b)
+        if (b < blocks) page_exp = max(page_exp, static_cast<int>(static_cast<int8_t>(value_exps >> (8 * b))));
+      f32x4 score[kSets][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        f16x8 kf[kRuns];
+#pragma unroll
+        for (int c = 0; c < kRuns; ++c)
+          kf[c] = __builtin_bit_cast(f16x8, now[(t * kRuns + c) * kOperand + (lane ^ key_place(t * kRuns + c, g))]);
+#pragma unroll
+        for (int n = 0; n < kSets; ++n) {
+          f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int c = 0; c < kRuns; ++c)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[c], q_lo[n][c], acc, 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < kRuns; ++c)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[c], q_hi[n][c], acc, 0, 0, 0);
+          score[n][t] = acc;
+        }
+      }
+      const int shift = 8 * (g / 2);  // of this lane's block of each half page
+      const float key_scale[2] = {ldexpf(1.0f, static_cast<int8_t>(key_exps >> shift)),
+                                  ldexpf(1.0f, static_cast<int8_t>(key_exps >> (16 + shift)))};
+      const bool edge = p * kKv8Page + kKv8Page - 1 > all_see;
+      float to_log2[kSets][2], page_top[kSets];
+      bool rises = page_exp > held_exp;
+#pragma unroll
+      for (int n = 0; n < kSets; ++n) {
+        to_log2[n][0] = unit[n] * key_scale[0];
+        to_log2[n][1] = unit[n] * key_scale[1];
+        if (edge) {
+          // Scaled first: a factor may be 0 or, of a block that holds anything, infinite.
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              score[n][t][i] = p * kKv8Page + 32 * (t / 2) + 8 * g + 4 * (t % 2) + i > limit[n]
+                                   ? -INFINITY
+                                   : score[n][t][i] * to_log2[n][t / 2];
+          to_log2[n][0] = to_log2[n][1] = 1.0f;
+        }
+        float top[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          top[u] = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[u] = fmaxf(top[u], score[n][2 * u + w][i]);
+        }
+        page_top[n] = fmaxf(top[0] * to_log2[n][0], top[1] * to_log2[n][1]);
+        rises = rises || page_top[n] > ref[n] + kLead;
+      }
+      if (__any(rises)) {
+        const int next_exp = max(held_exp, page_exp);
+#pragma unroll
+        for (int n = 0; n < kSets; ++n) {
+          const float next = fmaxf(ref[n], column_max(page_top[n]));
+          const float f = __builtin_amdgcn_exp2f(ref[n] - next);
+          l[n] *= f;
+          const float fo = ldexpf(f, held_exp - next_exp);
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) out[n][t] *= fo;
+          ref[n] = next;
+        }
+        held_exp = next_exp;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int my_exp = static_cast<int8_t>(value_exps >> (16 * u + shift));
+        const float f = ldexpf(1.0f, min(my_exp - held_exp, 0) + kRowsPBits);
+        f16x8 p_hi[kSets], p_lo[kSets];
+#pragma unroll
+        for (int n = 0; n < kSets; ++n) {
+          uint4 hi, lo;
+          uint32_t *ph = &hi.x, *pl = &lo.x;
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const float e0 = __builtin_amdgcn_exp2f(fmaf(score[n][2 * u + w][i], to_log2[n][u], -ref[n]));
+              const float e1 = __builtin_amdgcn_exp2f(fmaf(score[n][2 * u + w][i + 1], to_log2[n][u], -ref[n]));
+              l[n] += e0;
+              l[n] += e1;
+              split2_scaled(e0, e1, f, ph[2 * w + i / 2], pl[2 * w + i / 2]);
+            }
+          p_hi[n] = __builtin_bit_cast(f16x8, hi);
+          p_lo[n] = __builtin_bit_cast(f16x8, lo);
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          const f16x8 vf = __builtin_bit_cast(
+              f16x8, now[(4 * kRuns + u * kTiles + t) * kOperand + (lane ^ value_place(u, g))]);
+#pragma unroll
+          for (int n = 0; n < kSets; ++n) {
+            out[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p_lo[n], out[n][t], 0, 0, 0);
+            out[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p_hi[n], out[n][t], 0, 0, 0);
+          }
+        }
+      }
+    } else if (hidden && tid == 0) {
+      atomicOr(a.error, kKv8BadRows);
+    }
+    if (p + 1 < end) put(stage[(p + 1 - begin) % 2]);
+  }
+#pragma unroll
+  for (int n = 0; n < kSets; ++n) {
+    float total_l = column_sum(l[n]);
+    if (bad[n]) total_l = __builtin_nanf("");
+    if (limit[n] < 0) continue;
+    const float inv = used > 1 ? 1.0f : total_l != 0.0f ? 1.0f / total_l : 0.0f;
+    float* to = used > 1 ? a.part + (row[n] * splits + split) * D : a.out + row[n] * D;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      float4 o;
+      float* po = &o.x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) po[i] = ldexpf(out[n][t][i], held_exp - kRowsPBits) * inv;
+      *reinterpret_cast<float4*>(to + 16 * t + 4 * g) = o;
+    }
+    if (used > 1 && g == 0) store_ml(a, row[n], splits, split, D, ref[n], total_l);
+  }
+}
+
+// Splits of row `i` of a sequence's (token, head) rows.
+__device__ __forceinline__ int splits_of(const Kv8AttnArgs& a, const Kv8Span& span, int i, int chunk, int tile_rows) {
   const int token = i / a.hq, head = i - token * a.hq, group = a.hq / a.cache.hkv;
   const int m = token * group + head % group;
   const int tile_end = min((m / tile_rows + 1) * tile_rows, span.n * group);
   const int pages = (span.context + (tile_end - 1) / group) / kKv8Page + 1;
-  const int used = (pages + chunk - 1) / chunk;
+  return (pages + chunk - 1) / chunk;
+}
+
+// Joins a few splits of many rows: d / 4 threads a (token, head).
+__global__ __launch_bounds__(kAttnThreads) void kv8_combine_few_kernel(Kv8AttnArgs a, int chunk, int splits,
+                                                                       int tile_rows) {
+  const int s = blockIdx.y, d = a.cache.d, quads = d / 4, each = kAttnThreads / quads;
+  Kv8Span span;
+  if (!kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span)) return;
+  if (static_cast<int64_t>(span.context) + span.n > a.max_tokens) return;
+  const int part = threadIdx.x / quads, quad = threadIdx.x - part * quads, i = blockIdx.x * each + part;
+  if (part >= each || i >= span.n * a.hq) return;
+  const int used = splits_of(a, span, i, chunk, tile_rows);
+  if (used == 1) return;
+  const int64_t to = static_cast<int64_t>(span.first) * a.hq + i;
+  const float2* ml = reinterpret_cast<const float2*>(a.part + static_cast<int64_t>(a.rows) * a.hq * splits * d) + to * splits;
+  const float4* o = reinterpret_cast<const float4*>(a.part + to * splits * d) + quad;
+  float4 v[kFewSplits];
+  float2 of[kFewSplits];
+#pragma unroll
+  for (int y = 0; y < kFewSplits; ++y) {
+    v[y] = y < used ? o[y * quads] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    of[y] = y < used ? ml[y] : make_float2(kNoRow, 0.0f);
+  }
+  float top = of[0].x, l = 0.0f;
+#pragma unroll
+  for (int y = 1; y < kFewSplits; ++y) top = fmaxf(top, of[y].x);
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int y = 0; y < kFewSplits; ++y) {
+    const float w = __builtin_amdgcn_exp2f(of[y].x - top);
+    l += w * of[y].y;
+    sum.x += w * v[y].x, sum.y += w * v[y].y, sum.z += w * v[y].z, sum.w += w * v[y].w;
+  }
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  reinterpret_cast<float4*>(a.out + to * d)[quad] = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+}
+
+// Joins many splits, a block per (token, head): weights first, a split a thread, then groups of d / 4 threads take
+// splits in turn, four dimensions each.
+__global__ __launch_bounds__(kAttnThreads) void kv8_combine_kernel(Kv8AttnArgs a, int chunk, int splits,
+                                                                   int tile_rows) {
+  __shared__ float weight[kMostSplits], shared_top[kAttnWaves], shared_l[kAttnWaves];
+  __shared__ float4 shared_out[kAttnThreads];
+  const int s = blockIdx.y, d = a.cache.d, quads = d / 4, groups = kAttnThreads / quads;
+  Kv8Span span;
+  if (!kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span)) return;
+  if (static_cast<int64_t>(span.context) + span.n > a.max_tokens) return;
+  const int i = blockIdx.x;
+  if (i >= span.n * a.hq) return;
+  const int used = splits_of(a, span, i, chunk, tile_rows);
   if (used == 1) return;
   const int64_t to = static_cast<int64_t>(span.first) * a.hq + i;
   const float* ml = a.part + static_cast<int64_t>(a.rows) * a.hq * splits * d + to * splits * 2;
-  const float* o = a.part + to * splits * d;
-  float top = kNoRow;
-  for (int x = 0; x < used; ++x) top = fmaxf(top, ml[2 * x]);
-  float l = 0.0f, acc[2] = {0.0f, 0.0f};
-  for (int x = 0; x < used; ++x) {
-    const float f = __builtin_amdgcn_exp2f(ml[2 * x] - top);
-    l += f * ml[2 * x + 1];
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-      if (lane + 64 * c < d) acc[c] += f * o[static_cast<int64_t>(x) * d + lane + 64 * c];
+  const float4* o = reinterpret_cast<const float4*>(a.part + to * splits * d);
+  const int x = threadIdx.x, wave = x / kWave;
+  const float ref = x < used ? ml[2 * x] : kNoRow, part_l = x < used ? ml[2 * x + 1] : 0.0f;
+  float top = group_max<kWave>(ref);
+  if (x % kWave == 0) shared_top[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(shared_top[0], shared_top[1]), fmaxf(shared_top[2], shared_top[3]));
+  const float f = __builtin_amdgcn_exp2f(ref - top);
+  weight[x] = f;
+  const float l = group_sum<kWave>(f * part_l);
+  if (x % kWave == 0) shared_l[wave] = l;
+  __syncthreads();
+  const int g = x / quads, quad = x - g * quads;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (g < groups) {
+    for (int y = g; y < used; y += groups) {
+      const float4 v = o[y * quads + quad];
+      const float w = weight[y];
+      sum.x += w * v.x, sum.y += w * v.y, sum.z += w * v.z, sum.w += w * v.w;
+    }
   }
-#pragma unroll
-  for (int c = 0; c < 2; ++c)
-    if (lane + 64 * c < d) a.out[to * d + lane + 64 * c] = l != 0.0f ? acc[c] / l : 0.0f;
+  shared_out[x] = sum;
+  __syncthreads();
+  if (x < quads) {
+    for (int y = 1; y < min(groups, used); ++y) {
+      const float4 v = shared_out[y * quads + x];
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    const float total = shared_l[0] + shared_l[1] + shared_l[2] + shared_l[3];
+    const float inv = total != 0.0f ? 1.0f / total : 0.0f;
+    reinterpret_cast<float4*>(a.out + to * d)[x] = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+  }
 }
 
 }  // namespace
 
+// Splits along the context, sized by the longest one a launch may meet (blocks
+// past a sequence's end leave at once).  Measured in replayed graphs, d 96, two
+// KV heads, us a call:
+//   steps of at most kWidePages pages take one block and no join: 8.7 at 1,000
+//   tokens (8.9 split over four), while at 2,000 the split wins (9.1, 11.4);
+//   more take kStepBlocks blocks in all (32 sequences of up to 4,000 tokens
+//   15.3; with 512 blocks 15.9, with 128 18.5) and at most kMostSplits splits
+//   (one sequence of 32,768: 64 splits 13.5, 128 14.5).
+// Prompts: blocks that all run at once, two a compute unit.
 Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens) {
   Kv8AttnPlan p;
-  const int group = hq / hkv;
-  const int64_t most = static_cast<int64_t>(group) * max_rows;
+  const int64_t most = static_cast<int64_t>(hq / hkv) * max_rows;
   const int64_t pages = (max_tokens + kKv8Page - 1) / kKv8Page;
-  p.tile_rows = most <= 4 ? 4 : 16;
-  const int64_t tiles = (most + p.tile_rows - 1) / p.tile_rows;
-  const int64_t blocks = tiles * hkv * seqs;
-  if (blocks >= 1024) {
-    p.chunk_pages = static_cast<int>(std::max<int64_t>(pages, 1));
-    p.splits = 1;
-    return p;
-  }
-  p.chunk_pages = static_cast<int>(std::max<int64_t>(kAttnWaves, pages * blocks / 768));
-  p.splits = static_cast<int>(std::max<int64_t>(1, (pages + p.chunk_pages - 1) / p.chunk_pages));
+  p.tile_rows = most <= 4 ? 4 : kRowsTile;
+  const int64_t blocks = (most + p.tile_rows - 1) / p.tile_rows * hkv * seqs;
+  const int64_t wanted = p.tile_rows == 4 ? kStepBlocks : kRowsBlocks;
+  int64_t chunk = pages;
+  if (blocks < wanted && !(p.tile_rows == 4 && pages <= kWidePages))
+    chunk = std::max<int64_t>(
+        {kAttnWaves, (pages * blocks + wanted - 1) / wanted, (pages + kMostSplits - 1) / kMostSplits});
+  p.chunk_pages = static_cast<int>(chunk);
+  p.splits = static_cast<int>((pages + chunk - 1) / chunk);
   if (p.splits > 1) p.partial_floats = static_cast<int64_t>(rows) * hq * p.splits * (d + 2);
   return p;
 }
@@ -413,19 +785,20 @@ namespace {
 template <int D>
 void launch_attention_for(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t stream) {
   const int hkv = a.cache.hkv, most = a.hq / hkv * a.max_rows;
-  const int tiles = (most + p.tile_rows - 1) / p.tile_rows;
-  const dim3 grid(p.splits * tiles * hkv, a.cache.seqs);
-  if (p.tile_rows == 4)
-    kv8_attention_kernel<D, 4, true><<<grid, kAttnThreads, 0, stream>>>(a, p.chunk_pages, p.splits);
-  else if (p.splits > 1 || tiles < kAttnWaves)
-    kv8_attention_kernel<D, 16, true><<<grid, kAttnThreads, 0, stream>>>(a, p.chunk_pages, p.splits);
+  const dim3 grid(p.splits * ((most + p.tile_rows - 1) / p.tile_rows) * hkv, a.cache.seqs);
+  if (p.tile_rows != 4)
+    kv8_rows_kernel<D><<<grid, kRowsThreads, 0, stream>>>(a, p.chunk_pages, p.splits);
+  else if (p.splits == 1)
+    kv8_step_kernel<D, kWideWaves><<<grid, kWideWaves * kWave, 0, stream>>>(a, p.chunk_pages, p.splits);
   else
-    kv8_attention_kernel<D, 16, false>
-        <<<dim3((tiles + kAttnWaves - 1) / kAttnWaves * hkv, a.cache.seqs), kAttnThreads, 0, stream>>>(
-            a, p.chunk_pages, p.splits);
-  if (p.splits > 1)
-    kv8_combine_kernel<<<dim3((a.max_rows * a.hq + kAttnWaves - 1) / kAttnWaves, a.cache.seqs), kAttnThreads, 0,
-                         stream>>>(a, p.chunk_pages, p.splits, p.tile_rows);
+    kv8_step_kernel<D, kAttnWaves><<<grid, kAttnThreads, 0, stream>>>(a, p.chunk_pages, p.splits);
+  if (p.splits > 1 && p.splits <= kFewSplits) {
+    const int each = kAttnThreads / (D / 4);
+    kv8_combine_few_kernel<<<dim3((a.max_rows * a.hq + each - 1) / each, a.cache.seqs), kAttnThreads, 0, stream>>>(
+        a, p.chunk_pages, p.splits, p.tile_rows);
+  } else if (p.splits > 1)
+    kv8_combine_kernel<<<dim3(a.max_rows * a.hq, a.cache.seqs), kAttnThreads, 0, stream>>>(a, p.chunk_pages, p.splits,
+                                                                                         p.tile_rows);
 }
 
 }  // namespace

@@ -25,308 +25,490 @@ namespace mmr {
 
 namespace {
 
-constexpr int kQ4Waves = 4;
+constexpr int kQ4Waves = 8;
 constexpr int kQ4Threads = kQ4Waves * kWave;
-constexpr int kQ4Tile = 16;     // weight rows of a block
-constexpr int kQ4Batch = 4;     // batch rows of an x operand
-constexpr int kQ4Half = 1024;   // bytes of an x operand for 64 columns
+constexpr int kQ4Tile = 16;       // weight rows of a product
+constexpr int kQ4Batch = 4;       // batch rows of an x operand
+constexpr int kQ4Operands = 2048; // bytes of the two x operands of a run
 constexpr int kFusedCols = 8192;  // batch x cols that a block itself turns into digits
-constexpr int kManyTiles = 4;   // x operands of a block whose digits come from the workspace
+constexpr int kManyTiles = 4;     // x operands of a block whose digits come from the workspace
+constexpr int kAhead = 4;              // runs of a wave that are asked for together
+constexpr int kWideWaves = 16;         // of a block that takes many tiles
+constexpr int kWideThreads = kWideWaves * kWave;
+constexpr int kManyRowTiles = 1024;    // tiles from which that form is taken
+constexpr int kWideBlocks = 256;       // and its blocks: one a compute unit
+constexpr int kWideTiles = 512;        // tiles from which a block of the other form takes two
 
 using i32x4 = int __attribute__((ext_vector_type(4)));
 
-// 1 / sqrt(mean(x^2) + eps) of a row by the whole block.
-__device__ __forceinline__ float rms_scale(const float* x, int cols, float eps, float* partial) {
-  float ss = 0.0f;
-  for (int i = threadIdx.x; i < cols; i += kQ4Threads) ss += x[i] * x[i];
-  ss = group_sum<kWave>(ss);
-  __syncthreads();
-  if (threadIdx.x % kWave == 0) partial[threadIdx.x / kWave] = ss;
-  __syncthreads();
-  float total = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kQ4Waves; ++i) total += partial[i];
-  return 1.0f / sqrtf(total / static_cast<float>(cols) + eps);
+// What the launch decides, beside the shape.
+struct Q4Form {
+  GemvPrologue pro;
+  GemvEpilogue epi;
+  int runs, groups;
+  bool whole;   // the scales of a run are one load: every run is whole, and they are aligned
+  bool joined;  // those of kAhead runs are 8- or 16-byte loads
+};
+
+__device__ __forceinline__ float normalised(const Q4Form& f, float x, float w, float scale) {
+  return f.pro == kProRmsNorm ? x * (scale * w) : f.pro == kProRmsNormFinal ? (x * scale) * w : x;
 }
 
-template <GemvPrologue kPro>
-__device__ __forceinline__ float x_value(const float* x, const float* w, float scale, int c) {
-  if constexpr (kPro == kProRmsNorm) return x[c] * (scale * w[c]);
-  if constexpr (kPro == kProRmsNormFinal) return (x[c] * scale) * w[c];
-  return x[c];
+// Columns c + lane and c + 64 + lane of a run, and the weights of the norm.
+struct Columns {
+  float x[2], w[2];
+};
+__device__ __forceinline__ Columns load_columns(const MatvecQ4Args& a, const Q4Form& f, int b, int run) {
+  Columns v;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int c = run * kQ4Cols + 64 * k + threadIdx.x % kWave;
+    v.x[k] = c < a.cols ? a.x[static_cast<int64_t>(b) * a.cols + c] : 0.0f;
+    v.w[k] = c < a.cols && f.pro != kProPlain ? a.norm_w[c] : 0.0f;
+  }
+  return v;
 }
 
-// Digits of one 128-column run of row b of an x operand, by one wave: two
-// columns a lane.  to: [2 halves][rows][4 parts][16 bytes].  Returns the
-// power of two that the products come in, NaN if a value is not finite.
-template <GemvPrologue kPro>
-__device__ __forceinline__ float write_digits(const float* x, const float* w, float scale, int cols, int run, int b,
-                                              int rows, int8_t* to) {
-  const int lane = threadIdx.x % kWave, c = run * kQ4Cols + 2 * lane;
-  float v[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) v[i] = c + i < cols ? x_value<kPro>(x, w, scale, c + i) : 0.0f;
+// Digits of a run of row b of an x operand, by one wave.  to: [2 halves][rows]
+// [4 parts][16 bytes], half j / 2, part p and bytes 8 (j % 2) + i / 2 (even
+// columns) or + 4 (odd ones) for column 32 j + 8 p + i.  Returns the power of
+// two that the products come in, NaN if a value is not finite.
+__device__ __forceinline__ float write_digits(const float v[2], int b, int rows, int8_t* to) {
+  const int lane = threadIdx.x % kWave;
   const bool bad = __any(!(fabsf(v[0]) < __builtin_inff()) || !(fabsf(v[1]) < __builtin_inff()));
   const float top = group_max<kWave>(fmaxf(fabsf(v[0]), fabsf(v[1])));
   int e = 0;
   (void)frexpf(bad ? 0.0f : top, &e);
   e = max(e, -90);
-  const int j = lane / 16, p = lane % 16 / 4, i = lane % 4;  // columns 32 j + 8 p + 2 i and + 1
-  int8_t* at = to + (((j / 2) * rows + kQ4Batch * b) * 4 + p) * 16 + (j % 2) * 8 + i;
+  const int j = lane / 32, p = lane % 32 / 8, i = lane % 8;
+  int8_t* at = to + (kQ4Batch * b * 4 + p) * 16 + j * 8 + i % 2 * 4 + i / 2;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const uint32_t n = static_cast<uint32_t>(bad ? 0 : static_cast<int>(rintf(ldexpf(v[k], 30 - e)))) + 0x808080u;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
-      at[d * 64 + 4 * k] = static_cast<int8_t>((n >> (8 * d)) ^ (d < 3 ? 0x80u : 0u));
+      at[(k * rows + d) * 64] = static_cast<int8_t>((n >> (8 * d)) ^ (d < 3 ? 0x80u : 0u));
   }
   return bad ? __builtin_nanf("") : ldexpf(1.0f, e - 34);  // the weights come as 16 q
 }
 
-// The lane's share of a run: 4 groups of 32, 2 of 64 or 1 of 128 columns.
-// scales: of the lane's weight row from the run on, `left` of them there.
+// A lane's share of a run of its weight row: 16 bytes of codes, and the scales
+// of the run's groups.
 template <int kGroup>
-__device__ __forceinline__ float run_product(const uint4& codes, const i32x4 x[2], const __half* scales, int left) {
-  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-  uint32_t lo[4], hi[4];
+struct Run {
+  static constexpr int kGroups = kQ4Cols / kGroup;
+  uint4 codes;
+  __half scales[kGroups];
+};
+template <int kGroup>
+__device__ __forceinline__ void load_scales(const MatvecQ4Args& a, const Q4Form& f, int64_t row, int run, __half* to) {
+  constexpr int kGroups = Run<kGroup>::kGroups;
+  const __half* s = a.scales + row * f.groups + run * kGroups;
+  if (f.whole && kGroups == 4) {
+    *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(s);
+  } else if (f.whole && kGroups == 2) {
+    *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(s);
+  } else {
+#pragma unroll
+    for (int n = 0; n < kGroups; ++n) to[n] = run * kGroups + n < f.groups ? s[n] : __half(0.0f);
+  }
+}
+template <int kGroup>
+__device__ __forceinline__ Run<kGroup> load_run(const MatvecQ4Args& a, const Q4Form& f, int64_t row, int run) {
+  Run<kGroup> r;
+  r.codes = *reinterpret_cast<const uint4*>(a.codes + (row * f.runs + run) * 64 + threadIdx.x % kWave / 16 * 16);
+  load_scales<kGroup>(a, f, row, run, r.scales);
+  return r;
+}
+
+// The run's products with the x operand's row of this lane's part: batch row
+// lane / 16, weight row lane % 16.
+template <int kGroup>
+__device__ __forceinline__ float run_product(const Run<kGroup>& r, const i32x4& x0, const i32x4& x1) {
+  const uint32_t w[4] = {r.codes.x, r.codes.y, r.codes.z, r.codes.w};
+  int lo[4], hi[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) lo[j] = (w[j] << 4) & 0xF0F0F0F0u, hi[j] = w[j] & 0xF0F0F0F0u;
   float y = 0.0f;
-  auto join = [&](const i32x4& a, int n) {
-    const float top = static_cast<float>(a[3] * 256 + a[2]), low = static_cast<float>(a[1] * 256 + a[0]);
-    const float s = n < left ? __half2float(scales[n]) : 0.0f;
-    y = fmaf(fmaf(top, 65536.0f, low), s, y);
+  auto join = [&](const i32x4& d, __half scale) {
+    const float top = static_cast<float>(d[3] * 256 + d[2]), low = static_cast<float>(d[1] * 256 + d[0]);
+    y = fmaf(fmaf(top, 65536.0f, low), __half2float(scale), y);
   };
   const i32x4 zero = {0, 0, 0, 0};
   if constexpr (kGroup == 32) {
     // Half of a product's columns each, the other weights 0.
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int l = static_cast<int>(lo[j]), h = static_cast<int>(hi[j]);
-      const i32x4 b = j % 2 ? i32x4{0, 0, l, h} : i32x4{l, h, 0, 0};
-      join(__builtin_amdgcn_mfma_i32_16x16x64_i8(x[j / 2], b, zero, 0, 0, 0), j);
+      const i32x4 b = j % 2 ? i32x4{0, 0, lo[j], hi[j]} : i32x4{lo[j], hi[j], 0, 0};
+      join(__builtin_amdgcn_mfma_i32_16x16x64_i8(j < 2 ? x0 : x1, b, zero, 0, 0, 0), r.scales[j]);
     }
   } else {
-    i32x4 acc = zero;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const i32x4 b = {static_cast<int>(lo[2 * k]), static_cast<int>(hi[2 * k]), static_cast<int>(lo[2 * k + 1]),
-                       static_cast<int>(hi[2 * k + 1])};
-      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[k], b, kGroup == 64 ? zero : acc, 0, 0, 0);
-      if (kGroup == 64 || k == 1) join(acc, kGroup == 64 ? k : 0);
+    const i32x4 b0 = {lo[0], hi[0], lo[1], hi[1]}, b1 = {lo[2], hi[2], lo[3], hi[3]};
+    const i32x4 d0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(x0, b0, zero, 0, 0, 0);
+    if constexpr (kGroup == 64) {
+      join(d0, r.scales[0]);
+      join(__builtin_amdgcn_mfma_i32_16x16x64_i8(x1, b1, zero, 0, 0, 0), r.scales[1]);
+    } else {
+      join(__builtin_amdgcn_mfma_i32_16x16x64_i8(x1, b1, d0, 0, 0, 0), r.scales[0]);
     }
   }
   return y;
 }
 
 // Weight (r, c) as the formula has it.
-__device__ __forceinline__ float weight_at(const MatvecQ4Args& a, int64_t r, int c) {
-  const int64_t stride = static_cast<int64_t>((a.cols + kQ4Cols - 1) / kQ4Cols) * 64;
+__device__ __forceinline__ float weight_at(const MatvecQ4Args& a, const Q4Form& f, int64_t r, int c) {
   const int u = c % kQ4Cols;
-  const uint32_t byte = a.codes[r * stride + c / kQ4Cols * 64 + (u % 32 / 8 * 4 + u / 32) * 4 + u % 8 / 2];
+  const uint32_t byte = a.codes[(r * f.runs + c / kQ4Cols) * 64 + (u % 32 / 8 * 4 + u / 32) * 4 + u % 8 / 2];
   const int q = static_cast<int>((u & 1 ? byte >> 4 : byte & 15) ^ 8) - 8;
-  return static_cast<float>(q) * __half2float(a.scales[r * ((a.cols + a.group - 1) / a.group) + c / a.group]);
+  return static_cast<float>(q) * __half2float(a.scales[r * f.groups + c / a.group]);
 }
 
 // A result whose row of x holds an infinity or a NaN, which fixed point has no
 // digits for: the formula column by column.
-template <GemvPrologue kPro>
-__device__ __noinline__ float plain_product(const MatvecQ4Args& a, int b, int64_t r, float scale) {
+__device__ __forceinline__ float plain_product(const MatvecQ4Args& a, const Q4Form& f, int b, int64_t r, float scale) {
   const float* x = a.x + static_cast<int64_t>(b) * a.cols;
   float y = 0.0f;
-  for (int c = 0; c < a.cols; ++c) y = fmaf(weight_at(a, r, c), x_value<kPro>(x, a.norm_w, scale, c), y);
+  for (int c = 0; c < a.cols; ++c)
+    y = fmaf(weight_at(a, f, r, c), normalised(f, x[c], f.pro == kProPlain ? 0.0f : a.norm_w[c], scale), y);
   return y;
 }
 
-// sums: [batch rows of the block][kQ4Tile] of products, from row0 and batch row b0.
-template <GemvEpilogue kEpi>
-__device__ __forceinline__ void store_results(const MatvecQ4Args& a, const float* sums, int row0, int b0, int batch) {
-  constexpr int kOut = kEpi == kEpiSwiGlu ? kQ4Tile / 2 : kQ4Tile;
-  for (int i = threadIdx.x; i < batch * kOut; i += kQ4Threads) {
-    const int b = i / kOut, r = i % kOut;
-    const int64_t bg = b0 + b;
-    if constexpr (kEpi == kEpiSwiGlu) {
-      if (row0 + 2 * r < a.rows)
-        a.y[bg * (a.rows / 2) + row0 / 2 + r] = silu_fast(sums[b * kQ4Tile + 2 * r]) * sums[b * kQ4Tile + 2 * r + 1];
-    } else if (row0 + r < a.rows) {
-      const int64_t at = bg * a.rows + row0 + r;
-      a.y[at] = sums[b * kQ4Tile + r] + (kEpi == kEpiResidual ? a.residual[at] : 0.0f);
-    }
+// A wave's results: of batch row b and weight row `row` in each lane.
+__device__ __forceinline__ void finish(const MatvecQ4Args& a, const Q4Form& f, float y, int b, int row) {
+  const float pair = dpp_move<dpp::kQuadXor1>(y);
+  if (b >= a.batch || row >= a.rows) return;
+  const int64_t at = static_cast<int64_t>(b) * a.rows + row;
+  if (f.epi == kEpiSwiGlu) {
+    if (row % 2 == 0) a.y[at / 2] = silu_fast(y) * pair;
+  } else {
+    a.y[at] = f.epi == kEpiResidual ? y + a.residual[at] : y;
   }
 }
 
-// Up to four batch rows: every block writes the digits of x for itself.
-template <int kGroup, GemvPrologue kPro, GemvEpilogue kEpi>
-__global__ __launch_bounds__(kQ4Threads) void matvec_q4_kernel(MatvecQ4Args a) {
-  extern __shared__ __align__(16) int8_t digits[];  // [runs][2][4 batch][4 parts][16]
-  __shared__ float sums[kQ4Waves][kQ4Batch][kQ4Tile], partial[kQ4Waves], row_scale[kQ4Batch];
-  __shared__ int broken;
-  const int runs = (a.cols + kQ4Cols - 1) / kQ4Cols, groups = (a.cols + kGroup - 1) / kGroup;
-  float* const units = reinterpret_cast<float*>(digits + static_cast<int64_t>(runs) * a.batch * 512);  // [batch][runs]
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, g = lane / 16, col = lane % 16;
-  const int rows = kQ4Batch * a.batch;  // of the x operand
-  if (threadIdx.x == 0) broken = 0;
-  if constexpr (kPro != kProPlain) {
-    for (int b = 0; b < a.batch; ++b) {
-      const float scale = rms_scale(a.x + static_cast<int64_t>(b) * a.cols, a.cols, a.eps, partial);
-      if (threadIdx.x == 0) row_scale[b] = scale;
-    }
-  }
-  __syncthreads();
-  for (int u = wave; u < runs * a.batch; u += kQ4Waves) {
-    const int b = u / runs, run = u - b * runs;
-    const float unit = write_digits<kPro>(a.x + static_cast<int64_t>(b) * a.cols, a.norm_w,
-                                          kPro == kProPlain ? 1.0f : row_scale[b], a.cols, run, b, rows,
-                                          digits + static_cast<int64_t>(run) * rows * 128);
-    if (lane == 0) units[b * runs + run] = unit;
-    if (lane == 0 && unit != unit) broken = 1;
-  }
-  __syncthreads();
+// Up to four batch rows: every block writes the digits of x for itself, kUnits
+// runs of a row a wave.
+template <int kUnits, int kWaves>
+struct Digits {
+  static constexpr int kMost = kUnits * kWaves;  // runs of all rows
+  float units[kMost + kAhead][kQ4Batch];         // [runs], then zeros
+  float squares[kMost], row_scale[kQ4Batch];
+};
 
-  const int row0 = blockIdx.x * kQ4Tile;
-  const int64_t r = min(row0 + col, a.rows - 1);
-  const uint8_t* codes = a.codes + r * runs * 64 + 16 * g;
-  const __half* scales = a.scales + r * groups;
-  const int m = min(col, rows - 1), b = min(g, a.batch - 1);
-  float y = 0.0f;
-  for (int run = wave; run < runs; run += kQ4Waves) {
-    const uint4 w = *reinterpret_cast<const uint4*>(codes + run * 64);
-    const int8_t* d = digits + static_cast<int64_t>(run) * rows * 128;
-    const i32x4 x[2] = {*reinterpret_cast<const i32x4*>(d + (m * 4 + g) * 16),
-                        *reinterpret_cast<const i32x4*>(d + ((rows + m) * 4 + g) * 16)};
-    const int first = run * (kQ4Cols / kGroup);
-    y = fmaf(run_product<kGroup>(w, x, scales + first, groups - first), units[b * runs + run], y);
-  }
-  sums[wave][g][col] = y;
-  __syncthreads();
-  if (threadIdx.x < kQ4Batch * kQ4Tile) {
-    const int bb = threadIdx.x / kQ4Tile, rr = threadIdx.x % kQ4Tile;
-    float total = 0.0f;
+// Before: the loads of x; the caller's own loads go between.
+template <int kUnits, int kWaves>
+__device__ __forceinline__ void load_x(const MatvecQ4Args& a, const Q4Form& f, int wave, Columns v[kUnits]) {
 #pragma unroll
-    for (int w = 0; w < kQ4Waves; ++w) total += sums[w][bb][rr];
-    if (broken && bb < a.batch) {
-      bool bad = false;
-      for (int i = 0; i < runs; ++i) bad = bad || units[bb * runs + i] != units[bb * runs + i];
-      if (bad) total = plain_product<kPro>(a, bb, min(row0 + rr, a.rows - 1), kPro == kProPlain ? 1.0f : row_scale[bb]);
-    }
-    sums[0][bb][rr] = total;
+  for (int i = 0; i < kUnits; ++i) {
+    const int u = wave + kWaves * i;
+    if (u < f.runs * a.batch) v[i] = load_columns(a, f, u / f.runs, u % f.runs);
   }
+}
+// Returns whether a value is not finite.  to: [runs][2][4 batch][4 parts][16].
+template <int kUnits, int kWaves>
+__device__ __forceinline__ bool make_digits(const MatvecQ4Args& a, const Q4Form& f, int wave, const Columns v[kUnits],
+                                            Digits<kUnits, kWaves>& d, int8_t* to) {
+  const int lane = threadIdx.x % kWave, rows = kQ4Batch * a.batch;
+  if (f.pro != kProPlain) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int u = wave + kWaves * i;
+      if (u < f.runs * a.batch) {
+        const float ss = group_sum<kWave>(v[i].x[0] * v[i].x[0] + v[i].x[1] * v[i].x[1]);
+        if (lane == 0) d.squares[u] = ss;
+      }
+    }
+    __syncthreads();
+  }
+  bool broken = false;
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const int u = wave + kWaves * i;
+    if (u < f.runs * a.batch) {
+      const int b = u / f.runs, run = u - b * f.runs;
+      float scale = 1.0f;
+      if (f.pro != kProPlain) {
+        const float total = group_sum<kWave>(lane < f.runs ? d.squares[b * f.runs + lane] : 0.0f);  // runs <= 64
+        scale = 1.0f / sqrtf(total / static_cast<float>(a.cols) + a.eps);
+        if (run == 0 && lane == 0) d.row_scale[b] = scale;
+      }
+      float x[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) x[k] = normalised(f, v[i].x[k], v[i].w[k], scale);
+      const float unit = write_digits(x, b, rows, to + run * rows * 128);
+      if (lane == 0) d.units[run][b] = unit;
+      broken = broken || unit != unit;
+    }
+  }
+  if (threadIdx.x < kAhead * kQ4Batch) d.units[f.runs + threadIdx.x / kQ4Batch][threadIdx.x % kQ4Batch] = 0.0f;
+  return __syncthreads_or(broken);
+}
+
+// A run's products with the digits in LDS; runs past the last have unit 0.
+template <int kGroup, typename D>
+__device__ __forceinline__ float use_run(const Run<kGroup>& w, const D& d, const int8_t* operand, int rows, int run,
+                                         int b, float y) {
+  const i32x4 x0 = *reinterpret_cast<const i32x4*>(operand + run * rows * 128);
+  const i32x4 x1 = *reinterpret_cast<const i32x4*>(operand + run * rows * 128 + rows * 64);
+  return fmaf(run_product<kGroup>(w, x0, x1), d.units[run][b], y);
+}
+
+template <typename D>
+__device__ __forceinline__ void finish_checked(const MatvecQ4Args& a, const Q4Form& f, const D& d, bool broken, float y,
+                                               int row) {
+  const int g = threadIdx.x % kWave / 16;
+  if (broken && g < a.batch) {
+    bool bad = false;
+    for (int i = 0; i < f.runs; ++i) bad = bad || d.units[i][g] != d.units[i][g];
+    if (bad) y = plain_product(a, f, g, min(row, a.rows - 1), f.pro == kProPlain ? 1.0f : d.row_scale[g]);
+  }
+  finish(a, f, y, g, row);
+}
+
+// Few tiles of rows: one a block, whose waves share its columns.
+template <int kGroup, int kUnits>
+__global__ __launch_bounds__(kQ4Threads) void matvec_q4_kernel(MatvecQ4Args a, Q4Form f) {
+  extern __shared__ __align__(16) int8_t digits[];
+  __shared__ Digits<kUnits, kQ4Waves> d;
+  __shared__ float sums[kQ4Waves][kWave];
+  const int lane = threadIdx.x % kWave, g = lane / 16, col = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int row = blockIdx.x * kQ4Tile + col;
+  constexpr int kTogether = 2;
+  // Weights do not wait for x.  Runs past the last are read as the last.
+  Run<kGroup> w[kTogether];
+  auto ask = [&](int first) {
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j)
+      w[j] = load_run<kGroup>(a, f, min(row, a.rows - 1), min(first + j * kQ4Waves, f.runs - 1));
+  };
+  ask(wave);
+  Columns v[kUnits];
+  load_x<kUnits, kQ4Waves>(a, f, wave, v);
+  const bool broken = make_digits<kUnits, kQ4Waves>(a, f, wave, v, d, digits);
+  const int rows = kQ4Batch * a.batch, b = min(g, a.batch - 1);
+  const int8_t* const operand = digits + (min(col, rows - 1) * 4 + g) * 16;
+  float y = 0.0f;
+  for (int first = wave; first < f.runs; first += kTogether * kQ4Waves) {
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j)
+      y = use_run(w[j], d, operand, rows, min(first + j * kQ4Waves, f.runs), b, y);
+    if (first + kTogether * kQ4Waves < f.runs) ask(first + kTogether * kQ4Waves);
+  }
+  sums[wave][lane] = y;
   __syncthreads();
-  store_results<kEpi>(a, &sums[0][0][0], row0, 0, a.batch);
+  if (wave > 0) return;
+  y = sums[0][lane];
+#pragma unroll
+  for (int i = 1; i < kQ4Waves; ++i) y += sums[i][lane];
+  finish_checked(a, f, d, broken, y, row);
+}
+
+// Many tiles: two waves a tile, eight tiles of a block at a time, kRing chunks
+// of kAhead runs of a wave under way.
+template <int kGroup, int kUnits>
+__global__ __launch_bounds__(kWideThreads) void matvec_q4_wide_kernel(MatvecQ4Args a, Q4Form f) {
+  extern __shared__ __align__(16) int8_t digits[];
+  __shared__ Digits<kUnits, kWideWaves> d;
+  __shared__ float sums[2][kWideWaves / 2][kWave];
+  constexpr int kGroups = Run<kGroup>::kGroups, kRing = kGroup == 32 ? 2 : kGroup == 64 ? 3 : 4, kTiles = kWideWaves / 2;
+  const int lane = threadIdx.x % kWave, g = lane / 16, col = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), slot = wave / 2, half = wave % 2;
+  const int tiles = (a.rows + kQ4Tile - 1) / kQ4Tile, stride = gridDim.x * kTiles;
+  const int steps = (f.runs + 2 * kAhead - 1) / (2 * kAhead);  // chunks of a wave and tile
+  int ask_tile = blockIdx.x * kTiles + slot, ask_step = 0;
+  Run<kGroup> ring[kRing][kAhead];
+  auto ask = [&](Run<kGroup>* to) {  // what is past the last is read as the last, and not used
+    const int64_t row = min(min(ask_tile, tiles - 1) * kQ4Tile + col, a.rows - 1);
+    const int first = (2 * ask_step + half) * kAhead;
+    const uint8_t* codes = a.codes + row * f.runs * 64 + 16 * g;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      to[j].codes = *reinterpret_cast<const uint4*>(codes + min(first + j, f.runs - 1) * 64);
+    if (f.joined) {
+      // One load for all, or for 8 groups.
+      constexpr int kUnit = kGroups == 1 ? 4 : 8, kLoads = kAhead * kGroups / kUnit;
+      __half s[kAhead * kGroups];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const __half* at = a.scales + row * f.groups + min(first * kGroups + kUnit * i, f.groups - kUnit);
+        if constexpr (kUnit == 8)
+          *reinterpret_cast<uint4*>(s + 8 * i) = *reinterpret_cast<const uint4*>(at);
+        else
+          *reinterpret_cast<uint2*>(s + 4 * i) = *reinterpret_cast<const uint2*>(at);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+        for (int n = 0; n < kGroups; ++n) to[j].scales[n] = s[j * kGroups + n];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) load_scales<kGroup>(a, f, row, min(first + j, f.runs - 1), to[j].scales);
+    }
+    if (++ask_step == steps) ask_step = 0, ask_tile += stride;
+  };
+  Columns v[kUnits];
+  load_x<kUnits, kWideWaves>(a, f, wave, v);
+#pragma unroll
+  for (int i = 0; i < kRing; ++i) ask(ring[i]);
+  const bool broken = make_digits<kUnits, kWideWaves>(a, f, wave, v, d, digits);
+
+  const int rows = kQ4Batch * a.batch, b = min(g, a.batch - 1);
+  const int8_t* const operand = digits + (min(col, rows - 1) * 4 + g) * 16;
+  int base = blockIdx.x * kTiles, step = 0, round = 0;
+  int left = (tiles - base + stride - 1) / stride * steps;  // steps of this block's waves
+  float y = 0.0f;
+  auto use = [&](const Run<kGroup>* now) {
+    const int first = (2 * step + half) * kAhead;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) y = use_run(now[j], d, operand, rows, min(first + j, f.runs), b, y);
+    if (++step == steps) {
+      if (half == 1) sums[round % 2][slot][lane] = y;
+      __syncthreads();
+      if (half == 0) finish_checked(a, f, d, broken, y + sums[round % 2][slot][lane], (base + slot) * kQ4Tile + col);
+      y = 0.0f;
+      step = 0;
+      ++round;
+      base += stride;
+    }
+  };
+  // The loads of a chunk are waited for with those of the next kRing - 1 under
+  // way, so none of these is conditional; the last chunks ask for nothing.
+  for (; left > kRing; left -= kRing) {
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) {
+      use(ring[i]);
+      ask(ring[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRing; ++i)
+    if (i < left) use(ring[i]);
 }
 
 // Workspace of the two-launch form: digits [ceil(batch / 4)][runs][2 KB], then
 // fp32 units [batch][runs], then scales [batch].
 __host__ __device__ inline int64_t q4_units_offset(int runs, int batch) {
-  return static_cast<int64_t>((batch + kQ4Batch - 1) / kQ4Batch) * runs * (2 * kQ4Half);
+  return static_cast<int64_t>((batch + kQ4Batch - 1) / kQ4Batch) * runs * kQ4Operands;
 }
 
-template <GemvPrologue kPro>
-__global__ __launch_bounds__(kQ4Threads) void q4_digits_kernel(MatvecQ4Args a) {
+// A block a batch row.
+__global__ __launch_bounds__(kQ4Threads) void q4_digits_kernel(MatvecQ4Args a, Q4Form f) {
   __shared__ float partial[kQ4Waves];
-  const int b = blockIdx.x, runs = (a.cols + kQ4Cols - 1) / kQ4Cols;
-  const float* x = a.x + static_cast<int64_t>(b) * a.cols;
+  const int b = blockIdx.x, wave = threadIdx.x / kWave;
   int8_t* base = static_cast<int8_t*>(a.workspace);
-  float* units = reinterpret_cast<float*>(base + q4_units_offset(runs, a.batch));
-  const float scale = kPro == kProPlain ? 1.0f : rms_scale(x, a.cols, a.eps, partial);
-  if (threadIdx.x == 0) units[static_cast<int64_t>(a.batch) * runs + b] = scale;
-  int8_t* to = base + static_cast<int64_t>(b / kQ4Batch) * runs * (2 * kQ4Half);
-  for (int run = threadIdx.x / kWave; run < runs; run += kQ4Waves) {
-    const float unit = write_digits<kPro>(x, a.norm_w, scale, a.cols, run, b % kQ4Batch, 4 * kQ4Batch,
-                                          to + static_cast<int64_t>(run) * (2 * kQ4Half));
-    if (threadIdx.x % kWave == 0) units[static_cast<int64_t>(b) * runs + run] = unit;
-  }
-}
-
-// More rows: 16 weight rows x 16 batch rows a block, x digits from the workspace.
-template <int kGroup, GemvPrologue kPro, GemvEpilogue kEpi>
-__global__ __launch_bounds__(kQ4Threads) void matvec_q4_rows_kernel(MatvecQ4Args a) {
-  __shared__ float sums[kQ4Waves][kManyTiles * kQ4Batch][kQ4Tile];
-  const int runs = (a.cols + kQ4Cols - 1) / kQ4Cols, groups = (a.cols + kGroup - 1) / kGroup;
-  const int8_t* base = static_cast<const int8_t*>(a.workspace);
-  const float* units = reinterpret_cast<const float*>(base + q4_units_offset(runs, a.batch));
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, g = lane / 16, col = lane % 16;
-  const int row0 = blockIdx.x * kQ4Tile, b0 = blockIdx.y * kManyTiles * kQ4Batch;
-  const int batch = min(kManyTiles * kQ4Batch, a.batch - b0), tiles = (batch + kQ4Batch - 1) / kQ4Batch;
-  const int64_t r = min(row0 + col, a.rows - 1);
-  const uint8_t* codes = a.codes + r * runs * 64 + 16 * g;
-  const __half* scales = a.scales + r * groups;
-  float y[kManyTiles] = {};
-  for (int run = wave; run < runs; run += kQ4Waves) {
-    const uint4 w = *reinterpret_cast<const uint4*>(codes + static_cast<int64_t>(run) * 64);
-    const int first = run * (kQ4Cols / kGroup);
-#pragma unroll
-    for (int t = 0; t < kManyTiles; ++t) {
-      if (t < tiles) {
-        const int8_t* d = base + (static_cast<int64_t>(b0 / kQ4Batch + t) * runs + run) * (2 * kQ4Half);
-        const i32x4 x[2] = {*reinterpret_cast<const i32x4*>(d + (col * 4 + g) * 16),
-                            *reinterpret_cast<const i32x4*>(d + kQ4Half + (col * 4 + g) * 16)};
-        const int b = min(b0 + t * kQ4Batch + g, a.batch - 1);
-        y[t] = fmaf(run_product<kGroup>(w, x, scales + first, groups - first),
-                    units[static_cast<int64_t>(b) * runs + run], y[t]);
-      }
+  float* units = reinterpret_cast<float*>(base + q4_units_offset(f.runs, a.batch));
+  Columns v = {};
+  if (wave < f.runs) v = load_columns(a, f, b, wave);
+  float scale = 1.0f;
+  if (f.pro != kProPlain) {
+    float ss = v.x[0] * v.x[0] + v.x[1] * v.x[1];
+    for (int run = wave + kQ4Waves; run < f.runs; run += kQ4Waves) {
+      const Columns u = load_columns(a, f, b, run);
+      ss += u.x[0] * u.x[0] + u.x[1] * u.x[1];
     }
-  }
-#pragma unroll
-  for (int t = 0; t < kManyTiles; ++t) sums[wave][t * kQ4Batch + g][col] = y[t];
-  __syncthreads();
-  for (int i = threadIdx.x; i < batch * kQ4Tile; i += kQ4Threads) {
-    const int bb = i / kQ4Tile, rr = i % kQ4Tile;
+    ss = group_sum<kWave>(ss);
+    if (threadIdx.x % kWave == 0) partial[wave] = ss;
+    __syncthreads();
     float total = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kQ4Waves; ++w) total += sums[w][bb][rr];
-    if (total != total) {  // a unit of the row is NaN, or the sum overflowed
+    for (int i = 0; i < kQ4Waves; ++i) total += partial[i];
+    scale = 1.0f / sqrtf(total / static_cast<float>(a.cols) + a.eps);
+  }
+  if (threadIdx.x == 0) units[static_cast<int64_t>(a.batch) * f.runs + b] = scale;
+  int8_t* to = base + static_cast<int64_t>(b / kQ4Batch) * f.runs * kQ4Operands;
+  for (int run = wave; run < f.runs; run += kQ4Waves) {
+    if (run != wave) v = load_columns(a, f, b, run);
+    float x[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) x[k] = normalised(f, v.x[k], v.w[k], scale);
+    const float unit =
+        write_digits(x, b % kQ4Batch, 4 * kQ4Batch, to + static_cast<int64_t>(run) * kQ4Operands);
+    if (threadIdx.x % kWave == 0) units[static_cast<int64_t>(b) * f.runs + run] = unit;
+  }
+}
+
+// More rows of x: kTiles x 16 weight rows and 16 batch rows a block, whose
+// waves share the columns; x digits from the workspace.
+template <int kGroup, int kTiles>
+__global__ __launch_bounds__(kQ4Threads) void matvec_q4_rows_kernel(MatvecQ4Args a, Q4Form f) {
+  __shared__ float sums[kQ4Waves][kManyTiles][kTiles][kWave];
+  const int8_t* base = static_cast<const int8_t*>(a.workspace);
+  const float* units = reinterpret_cast<const float*>(base + q4_units_offset(f.runs, a.batch));
+  const int lane = threadIdx.x % kWave, g = lane / 16, col = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int row0 = blockIdx.x * kTiles * kQ4Tile, b0 = blockIdx.y * kManyTiles * kQ4Batch;
+  const int operands = (a.batch + kQ4Batch - 1) / kQ4Batch;
+  float y[kManyTiles][kTiles] = {};
+  for (int run = wave; run < f.runs; run += kQ4Waves) {
+    Run<kGroup> w[kTiles];
+#pragma unroll
+    for (int k = 0; k < kTiles; ++k)
+      w[k] = load_run<kGroup>(a, f, min(row0 + k * kQ4Tile + col, a.rows - 1), run);
+    // Operands past the last are read as the last and not stored.
+    i32x4 x[kManyTiles][2];
+    float unit[kManyTiles];
+#pragma unroll
+    for (int t = 0; t < kManyTiles; ++t) {
+      const int o = min(b0 / kQ4Batch + t, operands - 1);
+      const int8_t* d = base + (static_cast<int64_t>(o) * f.runs + run) * kQ4Operands + (col * 4 + g) * 16;
+      x[t][0] = *reinterpret_cast<const i32x4*>(d);
+      x[t][1] = *reinterpret_cast<const i32x4*>(d + kQ4Operands / 2);
+      unit[t] = units[static_cast<int64_t>(min(o * kQ4Batch + g, a.batch - 1)) * f.runs + run];
+    }
+#pragma unroll
+    for (int t = 0; t < kManyTiles; ++t)
+#pragma unroll
+      for (int k = 0; k < kTiles; ++k) y[t][k] = fmaf(run_product<kGroup>(w[k], x[t][0], x[t][1]), unit[t], y[t][k]);
+  }
+#pragma unroll
+  for (int t = 0; t < kManyTiles; ++t)
+#pragma unroll
+    for (int k = 0; k < kTiles; ++k) sums[wave][t][k][lane] = y[t][k];
+  __syncthreads();
+  for (int i = wave; i < kManyTiles * kTiles; i += kQ4Waves) {
+    const int t = i / kTiles, k = i % kTiles, b = b0 + t * kQ4Batch + g, row = row0 + k * kQ4Tile + col;
+    float total = sums[0][t][k][lane];
+#pragma unroll
+    for (int w = 1; w < kQ4Waves; ++w) total += sums[w][t][k][lane];
+    if (total != total && b < a.batch && row < a.rows) {  // a unit of the row is NaN, or the sum overflowed
       bool bad = false;
-      for (int u = 0; u < runs; ++u) {
-        const float unit = units[static_cast<int64_t>(b0 + bb) * runs + u];
+      for (int u = 0; u < f.runs; ++u) {
+        const float unit = units[static_cast<int64_t>(b) * f.runs + u];
         bad = bad || unit != unit;
       }
-      if (bad)
-        total = plain_product<kPro>(a, b0 + bb, min(row0 + rr, a.rows - 1),
-                                    units[static_cast<int64_t>(a.batch) * runs + b0 + bb]);
+      if (bad) total = plain_product(a, f, b, row, units[static_cast<int64_t>(a.batch) * f.runs + b]);
     }
-    sums[0][bb][rr] = total;
+    finish(a, f, total, b, row);
   }
-  __syncthreads();
-  store_results<kEpi>(a, &sums[0][0][0], row0, b0, batch);
 }
 
 bool fused_digits(int cols, int batch) {
   return batch <= kQ4Batch && static_cast<int64_t>(batch) * cols <= kFusedCols;
 }
 
-template <int kGroup, GemvPrologue kPro, GemvEpilogue kEpi>
-void launch_q4(const MatvecQ4Args& a, hipStream_t stream) {
-  const int tiles = (a.rows + kQ4Tile - 1) / kQ4Tile, runs = (a.cols + kQ4Cols - 1) / kQ4Cols;
+template <int kGroup>
+void launch_q4(const MatvecQ4Args& a, const Q4Form& f, hipStream_t stream) {
   if (fused_digits(a.cols, a.batch)) {
-    const size_t lds = static_cast<size_t>(runs) * a.batch * 516;
-    matvec_q4_kernel<kGroup, kPro, kEpi><<<tiles, kQ4Threads, lds, stream>>>(a);
+    const int tiles = (a.rows + kQ4Tile - 1) / kQ4Tile, all = f.runs * a.batch, each = kWideWaves / 2;
+    const size_t lds = static_cast<size_t>(f.runs + kAhead) * a.batch * 512;
+    const int blocks = std::min((tiles + each - 1) / each, kWideBlocks);
+    if (tiles < kManyRowTiles && all <= 2 * kQ4Waves)
+      matvec_q4_kernel<kGroup, 2><<<tiles, kQ4Threads, lds, stream>>>(a, f);
+    else if (tiles < kManyRowTiles)
+      matvec_q4_kernel<kGroup, 8><<<tiles, kQ4Threads, lds, stream>>>(a, f);
+    else if (all <= kWideWaves)
+      matvec_q4_wide_kernel<kGroup, 1><<<blocks, kWideThreads, lds, stream>>>(a, f);
+    else
+      matvec_q4_wide_kernel<kGroup, 4><<<blocks, kWideThreads, lds, stream>>>(a, f);
     return;
   }
-  const int many = kManyTiles * kQ4Batch;
-  q4_digits_kernel<kPro><<<a.batch, kQ4Threads, 0, stream>>>(a);
-  matvec_q4_rows_kernel<kGroup, kPro, kEpi>
-      <<<dim3(tiles, (a.batch + many - 1) / many), kQ4Threads, 0, stream>>>(a);
-}
-
-template <int kGroup, GemvPrologue kPro>
-void launch_q4_epi(const MatvecQ4Args& a, GemvEpilogue epi, hipStream_t stream) {
-  if (epi == kEpiResidual)
-    launch_q4<kGroup, kPro, kEpiResidual>(a, stream);
-  else if (epi == kEpiSwiGlu)
-    launch_q4<kGroup, kPro, kEpiSwiGlu>(a, stream);
+  const int tiles = (a.rows + kQ4Tile - 1) / kQ4Tile, many = kManyTiles * kQ4Batch;
+  q4_digits_kernel<<<a.batch, kQ4Threads, 0, stream>>>(a, f);
+  if (tiles >= kWideTiles)
+    matvec_q4_rows_kernel<kGroup, 2>
+        <<<dim3((tiles + 1) / 2, (a.batch + many - 1) / many), kQ4Threads, 0, stream>>>(a, f);
   else
-    launch_q4<kGroup, kPro, kEpiStore>(a, stream);
-}
-
-template <int kGroup>
-void launch_q4_pro(const MatvecQ4Args& a, GemvPrologue pro, GemvEpilogue epi, hipStream_t stream) {
-  if (pro == kProRmsNorm)
-    launch_q4_epi<kGroup, kProRmsNorm>(a, epi, stream);
-  else if (pro == kProRmsNormFinal)
-    launch_q4_epi<kGroup, kProRmsNormFinal>(a, epi, stream);
-  else
-    launch_q4_epi<kGroup, kProPlain>(a, epi, stream);
+    matvec_q4_rows_kernel<kGroup, 1><<<dim3(tiles, (a.batch + many - 1) / many), kQ4Threads, 0, stream>>>(a, f);
 }
 
 }  // namespace
@@ -338,10 +520,17 @@ int64_t matvec_q4_workspace(int cols, int batch) {
 }
 
 hipError_t launch_matvec_q4(const MatvecQ4Args& a, GemvPrologue pro, GemvEpilogue epi, hipStream_t stream) {
+  Q4Form f;
+  f.pro = pro;
+  f.epi = epi;
+  f.runs = (a.cols + kQ4Cols - 1) / kQ4Cols;
+  f.groups = (a.cols + a.group - 1) / a.group;
+  f.whole = a.cols % kQ4Cols == 0 && reinterpret_cast<uintptr_t>(a.scales) % 8 == 0;
+  f.joined = f.whole && f.groups % (a.group == 128 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(a.scales) % 16 == 0;
   switch (a.group) {
-    case 32: launch_q4_pro<32>(a, pro, epi, stream); break;
-    case 64: launch_q4_pro<64>(a, pro, epi, stream); break;
-    case 128: launch_q4_pro<128>(a, pro, epi, stream); break;
+    case 32: launch_q4<32>(a, f, stream); break;
+    case 64: launch_q4<64>(a, f, stream); break;
+    case 128: launch_q4<128>(a, f, stream); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
