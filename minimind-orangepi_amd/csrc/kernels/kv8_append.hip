@@ -24,6 +24,8 @@
 #include "device_common.h"
 #include "kv8_common.h"
 
+#include <algorithm>
+
 namespace mmr {
 
 namespace {
@@ -60,20 +62,25 @@ struct Quarter {
   static constexpr int kChunks = D / 32;
   double a[kChunks][4], b[kChunks][4];
 
-  __device__ __forceinline__ void load(const float* p, int j) {
+  struct Raw {
+    float4 lo[kChunks], hi[kChunks];
+    __device__ __forceinline__ void load(const float* p, int j, bool there) {
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        lo[c] = hi[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (there) {
+          lo[c] = *reinterpret_cast<const float4*>(p + 16 * c + 4 * j);
+          hi[c] = *reinterpret_cast<const float4*>(p + D / 2 + 16 * c + 4 * j);
+        }
+      }
+    }
+  };
+  __device__ __forceinline__ explicit Quarter(const Raw& r) {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      const float4 lo = *reinterpret_cast<const float4*>(p + 16 * c + 4 * j);
-      const float4 hi = *reinterpret_cast<const float4*>(p + D / 2 + 16 * c + 4 * j);
-      a[c][0] = lo.x, a[c][1] = lo.y, a[c][2] = lo.z, a[c][3] = lo.w;
-      b[c][0] = hi.x, b[c][1] = hi.y, b[c][2] = hi.z, b[c][3] = hi.w;
+      a[c][0] = r.lo[c].x, a[c][1] = r.lo[c].y, a[c][2] = r.lo[c].z, a[c][3] = r.lo[c].w;
+      b[c][0] = r.hi[c].x, b[c][1] = r.hi[c].y, b[c][2] = r.hi[c].z, b[c][3] = r.hi[c].w;
     }
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[c][i] = b[c][i] = 0.0;
   }
   // All four lanes of the row take part.
   __device__ __forceinline__ void normalise(const float* w, double eps, int j) {
@@ -137,9 +144,12 @@ __device__ __forceinline__ uint32_t moved(uint32_t codes, float scale) {
   return out;
 }
 
+// blockIdx.z 0 appends the block's keys and values, the others rotate a share
+// of its queries.  Everything that does not wait for the angles is asked for
+// before they are computed.
 template <int D>
 __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Kv8AppendArgs a) {
-  constexpr int kHalf = D / 2, kChunks = D / 32, kWaves = kAppendThreads / kWave;
+  constexpr int kHalf = D / 2, kChunks = D / 32, kWaves = kAppendThreads / kWave, kGroups = kAppendThreads / 4;
   __shared__ double2 turn[kKv8Block][kHalf];
   __shared__ __align__(16) int8_t tile[kWaves][D][kKv8Block];
   const int s = blockIdx.y, tid = threadIdx.x;
@@ -147,55 +157,76 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Kv8AppendArg
   const bool fine = kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span);
   const bool known = fine && (span.n == 0 || static_cast<int64_t>(span.context) + span.n <= a.max_positions);
   if (!known) {
-    if (blockIdx.x == 0 && tid == 0) atomicOr(a.error, kKv8BadRows);
+    if (blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) atomicOr(a.error, kKv8BadRows);
     return;
   }
   const int block = span.context / kKv8Block + blockIdx.x;
   const int lo = max(span.context, block * kKv8Block), hi = min(span.context + span.n, (block + 1) * kKv8Block);
   if (lo >= hi) return;
   const int page = a.cache.table[static_cast<int64_t>(s) * a.cache.per_seq + block / kKv8Blocks];
+  const int fresh = lo - block * kKv8Block, end = hi - block * kKv8Block;  // slots [fresh, end) are new
+  const int first_row = span.first + (lo - span.context);                  // of slot `fresh`
+  const int hq = a.hq, hkv = a.cache.hkv, j = tid & 3;
+  const int64_t stride = static_cast<int64_t>(hq + 2 * hkv) * D;
+
+  // What this thread's four lanes work on first.  Queries: (row, head) items.
+  // Keys and values: a wave each (K or V, head), lanes 4 i .. 4 i + 3 slot i.
+  const int wave = tid / kWave, lane = tid % kWave, slot = lane / 4;
+  const bool mine = slot >= fresh && slot < end;
+  const int items = (end - fresh) * hq;
+  int it = blockIdx.z == 0 ? wave : (blockIdx.z - 1) * kGroups + tid / 4;
+  typename Quarter<D>::Raw raw;
+  auto load_query = [&]() {
+    const int r = it / hq, h = it - r * hq;
+    raw.load(a.qkv + (first_row + r) * stride + h * D, j, it < items);
+  };
+  auto load_cached = [&]() {
+    raw.load(a.qkv + (first_row + slot - fresh) * stride + static_cast<int64_t>(hq + it) * D, j,
+             mine && it < 2 * hkv);
+  };
+  if (blockIdx.z == 0)
+    load_cached();
+  else if (it < items)
+    load_query();
+  for (int i = tid; i < (end - fresh) * kHalf; i += kAppendThreads) {
+    const int r = i / kHalf, d = i - r * kHalf;
+    const uint64_t t = static_cast<uint64_t>(lo + r) * a.turns[d];
+    double sn, cs;
+    sincospi(static_cast<double>(static_cast<int64_t>(t)) * 0x1p-63, &sn, &cs);
+    turn[fresh + r][d] = make_double2(cs, sn);
+  }
   if (page < 0 || page >= a.cache.pages) {
     if (tid == 0) atomicOr(a.error, kKv8BadRows);
     return;
   }
-  const int fresh = lo - block * kKv8Block, end = hi - block * kKv8Block;  // slots [fresh, end) are new
-  const int first_row = span.first + (lo - span.context);                  // of slot `fresh`
-  for (int i = tid; i < (end - fresh) * kHalf; i += kAppendThreads) {
-    const int r = i / kHalf, j = i - r * kHalf;
-    const uint64_t t = static_cast<uint64_t>(lo + r) * a.turns[j];
-    double sn, cs;
-    sincospi(static_cast<double>(static_cast<int64_t>(t)) * 0x1p-63, &sn, &cs);
-    turn[fresh + r][j] = make_double2(cs, sn);
-  }
   __syncthreads();
 
-  const int hq = a.hq, hkv = a.cache.hkv;
-  const int64_t stride = static_cast<int64_t>(hq + 2 * hkv) * D;
-  const int j = tid & 3;
-  for (int it = tid / 4; it < (end - fresh) * hq; it += kAppendThreads / 4) {
-    const int r = it / hq, h = it - r * hq;
-    Quarter<D> x;
-    x.load(a.qkv + (first_row + r) * stride + h * D, j);
-    if (a.q_norm) x.normalise(a.q_norm, a.eps, j);
-    x.rotate(turn[fresh + r], j);
-    float* out = a.query + (static_cast<int64_t>(first_row + r) * hq + h) * D;
+  if (blockIdx.z > 0) {
+    for (; it < items; it += kGroups * (gridDim.z - 1)) {
+      const int r = it / hq, h = it - r * hq;
+      Quarter<D> x(raw);
+      if (a.q_norm) x.normalise(a.q_norm, a.eps, j);
+      x.rotate(turn[fresh + r], j);
+      float* out = a.query + (static_cast<int64_t>(first_row + r) * hq + h) * D;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      *reinterpret_cast<float4*>(out + 16 * c + 4 * j) = make_float4(x.a[c][0], x.a[c][1], x.a[c][2], x.a[c][3]);
-      *reinterpret_cast<float4*>(out + kHalf + 16 * c + 4 * j) =
-          make_float4(x.b[c][0], x.b[c][1], x.b[c][2], x.b[c][3]);
+      for (int c = 0; c < kChunks; ++c) {
+        *reinterpret_cast<float4*>(out + 16 * c + 4 * j) = make_float4(x.a[c][0], x.a[c][1], x.a[c][2], x.a[c][3]);
+        *reinterpret_cast<float4*>(out + kHalf + 16 * c + 4 * j) =
+            make_float4(x.b[c][0], x.b[c][1], x.b[c][2], x.b[c][3]);
+      }
+      it += kGroups * (gridDim.z - 1);
+      if (it < items) load_query();
+      it -= kGroups * (gridDim.z - 1);
     }
+    return;
   }
-
-  // One wave a (K or V, head): lanes 4 i .. 4 i + 3 hold slot i of the block.
-  const int wave = tid / kWave, lane = tid % kWave, slot = lane / 4;
-  const bool mine = slot >= fresh && slot < end;
-  for (int it = wave; it < 2 * hkv; it += kWaves) {
+  for (; it < 2 * hkv; it += kWaves) {
     const bool is_key = it < hkv;
     const int h = is_key ? it : it - hkv;
-    Quarter<D> x;
-    x.zero();
-    if (mine) x.load(a.qkv + (first_row + slot - fresh) * stride + static_cast<int64_t>(hq + it) * D, j);
+    int8_t* exps = (is_key ? a.cache.key_exps : a.cache.value_exps) + kv8_exp_offset(page, h, hkv) + block % kKv8Blocks;
+    int8_t* codes = (is_key ? a.cache.keys : a.cache.values) + kv8_offset(page, h, hkv, D);
+    const int held = fresh > 0 ? *exps : kKv8MinExp;
+    Quarter<D> x(raw);
     if (is_key) {
       if (a.k_norm) x.normalise(a.k_norm, a.eps, j);
       if (mine) x.rotate(turn[slot], j);
@@ -205,14 +236,11 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Kv8AppendArg
     if (!mine) e = kKv8MinExp, bad = false;
     e = wave_max(e);
     if (bad) atomicOr(a.error, kKv8NotFinite);
-    int8_t* exps = (is_key ? a.cache.key_exps : a.cache.value_exps) + kv8_exp_offset(page, h, hkv) + block % kKv8Blocks;
-    const int held = fresh > 0 ? *exps : kKv8MinExp;
     const int grown = fresh > 0 ? max(0, e - held) : 0;  // earlier rows shift by this
     if (fresh > 0) e = max(e, held);
     const float shrink = ldexpf(1.0f, -grown);
     const double scale = pow2(-e);
     if (lane == 0) *exps = static_cast<int8_t>(e);
-    int8_t* codes = (is_key ? a.cache.keys : a.cache.values) + kv8_offset(page, h, hkv, D);
     if (is_key) {
       int8_t* row = codes + (block % kKv8Blocks * kKv8Block + slot) * D;
       if (mine) {
@@ -270,14 +298,19 @@ __global__ __launch_bounds__(kAppendThreads) void kv8_append_kernel(Kv8AppendArg
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
+    it += kWaves;
+    load_cached();
+    it -= kWaves;
   }
 }
 
 }  // namespace
 
 hipError_t launch_kv8_append(const Kv8AppendArgs& a, hipStream_t stream) {
-  // Rows that start anywhere in a block reach into this many blocks.
-  const dim3 grid((a.max_rows + 2 * (kKv8Block - 1)) / kKv8Block, a.cache.seqs);
+  // Rows that start anywhere in a block reach into this many blocks; of a full
+  // one, a thread group takes one query row of one head.
+  const int shares = (std::min(a.max_rows, kKv8Block) * a.hq + kAppendThreads / 4 - 1) / (kAppendThreads / 4);
+  const dim3 grid((a.max_rows + 2 * (kKv8Block - 1)) / kKv8Block, a.cache.seqs, 1 + shares);
   switch (a.cache.d) {
     case 32: kv8_append_kernel<32><<<grid, kAppendThreads, 0, stream>>>(a); break;
     case 64: kv8_append_kernel<64><<<grid, kAppendThreads, 0, stream>>>(a); break;
