@@ -47,10 +47,10 @@ constexpr float kNoRow = -FLT_MAX / 2;  // reference of a row that has met no ke
 constexpr float kLead = 5.0f;           // a score may pass the reference by 2^kLead
 constexpr int kRowsThreads = 256;
 constexpr int kFewSplits = 8;
-constexpr int kRowsTile = 128;          // rows of a block of the kernel for many
+constexpr int kRowsTile = 64;          // rows of a block of the kernel for many
 constexpr int kRowsPBits = 10;          // its p in units of 2^-10: at most 2^15 with the lead
 constexpr int kPBits = 25;              // p in units of 2^-25: at most 2^30 with the lead
-constexpr int kWidePages = 16, kStepBlocks = 256, kRowsBlocks = 512;  // see kv8_attention_plan
+constexpr int kWidePages = 16, kStepBlocks = 256, kRowsBlocks = 1280, kFewRows = 256;  // see kv8_attention_plan
 constexpr int kMostSplits = 64;  // at most one a thread of the combine
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 using f32x4 = float __attribute__((ext_vector_type(4)));
@@ -107,6 +107,9 @@ __device__ __forceinline__ int gather_digits(const int u[4], uint32_t sel, uint3
 __device__ __forceinline__ uint32_t digit_select(int k) { return k | (4 + k) << 8; }
 __device__ __forceinline__ uint32_t digit_flip(int k) { return k < 3 ? 0x80808080u : 0u; }
 
+// Splits of at most `chunk` pages each that a row's `pages` are dealt to, evenly.
+__device__ __forceinline__ int splits_used(int pages, int chunk) { return (pages + chunk - 1) / chunk; }
+
 // Reference and sum of a row's split, after all the splits' outputs.
 __device__ __forceinline__ void store_ml(const Kv8AttnArgs& a, int64_t row, int splits, int split, int d, float ref,
                                          float l) {
@@ -123,11 +126,6 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void kv8_step_kernel(Kv8AttnArgs 
   const int split = blockIdx.x % splits, h = blockIdx.x / splits;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int g = lane / 16, col = lane % 16;
-  // Page numbers of this wave's first 64 steps, one a lane: read along with the
-  // offsets, not after them.
-  const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
-  const int from = split * chunk + wave;
-  int numbers = table[min(from + kWaves * lane, a.cache.per_seq - 1)];
   Kv8Span span;
   const bool fine = kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span);
   if (!fine || (span.n > 0 && static_cast<int64_t>(span.context) + span.n > a.max_tokens)) {
@@ -137,9 +135,14 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void kv8_step_kernel(Kv8AttnArgs 
   const int total = span.n * group;  // rows of this group of heads
   if (total == 0) return;
   const int pages = (span.context + span.n - 1) / kKv8Page + 1;
-  const int begin = split * chunk, end = min(begin + chunk, pages);
-  if (begin >= end) return;
-  const int used = (pages + chunk - 1) / chunk;
+  const int used = splits_used(pages, chunk);
+  if (split >= used) return;
+  const int each = (pages + used - 1) / used, begin = split * each, end = min(begin + each, pages);
+
+  // Page numbers of this wave's next 64 steps, one a lane.
+  const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
+  const int from = begin + wave;
+  int numbers = table[min(from + kWaves * lane, a.cache.per_seq - 1)];
 
   // This lane's column: digit `digit` of row m.
   const int m = col / 4, digit = col % 4;
@@ -376,25 +379,25 @@ __device__ __forceinline__ void widen(const uint4& codes, uint4* lo, uint4* hi) 
   *hi = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
-// x * f = hi + lo in fp16, two at a time (split2 with the product inside).
-__device__ __forceinline__ void split2_scaled(float x0, float x1, float f, uint32_t& hi, uint32_t& lo) {
-  asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(hi) : "v"(x0), "v"(f));
-  asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(hi) : "v"(x1), "v"(f));
-  asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(lo) : "v"(x0), "v"(f), "v"(hi));
-  asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(lo) : "v"(x1), "v"(f), "v"(hi));
+// x = hi + lo in fp16 with hi truncated, which packs two in one instruction;
+// lo takes up the difference (split2 rounds hi, in three): 21 bits.
+__device__ __forceinline__ void split2_truncated(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+  asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(hi), "v"(x0));
+  asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(lo) : "v"(hi), "v"(x1));
 }
 
-// 32 rows a wave, all waves over the same pages, which the block widens into
+// 16 rows a wave, all waves over the same pages, which the block widens into
 // LDS: the operands of every product, 16 bytes a lane in the order of lanes.
 template <int D>
-__global__ __launch_bounds__(kRowsThreads, 2) void kv8_rows_kernel(Kv8AttnArgs a, int chunk, int splits) {
+__global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel(Kv8AttnArgs a, int chunk, int splits) {
   constexpr int kTiles = D / 16, kRuns = D / 32;  // tiles of the output, products along D
   constexpr int kPieces = D / 32;                 // 16-byte pieces of a page that a thread widens
   constexpr int kOperand = kWave;                 // of uint4
-  constexpr int kSets = 2;                        // of 16 rows of a wave
   __shared__ uint4 stage[2][(4 * kRuns + 2 * kTiles) * kOperand];  // K [4 t][runs], then V [2 u][tiles]
   const int s = blockIdx.y, hkv = a.cache.hkv, group = a.hq / hkv;
-  const int split = blockIdx.x % splits, unit_of_grid = blockIdx.x / splits;
+  const int grid_tiles = gridDim.x / (splits * hkv);
+  const int grid_tile = blockIdx.x % grid_tiles, h = blockIdx.x / grid_tiles % hkv, split = blockIdx.x / grid_tiles / hkv;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int g = lane / 16, col = lane % 16;
   Kv8Span span;
@@ -403,29 +406,25 @@ __global__ __launch_bounds__(kRowsThreads, 2) void kv8_rows_kernel(Kv8AttnArgs a
     if (blockIdx.x == 0 && tid == 0) atomicOr(a.error, kKv8BadRows);
     return;
   }
-  const int total = span.n * group, h = unit_of_grid % hkv;
-  const int tiles = (total + kRowsTile - 1) / kRowsTile, tile = tiles - 1 - unit_of_grid / hkv;  // the longest first
+  const int total = span.n * group;
+  const int tiles = (total + kRowsTile - 1) / kRowsTile, tile = tiles - 1 - grid_tile;  // the longest first
   if (tile < 0) return;
   const int first = tile * kRowsTile;
   const int last_token = (min(first + kRowsTile, total) - 1) / group;
   const int pages = (span.context + last_token) / kKv8Page + 1;
-  const int begin = split * chunk, end = min(begin + chunk, pages);
-  if (begin >= end) return;
-  const int used = (pages + chunk - 1) / chunk;
+  const int used = splits_used(pages, chunk);
+  if (split >= used) return;
+  const int each = (pages + used - 1) / used, begin = split * each, end = min(begin + each, pages);
 
-  // This lane's rows, one a set.
-  const int wave_first = first + 16 * kSets * wave;
+  // This lane's row.
+  const int wave_first = first + 16 * wave;
   const bool works = wave_first < total;
   const int all_see = span.context + min(wave_first, total - 1) / group;
-  const int wave_last = span.context + (min(wave_first + 16 * kSets, total) - 1) / group;  // last key of any row
-  int limit[kSets];
-  int64_t row[kSets];
-#pragma unroll
-  for (int n = 0; n < kSets; ++n) {
-    const int m = wave_first + 16 * n + col, token = m < total ? m / group : 0;
-    limit[n] = m < total ? span.context + token : -1;
-    row[n] = (static_cast<int64_t>(span.first) + token) * a.hq + h * group + (m < total ? m % group : 0);
-  }
+  const int wave_last = span.context + (min(wave_first + 16, total) - 1) / group;  // last key of any row
+  const int m = wave_first + col, token = m < total ? m / group : 0;
+  const int limit = m < total ? span.context + token : -1;  // its last key
+  const int64_t row =
+      (static_cast<int64_t>(span.first) + token) * a.hq + h * group + (m < total ? m % group : 0);
 
   const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
   int numbers = table[min(begin + lane, a.cache.per_seq - 1)];
@@ -479,29 +478,27 @@ __global__ __launch_bounds__(kRowsThreads, 2) void kv8_rows_kernel(Kv8AttnArgs a
   };
   ask(begin);
 
-  f16x8 q_hi[kSets][kRuns], q_lo[kSets][kRuns];
-  float unit[kSets];
-  bool bad[kSets];
-#pragma unroll
-  for (int n = 0; n < kSets; ++n) {
+  f16x8 q_hi[kRuns], q_lo[kRuns];
+  float unit;        // of a score, in log2
+  bool bad = false;  // a query that is not finite gives a row of NaN
+  {
     float v[8 * kRuns];
 #pragma unroll
     for (int c = 0; c < kRuns; ++c)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         *reinterpret_cast<float4*>(v + 8 * c + 4 * i) =
-            *reinterpret_cast<const float4*>(a.query + row[n] * D + 32 * c + 8 * g + 4 * i);
+            *reinterpret_cast<const float4*>(a.query + row * D + 32 * c + 8 * g + 4 * i);
     float top = 0.0f;
-    bool broken = false;
 #pragma unroll
     for (int i = 0; i < 8 * kRuns; ++i) {
-      broken = broken || !(fabsf(v[i]) < __builtin_inff());
+      bad = bad || !(fabsf(v[i]) < __builtin_inff());
       top = fmaxf(top, fabsf(v[i]));
     }
     top = column_max(top);
-    bad[n] = column_max(broken ? 1.0f : 0.0f) > 0.0f;
+    bad = column_max(bad ? 1.0f : 0.0f) > 0.0f;
     int x = 0;
-    if (top > 0.0f && !bad[n]) (void)frexpf(top, &x);
+    if (top > 0.0f && !bad) (void)frexpf(top, &x);
     // The largest below 2^15: what is rounded off is under 2^-39 of it.
 #pragma unroll
     for (int c = 0; c < kRuns; ++c) {
@@ -509,153 +506,151 @@ __global__ __launch_bounds__(kRowsThreads, 2) void kv8_rows_kernel(Kv8AttnArgs a
       uint32_t *ph = &hi.x, *pl = &lo.x;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        split2(bad[n] ? 0.0f : ldexpf(v[8 * c + 2 * i], 15 - x), bad[n] ? 0.0f : ldexpf(v[8 * c + 2 * i + 1], 15 - x),
-               ph[i], pl[i]);
-      q_hi[n][c] = __builtin_bit_cast(f16x8, hi);
-      q_lo[n][c] = __builtin_bit_cast(f16x8, lo);
+        split2(bad ? 0.0f : ldexpf(v[8 * c + 2 * i], 15 - x), bad ? 0.0f : ldexpf(v[8 * c + 2 * i + 1], 15 - x), ph[i],
+               pl[i]);
+      q_hi[c] = __builtin_bit_cast(f16x8, hi);
+      q_lo[c] = __builtin_bit_cast(f16x8, lo);
     }
-    unit[n] = ldexpf(1.4426950408889634f / sqrtf(static_cast<float>(D)), x - 15);
+    unit = ldexpf(1.4426950408889634f / sqrtf(static_cast<float>(D)), x - 15);
   }
 
-  f32x4 out[kSets][kTiles] = {};
-  float ref[kSets], l[kSets];
-#pragma unroll
-  for (int n = 0; n < kSets; ++n) ref[n] = kNoRow, l[n] = 0.0f;
+  f32x4 out[kTiles] = {};
+  float ref = kNoRow, l = 0.0f;
   int held_exp = kKv8MinExp - 1;
   put(stage[0]);
+  if (!works) {  // rows past the last: this wave only helps with the pages
+    for (int p = begin; p < end; ++p) {
+      if (next_hidden && tid == 0) atomicOr(a.error, kKv8BadRows);
+      __syncthreads();
+      if (p + 1 < end) {
+        ask(p + 1);
+        put(stage[(p + 1 - begin) % 2]);
+      }
+    }
+    return;
+  }
+  // No branch around the loop's sums, of which the compiler would keep copies:
+  // a page that no row sees, the last of a tile for some waves or one with a
+  // bad number, has all its keys masked.
   for (int p = begin; p < end; ++p) {
     const uint4* now = stage[(p - begin) % 2];
     const uint32_t key_exps = next_key_exps, value_exps = next_value_exps;
     const bool hidden = next_hidden;
+    if (hidden && tid == 0) atomicOr(a.error, kKv8BadRows);
     __syncthreads();  // this page is in LDS, and every wave is done with the one before
     if (p + 1 < end) ask(p + 1);
-    if (works && p * kKv8Page <= wave_last && !hidden) {
-      const int blocks = min(kKv8Blocks, (wave_last - p * kKv8Page) / kKv8Block + 1);
+    {
+      const int blocks = hidden ? 0 : min(kKv8Blocks, (wave_last - p * kKv8Page + kKv8Block) / kKv8Block);
       int page_exp = kKv8MinExp - 1;
 #pragma unroll
       for (int b = 0; b < kKv8Blocks; ++b)
         if (b < blocks) page_exp = max(page_exp, static_cast<int>(static_cast<int8_t>(value_exps >> (8 * b))));
-      f32x4 score[kSets][4];
+      // Two sums at a time: a sum's products wait for each other.
+      f32x4 score[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        f16x8 kf[kRuns];
+      for (int t = 0; t < 4; t += 2) {
+        f16x8 kf[2][kRuns];
 #pragma unroll
-        for (int c = 0; c < kRuns; ++c)
-          kf[c] = __builtin_bit_cast(f16x8, now[(t * kRuns + c) * kOperand + (lane ^ key_place(t * kRuns + c, g))]);
+        for (int w = 0; w < 2; ++w) {
+          score[t + w] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int n = 0; n < kSets; ++n) {
-          f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int c = 0; c < kRuns; ++c)
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[c], q_lo[n][c], acc, 0, 0, 0);
-#pragma unroll
-          for (int c = 0; c < kRuns; ++c)
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[c], q_hi[n][c], acc, 0, 0, 0);
-          score[n][t] = acc;
+          for (int c = 0; c < kRuns; ++c) {
+            const int o = (t + w) * kRuns + c;
+            kf[w][c] = __builtin_bit_cast(f16x8, now[o * kOperand + (lane ^ key_place(o, g))]);
+          }
         }
+#pragma unroll
+        for (int c = 0; c < 2 * kRuns; ++c)
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+            score[t + w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                kf[w][c % kRuns], c < kRuns ? q_lo[c % kRuns] : q_hi[c % kRuns], score[t + w], 0, 0, 0);
       }
       const int shift = 8 * (g / 2);  // of this lane's block of each half page
       const float key_scale[2] = {ldexpf(1.0f, static_cast<int8_t>(key_exps >> shift)),
                                   ldexpf(1.0f, static_cast<int8_t>(key_exps >> (16 + shift)))};
-      const bool edge = p * kKv8Page + kKv8Page - 1 > all_see;
-      float to_log2[kSets][2], page_top[kSets];
-      bool rises = page_exp > held_exp;
+      float to_log2[2] = {unit * key_scale[0], unit * key_scale[1]};
+      if (hidden || p * kKv8Page + kKv8Page - 1 > all_see) {
+        // Scaled first: a factor may be 0 or, of a block that holds anything, infinite.
 #pragma unroll
-      for (int n = 0; n < kSets; ++n) {
-        to_log2[n][0] = unit[n] * key_scale[0];
-        to_log2[n][1] = unit[n] * key_scale[1];
-        if (edge) {
-          // Scaled first: a factor may be 0 or, of a block that holds anything, infinite.
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              score[n][t][i] = p * kKv8Page + 32 * (t / 2) + 8 * g + 4 * (t % 2) + i > limit[n]
-                                   ? -INFINITY
-                                   : score[n][t][i] * to_log2[n][t / 2];
-          to_log2[n][0] = to_log2[n][1] = 1.0f;
-        }
-        float top[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          top[u] = -INFINITY;
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top[u] = fmaxf(top[u], score[n][2 * u + w][i]);
-        }
-        page_top[n] = fmaxf(top[0] * to_log2[n][0], top[1] * to_log2[n][1]);
-        rises = rises || page_top[n] > ref[n] + kLead;
+          for (int i = 0; i < 4; ++i)
+            score[t][i] = hidden || p * kKv8Page + 32 * (t / 2) + 8 * g + 4 * (t % 2) + i > limit
+                              ? -INFINITY
+                              : score[t][i] * to_log2[t / 2];
+        to_log2[0] = to_log2[1] = 1.0f;
       }
-      if (__any(rises)) {
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[t / 2] = fmaxf(top[t / 2], score[t][i]);
+      const float page_top = fmaxf(top[0] * to_log2[0], top[1] * to_log2[1]);
+      if (__any(page_top > ref + kLead) || page_exp > held_exp) {
+        const float next = fmaxf(ref, column_max(page_top));
         const int next_exp = max(held_exp, page_exp);
+        const float f = __builtin_amdgcn_exp2f(ref - next), down = ldexpf(f, held_exp - next_exp);
+        l *= f;
 #pragma unroll
-        for (int n = 0; n < kSets; ++n) {
-          const float next = fmaxf(ref[n], column_max(page_top[n]));
-          const float f = __builtin_amdgcn_exp2f(ref[n] - next);
-          l[n] *= f;
-          const float fo = ldexpf(f, held_exp - next_exp);
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) out[n][t] *= fo;
-          ref[n] = next;
-        }
+        for (int t = 0; t < kTiles; ++t) out[t] *= down;
+        ref = next;
         held_exp = next_exp;
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
+        // The value block's factor goes into the exponent.  Below 2^-60 of the
+        // largest block it no longer falls: what it weighs is nothing in fp16.
         const int my_exp = static_cast<int8_t>(value_exps >> (16 * u + shift));
-        const float f = ldexpf(1.0f, min(my_exp - held_exp, 0) + kRowsPBits);
-        f16x8 p_hi[kSets], p_lo[kSets];
+        const int bias = min(max(my_exp - held_exp, -60), 0) + kRowsPBits;
+        const float from = static_cast<float>(bias) - ref;
+        float part = 0.0f;
+        uint4 hi, lo;
+        uint32_t *ph = &hi.x, *pl = &lo.x;
 #pragma unroll
-        for (int n = 0; n < kSets; ++n) {
-          uint4 hi, lo;
-          uint32_t *ph = &hi.x, *pl = &lo.x;
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(fmaf(score[2 * u + w][i], to_log2[u], from));
+            const float e1 = __builtin_amdgcn_exp2f(fmaf(score[2 * u + w][i + 1], to_log2[u], from));
+            part += e0;
+            part += e1;
+            split2_truncated(e0, e1, ph[2 * w + i / 2], pl[2 * w + i / 2]);
+          }
+        l = fmaf(part, ldexpf(1.0f, -bias), l);
+        const f16x8 p_hi = __builtin_bit_cast(f16x8, hi), p_lo = __builtin_bit_cast(f16x8, lo);
+#pragma unroll
+        for (int t = 0; t < kTiles; t += 2) {
+          f16x8 vf[2];
 #pragma unroll
           for (int w = 0; w < 2; ++w)
+            vf[w] = __builtin_bit_cast(
+                f16x8, now[(4 * kRuns + u * kTiles + t + w) * kOperand + (lane ^ value_place(u, g))]);
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-              const float e0 = __builtin_amdgcn_exp2f(fmaf(score[n][2 * u + w][i], to_log2[n][u], -ref[n]));
-              const float e1 = __builtin_amdgcn_exp2f(fmaf(score[n][2 * u + w][i + 1], to_log2[n][u], -ref[n]));
-              l[n] += e0;
-              l[n] += e1;
-              split2_scaled(e0, e1, f, ph[2 * w + i / 2], pl[2 * w + i / 2]);
-            }
-          p_hi[n] = __builtin_bit_cast(f16x8, hi);
-          p_lo[n] = __builtin_bit_cast(f16x8, lo);
-        }
+          for (int w = 0; w < 2; ++w)
+            out[t + w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[w], p_lo, out[t + w], 0, 0, 0);
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          const f16x8 vf = __builtin_bit_cast(
-              f16x8, now[(4 * kRuns + u * kTiles + t) * kOperand + (lane ^ value_place(u, g))]);
-#pragma unroll
-          for (int n = 0; n < kSets; ++n) {
-            out[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p_lo[n], out[n][t], 0, 0, 0);
-            out[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p_hi[n], out[n][t], 0, 0, 0);
-          }
+          for (int w = 0; w < 2; ++w)
+            out[t + w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[w], p_hi, out[t + w], 0, 0, 0);
         }
       }
-    } else if (hidden && tid == 0) {
-      atomicOr(a.error, kKv8BadRows);
     }
     if (p + 1 < end) put(stage[(p + 1 - begin) % 2]);
   }
+  l = column_sum(l);
+  if (bad) l = __builtin_nanf("");
+  if (m >= total) return;
+  const float inv = used > 1 ? 1.0f : l != 0.0f ? 1.0f / l : 0.0f;
+  float* to = used > 1 ? a.part + (row * splits + split) * D : a.out + row * D;
 #pragma unroll
-  for (int n = 0; n < kSets; ++n) {
-    float total_l = column_sum(l[n]);
-    if (bad[n]) total_l = __builtin_nanf("");
-    if (limit[n] < 0) continue;
-    const float inv = used > 1 ? 1.0f : total_l != 0.0f ? 1.0f / total_l : 0.0f;
-    float* to = used > 1 ? a.part + (row[n] * splits + split) * D : a.out + row[n] * D;
+  for (int t = 0; t < kTiles; ++t) {
+    float4 o;
+    float* po = &o.x;
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      float4 o;
-      float* po = &o.x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) po[i] = ldexpf(out[n][t][i], held_exp - kRowsPBits) * inv;
-      *reinterpret_cast<float4*>(to + 16 * t + 4 * g) = o;
-    }
-    if (used > 1 && g == 0) store_ml(a, row[n], splits, split, D, ref[n], total_l);
+    for (int i = 0; i < 4; ++i) po[i] = ldexpf(out[t][i], held_exp - kRowsPBits) * inv;
+    *reinterpret_cast<float4*>(to + 16 * t + 4 * g) = o;
   }
+  if (used > 1 && g == 0) store_ml(a, row, splits, split, D, ref, l);
 }
 
 // Splits of row `i` of a sequence's (token, head) rows.
@@ -664,7 +659,7 @@ __device__ __forceinline__ int splits_of(const Kv8AttnArgs& a, const Kv8Span& sp
   const int m = token * group + head % group;
   const int tile_end = min((m / tile_rows + 1) * tile_rows, span.n * group);
   const int pages = (span.context + (tile_end - 1) / group) / kKv8Page + 1;
-  return (pages + chunk - 1) / chunk;
+  return splits_used(pages, chunk);
 }
 
 // Joins a few splits of many rows: d / 4 threads a (token, head).
@@ -761,19 +756,25 @@ __global__ __launch_bounds__(kAttnThreads) void kv8_combine_kernel(Kv8AttnArgs a
 //   tokens (8.9 split over four), while at 2,000 the split wins (9.1, 11.4);
 //   more take kStepBlocks blocks in all (32 sequences of up to 4,000 tokens
 //   15.3; with 512 blocks 15.9, with 128 18.5) and at most kMostSplits splits
-//   (one sequence of 32,768: 64 splits 13.5, 128 14.5).
-// Prompts: blocks that all run at once, two a compute unit.
+//   (one sequence of 32,768: 64 splits 13.5, 128 14.5);
+//   many rows take kRowsBlocks blocks, whose tiles see different numbers of
+//   keys (3,000 rows after 1,111: 80; with 768 blocks 87, 256 104), but at most
+//   kFewSplits splits, whose join is cheap, unless there are few rows (512 rows
+//   after 2,000: 24 with 8 splits, 32 with 16).
 Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens) {
   Kv8AttnPlan p;
   const int64_t most = static_cast<int64_t>(hq / hkv) * max_rows;
   const int64_t pages = (max_tokens + kKv8Page - 1) / kKv8Page;
   p.tile_rows = most <= 4 ? 4 : kRowsTile;
+  const bool step = p.tile_rows == 4;
   const int64_t blocks = (most + p.tile_rows - 1) / p.tile_rows * hkv * seqs;
-  const int64_t wanted = p.tile_rows == 4 ? kStepBlocks : kRowsBlocks;
+  const int64_t wanted = step ? kStepBlocks : kRowsBlocks;
+  const int64_t splits = step || static_cast<int64_t>(rows) * hq <= kFewRows ? kMostSplits : kFewSplits;
+  // Of a prompt's tiles, the first sees the context and the last all of max_tokens.
+  const int64_t mean = step ? pages : std::max<int64_t>(1, (2 * max_tokens - max_rows) / (2 * kKv8Page));
   int64_t chunk = pages;
-  if (blocks < wanted && !(p.tile_rows == 4 && pages <= kWidePages))
-    chunk = std::max<int64_t>(
-        {kAttnWaves, (pages * blocks + wanted - 1) / wanted, (pages + kMostSplits - 1) / kMostSplits});
+  if (blocks < wanted && !(step && pages <= kWidePages))
+    chunk = std::max<int64_t>({kAttnWaves, (mean * blocks + wanted - 1) / wanted, (pages + splits - 1) / splits});
   p.chunk_pages = static_cast<int>(chunk);
   p.splits = static_cast<int>((pages + chunk - 1) / chunk);
   if (p.splits > 1) p.partial_floats = static_cast<int64_t>(rows) * hq * p.splits * (d + 2);
