@@ -32,17 +32,17 @@ namespace {
 
 constexpr int kAppendThreads = 256;
 
+template <int kCtrl>
+__device__ __forceinline__ double dpp_move_double(double v) {
+  return __hiloint2double(dpp_move_int<kCtrl>(__double2hiint(v)), dpp_move_int<kCtrl>(__double2loint(v)));
+}
 __device__ __forceinline__ double quad_sum(double v) {
-  v += __shfl_xor(v, 1);
-  v += __shfl_xor(v, 2);
-  return v;
+  v += dpp_move_double<dpp::kQuadXor1>(v);
+  return v + dpp_move_double<dpp::kQuadXor2>(v);
 }
 
-__device__ __forceinline__ int wave_max(int v) {
-#pragma unroll
-  for (int m = 1; m < kWave; m *= 2) v = max(v, __shfl_xor(v, m));
-  return v;
-}
+// Of small whole numbers.
+__device__ __forceinline__ int wave_max(int v) { return static_cast<int>(group_max<kWave>(static_cast<float>(v))); }
 
 // 2^n for |n| <= 1000.
 __device__ __forceinline__ double pow2(int n) { return __longlong_as_double(static_cast<long long>(1023 + n) << 52); }

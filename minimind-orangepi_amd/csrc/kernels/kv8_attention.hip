@@ -40,9 +40,8 @@ namespace mmr {
 
 namespace {
 
-constexpr int kAttnWaves = 4;
-constexpr int kAttnThreads = kAttnWaves * kWave;
-constexpr int kWideWaves = 8;  // of a block that takes a short context without a split
+constexpr int kStepWaves = 8, kStepThreads = kStepWaves * kWave;
+constexpr int kJoinWaves = 4, kJoinThreads = kJoinWaves * kWave;
 constexpr float kNoRow = -FLT_MAX / 2;  // reference of a row that has met no key
 constexpr float kLead = 5.0f;           // a score may pass the reference by 2^kLead
 constexpr int kRowsThreads = 256;
@@ -50,7 +49,7 @@ constexpr int kFewSplits = 8;
 constexpr int kRowsTile = 64;          // rows of a block of the kernel for many
 constexpr int kRowsPBits = 10;          // its p in units of 2^-10: at most 2^15 with the lead
 constexpr int kPBits = 25;              // p in units of 2^-25: at most 2^30 with the lead
-constexpr int kWidePages = 16, kStepBlocks = 256, kRowsBlocks = 1280, kFewRows = 256;  // see kv8_attention_plan
+constexpr int kLeastPages = 4, kWidePages = 16, kStepBlocks = 256, kRowsBlocks = 1280, kFewRows = 256;  // see kv8_attention_plan
 constexpr int kMostSplits = 64;  // at most one a thread of the combine
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 using f32x4 = float __attribute__((ext_vector_type(4)));
@@ -119,13 +118,18 @@ __device__ __forceinline__ void store_ml(const Kv8AttnArgs& a, int64_t row, int 
 }
 
 // Waves take the pages of a split in turn and join their results at the end.
-template <int D, int kWaves>
-__global__ __launch_bounds__(kWaves* kWave, 2) void kv8_step_kernel(Kv8AttnArgs a, int chunk, int splits) {
+template <int D>
+__global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a, int chunk, int splits) {
   constexpr int kRows = 4, kTiles = D / 16;  // tiles of the output's dimensions
   const int s = blockIdx.y, hkv = a.cache.hkv, group = a.hq / hkv;
   const int split = blockIdx.x % splits, h = blockIdx.x / splits;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int g = lane / 16, col = lane % 16;
+  // Page numbers of this wave's next 64 steps, one a lane: read along with the
+  // offsets, not after them.
+  const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
+  const int begin = split * chunk, from = begin + wave;
+  int numbers = table[min(from + kStepWaves * lane, a.cache.per_seq - 1)];
   Kv8Span span;
   const bool fine = kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span);
   if (!fine || (span.n > 0 && static_cast<int64_t>(span.context) + span.n > a.max_tokens)) {
@@ -135,14 +139,8 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void kv8_step_kernel(Kv8AttnArgs 
   const int total = span.n * group;  // rows of this group of heads
   if (total == 0) return;
   const int pages = (span.context + span.n - 1) / kKv8Page + 1;
-  const int used = splits_used(pages, chunk);
+  const int used = splits_used(pages, chunk), end = min(begin + chunk, pages);
   if (split >= used) return;
-  const int each = (pages + used - 1) / used, begin = split * each, end = min(begin + each, pages);
-
-  // Page numbers of this wave's next 64 steps, one a lane.
-  const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
-  const int from = begin + wave;
-  int numbers = table[min(from + kWaves * lane, a.cache.per_seq - 1)];
 
   // This lane's column: digit `digit` of row m.
   const int m = col / 4, digit = col % 4;
@@ -160,8 +158,8 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void kv8_step_kernel(Kv8AttnArgs 
   const int8_t *next_k, *next_v;
   int ask_at = 0;
   auto ask = [&]() {  // addresses and exponents of step ask_at, at most the last
-    const int step = min(ask_at, (end - 1 - from) / kWaves);
-    if (ask_at > 0 && step % kWave == 0) numbers = table[min(from + kWaves * (step + lane), a.cache.per_seq - 1)];
+    const int step = min(ask_at, (end - 1 - from) / kStepWaves);
+    if (ask_at > 0 && step % kWave == 0) numbers = table[min(from + kStepWaves * (step + lane), a.cache.per_seq - 1)];
     ++ask_at;
     const int number = __builtin_amdgcn_readlane(numbers, step % kWave);
     next_hidden = number < 0 || number >= a.cache.pages;
@@ -252,7 +250,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void kv8_step_kernel(Kv8AttnArgs 
     since = 0;
   };
 
-  for (int p = from; p < end; p += kWaves) {
+  for (int p = from; p < end; p += kStepWaves) {
     const uint32_t key_exps = next_key_exps, value_exps = next_value_exps;
     const bool hidden = next_hidden;
     // Blocks past the last key hold anything: their exponents don't count.
@@ -294,7 +292,7 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void kv8_step_kernel(Kv8AttnArgs 
 
     if (__any(top > ref + kLead) || page_exp > held_exp || since == kMostPages) {
       const float next = fmaxf(ref, column_max(top));
-      move(__builtin_amdgcn_exp2f(ref - next));
+      if (since > 0) move(__builtin_amdgcn_exp2f(ref - next));  // not before the first page
       ref = next;
       held_exp = max(held_exp, page_exp);
     }
@@ -326,8 +324,8 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void kv8_step_kernel(Kv8AttnArgs 
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[t][i] = quad_add(out[t][i]);
 
-  __shared__ float sh_ref[kWaves][kRows], sh_l[kWaves][kRows];
-  __shared__ __align__(16) float sh_out[kWaves][kRows][D];
+  __shared__ float sh_ref[kStepWaves][kRows], sh_l[kStepWaves][kRows];
+  __shared__ __align__(16) float sh_out[kStepWaves][kRows][D];
   if (digit == 0) {
     if (g == 0) {
       sh_ref[wave][m] = ref;
@@ -339,14 +337,14 @@ __global__ __launch_bounds__(kWaves* kWave, 2) void kv8_step_kernel(Kv8AttnArgs 
           make_float4(out[t][0], out[t][1], out[t][2], out[t][3]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < total * D; i += kWaves * kWave) {
+  for (int i = threadIdx.x; i < total * D; i += kStepThreads) {
     const int mr = i / D, dim = i - mr * D;
     float top = sh_ref[0][mr];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sh_ref[w][mr]);
+    for (int w = 1; w < kStepWaves; ++w) top = fmaxf(top, sh_ref[w][mr]);
     float o = 0.0f, ll = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kStepWaves; ++w) {
       const float f = __builtin_amdgcn_exp2f(sh_ref[w][mr] - top);
       o += f * sh_out[w][mr][dim];
       ll += f * sh_l[w][mr];
@@ -663,9 +661,9 @@ __device__ __forceinline__ int splits_of(const Kv8AttnArgs& a, const Kv8Span& sp
 }
 
 // Joins a few splits of many rows: d / 4 threads a (token, head).
-__global__ __launch_bounds__(kAttnThreads) void kv8_combine_few_kernel(Kv8AttnArgs a, int chunk, int splits,
+__global__ __launch_bounds__(kJoinThreads) void kv8_combine_few_kernel(Kv8AttnArgs a, int chunk, int splits,
                                                                        int tile_rows) {
-  const int s = blockIdx.y, d = a.cache.d, quads = d / 4, each = kAttnThreads / quads;
+  const int s = blockIdx.y, d = a.cache.d, quads = d / 4, each = kJoinThreads / quads;
   Kv8Span span;
   if (!kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span)) return;
   if (static_cast<int64_t>(span.context) + span.n > a.max_tokens) return;
@@ -699,11 +697,11 @@ __global__ __launch_bounds__(kAttnThreads) void kv8_combine_few_kernel(Kv8AttnAr
 
 // Joins many splits, a block per (token, head): weights first, a split a thread, then groups of d / 4 threads take
 // splits in turn, four dimensions each.
-__global__ __launch_bounds__(kAttnThreads) void kv8_combine_kernel(Kv8AttnArgs a, int chunk, int splits,
+__global__ __launch_bounds__(kJoinThreads) void kv8_combine_kernel(Kv8AttnArgs a, int chunk, int splits,
                                                                    int tile_rows) {
-  __shared__ float weight[kMostSplits], shared_top[kAttnWaves], shared_l[kAttnWaves];
-  __shared__ float4 shared_out[kAttnThreads];
-  const int s = blockIdx.y, d = a.cache.d, quads = d / 4, groups = kAttnThreads / quads;
+  __shared__ float weight[kMostSplits], shared_top[kJoinWaves], shared_l[kJoinWaves];
+  __shared__ float4 shared_out[kJoinThreads];
+  const int s = blockIdx.y, d = a.cache.d, quads = d / 4, groups = kJoinThreads / quads;
   Kv8Span span;
   if (!kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span)) return;
   if (static_cast<int64_t>(span.context) + span.n > a.max_tokens) return;
@@ -774,7 +772,7 @@ Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int m
   const int64_t mean = step ? pages : std::max<int64_t>(1, (2 * max_tokens - max_rows) / (2 * kKv8Page));
   int64_t chunk = pages;
   if (blocks < wanted && !(step && pages <= kWidePages))
-    chunk = std::max<int64_t>({kAttnWaves, (mean * blocks + wanted - 1) / wanted, (pages + splits - 1) / splits});
+    chunk = std::max<int64_t>({kLeastPages, (mean * blocks + wanted - 1) / wanted, (pages + splits - 1) / splits});
   p.chunk_pages = static_cast<int>(chunk);
   p.splits = static_cast<int>((pages + chunk - 1) / chunk);
   if (p.splits > 1) p.partial_floats = static_cast<int64_t>(rows) * hq * p.splits * (d + 2);
@@ -789,16 +787,14 @@ void launch_attention_for(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_
   const dim3 grid(p.splits * ((most + p.tile_rows - 1) / p.tile_rows) * hkv, a.cache.seqs);
   if (p.tile_rows != 4)
     kv8_rows_kernel<D><<<grid, kRowsThreads, 0, stream>>>(a, p.chunk_pages, p.splits);
-  else if (p.splits == 1)
-    kv8_step_kernel<D, kWideWaves><<<grid, kWideWaves * kWave, 0, stream>>>(a, p.chunk_pages, p.splits);
   else
-    kv8_step_kernel<D, kAttnWaves><<<grid, kAttnThreads, 0, stream>>>(a, p.chunk_pages, p.splits);
+    kv8_step_kernel<D><<<grid, kStepThreads, 0, stream>>>(a, p.chunk_pages, p.splits);
   if (p.splits > 1 && p.splits <= kFewSplits) {
-    const int each = kAttnThreads / (D / 4);
-    kv8_combine_few_kernel<<<dim3((a.max_rows * a.hq + each - 1) / each, a.cache.seqs), kAttnThreads, 0, stream>>>(
+    const int each = kJoinThreads / (D / 4);
+    kv8_combine_few_kernel<<<dim3((a.max_rows * a.hq + each - 1) / each, a.cache.seqs), kJoinThreads, 0, stream>>>(
         a, p.chunk_pages, p.splits, p.tile_rows);
   } else if (p.splits > 1)
-    kv8_combine_kernel<<<dim3(a.max_rows * a.hq, a.cache.seqs), kAttnThreads, 0, stream>>>(a, p.chunk_pages, p.splits,
+    kv8_combine_kernel<<<dim3(a.max_rows * a.hq, a.cache.seqs), kJoinThreads, 0, stream>>>(a, p.chunk_pages, p.splits,
                                                                                          p.tile_rows);
 }
 
