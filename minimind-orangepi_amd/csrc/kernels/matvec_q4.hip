@@ -27,17 +27,27 @@ namespace {
 
 constexpr int kQ4Waves = 8;
 constexpr int kQ4Threads = kQ4Waves * kWave;
-constexpr int kQ4Tile = 16;       // weight rows of a product
-constexpr int kQ4Batch = 4;       // batch rows of an x operand
-constexpr int kQ4Operands = 2048; // bytes of the two x operands of a run
-constexpr int kFusedCols = 8192;  // batch x cols that a block itself turns into digits
-constexpr int kManyTiles = 4;     // x operands of a block whose digits come from the workspace
-constexpr int kAhead = 4;              // runs of a wave that are asked for together
-constexpr int kWideWaves = 16;         // of a block that takes many tiles
-constexpr int kWideThreads = kWideWaves * kWave;
-constexpr int kManyRowTiles = 1024;    // tiles from which that form is taken
-constexpr int kWideBlocks = 256;       // and its blocks: one a compute unit
-constexpr int kWideTiles = 512;        // tiles from which a block of the other form takes two
+constexpr int kQ4Tile = 16;        // weight rows of a product
+constexpr int kQ4Batch = 4;        // batch rows of an x operand
+constexpr int kQ4Operands = 2048;  // bytes of the two x operands of a run
+// batch x cols that a block itself turns into digits, of up to kQ4Batch rows:
+// more of them cost a second launch less (768 x 2048 for 4 rows 9.2 us here and
+// 8.6 in two launches, 4096 x 2048 9.6 and 10.5; replayed graphs).
+constexpr int kFusedCols = 8192;
+// Tiles of rows from which blocks take several in turn, so that x is turned
+// into digits once a compute unit (8192 x 4096 in groups of 32: 11.7 us with a
+// tile a block, 9.4; 4096 x 768 with 256 tiles 4.2 and 4.9).
+constexpr int kManyRowTiles = 512;
+constexpr int kWideBlocks = 256;    // then: one a compute unit
+constexpr int kManyWaves = 2048;    // and its waves
+constexpr int kAhead = 4;           // runs of a chunk of them
+constexpr int kRing = 3;            // chunks of a wave under way
+constexpr int kCodeBytes = 4096;    // of a chunk of 16 rows
+constexpr int kChunkBytes = kCodeBytes + 512;  // with their scales
+constexpr int kManyTiles = 4;       // x operands of a block whose digits come from the workspace
+// Tiles from which such a block takes two and reads the operands for both
+// (4096 x 768 for 32 rows: 6.8 us with one, 6.4; 768 x 2048 8.4 and 9.9).
+constexpr int kTwoTiles = 256;
 
 using i32x4 = int __attribute__((ext_vector_type(4)));
 
@@ -46,8 +56,9 @@ struct Q4Form {
   GemvPrologue pro;
   GemvEpilogue epi;
   int runs, groups;
-  bool whole;   // the scales of a run are one load: every run is whole, and they are aligned
-  bool joined;  // those of kAhead runs are 8- or 16-byte loads
+  bool whole;  // the scales of a run are one load: every run is whole, and they are aligned
+  bool even;   // then: a row has an even number of groups
+  int share;   // waves of the form for many tiles that share a tile's columns
 };
 
 __device__ __forceinline__ float normalised(const Q4Form& f, float x, float w, float scale) {
@@ -69,9 +80,10 @@ __device__ __forceinline__ Columns load_columns(const MatvecQ4Args& a, const Q4F
   return v;
 }
 
-// Digits of a run of row b of an x operand, by one wave.  to: [2 halves][rows]
-// [4 parts][16 bytes], half j / 2, part p and bytes 8 (j % 2) + i / 2 (even
-// columns) or + 4 (odd ones) for column 32 j + 8 p + i.  Returns the power of
+// Digits of a run of row b of an x operand, by one wave.  to: [2 halves][4 parts]
+// [rows][16 bytes] (16 rows: in the order of the lanes that read them), half
+// j / 2, part p and bytes 8 (j % 2) + i / 2 (even columns) or + 4 (odd ones)
+// for column 32 j + 8 p + i.  Returns the power of
 // two that the products come in, NaN if a value is not finite.
 __device__ __forceinline__ float write_digits(const float v[2], int b, int rows, int8_t* to) {
   const int lane = threadIdx.x % kWave;
@@ -81,13 +93,13 @@ __device__ __forceinline__ float write_digits(const float v[2], int b, int rows,
   (void)frexpf(bad ? 0.0f : top, &e);
   e = max(e, -90);
   const int j = lane / 32, p = lane % 32 / 8, i = lane % 8;
-  int8_t* at = to + (kQ4Batch * b * 4 + p) * 16 + j * 8 + i % 2 * 4 + i / 2;
+  int8_t* at = to + (p * rows + kQ4Batch * b) * 16 + j * 8 + i % 2 * 4 + i / 2;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const uint32_t n = static_cast<uint32_t>(bad ? 0 : static_cast<int>(rintf(ldexpf(v[k], 30 - e)))) + 0x808080u;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
-      at[(k * rows + d) * 64] = static_cast<int8_t>((n >> (8 * d)) ^ (d < 3 ? 0x80u : 0u));
+      at[(k * 4 * rows + d) * 16] = static_cast<int8_t>((n >> (8 * d)) ^ (d < 3 ? 0x80u : 0u));
   }
   return bad ? __builtin_nanf("") : ldexpf(1.0f, e - 34);  // the weights come as 16 q
 }
@@ -203,7 +215,7 @@ __device__ __forceinline__ void load_x(const MatvecQ4Args& a, const Q4Form& f, i
     if (u < f.runs * a.batch) v[i] = load_columns(a, f, u / f.runs, u % f.runs);
   }
 }
-// Returns whether a value is not finite.  to: [runs][2][4 batch][4 parts][16].
+// Returns whether a value is not finite.  to: [runs][2][4 parts][4 batch][16].
 template <int kUnits, int kWaves>
 __device__ __forceinline__ bool make_digits(const MatvecQ4Args& a, const Q4Form& f, int wave, const Columns v[kUnits],
                                             Digits<kUnits, kWaves>& d, int8_t* to) {
@@ -286,7 +298,7 @@ __global__ __launch_bounds__(kQ4Threads) void matvec_q4_kernel(MatvecQ4Args a, Q
   load_x<kUnits, kQ4Waves>(a, f, wave, v);
   const bool broken = make_digits<kUnits, kQ4Waves>(a, f, wave, v, d, digits);
   const int rows = kQ4Batch * a.batch, b = min(g, a.batch - 1);
-  const int8_t* const operand = digits + (min(col, rows - 1) * 4 + g) * 16;
+  const int8_t* const operand = digits + (g * rows + min(col, rows - 1)) * 16;
   float y = 0.0f;
   for (int first = wave; first < f.runs; first += kTogether * kQ4Waves) {
 #pragma unroll
@@ -303,86 +315,117 @@ __global__ __launch_bounds__(kQ4Threads) void matvec_q4_kernel(MatvecQ4Args a, Q
   finish_checked(a, f, d, broken, y, row);
 }
 
-// Many tiles: two waves a tile, eight tiles of a block at a time, kRing chunks
-// of kAhead runs of a wave under way.
+// Many tiles: a block takes kQ4Waves / f.share of them at a time, and then
+// further ones; f.share waves share a tile's columns, a chunk of kAhead runs
+// each in turn.  For whole runs with an even number of groups in a row.
+//
+// A lane of a product needs 16 bytes of its own weight row, and a load that
+// goes by that asks for 64 places a row apart, one a cycle.  So a chunk's codes
+// go to LDS with direct loads, 256 bytes of four rows each, and its scales four
+// bytes a lane, kRing chunks of a wave under way; pieces of 16 bytes change
+// places within a row by its number, so that lanes that read the same piece of
+// 16 rows use all banks.  The waits are counted by hand: all that a wave has
+// under way are its chunks, kChunkLoads loads each, which return in order.
+template <int kLoads>
+__device__ __forceinline__ void wait_for_chunk(int later) {  // while `later` chunks after it are under way
+  static_assert(kRing == 3, "one wait for each number of later chunks");
+  if (later >= 2)
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * kLoads) : "memory");
+  else if (later == 1)
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kLoads) : "memory");
+  else
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+}
+
 template <int kGroup, int kUnits>
-__global__ __launch_bounds__(kWideThreads) void matvec_q4_wide_kernel(MatvecQ4Args a, Q4Form f) {
-  extern __shared__ __align__(16) int8_t digits[];
-  __shared__ Digits<kUnits, kWideWaves> d;
-  __shared__ float sums[2][kWideWaves / 2][kWave];
-  constexpr int kGroups = Run<kGroup>::kGroups, kRing = kGroup == 32 ? 2 : kGroup == 64 ? 3 : 4, kTiles = kWideWaves / 2;
+__global__ __launch_bounds__(kQ4Threads) void matvec_q4_wide_kernel(MatvecQ4Args a, Q4Form f) {
+  extern __shared__ __align__(16) int8_t shared[];  // chunks [waves][kRing][codes, scales], then digits
+  __shared__ Digits<kUnits, kQ4Waves> d;
+  __shared__ float sums[2][kQ4Waves][kWave];
+  constexpr int kGroups = Run<kGroup>::kGroups;
+  constexpr int kWords = kAhead * kGroups / 2;            // of a row's scales in a chunk
+  constexpr int kScaleLoads = (16 * kWords + kWave - 1) / kWave, kChunkLoads = kAhead + kScaleLoads;
+  int8_t* const digits = shared + kQ4Waves * kRing * kChunkBytes;
   const int lane = threadIdx.x % kWave, g = lane / 16, col = lane % 16;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), slot = wave / 2, half = wave % 2;
-  const int tiles = (a.rows + kQ4Tile - 1) / kQ4Tile, stride = gridDim.x * kTiles;
-  const int steps = (f.runs + 2 * kAhead - 1) / (2 * kAhead);  // chunks of a wave and tile
-  int ask_tile = blockIdx.x * kTiles + slot, ask_step = 0;
-  Run<kGroup> ring[kRing][kAhead];
-  auto ask = [&](Run<kGroup>* to) {  // what is past the last is read as the last, and not used
-    const int64_t row = min(min(ask_tile, tiles - 1) * kQ4Tile + col, a.rows - 1);
-    const int first = (2 * ask_step + half) * kAhead;
-    const uint8_t* codes = a.codes + row * f.runs * 64 + 16 * g;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int at_once = kQ4Waves / f.share, part = wave % f.share, slot = wave / f.share;
+  const int tiles = (a.rows + kQ4Tile - 1) / kQ4Tile, stride = gridDim.x * at_once, row_bytes = f.runs * 64;
+  const int turns = (tiles - static_cast<int>(blockIdx.x) * at_once + stride - 1) / stride;  // of this block
+  const int chunks = (f.runs + kAhead - 1) / kAhead, steps = (chunks + f.share - 1) / f.share;
+  int8_t* const ring = shared + wave * kRing * kChunkBytes;
+  const uint32_t ring_at = __builtin_amdgcn_readfirstlane(lds_address(ring));
+
+  // What is past the last tile, row, run or group is read as the last, and not used.
+  int ask_tile = blockIdx.x * at_once + slot, ask_step = 0, ask_place = 0;
+  auto ask = [&]() {
+    const int tile = min(ask_tile, tiles - 1), first = (ask_step * f.share + part) * kAhead;
+    const int last_row = a.rows - 1 - tile * kQ4Tile;
+    const uint8_t* codes = a.codes + static_cast<int64_t>(tile) * kQ4Tile * row_bytes;
+    const __half* scales = a.scales + static_cast<int64_t>(tile) * kQ4Tile * f.groups;
+    const uint32_t to = ring_at + ask_place * kChunkBytes;
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      to[j].codes = *reinterpret_cast<const uint4*>(codes + min(first + j, f.runs - 1) * 64);
-    if (f.joined) {
-      // One load for all, or for 8 groups.
-      constexpr int kUnit = kGroups == 1 ? 4 : 8, kLoads = kAhead * kGroups / kUnit;
-      __half s[kAhead * kGroups];
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const __half* at = a.scales + row * f.groups + min(first * kGroups + kUnit * i, f.groups - kUnit);
-        if constexpr (kUnit == 8)
-          *reinterpret_cast<uint4*>(s + 8 * i) = *reinterpret_cast<const uint4*>(at);
-        else
-          *reinterpret_cast<uint2*>(s + 4 * i) = *reinterpret_cast<const uint2*>(at);
-      }
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-#pragma unroll
-        for (int n = 0; n < kGroups; ++n) to[j].scales[n] = s[j * kGroups + n];
-    } else {
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) load_scales<kGroup>(a, f, row, min(first + j, f.runs - 1), to[j].scales);
+    for (int q = 0; q < kAhead; ++q) {
+      const int row = 4 * q + g, piece = col ^ row;
+      dma_load<16>(codes,
+                   min(row, last_row) * row_bytes + min(first + piece / 4, f.runs - 1) * 64 + piece % 4 * 16,
+                   to + q * 1024);
     }
+#pragma unroll
+    for (int q = 0; q < kScaleLoads; ++q) {
+      const int i = q * kWave + lane, row = min(i / kWords, min(last_row, kQ4Tile - 1));
+      const int word = min(first * kGroups / 2 + i % kWords, f.groups / 2 - 1);
+      dma_load<4>(scales, (row * f.groups + 2 * word) * 2, to + kCodeBytes + q * 256);
+    }
+    ask_place = ask_place + 1 < kRing ? ask_place + 1 : 0;
     if (++ask_step == steps) ask_step = 0, ask_tile += stride;
   };
+  const int total = turns * steps;
   Columns v[kUnits];
-  load_x<kUnits, kWideWaves>(a, f, wave, v);
+  load_x<kUnits, kQ4Waves>(a, f, wave, v);
+  // After x has come: the compiler, which counts only the loads it makes, would
+  // else wait for the chunks with it.
 #pragma unroll
-  for (int i = 0; i < kRing; ++i) ask(ring[i]);
-  const bool broken = make_digits<kUnits, kWideWaves>(a, f, wave, v, d, digits);
+  for (int i = 0; i < kUnits; ++i)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) asm volatile("" : "+v"(v[i].x[k]), "+v"(v[i].w[k]) : : "memory");
+  for (int i = 0; i < min(kRing, total); ++i) ask();
+  const bool broken = make_digits<kUnits, kQ4Waves>(a, f, wave, v, d, digits);
 
   const int rows = kQ4Batch * a.batch, b = min(g, a.batch - 1);
-  const int8_t* const operand = digits + (min(col, rows - 1) * 4 + g) * 16;
-  int base = blockIdx.x * kTiles, step = 0, round = 0;
-  int left = (tiles - base + stride - 1) / stride * steps;  // steps of this block's waves
+  const int8_t* const operand = digits + (g * rows + min(col, rows - 1)) * 16;
+  int tile = blockIdx.x * at_once + slot, step = 0, turn = 0, place = 0;
   float y = 0.0f;
-  auto use = [&](const Run<kGroup>* now) {
-    const int first = (2 * step + half) * kAhead;
+  for (int at = 0; at < total; ++at) {
+    wait_for_chunk<kChunkLoads>(total - 1 - at);
+    const int8_t* chunk = ring + place * kChunkBytes;
+    place = place + 1 < kRing ? place + 1 : 0;
+    const int first = (step * f.share + part) * kAhead;
+    Run<kGroup> w[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) y = use_run(now[j], d, operand, rows, min(first + j, f.runs), b, y);
+    for (int j = 0; j < kAhead; ++j) {
+      w[j].codes = *reinterpret_cast<const uint4*>(chunk + col * 256 + ((4 * j + g) ^ col) * 16);
+      const __half* s = reinterpret_cast<const __half*>(chunk + kCodeBytes) + col * 2 * kWords + j * kGroups;
+#pragma unroll
+      for (int n = 0; n < kGroups; ++n) w[j].scales[n] = s[n];
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) y = use_run(w[j], d, operand, rows, min(first + j, f.runs), b, y);
+    asm volatile("" : "+v"(y) : : "memory");  // the chunk is read
+    if (at + kRing < total) ask();
     if (++step == steps) {
-      if (half == 1) sums[round % 2][slot][lane] = y;
-      __syncthreads();
-      if (half == 0) finish_checked(a, f, d, broken, y + sums[round % 2][slot][lane], (base + slot) * kQ4Tile + col);
+      if (f.share > 1) {
+        sums[turn % 2][wave][lane] = y;
+        __syncthreads();
+        if (part == 0)
+          for (int n = 1; n < f.share; ++n) y += sums[turn % 2][wave + n][lane];
+      }
+      if (part == 0) finish_checked(a, f, d, broken, y, tile * kQ4Tile + col);
       y = 0.0f;
       step = 0;
-      ++round;
-      base += stride;
-    }
-  };
-  // The loads of a chunk are waited for with those of the next kRing - 1 under
-  // way, so none of these is conditional; the last chunks ask for nothing.
-  for (; left > kRing; left -= kRing) {
-#pragma unroll
-    for (int i = 0; i < kRing; ++i) {
-      use(ring[i]);
-      ask(ring[i]);
+      ++turn;
+      tile += stride;
     }
   }
-#pragma unroll
-  for (int i = 0; i < kRing; ++i)
-    if (i < left) use(ring[i]);
 }
 
 // Workspace of the two-launch form: digits [ceil(batch / 4)][runs][2 KB], then
@@ -450,7 +493,7 @@ __global__ __launch_bounds__(kQ4Threads) void matvec_q4_rows_kernel(MatvecQ4Args
 #pragma unroll
     for (int t = 0; t < kManyTiles; ++t) {
       const int o = min(b0 / kQ4Batch + t, operands - 1);
-      const int8_t* d = base + (static_cast<int64_t>(o) * f.runs + run) * kQ4Operands + (col * 4 + g) * 16;
+      const int8_t* d = base + (static_cast<int64_t>(o) * f.runs + run) * kQ4Operands + lane * 16;
       x[t][0] = *reinterpret_cast<const i32x4*>(d);
       x[t][1] = *reinterpret_cast<const i32x4*>(d + kQ4Operands / 2);
       unit[t] = units[static_cast<int64_t>(min(o * kQ4Batch + g, a.batch - 1)) * f.runs + run];
@@ -488,27 +531,31 @@ bool fused_digits(int cols, int batch) {
 
 template <int kGroup>
 void launch_q4(const MatvecQ4Args& a, const Q4Form& f, hipStream_t stream) {
+  const int tiles = (a.rows + kQ4Tile - 1) / kQ4Tile;
   if (fused_digits(a.cols, a.batch)) {
-    const int tiles = (a.rows + kQ4Tile - 1) / kQ4Tile, all = f.runs * a.batch, each = kWideWaves / 2;
     const size_t lds = static_cast<size_t>(f.runs + kAhead) * a.batch * 512;
-    const int blocks = std::min((tiles + each - 1) / each, kWideBlocks);
-    if (tiles < kManyRowTiles && all <= 2 * kQ4Waves)
-      matvec_q4_kernel<kGroup, 2><<<tiles, kQ4Threads, lds, stream>>>(a, f);
-    else if (tiles < kManyRowTiles)
-      matvec_q4_kernel<kGroup, 8><<<tiles, kQ4Threads, lds, stream>>>(a, f);
-    else if (all <= kWideWaves)
-      matvec_q4_wide_kernel<kGroup, 1><<<blocks, kWideThreads, lds, stream>>>(a, f);
-    else
-      matvec_q4_wide_kernel<kGroup, 4><<<blocks, kWideThreads, lds, stream>>>(a, f);
+    const bool few = f.runs * a.batch <= 2 * kQ4Waves;
+    if (tiles < kManyRowTiles || !f.even) {
+      if (few)
+        matvec_q4_kernel<kGroup, 2><<<tiles, kQ4Threads, lds, stream>>>(a, f);
+      else
+        matvec_q4_kernel<kGroup, 8><<<tiles, kQ4Threads, lds, stream>>>(a, f);
+    } else {
+      const int at_once = kQ4Waves / f.share, blocks = std::min((tiles + at_once - 1) / at_once, kWideBlocks);
+      const size_t more = lds + kQ4Waves * kRing * kChunkBytes;
+      if (few)
+        matvec_q4_wide_kernel<kGroup, 2><<<blocks, kQ4Threads, more, stream>>>(a, f);
+      else
+        matvec_q4_wide_kernel<kGroup, 8><<<blocks, kQ4Threads, more, stream>>>(a, f);
+    }
     return;
   }
-  const int tiles = (a.rows + kQ4Tile - 1) / kQ4Tile, many = kManyTiles * kQ4Batch;
+  const int many = (a.batch + kManyTiles * kQ4Batch - 1) / (kManyTiles * kQ4Batch);
   q4_digits_kernel<<<a.batch, kQ4Threads, 0, stream>>>(a, f);
-  if (tiles >= kWideTiles)
-    matvec_q4_rows_kernel<kGroup, 2>
-        <<<dim3((tiles + 1) / 2, (a.batch + many - 1) / many), kQ4Threads, 0, stream>>>(a, f);
+  if (tiles >= kTwoTiles)
+    matvec_q4_rows_kernel<kGroup, 2><<<dim3((tiles + 1) / 2, many), kQ4Threads, 0, stream>>>(a, f);
   else
-    matvec_q4_rows_kernel<kGroup, 1><<<dim3(tiles, (a.batch + many - 1) / many), kQ4Threads, 0, stream>>>(a, f);
+    matvec_q4_rows_kernel<kGroup, 1><<<dim3(tiles, many), kQ4Threads, 0, stream>>>(a, f);
 }
 
 }  // namespace
@@ -526,7 +573,11 @@ hipError_t launch_matvec_q4(const MatvecQ4Args& a, GemvPrologue pro, GemvEpilogu
   f.runs = (a.cols + kQ4Cols - 1) / kQ4Cols;
   f.groups = (a.cols + a.group - 1) / a.group;
   f.whole = a.cols % kQ4Cols == 0 && reinterpret_cast<uintptr_t>(a.scales) % 8 == 0;
-  f.joined = f.whole && f.groups % (a.group == 128 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(a.scales) % 16 == 0;
+  // As many as give every wave a tile, while each has a chunk.
+  f.share = 1;
+  while (f.share < kQ4Waves && f.share * kAhead < f.runs && (a.rows + kQ4Tile - 1) / kQ4Tile * f.share < kManyWaves)
+    f.share *= 2;
+  f.even = f.whole && f.groups % 2 == 0;
   switch (a.group) {
     case 32: launch_q4<32>(a, f, stream); break;
     case 64: launch_q4<64>(a, f, stream); break;

@@ -96,6 +96,22 @@ def test_product(gpu, rows, cols, group, batch):
     Call(gpu, np.random.default_rng(rows + cols + group + batch), rows, cols, group, batch).check()
 
 
+@pytest.mark.parametrize("rows,cols", [(8192, 768), (8210, 1408), (8200, 4096), (9001, 96), (40000, 256), (8250, 896),
+                                       (16400, 2048), (33000, 128)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("batch", [1, 2, 4])
+def test_product_of_many_rows(gpu, rows, cols, group, batch):
+    """Blocks that take several tiles of rows in turn; ragged rows, runs, chunks and turns."""
+    print(f"[case] q4 {rows}x{cols} group {group} batch {batch}", flush=True)
+    Call(gpu, np.random.default_rng(rows + cols + group + batch), rows, cols, group, batch).check()
+
+
+@pytest.mark.parametrize("prologue,epilogue", [(1, 2), (2, 1), (0, 2)])
+@pytest.mark.parametrize("batch", [1, 3])
+def test_fused_forms_of_many_rows(gpu, prologue, epilogue, batch):
+    Call(gpu, np.random.default_rng(prologue + batch), 8222, 768, 32, batch, prologue, epilogue).check()
+
+
 @pytest.mark.parametrize("prologue", [0, 1, 2])
 @pytest.mark.parametrize("epilogue", [0, 1, 2])
 @pytest.mark.parametrize("batch", [1, 3, 18])
@@ -130,11 +146,11 @@ def test_x_of_any_size(gpu, batch):
 
 
 @pytest.mark.parametrize("prologue", [0, 1])
-@pytest.mark.parametrize("batch", [1, 3, 9])
-def test_x_that_is_not_finite(gpu, batch, prologue):
+@pytest.mark.parametrize("batch,rows", [(1, 70), (3, 70), (9, 70), (2, 8230)])
+def test_x_that_is_not_finite(gpu, batch, rows, prologue):
     """Infinities and NaN go where the formula takes them, and to no other row of x."""
     rng = np.random.default_rng(13)
-    c = Call(gpu, rng, 70, 320, 32, batch, prologue)
+    c = Call(gpu, rng, rows, 384, 32, batch, prologue)
     clean = c.run().numpy()
     x = c.x.copy()
     x[batch - 1, 300] = np.inf
