@@ -367,7 +367,7 @@ int mmr_prefill_attention(const float* query, const mmr_kv_cache* cache, int64_t
  *   key_exps, value_exps  int8 [pages][kv_heads][4]
  *   table       int32 [seqs][pages_per_seq]: page p of sequence s holds its
  *               positions 64 p .. 64 p + 63; entries past a sequence's last
- *               page are not read.
+ *               page may be anything.
  * keys and values are 16-byte aligned, the rest 4-byte aligned; head_dim is
  * 32, 64, 96 or 128, kv_heads at most 64, seqs at most 65535.  Sequences may
  * share pages that neither of them appends to.
@@ -377,8 +377,11 @@ int mmr_prefill_attention(const float* query, const mmr_kv_cache* cache, int64_t
  * take its positions context[s] .. context[s] + n - 1.  offsets [seqs + 1]
  * and context [seqs] are int32 on the device, so a recorded graph serves
  * every step; rows is what the row buffers hold, max_rows the most that one
- * sequence brings (both size the launch).  Rows outside [offsets[0],
- * offsets[seqs]) are left as they are.  rows or max_rows of 0 is no work.
+ * sequence brings (both size the launch: max_rows x seqs is at most 2^26, and
+ * a long prompt is better in a call of its own than among single rows).  Rows
+ * outside [offsets[0], offsets[seqs]) are left as they are.  rows or max_rows
+ * of 0 is no work.  As for all op-level calls, the current device is the one
+ * that holds the buffers and the stream.
  *
  * *error (device int32, never cleared here) gets bits: 1 if a sequence's
  * offsets fall or leave [0, rows], it brings more than max_rows rows, reaches
@@ -426,12 +429,13 @@ int mmr_kv8_append(const float* qkv, const float* q_norm, const float* k_norm, f
  * softmax(q.k / sqrt(d)) v per head, GQA mapping kv = h / (Hq/Hkv).  query
  * and out fp32 [rows][q_heads d], 16-byte aligned, q_heads a multiple of
  * kv_heads.  max_tokens bounds context[s] + n over all sequences and sizes
- * the split along the context.  A query row that is not finite gives a row of
- * NaN and no other.  The workspace
- * (mmr_kv8_attention_workspace_size bytes of the same sizes, possibly 0;
- * 16-byte aligned) holds the split partials and is the call's own until it
- * has run; it keeps nothing between calls.  No allocation, no
- * synchronisation, graph-capturable. */
+ * the split along the context.  Scores, weights and sums carry 21 bits or
+ * more, the sums relative to the largest exponent among a row's values.  A
+ * query row that is not finite gives a row of NaN and no other; out may alias
+ * query.  The workspace (mmr_kv8_attention_workspace_size bytes of the same
+ * sizes, possibly 0; 16-byte aligned) holds the split partials and is the
+ * call's own until it has run; it keeps nothing between calls.  No allocation,
+ * no synchronisation, graph-capturable. */
 size_t mmr_kv8_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
                                         int64_t rows, int64_t max_rows, int64_t max_tokens);
 int mmr_kv8_attention(const float* query, const mmr_kv8_pages* cache, const int32_t* offsets, const int32_t* context,

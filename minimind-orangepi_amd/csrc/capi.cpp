@@ -1019,6 +1019,8 @@ void check_kv8_sizes(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_
   require(seqs >= 1 && seqs <= 65535, "seqs must be in [1, 65535]");
   require(rows >= 0 && max_rows >= 0 && max_rows <= rows, "need 0 <= max_rows <= rows");
   require(rows <= (int64_t{1} << 24) && rows * (q_heads + 2 * kv_heads) <= (int64_t{1} << 27), "too many rows");
+  // Every sequence gets blocks for max_rows rows, most of which leave at once.
+  require(max_rows * seqs <= (int64_t{1} << 26), "max_rows x seqs over 2^26: pass sequences of like lengths together");
 }
 
 mmr::Kv8Pages kv8_pages(const mmr_kv8_pages* c) {

@@ -4,7 +4,7 @@
 //   s_mj = (q_m . k_j) log2(e) / sqrt(d)     for keys j <= context + token(m)
 //
 // with one pass over the keys and a running reference r_m in place of the row
-// maximum: a score may pass it by kLead before everything is scaled down to a
+// maximum: a score may pass it a little before everything is scaled down to a
 // new one.  Two kernels, by the rows (token, head) that a sequence brings to a
 // group of heads that share their keys:
 //
@@ -13,7 +13,7 @@
 // an integer n is the sum of d_k 256^k with d_k in [-128, 127], and the bytes
 // of n + 0x808080 are those digits, the lower three with their top bit
 // flipped.  Products and sums of digits and codes are exact in int32; rounded
-// are q (to 2^-30 of its row's largest value), p (2^-26) and the fp32 sums
+// are q (to 2^-30 of its row's largest value), p (2^-29) and the fp32 sums
 // over pages.  The 16 columns of a product are 4 rows x 4 digits, so K and V
 // are each the operand of one product, and a score is the sum over four lanes.
 //
@@ -43,12 +43,12 @@ namespace {
 constexpr int kStepWaves = 8, kStepThreads = kStepWaves * kWave;
 constexpr int kJoinWaves = 4, kJoinThreads = kJoinWaves * kWave;
 constexpr float kNoRow = -FLT_MAX / 2;  // reference of a row that has met no key
-constexpr float kLead = 5.0f;           // a score may pass the reference by 2^kLead
+constexpr float kStepLead = 2.0f, kRowsLead = 5.0f;  // a score may pass the reference by this much (log2)
 constexpr int kRowsThreads = 256;
 constexpr int kFewSplits = 8;
 constexpr int kRowsTile = 64;          // rows of a block of the kernel for many
 constexpr int kRowsPBits = 10;          // its p in units of 2^-10: at most 2^15 with the lead
-constexpr int kPBits = 25;              // p in units of 2^-25: at most 2^30 with the lead
+constexpr int kPBits = 28;              // p of steps in units of 2^-28: at most 2^30 with the lead
 constexpr int kLeastPages = 4, kWidePages = 16, kStepBlocks = 256, kRowsBlocks = 1280, kFewRows = 256;  // see kv8_attention_plan
 constexpr int kMostSplits = 64;  // at most one a thread of the combine
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, score[t][i]);
 
-    if (__any(top > ref + kLead) || page_exp > held_exp || since == kMostPages) {
+    if (__any(top > ref + kStepLead) || page_exp > held_exp || since == kMostPages) {
       const float next = fmaxf(ref, column_max(top));
       if (since > 0) move(__builtin_amdgcn_exp2f(ref - next));  // not before the first page
       ref = next;
@@ -585,7 +585,7 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
 #pragma unroll
         for (int i = 0; i < 4; ++i) top[t / 2] = fmaxf(top[t / 2], score[t][i]);
       const float page_top = fmaxf(top[0] * to_log2[0], top[1] * to_log2[1]);
-      if (__any(page_top > ref + kLead) || page_exp > held_exp) {
+      if (__any(page_top > ref + kRowsLead) || page_exp > held_exp) {
         const float next = fmaxf(ref, column_max(page_top));
         const int next_exp = max(held_exp, page_exp);
         const float f = __builtin_amdgcn_exp2f(ref - next), down = ldexpf(f, held_exp - next_exp);

@@ -356,3 +356,57 @@ def test_no_rows_is_no_work(gpu):
     mmr.synchronize()
     assert error == 0 and (got == 7.5).all() and (one.numpy() == 7.5).all() and int(step.error.numpy()[0]) == 0
     cache.assert_equals(step.device)
+
+
+def test_thousands_of_sequences(gpu):
+    """One row each, on caches of one to three pages, in one call."""
+    rng = np.random.default_rng(43)
+    seqs, per, hq, hkv, d = 3000, 3, 2, 1, 32
+    cache = ref.Cache(rng, seqs * per, seqs, per, hkv, d)
+    context = [int(c) for c in rng.integers(0, 190, seqs)]
+    step = Append(gpu, cache, hq, rng=rng)
+    step.check(qkv_rows(rng, seqs, hq, hkv, d), [1] * seqs, context)
+    # Cached tokens before the new rows are whatever the pages held: their exponents can be anything a block may have.
+    cache.key_exps[:] = np.clip(cache.key_exps, -12, -4)
+    cache.value_exps[:] = np.clip(cache.value_exps, -12, -4)
+    check_attention(gpu, cache, rng.standard_normal((seqs, hq * d)).astype(np.float32), [1] * seqs, context, hq)
+
+
+def test_calls_on_two_streams_at_once(gpu):
+    """Caches, workspaces and errors of their own: neither call sees the other."""
+    mmr = gpu
+    runs = []
+    for seed in (45, 46):
+        rng = np.random.default_rng(seed)
+        cache = ref.Cache(rng, 2 * 20, 2, 20, 2, 96)
+        cache.fill(rng, [1200, 700])
+        query = rng.standard_normal((2, 8 * 96)).astype(np.float32)
+        size = mmr.kv8_attention_workspace_size(8, 2, 96, 2, 2, 1, 1280)
+        runs.append(dict(cache=cache, device=cache.upload(mmr), query=query, dq=mmr.DeviceArray.from_numpy(query),
+                         out=mmr.DeviceArray((2, 768), np.float32), ws=mmr.DeviceArray(size, np.uint8),
+                         offsets=ints(mmr, [0, 1, 2]), context=ints(mmr, [1199, 699]), error=ints(mmr, [0]),
+                         stream=mmr.Stream()))
+    mmr.synchronize()
+    for _ in range(20):
+        for r in runs:
+            mmr.kv8_attention(r["dq"], r["device"], r["offsets"], r["context"], 2, 1, 1280, 8, r["out"], r["ws"],
+                              r["error"], stream=r["stream"])
+    mmr.synchronize()
+    for r in runs:
+        want, bound = ref.attention(r["cache"], r["query"], [0, 1, 2], [1199, 699], 8, r["query"])
+        assert (np.abs(r["out"].numpy() - want) <= bound).all()
+
+
+@pytest.mark.parametrize("rows,context", [([1, 1], [100, 2000]), ([40, 90], [3, 600])])
+def test_out_in_place_of_the_query(gpu, rows, context):
+    mmr, rng = gpu, np.random.default_rng(47)
+    per = pages_for(rows, context)
+    cache = ref.Cache(rng, 2 * per, 2, per, 2, 64)
+    cache.fill(rng, [a + b for a, b in zip(rows, context)])
+    query = rng.standard_normal((sum(rows), 8 * 64)).astype(np.float32)
+    both, error, max_rows = mmr.DeviceArray.from_numpy(query), ints(mmr, [0]), max(rows)
+    size = mmr.kv8_attention_workspace_size(8, 2, 64, 2, len(query), max_rows, per * 64)
+    mmr.kv8_attention(both, cache.upload(mmr), ints(mmr, offsets_of(rows)), ints(mmr, context), len(query), max_rows,
+                      per * 64, 8, both, mmr.DeviceArray(max(size, 1), np.uint8), error)
+    want, bound = ref.attention(cache, query, offsets_of(rows), context, 8, query)
+    assert (np.abs(both.numpy() - want) <= bound).all()

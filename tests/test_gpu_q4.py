@@ -97,7 +97,7 @@ def test_product(gpu, rows, cols, group, batch):
 
 
 @pytest.mark.parametrize("rows,cols", [(8192, 768), (8210, 1408), (8200, 4096), (9001, 96), (40000, 256), (8250, 896),
-                                       (16400, 2048), (33000, 128)])
+                                       (16400, 2048), (33000, 128), (8192, 8192)])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("batch", [1, 2, 4])
 def test_product_of_many_rows(gpu, rows, cols, group, batch):

@@ -133,6 +133,7 @@ def test_attention_refuses(mmr):
     refused("max_rows", max_rows=5)
     refused("max_rows", max_rows=-1)
     refused("rows", rows=1 << 25)
+    refused("like lengths", cache=pages(mmr, seqs=4096), rows=1 << 17, max_rows=1 << 15)
     refused("q_heads", q_heads=3)
     refused("q_heads", q_heads=0)
     refused("max_tokens", max_tokens=0)
