@@ -41,7 +41,7 @@ namespace mmr {
 namespace {
 
 constexpr int kStepWaves = 8, kStepThreads = kStepWaves * kWave;
-constexpr int kJoinWaves = 4, kJoinThreads = kJoinWaves * kWave;
+constexpr int kJoinThreads = 256;
 constexpr float kNoRow = -FLT_MAX / 2;  // reference of a row that has met no key
 constexpr float kStepLead = 2.0f, kRowsLead = 5.0f;  // a score may pass the reference by this much (log2)
 constexpr int kRowsThreads = 256;
@@ -50,7 +50,7 @@ constexpr int kRowsTile = 64;          // rows of a block of the kernel for many
 constexpr int kRowsPBits = 10;          // its p in units of 2^-10: at most 2^15 with the lead
 constexpr int kPBits = 28;              // p of steps in units of 2^-28: at most 2^30 with the lead
 constexpr int kLeastPages = 4, kWidePages = 16, kStepBlocks = 256, kRowsBlocks = 1280, kFewRows = 256;  // see kv8_attention_plan
-constexpr int kMostSplits = 64;  // at most one a thread of the combine
+constexpr int kMostSplits = 64;         // a lane of a wave each in the join
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 using f32x4 = float __attribute__((ext_vector_type(4)));
 constexpr int kMostPages = 1024;        // int32 sums: 64 keys x 128 x 127 < 2^20 a page
@@ -117,7 +117,12 @@ __device__ __forceinline__ void store_ml(const Kv8AttnArgs& a, int64_t row, int 
   ml[1] = l;
 }
 
-// Waves take the pages of a split in turn and join their results at the end.
+// Steps: waves take the pages of a split in turn and join their results at the
+// end.  Waves wait for memory half of their time, the vector units are busy 19 %
+// of it: what counts is that a wave always has a page under way.  32 sequences
+// of up to 8,192 tokens, two KV heads of d 96: 72 MB in 19.2 us with the join, 3.8
+// TB/s; one query over 32,768 13.1 us, over 500 7.2 (replayed graph, 1.6 of them
+// any kernel's): two dependent loads, one page's arithmetic, the join in LDS.
 template <int D>
 __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a, int chunk, int splits) {
   constexpr int kRows = 4, kTiles = D / 16;  // tiles of the output's dimensions
@@ -387,6 +392,15 @@ __device__ __forceinline__ void split2_truncated(float x0, float x1, uint32_t& h
 
 // 16 rows a wave, all waves over the same pages, which the block widens into
 // LDS: the operands of every product, 16 bytes a lane in the order of lanes.
+//
+// Measured: 3,000 rows after 1,111, 8 heads of d 96 over two KV heads, 77 us a
+// call (9 of them the join), 311 TFLOP/s of the formula's products, of which
+// the two planes make twice as many.  Vector units are busy 48 % of the
+// kernel, matrix cores 26 %, LDS 26 %; with the lower planes' products, the
+// exponentials or the widening of pages left out, one at a time, it takes 70
+// to 75 us, so it is none of them but the chain barrier - LDS - products -
+// weights - products with three waves a SIMD.  32 rows a wave (half the LDS reads a row, two waves
+// a SIMD) took 84 us, blocks of eight waves 101.
 template <int D>
 __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel(Kv8AttnArgs a, int chunk, int splits) {
   constexpr int kTiles = D / 16, kRuns = D / 32;  // tiles of the output, products along D
@@ -518,7 +532,6 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
   put(stage[0]);
   if (!works) {  // rows past the last: this wave only helps with the pages
     for (int p = begin; p < end; ++p) {
-      if (next_hidden && tid == 0) atomicOr(a.error, kKv8BadRows);
       __syncthreads();
       if (p + 1 < end) {
         ask(p + 1);
@@ -537,100 +550,98 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
     if (hidden && tid == 0) atomicOr(a.error, kKv8BadRows);
     __syncthreads();  // this page is in LDS, and every wave is done with the one before
     if (p + 1 < end) ask(p + 1);
-    {
-      const int blocks = hidden ? 0 : min(kKv8Blocks, (wave_last - p * kKv8Page + kKv8Block) / kKv8Block);
-      int page_exp = kKv8MinExp - 1;
+    const int blocks = hidden ? 0 : min(kKv8Blocks, (wave_last - p * kKv8Page + kKv8Block) / kKv8Block);
+    int page_exp = kKv8MinExp - 1;
 #pragma unroll
-      for (int b = 0; b < kKv8Blocks; ++b)
-        if (b < blocks) page_exp = max(page_exp, static_cast<int>(static_cast<int8_t>(value_exps >> (8 * b))));
-      // Two sums at a time: a sum's products wait for each other.
-      f32x4 score[4];
+    for (int b = 0; b < kKv8Blocks; ++b)
+      if (b < blocks) page_exp = max(page_exp, static_cast<int>(static_cast<int8_t>(value_exps >> (8 * b))));
+    // Two sums at a time: a sum's products wait for each other.
+    f32x4 score[4];
 #pragma unroll
-      for (int t = 0; t < 4; t += 2) {
-        f16x8 kf[2][kRuns];
+    for (int t = 0; t < 4; t += 2) {
+      f16x8 kf[2][kRuns];
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          score[t + w] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int w = 0; w < 2; ++w) {
+        score[t + w] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int c = 0; c < kRuns; ++c) {
-            const int o = (t + w) * kRuns + c;
-            kf[w][c] = __builtin_bit_cast(f16x8, now[o * kOperand + (lane ^ key_place(o, g))]);
-          }
+        for (int c = 0; c < kRuns; ++c) {
+          const int o = (t + w) * kRuns + c;
+          kf[w][c] = __builtin_bit_cast(f16x8, now[o * kOperand + (lane ^ key_place(o, g))]);
         }
-#pragma unroll
-        for (int c = 0; c < 2 * kRuns; ++c)
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-            score[t + w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                kf[w][c % kRuns], c < kRuns ? q_lo[c % kRuns] : q_hi[c % kRuns], score[t + w], 0, 0, 0);
       }
-      const int shift = 8 * (g / 2);  // of this lane's block of each half page
-      const float key_scale[2] = {ldexpf(1.0f, static_cast<int8_t>(key_exps >> shift)),
-                                  ldexpf(1.0f, static_cast<int8_t>(key_exps >> (16 + shift)))};
-      float to_log2[2] = {unit * key_scale[0], unit * key_scale[1]};
-      if (hidden || p * kKv8Page + kKv8Page - 1 > all_see) {
-        // Scaled first: a factor may be 0 or, of a block that holds anything, infinite.
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+      for (int c = 0; c < 2 * kRuns; ++c)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            score[t][i] = hidden || p * kKv8Page + 32 * (t / 2) + 8 * g + 4 * (t % 2) + i > limit
-                              ? -INFINITY
-                              : score[t][i] * to_log2[t / 2];
-        to_log2[0] = to_log2[1] = 1.0f;
-      }
-      float top[2] = {-INFINITY, -INFINITY};
+        for (int w = 0; w < 2; ++w)
+          score[t + w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              kf[w][c % kRuns], c < kRuns ? q_lo[c % kRuns] : q_hi[c % kRuns], score[t + w], 0, 0, 0);
+    }
+    const int shift = 8 * (g / 2);  // of this lane's block of each half page
+    const float key_scale[2] = {ldexpf(1.0f, static_cast<int8_t>(key_exps >> shift)),
+                                ldexpf(1.0f, static_cast<int8_t>(key_exps >> (16 + shift)))};
+    float to_log2[2] = {unit * key_scale[0], unit * key_scale[1]};
+    if (hidden || p * kKv8Page + kKv8Page - 1 > all_see) {
+      // Scaled first: a factor may be 0 or, of a block that holds anything, infinite.
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top[t / 2] = fmaxf(top[t / 2], score[t][i]);
-      const float page_top = fmaxf(top[0] * to_log2[0], top[1] * to_log2[1]);
-      if (__any(page_top > ref + kRowsLead) || page_exp > held_exp) {
-        const float next = fmaxf(ref, column_max(page_top));
-        const int next_exp = max(held_exp, page_exp);
-        const float f = __builtin_amdgcn_exp2f(ref - next), down = ldexpf(f, held_exp - next_exp);
-        l *= f;
+        for (int i = 0; i < 4; ++i)
+          score[t][i] = hidden || p * kKv8Page + 32 * (t / 2) + 8 * g + 4 * (t % 2) + i > limit
+                            ? -INFINITY
+                            : score[t][i] * to_log2[t / 2];
+      to_log2[0] = to_log2[1] = 1.0f;
+    }
+    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) out[t] *= down;
-        ref = next;
-        held_exp = next_exp;
-      }
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        // The value block's factor goes into the exponent.  Below 2^-60 of the
-        // largest block it no longer falls: what it weighs is nothing in fp16.
-        const int my_exp = static_cast<int8_t>(value_exps >> (16 * u + shift));
-        const int bias = min(max(my_exp - held_exp, -60), 0) + kRowsPBits;
-        const float from = static_cast<float>(bias) - ref;
-        float part = 0.0f;
-        uint4 hi, lo;
-        uint32_t *ph = &hi.x, *pl = &lo.x;
+      for (int i = 0; i < 4; ++i) top[t / 2] = fmaxf(top[t / 2], score[t][i]);
+    const float page_top = fmaxf(top[0] * to_log2[0], top[1] * to_log2[1]);
+    if (__any(page_top > ref + kRowsLead) || page_exp > held_exp) {
+      const float next = fmaxf(ref, column_max(page_top));
+      const int next_exp = max(held_exp, page_exp);
+      const float f = __builtin_amdgcn_exp2f(ref - next), down = ldexpf(f, held_exp - next_exp);
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) out[t] *= down;
+      ref = next;
+      held_exp = next_exp;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      // The value block's factor goes into the exponent.  Below 2^-60 of the
+      // largest block it no longer falls: what it weighs is nothing in fp16.
+      const int my_exp = static_cast<int8_t>(value_exps >> (16 * u + shift));
+      const int bias = min(max(my_exp - held_exp, -60), 0) + kRowsPBits;
+      const float from = static_cast<float>(bias) - ref;
+      float part = 0.0f;
+      uint4 hi, lo;
+      uint32_t *ph = &hi.x, *pl = &lo.x;
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const float e0 = __builtin_amdgcn_exp2f(fmaf(score[2 * u + w][i], to_log2[u], from));
+          const float e1 = __builtin_amdgcn_exp2f(fmaf(score[2 * u + w][i + 1], to_log2[u], from));
+          part += e0;
+          part += e1;
+          split2_truncated(e0, e1, ph[2 * w + i / 2], pl[2 * w + i / 2]);
+        }
+      l = fmaf(part, ldexpf(1.0f, -bias), l);
+      const f16x8 p_hi = __builtin_bit_cast(f16x8, hi), p_lo = __builtin_bit_cast(f16x8, lo);
+#pragma unroll
+      for (int t = 0; t < kTiles; t += 2) {
+        f16x8 vf[2];
 #pragma unroll
         for (int w = 0; w < 2; ++w)
+          vf[w] = __builtin_bit_cast(
+              f16x8, now[(4 * kRuns + u * kTiles + t + w) * kOperand + (lane ^ value_place(u, g))]);
 #pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            const float e0 = __builtin_amdgcn_exp2f(fmaf(score[2 * u + w][i], to_log2[u], from));
-            const float e1 = __builtin_amdgcn_exp2f(fmaf(score[2 * u + w][i + 1], to_log2[u], from));
-            part += e0;
-            part += e1;
-            split2_truncated(e0, e1, ph[2 * w + i / 2], pl[2 * w + i / 2]);
-          }
-        l = fmaf(part, ldexpf(1.0f, -bias), l);
-        const f16x8 p_hi = __builtin_bit_cast(f16x8, hi), p_lo = __builtin_bit_cast(f16x8, lo);
+        for (int w = 0; w < 2; ++w)
+          out[t + w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[w], p_lo, out[t + w], 0, 0, 0);
 #pragma unroll
-        for (int t = 0; t < kTiles; t += 2) {
-          f16x8 vf[2];
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-            vf[w] = __builtin_bit_cast(
-                f16x8, now[(4 * kRuns + u * kTiles + t + w) * kOperand + (lane ^ value_place(u, g))]);
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-            out[t + w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[w], p_lo, out[t + w], 0, 0, 0);
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-            out[t + w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[w], p_hi, out[t + w], 0, 0, 0);
-        }
+        for (int w = 0; w < 2; ++w)
+          out[t + w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[w], p_hi, out[t + w], 0, 0, 0);
       }
     }
     if (p + 1 < end) put(stage[(p + 1 - begin) % 2]);
@@ -695,53 +706,59 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_few_kernel(Kv8AttnAr
   reinterpret_cast<float4*>(a.out + to * d)[quad] = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
 }
 
-// Joins many splits, a block per (token, head): weights first, a split a thread, then groups of d / 4 threads take
-// splits in turn, four dimensions each.
+// Joins many splits, a block per (token, head): groups of d / 4 threads take
+// splits in turn, four dimensions each, with all loads under way before the
+// first wave, a split a lane, has the weights.
+template <int D>
 __global__ __launch_bounds__(kJoinThreads) void kv8_combine_kernel(Kv8AttnArgs a, int chunk, int splits,
                                                                    int tile_rows) {
-  __shared__ float weight[kMostSplits], shared_top[kJoinWaves], shared_l[kJoinWaves];
-  __shared__ float4 shared_out[kJoinThreads];
-  const int s = blockIdx.y, d = a.cache.d, quads = d / 4, groups = kJoinThreads / quads;
+  constexpr int kQuads = D / 4, kGroups = kJoinThreads / kQuads, kEach = (kMostSplits + kGroups - 1) / kGroups;
+  static_assert(kMostSplits == kWave, "a split a lane");
+  __shared__ float weight[kMostSplits], shared_l;
+  __shared__ float4 shared_out[kGroups][kQuads];
+  const int s = blockIdx.y, i = blockIdx.x, x = threadIdx.x, g = x / kQuads, quad = x - g * kQuads;
   Kv8Span span;
   if (!kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span)) return;
   if (static_cast<int64_t>(span.context) + span.n > a.max_tokens) return;
-  const int i = blockIdx.x;
   if (i >= span.n * a.hq) return;
   const int used = splits_of(a, span, i, chunk, tile_rows);
   if (used == 1) return;
   const int64_t to = static_cast<int64_t>(span.first) * a.hq + i;
-  const float* ml = a.part + static_cast<int64_t>(a.rows) * a.hq * splits * d + to * splits * 2;
-  const float4* o = reinterpret_cast<const float4*>(a.part + to * splits * d);
-  const int x = threadIdx.x, wave = x / kWave;
-  const float ref = x < used ? ml[2 * x] : kNoRow, part_l = x < used ? ml[2 * x + 1] : 0.0f;
-  float top = group_max<kWave>(ref);
-  if (x % kWave == 0) shared_top[wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(shared_top[0], shared_top[1]), fmaxf(shared_top[2], shared_top[3]));
-  const float f = __builtin_amdgcn_exp2f(ref - top);
-  weight[x] = f;
-  const float l = group_sum<kWave>(f * part_l);
-  if (x % kWave == 0) shared_l[wave] = l;
-  __syncthreads();
-  const int g = x / quads, quad = x - g * quads;
-  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (g < groups) {
-    for (int y = g; y < used; y += groups) {
-      const float4 v = o[y * quads + quad];
-      const float w = weight[y];
-      sum.x += w * v.x, sum.y += w * v.y, sum.z += w * v.z, sum.w += w * v.w;
-    }
+  const float2* ml = reinterpret_cast<const float2*>(a.part + static_cast<int64_t>(a.rows) * a.hq * splits * D) + to * splits;
+  const float4* o = reinterpret_cast<const float4*>(a.part + to * splits * D) + quad;
+  float2 of = make_float2(kNoRow, 0.0f);
+  if (x < used) of = ml[x];
+  float4 v[kEach];
+#pragma unroll
+  for (int n = 0; n < kEach; ++n) {
+    const int y = g + kGroups * n;
+    v[n] = g < kGroups && y < used ? o[y * kQuads] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
-  shared_out[x] = sum;
+  if (x < kWave) {
+    const float w = __builtin_amdgcn_exp2f(of.x - group_max<kWave>(of.x));
+    const float l = group_sum<kWave>(w * of.y);
+    weight[x] = w;
+    if (x == 0) shared_l = l;
+  }
   __syncthreads();
-  if (x < quads) {
-    for (int y = 1; y < min(groups, used); ++y) {
-      const float4 v = shared_out[y * quads + x];
-      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+  if (g < kGroups) {
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+      const float w = weight[min(g + kGroups * n, kMostSplits - 1)];  // of splits past the last: times 0
+      sum.x += w * v[n].x, sum.y += w * v[n].y, sum.z += w * v[n].z, sum.w += w * v[n].w;
     }
-    const float total = shared_l[0] + shared_l[1] + shared_l[2] + shared_l[3];
-    const float inv = total != 0.0f ? 1.0f / total : 0.0f;
-    reinterpret_cast<float4*>(a.out + to * d)[x] = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+    shared_out[g][quad] = sum;
+  }
+  __syncthreads();
+  if (x < kQuads) {
+    float4 sum = shared_out[0][x];
+    for (int y = 1; y < min(kGroups, used); ++y) {
+      const float4 more = shared_out[y][x];
+      sum.x += more.x, sum.y += more.y, sum.z += more.z, sum.w += more.w;
+    }
+    const float inv = shared_l != 0.0f ? 1.0f / shared_l : 0.0f;
+    reinterpret_cast<float4*>(a.out + to * D)[x] = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
   }
 }
 
@@ -794,8 +811,8 @@ void launch_attention_for(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_
     kv8_combine_few_kernel<<<dim3((a.max_rows * a.hq + each - 1) / each, a.cache.seqs), kJoinThreads, 0, stream>>>(
         a, p.chunk_pages, p.splits, p.tile_rows);
   } else if (p.splits > 1)
-    kv8_combine_kernel<<<dim3(a.max_rows * a.hq, a.cache.seqs), kJoinThreads, 0, stream>>>(a, p.chunk_pages, p.splits,
-                                                                                         p.tile_rows);
+    kv8_combine_kernel<D><<<dim3(a.max_rows * a.hq, a.cache.seqs), kJoinThreads, 0, stream>>>(
+        a, p.chunk_pages, p.splits, p.tile_rows);
 }
 
 }  // namespace

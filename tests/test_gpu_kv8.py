@@ -210,6 +210,24 @@ def test_attention_over_many_rows_of_blocks(gpu, rows):
                     hq)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(4, 1, 32), (4, 4, 64), (8, 2, 96), (6, 3, 128)])
+@pytest.mark.parametrize("rows,context", [([1, 1], [20000, 16300]), ([30], [9000])])
+def test_attention_joins_many_splits(gpu, hq, hkv, d, rows, context):
+    """As many splits as one join takes, and fewer of the second sequence; the same bits whenever it is called."""
+    print(f"[case] joins {hq},{hkv},{d} rows {rows} context {context}", flush=True)
+    rng = np.random.default_rng(sum(context) + d)
+    per = pages_for(rows, context)
+    cache = ref.Cache(rng, len(rows) * per, len(rows), per, hkv, d)
+    cache.fill(rng, [a + b for a, b in zip(rows, context)])
+    query = rng.standard_normal((sum(rows), hq * d)).astype(np.float32)
+    check_attention(gpu, cache, query, rows, context, hq)
+    device, offsets = cache.upload(gpu), offsets_of(rows)
+    first, _ = attend(gpu, device, cache, query, offsets, context, hq, max_rows=max(rows))
+    for _ in range(20):
+        again, _ = attend(gpu, device, cache, query, offsets, context, hq, max_rows=max(rows))
+        np.testing.assert_array_equal(again, first)
+
+
 @pytest.mark.parametrize("rows", [1, 9])
 def test_attention_over_values_of_any_size(gpu, rows):
     """Blocks whose values are 2^40 apart, all zero, or at the ends of the exponents; peaked and flat rows."""
