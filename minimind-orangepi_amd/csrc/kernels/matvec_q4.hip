@@ -17,6 +17,11 @@
 // 32 j + 8 p + 0 .. 7, column 2 i in the low nibble of byte i and 2 i + 1 in
 // the high one.  Part p of a product's K is lanes 16 p .. 16 p + 15, so a lane
 // loads 16 bytes and has a share of every group, whatever the group's size.
+//
+// Measured in replayed graphs, 1.6 us of them any kernel's: 1152 x 768 in groups
+// of 32 for one row 4.1 us (latency), 32768 x 4096 in groups of 128 15.5 us, 69.4
+// MB at 4.5 TB/s, 4096 x 768 for 32 rows 6.4 us (two launches), 16384 x 4096 for 32
+// rows 39.7: there each lane's 16 bytes of codes are a line of their own.
 #include "device_common.h"
 
 #include <algorithm>
@@ -30,10 +35,10 @@ constexpr int kQ4Threads = kQ4Waves * kWave;
 constexpr int kQ4Tile = 16;        // weight rows of a product
 constexpr int kQ4Batch = 4;        // batch rows of an x operand
 constexpr int kQ4Operands = 2048;  // bytes of the two x operands of a run
-// batch x cols that a block itself turns into digits, of up to kQ4Batch rows:
-// more of them cost a second launch less (768 x 2048 for 4 rows 9.2 us here and
-// 8.6 in two launches, 4096 x 2048 9.6 and 10.5; replayed graphs).
-constexpr int kFusedCols = 8192;
+// Runs of all rows of x, up to kQ4Batch rows, that a block itself turns into
+// digits: more of them cost a second launch less (768 x 2048 for 4 rows 9.2 us
+// here and 8.6 in two launches, 4096 x 2048 9.6 and 10.5; replayed graphs).
+constexpr int kFusedRuns = 64;
 // Tiles of rows from which blocks take several in turn, so that x is turned
 // into digits once a compute unit (8192 x 4096 in groups of 32: 11.7 us with a
 // tile a block, 9.4; 4096 x 768 with 256 tiles 4.2 and 4.9).
@@ -202,6 +207,7 @@ __device__ __forceinline__ void finish(const MatvecQ4Args& a, const Q4Form& f, f
 template <int kUnits, int kWaves>
 struct Digits {
   static constexpr int kMost = kUnits * kWaves;  // runs of all rows
+  static_assert(kMost <= kFusedRuns, "and kFusedRuns in the larger form");
   float units[kMost + kAhead][kQ4Batch];         // [runs], then zeros
   float squares[kMost], row_scale[kQ4Batch];
 };
@@ -526,7 +532,7 @@ __global__ __launch_bounds__(kQ4Threads) void matvec_q4_rows_kernel(MatvecQ4Args
 }
 
 bool fused_digits(int cols, int batch) {
-  return batch <= kQ4Batch && static_cast<int64_t>(batch) * cols <= kFusedCols;
+  return batch <= kQ4Batch && batch * ((cols + kQ4Cols - 1) / kQ4Cols) <= kFusedRuns;
 }
 
 template <int kGroup>

@@ -106,6 +106,19 @@ def test_product_of_many_rows(gpu, rows, cols, group, batch):
     Call(gpu, np.random.default_rng(rows + cols + group + batch), rows, cols, group, batch).check()
 
 
+@pytest.mark.parametrize("batch,cols", [(1, 8192), (1, 8224), (2, 4096), (2, 4128), (3, 2688), (3, 2720), (3, 2752),
+                                        (4, 2048), (4, 2080)])
+@pytest.mark.parametrize("rows", [40, 8200])
+def test_most_columns_of_one_launch(gpu, batch, cols, rows):
+    """Where the runs of all rows of x just fit one launch, and just don't: a ragged run counts as a whole one."""
+    print(f"[case] q4 {rows}x{cols} batch {batch}", flush=True)
+    Call(gpu, np.random.default_rng(cols + batch), rows, cols, 32, batch, 1).check()
+
+
+def test_most_rows_of_x(gpu):
+    Call(gpu, np.random.default_rng(19), 18, 160, 32, 65536).check()
+
+
 @pytest.mark.parametrize("prologue,epilogue", [(1, 2), (2, 1), (0, 2)])
 @pytest.mark.parametrize("batch", [1, 3])
 def test_fused_forms_of_many_rows(gpu, prologue, epilogue, batch):
