@@ -106,6 +106,15 @@ __device__ __forceinline__ int gather_digits(const int u[4], uint32_t sel, uint3
 __device__ __forceinline__ uint32_t digit_select(int k) { return k | (4 + k) << 8; }
 __device__ __forceinline__ uint32_t digit_flip(int k) { return k < 3 ? 0x80808080u : 0u; }
 
+// 0, but not to the compiler: the result of a load that it sees to be the same
+// in all lanes it moves to a scalar register right behind the load, which waits
+// for it and for all that was asked for before.
+__device__ __forceinline__ int zero_of_lanes() {
+  int zero = 0;
+  asm volatile("" : "+v"(zero));
+  return zero;
+}
+
 // Splits of at most `chunk` pages each that a row's `pages` are dealt to, evenly.
 __device__ __forceinline__ int splits_used(int pages, int chunk) { return (pages + chunk - 1) / chunk; }
 
@@ -162,9 +171,13 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
   bool next_hidden;
   const int8_t *next_k, *next_v;
   int ask_at = 0;
+  const int lane_zero = zero_of_lanes();
   auto ask = [&]() {  // addresses and exponents of step ask_at, at most the last
     const int step = min(ask_at, (end - 1 - from) / kStepWaves);
-    if (ask_at > 0 && step % kWave == 0) numbers = table[min(from + kStepWaves * (step + lane), a.cache.per_seq - 1)];
+    if (ask_at > 0 && step % kWave == 0) {
+      numbers = table[min(from + kStepWaves * (step + lane), a.cache.per_seq - 1)];
+      asm volatile("" : "+v"(numbers));  // waited for here, not wherever it is read
+    }
     ++ask_at;
     const int number = __builtin_amdgcn_readlane(numbers, step % kWave);
     next_hidden = number < 0 || number >= a.cache.pages;
@@ -172,8 +185,8 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
     const int64_t at = kv8_offset(page, h, hkv, D), exp_at = kv8_exp_offset(page, h, hkv);
     next_k = a.cache.keys + at;
     next_v = a.cache.values + at;
-    next_key_exps = *reinterpret_cast<const uint32_t*>(a.cache.key_exps + exp_at);
-    next_value_exps = *reinterpret_cast<const uint32_t*>(a.cache.value_exps + exp_at);
+    next_key_exps = *reinterpret_cast<const uint32_t*>(a.cache.key_exps + exp_at + lane_zero);
+    next_value_exps = *reinterpret_cast<const uint32_t*>(a.cache.value_exps + exp_at + lane_zero);
   };
   // Row 4 g + i of the t-th product is key 16 g + 4 t + i: a lane's scores are
   // those of part g's 16 keys of P.
@@ -256,7 +269,7 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
   };
 
   for (int p = from; p < end; p += kStepWaves) {
-    const uint32_t key_exps = next_key_exps, value_exps = next_value_exps;
+    const uint32_t key_exps = next_key_exps, value_exps = __builtin_amdgcn_readfirstlane(next_value_exps);
     const bool hidden = next_hidden;
     // Blocks past the last key hold anything: their exponents don't count.
     const int blocks = hidden ? 0 : min(kKv8Blocks, (span.context + span.n - 1 - p * kKv8Page) / kKv8Block + 1);
@@ -443,9 +456,13 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
   uint4 piece[kPieces];
   uint32_t next_key_exps, next_value_exps;
   bool next_hidden;
+  const int lane_zero = zero_of_lanes();
   auto ask = [&](int p) {
     const int step = p - begin;
-    if (step > 0 && step % kWave == 0) numbers = table[min(p + lane, a.cache.per_seq - 1)];
+    if (step > 0 && step % kWave == 0) {
+      numbers = table[min(p + lane, a.cache.per_seq - 1)];
+      asm volatile("" : "+v"(numbers));  // waited for here, not wherever it is read
+    }
     const int number = __builtin_amdgcn_readlane(numbers, step % kWave);
     next_hidden = number < 0 || number >= a.cache.pages;
     const int page = next_hidden ? 0 : number;
@@ -456,8 +473,8 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
       piece[j] = *reinterpret_cast<const uint4*>(x < 4 * D ? a.cache.keys + at + 16 * x
                                                            : a.cache.values + at + 16 * (x - 4 * D));
     }
-    next_key_exps = *reinterpret_cast<const uint32_t*>(a.cache.key_exps + exp_at);
-    next_value_exps = *reinterpret_cast<const uint32_t*>(a.cache.value_exps + exp_at);
+    next_key_exps = *reinterpret_cast<const uint32_t*>(a.cache.key_exps + exp_at + lane_zero);
+    next_value_exps = *reinterpret_cast<const uint32_t*>(a.cache.value_exps + exp_at + lane_zero);
   };
   // Key 32 u + 8 g + 4 w + i is row 4 g + i of product t = 2 u + w, so a lane's
   // scores of products 2 u and 2 u + 1 are of the 8 keys that are its run of
@@ -545,7 +562,7 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
   // bad number, has all its keys masked.
   for (int p = begin; p < end; ++p) {
     const uint4* now = stage[(p - begin) % 2];
-    const uint32_t key_exps = next_key_exps, value_exps = next_value_exps;
+    const uint32_t key_exps = next_key_exps, value_exps = __builtin_amdgcn_readfirstlane(next_value_exps);
     const bool hidden = next_hidden;
     if (hidden && tid == 0) atomicOr(a.error, kKv8BadRows);
     __syncthreads();  // this page is in LDS, and every wave is done with the one before
