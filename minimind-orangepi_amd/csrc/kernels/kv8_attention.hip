@@ -453,6 +453,13 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
 
   const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
   int numbers = table[min(begin + lane, a.cache.per_seq - 1)];
+  float v[8 * kRuns];  // of the query, which does not wait for a page's number
+#pragma unroll
+  for (int c = 0; c < kRuns; ++c)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<float4*>(v + 8 * c + 4 * i) =
+          *reinterpret_cast<const float4*>(a.query + row * D + 32 * c + 8 * g + 4 * i);
   uint4 piece[kPieces];
   uint32_t next_key_exps, next_value_exps;
   bool next_hidden;
@@ -511,13 +518,6 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
   float unit;        // of a score, in log2
   bool bad = false;  // a query that is not finite gives a row of NaN
   {
-    float v[8 * kRuns];
-#pragma unroll
-    for (int c = 0; c < kRuns; ++c)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<float4*>(v + 8 * c + 4 * i) =
-            *reinterpret_cast<const float4*>(a.query + row * D + 32 * c + 8 * g + 4 * i);
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8 * kRuns; ++i) {

@@ -21,7 +21,8 @@
 // Measured in replayed graphs, 1.6 us of them any kernel's: 1152 x 768 in groups
 // of 32 for one row 4.1 us (latency), 32768 x 4096 in groups of 128 15.5 us, 69.4
 // MB at 4.5 TB/s, 4096 x 768 for 32 rows 6.4 us (two launches), 16384 x 4096 for 32
-// rows 39.7: there each lane's 16 bytes of codes are a line of their own.
+// rows 28.7: there every two tiles of weight rows read all digits of 16 rows of
+// x, 256 KB, from the L2.
 #include "device_common.h"
 
 #include <algorithm>
@@ -53,6 +54,13 @@ constexpr int kManyTiles = 4;       // x operands of a block whose digits come f
 // Tiles from which such a block takes two and reads the operands for both
 // (4096 x 768 for 32 rows: 6.8 us with one, 6.4; 768 x 2048 8.4 and 9.9).
 constexpr int kTwoTiles = 256;
+
+// Blocks of the form whose codes go through LDS, with kTilesOfWave tiles a wave,
+// from which it is taken for many rows of x: one a compute unit (groups of 64,
+// 32 rows: 8192 x 2048, 256 blocks, 11.9 us and 14.5 without; 4096 x 2048, 128
+// blocks, 11.1 and 10.3; 16384 x 4096, 1024 blocks, 28.7 and 39.5).
+constexpr int kWideRowsBlocks = 256;
+constexpr int kTilesOfWave = 2;
 
 using i32x4 = int __attribute__((ext_vector_type(4)));
 
@@ -321,19 +329,53 @@ __global__ __launch_bounds__(kQ4Threads) void matvec_q4_kernel(MatvecQ4Args a, Q
   finish_checked(a, f, d, broken, y, row);
 }
 
-// Many tiles: a block takes kQ4Waves / f.share of them at a time, and then
-// further ones; f.share waves share a tile's columns, a chunk of kAhead runs
-// each in turn.  For whole runs with an even number of groups in a row.
-//
-// A lane of a product needs 16 bytes of its own weight row, and a load that
-// goes by that asks for 64 places a row apart, one a cycle.  So a chunk's codes
-// go to LDS with direct loads, 256 bytes of four rows each, and its scales four
-// bytes a lane, kRing chunks of a wave under way; pieces of 16 bytes change
-// places within a row by its number, so that lanes that read the same piece of
-// 16 rows use all banks.  The waits are counted by hand: all that a wave has
-// under way are its chunks, kChunkLoads loads each, which return in order.
+// Many tiles.  A lane of a product needs 16 bytes of its own weight row, and a
+// load that goes by that asks for 64 places a row apart, one a cycle.  So the
+// codes of a chunk, kAhead runs of 16 rows, go to LDS with direct loads, 256
+// bytes of four rows each, and its scales four bytes a lane; pieces of 16 bytes
+// change places within a row by its number, so that lanes that read the same
+// piece of 16 rows use all banks.  For whole runs with an even number of groups
+// in a row.
+template <int kGroup>
+struct Chunk {
+  static constexpr int kGroups = Run<kGroup>::kGroups;
+  static constexpr int kWords = kAhead * kGroups / 2;  // of a row's scales
+  static constexpr int kScaleLoads = (16 * kWords + kWave - 1) / kWave;
+  static constexpr int kLoads = kAhead + kScaleLoads;
+
+  // Into LDS at `to`.  What is past the last row, run or group is read as the last.
+  static __device__ __forceinline__ void ask(const MatvecQ4Args& a, const Q4Form& f, int tile, int first, uint32_t to) {
+    const int lane = threadIdx.x % kWave, g = lane / 16, col = lane % 16, row_bytes = f.runs * 64;
+    const int last_row = a.rows - 1 - tile * kQ4Tile;
+    const uint8_t* codes = a.codes + static_cast<int64_t>(tile) * kQ4Tile * row_bytes;
+    const __half* scales = a.scales + static_cast<int64_t>(tile) * kQ4Tile * f.groups;
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int row = 4 * q + g, piece = col ^ row;
+      dma_load<16>(codes, min(row, last_row) * row_bytes + min(first + piece / 4, f.runs - 1) * 64 + piece % 4 * 16,
+                   to + q * 1024);
+    }
+#pragma unroll
+    for (int q = 0; q < kScaleLoads; ++q) {
+      const int i = q * kWave + lane, row = min(i / kWords, min(last_row, kQ4Tile - 1));
+      const int word = min(first * kGroups / 2 + i % kWords, f.groups / 2 - 1);
+      dma_load<4>(scales, (row * f.groups + 2 * word) * 2, to + kCodeBytes + q * 256);
+    }
+  }
+  static __device__ __forceinline__ Run<kGroup> run(const int8_t* chunk, int j) {
+    const int lane = threadIdx.x % kWave, g = lane / 16, col = lane % 16;
+    Run<kGroup> w;
+    w.codes = *reinterpret_cast<const uint4*>(chunk + col * 256 + ((4 * j + g) ^ col) * 16);
+    const __half* s = reinterpret_cast<const __half*>(chunk + kCodeBytes) + col * 2 * kWords + j * kGroups;
+#pragma unroll
+    for (int n = 0; n < kGroups; ++n) w.scales[n] = s[n];
+    return w;
+  }
+};
+
+// While `later` chunks after it are under way.
 template <int kLoads>
-__device__ __forceinline__ void wait_for_chunk(int later) {  // while `later` chunks after it are under way
+__device__ __forceinline__ void wait_for_chunk(int later) {
   static_assert(kRing == 3, "one wait for each number of later chunks");
   if (later >= 2)
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * kLoads) : "memory");
@@ -343,45 +385,30 @@ __device__ __forceinline__ void wait_for_chunk(int later) {  // while `later` ch
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
 }
 
+// Up to four batch rows: a block takes kQ4Waves / f.share tiles at a time, and
+// then further ones; f.share waves share a tile's columns, a chunk each in turn,
+// with kRing chunks of a wave under way.  The waits are counted by hand: all that
+// a wave has under way are its chunks, kLoads loads each, which return in order.
 template <int kGroup, int kUnits>
 __global__ __launch_bounds__(kQ4Threads) void matvec_q4_wide_kernel(MatvecQ4Args a, Q4Form f) {
   extern __shared__ __align__(16) int8_t shared[];  // chunks [waves][kRing][codes, scales], then digits
   __shared__ Digits<kUnits, kQ4Waves> d;
   __shared__ float sums[2][kQ4Waves][kWave];
-  constexpr int kGroups = Run<kGroup>::kGroups;
-  constexpr int kWords = kAhead * kGroups / 2;            // of a row's scales in a chunk
-  constexpr int kScaleLoads = (16 * kWords + kWave - 1) / kWave, kChunkLoads = kAhead + kScaleLoads;
   int8_t* const digits = shared + kQ4Waves * kRing * kChunkBytes;
   const int lane = threadIdx.x % kWave, g = lane / 16, col = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int at_once = kQ4Waves / f.share, part = wave % f.share, slot = wave / f.share;
-  const int tiles = (a.rows + kQ4Tile - 1) / kQ4Tile, stride = gridDim.x * at_once, row_bytes = f.runs * 64;
+  const int tiles = (a.rows + kQ4Tile - 1) / kQ4Tile, stride = gridDim.x * at_once;
   const int turns = (tiles - static_cast<int>(blockIdx.x) * at_once + stride - 1) / stride;  // of this block
   const int chunks = (f.runs + kAhead - 1) / kAhead, steps = (chunks + f.share - 1) / f.share;
   int8_t* const ring = shared + wave * kRing * kChunkBytes;
   const uint32_t ring_at = __builtin_amdgcn_readfirstlane(lds_address(ring));
 
-  // What is past the last tile, row, run or group is read as the last, and not used.
+  // What is past the last tile is read as the last, and not used.
   int ask_tile = blockIdx.x * at_once + slot, ask_step = 0, ask_place = 0;
   auto ask = [&]() {
-    const int tile = min(ask_tile, tiles - 1), first = (ask_step * f.share + part) * kAhead;
-    const int last_row = a.rows - 1 - tile * kQ4Tile;
-    const uint8_t* codes = a.codes + static_cast<int64_t>(tile) * kQ4Tile * row_bytes;
-    const __half* scales = a.scales + static_cast<int64_t>(tile) * kQ4Tile * f.groups;
-    const uint32_t to = ring_at + ask_place * kChunkBytes;
-#pragma unroll
-    for (int q = 0; q < kAhead; ++q) {
-      const int row = 4 * q + g, piece = col ^ row;
-      dma_load<16>(codes,
-                   min(row, last_row) * row_bytes + min(first + piece / 4, f.runs - 1) * 64 + piece % 4 * 16,
-                   to + q * 1024);
-    }
-#pragma unroll
-    for (int q = 0; q < kScaleLoads; ++q) {
-      const int i = q * kWave + lane, row = min(i / kWords, min(last_row, kQ4Tile - 1));
-      const int word = min(first * kGroups / 2 + i % kWords, f.groups / 2 - 1);
-      dma_load<4>(scales, (row * f.groups + 2 * word) * 2, to + kCodeBytes + q * 256);
-    }
+    Chunk<kGroup>::ask(a, f, min(ask_tile, tiles - 1), (ask_step * f.share + part) * kAhead,
+                       ring_at + ask_place * kChunkBytes);
     ask_place = ask_place + 1 < kRing ? ask_place + 1 : 0;
     if (++ask_step == steps) ask_step = 0, ask_tile += stride;
   };
@@ -402,18 +429,13 @@ __global__ __launch_bounds__(kQ4Threads) void matvec_q4_wide_kernel(MatvecQ4Args
   int tile = blockIdx.x * at_once + slot, step = 0, turn = 0, place = 0;
   float y = 0.0f;
   for (int at = 0; at < total; ++at) {
-    wait_for_chunk<kChunkLoads>(total - 1 - at);
+    wait_for_chunk<Chunk<kGroup>::kLoads>(total - 1 - at);
     const int8_t* chunk = ring + place * kChunkBytes;
     place = place + 1 < kRing ? place + 1 : 0;
     const int first = (step * f.share + part) * kAhead;
     Run<kGroup> w[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      w[j].codes = *reinterpret_cast<const uint4*>(chunk + col * 256 + ((4 * j + g) ^ col) * 16);
-      const __half* s = reinterpret_cast<const __half*>(chunk + kCodeBytes) + col * 2 * kWords + j * kGroups;
-#pragma unroll
-      for (int n = 0; n < kGroups; ++n) w[j].scales[n] = s[n];
-    }
+    for (int j = 0; j < kAhead; ++j) w[j] = Chunk<kGroup>::run(chunk, j);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) y = use_run(w[j], d, operand, rows, min(first + j, f.runs), b, y);
     asm volatile("" : "+v"(y) : : "memory");  // the chunk is read
@@ -476,6 +498,19 @@ __global__ __launch_bounds__(kQ4Threads) void q4_digits_kernel(MatvecQ4Args a, Q
   }
 }
 
+__device__ __forceinline__ void finish_rows(const MatvecQ4Args& a, const Q4Form& f, const float* units, float y, int b,
+                                            int row) {
+  if (y != y && b < a.batch && row < a.rows) {  // a unit of the row is NaN, or the sum overflowed
+    bool bad = false;
+    for (int u = 0; u < f.runs; ++u) {
+      const float unit = units[static_cast<int64_t>(b) * f.runs + u];
+      bad = bad || unit != unit;
+    }
+    if (bad) y = plain_product(a, f, b, row, units[static_cast<int64_t>(a.batch) * f.runs + b]);
+  }
+  finish(a, f, y, b, row);
+}
+
 // More rows of x: kTiles x 16 weight rows and 16 batch rows a block, whose
 // waves share the columns; x digits from the workspace.
 template <int kGroup, int kTiles>
@@ -519,15 +554,74 @@ __global__ __launch_bounds__(kQ4Threads) void matvec_q4_rows_kernel(MatvecQ4Args
     float total = sums[0][t][k][lane];
 #pragma unroll
     for (int w = 1; w < kQ4Waves; ++w) total += sums[w][t][k][lane];
-    if (total != total && b < a.batch && row < a.rows) {  // a unit of the row is NaN, or the sum overflowed
-      bool bad = false;
-      for (int u = 0; u < f.runs; ++u) {
-        const float unit = units[static_cast<int64_t>(b) * f.runs + u];
-        bad = bad || unit != unit;
+    finish_rows(a, f, units, total, b, row);
+  }
+}
+
+// The same where there are tiles or batch rows enough: two tiles and 16 batch
+// rows a group of f.share waves, which share the columns a chunk each in turn,
+// codes through LDS (Chunk).  One chunk of a wave at a time: 16 waves a compute
+// unit hide each other's waits.
+template <int kGroup>
+__global__ __launch_bounds__(kQ4Threads, 4) void matvec_q4_wide_rows_kernel(MatvecQ4Args a, Q4Form f) {
+  constexpr int kTiles = kTilesOfWave;
+  __shared__ __align__(16) int8_t shared[kQ4Waves * kTiles * kChunkBytes];  // chunks, then sums
+  const int8_t* base = static_cast<const int8_t*>(a.workspace);
+  const float* units = reinterpret_cast<const float*>(base + q4_units_offset(f.runs, a.batch));
+  const int lane = threadIdx.x % kWave, g = lane / 16, col = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int part = wave % f.share, slot = wave / f.share, tiles = (a.rows + kQ4Tile - 1) / kQ4Tile;
+  const int tile0 = (blockIdx.x * (kQ4Waves / f.share) + slot) * kTiles, b0 = blockIdx.y * kManyTiles * kQ4Batch;
+  const int operands = (a.batch + kQ4Batch - 1) / kQ4Batch, chunks = (f.runs + kAhead - 1) / kAhead;
+  const int8_t* const own = shared + wave * kTiles * kChunkBytes;
+  const uint32_t own_at = __builtin_amdgcn_readfirstlane(lds_address(own));
+  float y[kManyTiles][kTiles] = {};
+  for (int chunk = part; chunk < chunks; chunk += f.share) {
+    // Tiles past the last are read as the last and not stored.
+#pragma unroll
+    for (int k = 0; k < kTiles; ++k)
+      Chunk<kGroup>::ask(a, f, min(tile0 + k, tiles - 1), chunk * kAhead, own_at + k * kChunkBytes);
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+#pragma unroll 1
+    for (int j = 0; j < min(kAhead, f.runs - chunk * kAhead); ++j) {
+      const int run = chunk * kAhead + j;
+      Run<kGroup> w[kTiles];
+#pragma unroll
+      for (int k = 0; k < kTiles; ++k) w[k] = Chunk<kGroup>::run(own + k * kChunkBytes, j);
+      // Operands past the last are read as the last and not stored.
+      i32x4 x[kManyTiles][2];
+      float unit[kManyTiles];
+#pragma unroll
+      for (int t = 0; t < kManyTiles; ++t) {
+        const int o = min(b0 / kQ4Batch + t, operands - 1);
+        const int8_t* d = base + (static_cast<int64_t>(o) * f.runs + run) * kQ4Operands + lane * 16;
+        x[t][0] = *reinterpret_cast<const i32x4*>(d);
+        x[t][1] = *reinterpret_cast<const i32x4*>(d + kQ4Operands / 2);
+        unit[t] = units[static_cast<int64_t>(min(o * kQ4Batch + g, a.batch - 1)) * f.runs + run];
       }
-      if (bad) total = plain_product(a, f, b, row, units[static_cast<int64_t>(a.batch) * f.runs + b]);
+#pragma unroll
+      for (int t = 0; t < kManyTiles; ++t)
+#pragma unroll
+        for (int k = 0; k < kTiles; ++k) y[t][k] = fmaf(run_product<kGroup>(w[k], x[t][0], x[t][1]), unit[t], y[t][k]);
     }
-    finish(a, f, total, b, row);
+#pragma unroll
+    for (int t = 0; t < kManyTiles; ++t)
+#pragma unroll
+      for (int k = 0; k < kTiles; ++k) asm volatile("" : "+v"(y[t][k]) : : "memory");  // the chunk is read
+  }
+  __syncthreads();
+  float* const sums = reinterpret_cast<float*>(shared);  // [waves][batch tiles][tiles][lanes]
+#pragma unroll
+  for (int t = 0; t < kManyTiles; ++t)
+#pragma unroll
+    for (int k = 0; k < kTiles; ++k) sums[((wave * kManyTiles + t) * kTiles + k) * kWave + lane] = y[t][k];
+  __syncthreads();
+  for (int i = part; i < kManyTiles * kTiles; i += f.share) {
+    const int t = i / kTiles, k = i % kTiles, b = b0 + t * kQ4Batch + g, row = (tile0 + k) * kQ4Tile + col;
+    float total = 0.0f;
+    for (int n = 0; n < f.share; ++n)
+      total += sums[((slot * f.share + n) * kManyTiles * kTiles + i) * kWave + lane];
+    finish_rows(a, f, units, total, b, row);
   }
 }
 
@@ -558,7 +652,13 @@ void launch_q4(const MatvecQ4Args& a, const Q4Form& f, hipStream_t stream) {
   }
   const int many = (a.batch + kManyTiles * kQ4Batch - 1) / (kManyTiles * kQ4Batch);
   q4_digits_kernel<<<a.batch, kQ4Threads, 0, stream>>>(a, f);
-  if (tiles >= kTwoTiles)
+  Q4Form wide = f;
+  wide.share = 1;
+  while (wide.share < kQ4Waves && wide.share * kAhead < f.runs) wide.share *= 2;
+  const int at_once = kTilesOfWave * (kQ4Waves / wide.share), blocks = (tiles + at_once - 1) / at_once;
+  if (f.even && static_cast<int64_t>(blocks) * many >= kWideRowsBlocks) {
+    matvec_q4_wide_rows_kernel<kGroup><<<dim3(blocks, many), kQ4Threads, 0, stream>>>(a, wide);
+  } else if (tiles >= kTwoTiles)
     matvec_q4_rows_kernel<kGroup, 2><<<dim3((tiles + 1) / 2, many), kQ4Threads, 0, stream>>>(a, f);
   else
     matvec_q4_rows_kernel<kGroup, 1><<<dim3(tiles, many), kQ4Threads, 0, stream>>>(a, f);

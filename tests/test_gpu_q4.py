@@ -115,6 +115,20 @@ def test_most_columns_of_one_launch(gpu, batch, cols, rows):
     Call(gpu, np.random.default_rng(cols + batch), rows, cols, 32, batch, 1).check()
 
 
+@pytest.mark.parametrize("rows,cols,batch", [(8210, 2048, 20), (4112, 4096, 33), (1030, 4096, 130), (16390, 768, 17),
+                                             (520, 8192, 260), (40, 512, 4100)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_product_of_many_rows_and_many_of_x(gpu, rows, cols, batch, group):
+    """Two tiles a wave and 16 rows of x, the codes in chunks of four runs; ragged rows, tiles, chunks and rows of x."""
+    print(f"[case] q4 {rows}x{cols} group {group} batch {batch}", flush=True)
+    Call(gpu, np.random.default_rng(rows + cols + group + batch), rows, cols, group, batch).check()
+
+
+@pytest.mark.parametrize("prologue,epilogue", [(1, 2), (2, 1), (0, 2)])
+def test_fused_forms_of_many_rows_and_many_of_x(gpu, prologue, epilogue):
+    Call(gpu, np.random.default_rng(prologue + epilogue), 8222, 2048, 32, 19, prologue, epilogue).check()
+
+
 def test_most_rows_of_x(gpu):
     Call(gpu, np.random.default_rng(19), 18, 160, 32, 65536).check()
 
@@ -159,7 +173,7 @@ def test_x_of_any_size(gpu, batch):
 
 
 @pytest.mark.parametrize("prologue", [0, 1])
-@pytest.mark.parametrize("batch,rows", [(1, 70), (3, 70), (9, 70), (2, 8230)])
+@pytest.mark.parametrize("batch,rows", [(1, 70), (3, 70), (9, 70), (2, 8230), (140, 8230)])
 def test_x_that_is_not_finite(gpu, batch, rows, prologue):
     """Infinities and NaN go where the formula takes them, and to no other row of x."""
     rng = np.random.default_rng(13)
