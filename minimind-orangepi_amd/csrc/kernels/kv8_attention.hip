@@ -129,8 +129,8 @@ __device__ __forceinline__ void store_ml(const Kv8AttnArgs& a, int64_t row, int 
 // Steps: waves take the pages of a split in turn and join their results at the
 // end.  Waves wait for memory half of their time, the vector units are busy 19 %
 // of it: what counts is that a wave always has a page under way.  32 sequences
-// of up to 8,192 tokens, two KV heads of d 96: 72 MB in 19.2 us with the join, 3.8
-// TB/s; one query over 32,768 13.1 us, over 500 7.2 (replayed graph, 1.6 of them
+// of up to 8,192 tokens, two KV heads of d 96: 72 MB in 18.5 us with the join, 3.9
+// TB/s; one query over 32,768 11.5 us, over 500 7.2 (replayed graph, 1.6 of them
 // any kernel's): two dependent loads, one page's arithmetic, the join in LDS.
 template <int D>
 __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a, int chunk, int splits) {
@@ -406,14 +406,14 @@ __device__ __forceinline__ void split2_truncated(float x0, float x1, uint32_t& h
 // 16 rows a wave, all waves over the same pages, which the block widens into
 // LDS: the operands of every product, 16 bytes a lane in the order of lanes.
 //
-// Measured: 3,000 rows after 1,111, 8 heads of d 96 over two KV heads, 77 us a
-// call (9 of them the join), 311 TFLOP/s of the formula's products, of which
-// the two planes make twice as many.  Vector units are busy 48 % of the
-// kernel, matrix cores 26 %, LDS 26 %; with the lower planes' products, the
-// exponentials or the widening of pages left out, one at a time, it takes 70
-// to 75 us, so it is none of them but the chain barrier - LDS - products -
-// weights - products with three waves a SIMD.  32 rows a wave (half the LDS reads a row, two waves
-// a SIMD) took 84 us, blocks of eight waves 101.
+// Measured: 3,000 rows after 1,111, 8 heads of d 96 over two KV heads, 75 us a
+// call (9 of them the join), 320 TFLOP/s of the formula's products, of which
+// the two planes make twice as many.  Vector units are busy 50 % of the
+// kernel, matrix cores 27 %, LDS 28 %; with the lower planes' products, the
+// exponentials or the widening of pages left out, one at a time, it took 70 to
+// 75 us of 78, so it is none of them but the chain barrier - LDS - products -
+// weights - products with three waves a SIMD.  32 rows a wave (half the LDS
+// reads a row, two waves a SIMD) took as long, blocks of eight waves 101.
 template <int D>
 __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel(Kv8AttnArgs a, int chunk, int splits) {
   constexpr int kTiles = D / 16, kRuns = D / 32;  // tiles of the output, products along D
