@@ -75,6 +75,73 @@ def test_append(gpu, hq, hkv, d, rows, context):
     Append(gpu, cache, hq, rng=rng).check(qkv_rows(rng, sum(rows) + 2, hq, hkv, d), rows, context)
 
 
+@pytest.mark.parametrize("which", [0, 1])
+def test_append_with_one_norm(gpu, which):
+    rng = np.random.default_rng(51)
+    cache = ref.Cache(rng, 4, 1, 4, 2, 96)
+    step = Append(gpu, cache, 8, rng=rng)
+    step.norms[which] = step.dnorms[which] = None
+    step.check(qkv_rows(rng, 70, 8, 2, 96), [70], [3])
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(130, 1, 32), (64, 64, 32), (24, 3, 64)])
+@pytest.mark.parametrize("rows,context", [([1, 1], [200, 30]), ([4, 70], [77, 0])])
+def test_many_heads(gpu, hq, hkv, d, rows, context):
+    """More heads than a tile of the attention has rows, and as many KV heads as there may be."""
+    print(f"[case] heads {hq},{hkv},{d} rows {rows}", flush=True)
+    rng = np.random.default_rng(hq + sum(rows))
+    per = pages_for(rows, context)
+    cache = ref.Cache(rng, 2 * per, 2, per, hkv, d)
+    cache.fill(rng, context)
+    Append(gpu, cache, hq, rng=rng).check(qkv_rows(rng, sum(rows), hq, hkv, d), rows, context)
+    query = rng.standard_normal((sum(rows), hq * d)).astype(np.float32)
+    check_attention(gpu, cache, query, rows, context, hq)
+
+
+def test_rows_before_the_first_sequence(gpu):
+    """offsets[0] above 0: the rows before it are nobody's, and stay."""
+    mmr, rng = gpu, np.random.default_rng(53)
+    hq, hkv, d = 8, 2, 96
+    cache = ref.Cache(rng, 4, 2, 2, hkv, d)
+    cache.fill(rng, [40, 3])
+    step = Append(mmr, cache, hq, rng=rng)
+    qkv, offsets, context = qkv_rows(rng, 20, hq, hkv, d), np.array([5, 6, 18], np.int32), [40, 3]
+    fill = np.full((20, hq * d), 7.5, np.float32)
+    query = mmr.DeviceArray.from_numpy(fill)
+    mmr.kv8_append(mmr.DeviceArray.from_numpy(qkv), *step.dnorms, EPS, step.rope, step.device, ints(mmr, offsets),
+                   ints(mmr, context), 20, 12, hq, query, step.error)
+    want = ref.append(cache, qkv, offsets, context, hq, THETA, *step.norms, EPS, fill)
+    cache.assert_equals(step.device)
+    assert (np.abs(query.numpy() - want) <= HALF_STEP * np.abs(want) + 1e-12).all()
+    q = query.numpy()
+    got, error = attend(mmr, step.device, cache, q, offsets, context, hq, max_rows=12)
+    want, bound = ref.attention(cache, q, offsets, context, hq, fill)
+    assert error == 0 and int(step.error.numpy()[0]) == 0
+    assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("seqs,rows", [(65535, 1), (9000, 3)])
+def test_most_sequences_on_shared_pages(gpu, seqs, rows):
+    """Every sequence has the same pages, one of them twice."""
+    rng = np.random.default_rng(55)
+    hq, hkv, d, kinds = 4, 2, 32, 5
+    cache = ref.Cache(rng, kinds * 3, kinds, 3, hkv, d)
+    cache.table[:] = [4, 9, 4]
+    cache.fill(rng, [192] * kinds)
+    context = np.array([0, 63, 64, 100, 188], np.int32)
+    query = rng.standard_normal((kinds * rows, hq * d)).astype(np.float32)
+    want, bound = ref.attention(cache, query, np.arange(kinds + 1) * rows, context, hq, query)
+    kind = np.arange(seqs) % kinds
+    row = (kind[:, None] * rows + np.arange(rows)).reshape(-1)
+    good = cache.upload(gpu)
+    table = gpu.DeviceArray.from_numpy(np.tile(cache.table[:1], (seqs, 1)))
+    many = gpu.Kv8Pages(*good.buffers[:4], table, cache.pages, seqs, 3, hkv, d)
+    cache.seqs = seqs
+    got, error = attend(gpu, many, cache, query[row], np.arange(seqs + 1) * rows, context[kind], hq, max_rows=rows)
+    assert error == 0
+    assert (np.abs(got - want[row]) <= bound[row]).all()
+
+
 def test_append_token_by_token_moves_blocks(gpu):
     """Every token larger than the ones before: the block's codes move to a larger exponent again and again."""
     rng = np.random.default_rng(5)

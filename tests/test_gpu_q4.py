@@ -172,6 +172,38 @@ def test_x_of_any_size(gpu, batch):
     c.check()
 
 
+class Behind:
+    """An array behind a few elements of its type: aligned to that type only."""
+
+    def __init__(self, mmr, a, skip):
+        self.whole = mmr.DeviceArray.from_numpy(np.concatenate([np.zeros(skip, a.dtype), a.reshape(-1)]))
+        self.skip, self.shape, self.nbytes = skip, a.shape, a.nbytes
+        self.ptr = self.whole.ptr + skip * a.dtype.itemsize
+
+    def numpy(self):
+        return self.whole.numpy()[self.skip:].reshape(self.shape)
+
+
+@pytest.mark.parametrize("rows,batch", [(70, 1), (70, 9), (8230, 2), (8230, 40)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_operands_aligned_to_their_type_only(gpu, rows, batch, group):
+    c = Call(gpu, np.random.default_rng(rows + batch), rows, 768, group, batch, 1, gpu.EPI_RESIDUAL)
+    c.dw = c.dw[0], Behind(gpu, c.scales, 1)
+    c.dnorm, c.dres = Behind(gpu, c.norm, 1), Behind(gpu, c.residual, 3)
+    y = Behind(gpu, np.zeros((batch, rows), np.float32), 1)
+    got, (want, off) = c.run(dx=Behind(gpu, c.x, 3), y=y).numpy(), c.expected()
+    assert (np.abs(got - want) <= off).all()
+    assert y.whole.numpy()[0] == 0
+
+
+@pytest.mark.parametrize("batch", [1, 3, 20])
+def test_norm_of_zeros(gpu, batch):
+    c = Call(gpu, np.random.default_rng(21), 64, 256, 32, batch, 1)
+    c.x[-1] = 0
+    got, (want, off) = c.run().numpy(), c.expected()
+    assert (np.abs(got - want) <= off).all() and (got[-1] == 0).all()
+
+
 @pytest.mark.parametrize("prologue", [0, 1])
 @pytest.mark.parametrize("batch,rows", [(1, 70), (3, 70), (9, 70), (2, 8230), (140, 8230)])
 def test_x_that_is_not_finite(gpu, batch, rows, prologue):
