@@ -49,7 +49,9 @@ constexpr int kFewSplits = 8;
 constexpr int kRowsTile = 64;          // rows of a block of the kernel for many
 constexpr int kRowsPBits = 10;          // its p in units of 2^-10: at most 2^15 with the lead
 constexpr int kPBits = 28;              // p of steps in units of 2^-28: at most 2^30 with the lead
-constexpr int kLeastPages = 4, kWidePages = 16, kStepBlocks = 256, kRowsBlocks = 1280, kFewRows = 256;  // see kv8_attention_plan
+// See kv8_attention_plan.
+constexpr int kLeastPages = 2, kLeastRowsPages = 4, kWidePages = 16;
+constexpr int kStepBlocks = 256, kRowsBlocks = 1280, kFewRows = 256;
 constexpr int kMostSplits = 64;         // a lane of a wave each in the join
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 using f32x4 = float __attribute__((ext_vector_type(4)));
@@ -422,7 +424,8 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
   __shared__ uint4 stage[2][(4 * kRuns + 2 * kTiles) * kOperand];  // K [4 t][runs], then V [2 u][tiles]
   const int s = blockIdx.y, hkv = a.cache.hkv, group = a.hq / hkv;
   const int grid_tiles = gridDim.x / (splits * hkv);
-  const int grid_tile = blockIdx.x % grid_tiles, h = blockIdx.x / grid_tiles % hkv, split = blockIdx.x / grid_tiles / hkv;
+  const int grid_tile = blockIdx.x % grid_tiles, h = blockIdx.x / grid_tiles % hkv;
+  const int split = blockIdx.x / grid_tiles / hkv;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int g = lane / 16, col = lane % 16;
   Kv8Span span;
@@ -700,7 +703,8 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_few_kernel(Kv8AttnAr
   const int used = splits_of(a, span, i, chunk, tile_rows);
   if (used == 1) return;
   const int64_t to = static_cast<int64_t>(span.first) * a.hq + i;
-  const float2* ml = reinterpret_cast<const float2*>(a.part + static_cast<int64_t>(a.rows) * a.hq * splits * d) + to * splits;
+  const float2* ml =
+      reinterpret_cast<const float2*>(a.part + static_cast<int64_t>(a.rows) * a.hq * splits * d) + to * splits;
   const float4* o = reinterpret_cast<const float4*>(a.part + to * splits * d) + quad;
   float4 v[kFewSplits];
   float2 of[kFewSplits];
@@ -741,7 +745,8 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_kernel(Kv8AttnArgs a
   const int used = splits_of(a, span, i, chunk, tile_rows);
   if (used == 1) return;
   const int64_t to = static_cast<int64_t>(span.first) * a.hq + i;
-  const float2* ml = reinterpret_cast<const float2*>(a.part + static_cast<int64_t>(a.rows) * a.hq * splits * D) + to * splits;
+  const float2* ml =
+      reinterpret_cast<const float2*>(a.part + static_cast<int64_t>(a.rows) * a.hq * splits * D) + to * splits;
   const float4* o = reinterpret_cast<const float4*>(a.part + to * splits * D) + quad;
   float2 of = make_float2(kNoRow, 0.0f);
   if (x < used) of = ml[x];
@@ -784,15 +789,19 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_kernel(Kv8AttnArgs a
 // Splits along the context, sized by the longest one a launch may meet (blocks
 // past a sequence's end leave at once).  Measured in replayed graphs, d 96, two
 // KV heads, us a call:
-//   steps of at most kWidePages pages take one block and no join: 8.7 at 1,000
-//   tokens (8.9 split over four), while at 2,000 the split wins (9.1, 11.4);
+//   steps of at most kWidePages pages take one block and no join: 9.0 for 32
+//   sequences of 1,000 tokens (10.1 split), while at 2,000 the split wins (8.7,
+//   11.3);
 //   more take kStepBlocks blocks in all (32 sequences of up to 4,000 tokens
-//   15.3; with 512 blocks 15.9, with 128 18.5) and at most kMostSplits splits
+//   14.2; with 384 blocks 19.6, with 192 15.1) and at most kMostSplits splits
 //   (one sequence of 32,768: 64 splits 13.5, 128 14.5);
 //   many rows take kRowsBlocks blocks, whose tiles see different numbers of
 //   keys (3,000 rows after 1,111: 80; with 768 blocks 87, 256 104), but at most
 //   kFewSplits splits, whose join is cheap, unless there are few rows (512 rows
-//   after 2,000: 24 with 8 splits, 32 with 16).
+//   after 2,000: 24 with 8 splits, 32 with 16);
+//   a split has kLeastPages pages (one query at 4,000 tokens 8.8, 5 rows there
+//   10.0; with four 9.1 and 12.5), of many rows kLeastRowsPages, which are more
+//   to join (1,500 rows 24.9; with three 28.4).
 Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens) {
   Kv8AttnPlan p;
   const int64_t most = static_cast<int64_t>(hq / hkv) * max_rows;
@@ -801,12 +810,13 @@ Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int m
   const bool step = p.tile_rows == 4;
   const int64_t blocks = (most + p.tile_rows - 1) / p.tile_rows * hkv * seqs;
   const int64_t wanted = step ? kStepBlocks : kRowsBlocks;
-  const int64_t splits = step || static_cast<int64_t>(rows) * hq <= kFewRows ? kMostSplits : kFewSplits;
+  const bool few = step || static_cast<int64_t>(rows) * hq <= kFewRows;
+  const int64_t splits = few ? kMostSplits : kFewSplits, least = few ? kLeastPages : kLeastRowsPages;
   // Of a prompt's tiles, the first sees the context and the last all of max_tokens.
   const int64_t mean = step ? pages : std::max<int64_t>(1, (2 * max_tokens - max_rows) / (2 * kKv8Page));
   int64_t chunk = pages;
   if (blocks < wanted && !(step && pages <= kWidePages))
-    chunk = std::max<int64_t>({kLeastPages, (mean * blocks + wanted - 1) / wanted, (pages + splits - 1) / splits});
+    chunk = std::max<int64_t>({least, (mean * blocks + wanted - 1) / wanted, (pages + splits - 1) / splits});
   p.chunk_pages = static_cast<int>(chunk);
   p.splits = static_cast<int>((pages + chunk - 1) / chunk);
   if (p.splits > 1) p.partial_floats = static_cast<int64_t>(rows) * hq * p.splits * (d + 2);
