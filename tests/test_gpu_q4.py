@@ -26,7 +26,7 @@ def product(w, x, norm, prologue, eps, epilogue, residual, mmr):
 
     A result is a sum of one product a group, each exact up to the rounding of x to 2^-31 of its run's largest value
     (a half step at most of that value, on at most 128 weights of 8 scales) and three fp32 roundings, added one after
-    another within a wave and then over four waves: (groups + 8) half steps of the sum of |w x|.  The normalised x is
+    another within a wave and then over eight waves: (groups + 8) half steps of the sum of |w x|.  The normalised x is
     off by a serial sum of cols / 256 squares, ten more roundings of its joins, the root, the quotient and two
     products."""
     batch, cols = x.shape
