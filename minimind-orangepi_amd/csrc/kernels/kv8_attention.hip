@@ -8,8 +8,8 @@
 // new one.  Two kernels, by the rows (token, head) that a sequence brings to a
 // group of heads that share their keys:
 //
-// Steps, up to 4 rows (a decode step of four heads): int8 matrix cores on the
-// codes as they are stored.  The fp32 operand goes in as fixed-point digits:
+// Steps, up to 8 rows (a decode step of eight heads), 4 a block: int8 matrix
+// cores on the codes as they are stored.  The fp32 operand goes in as fixed-point digits:
 // an integer n is the sum of d_k 256^k with d_k in [-128, 127], and the bytes
 // of n + 0x808080 are those digits, the lower three with their top bit
 // flipped.  Products and sums of digits and codes are exact in int32; rounded
@@ -44,6 +44,7 @@ constexpr int kStepWaves = 8, kStepThreads = kStepWaves * kWave;
 constexpr int kJoinThreads = 256;
 constexpr float kNoRow = -FLT_MAX / 2;  // reference of a row that has met no key
 constexpr float kStepLead = 2.0f, kRowsLead = 5.0f;  // a score may pass the reference by this much (log2)
+constexpr int kStepRows = 8, kStepTile = 4;  // rows that the kernel for steps takes, and of a block
 constexpr int kRowsThreads = 256;
 constexpr int kFewSplits = 8;
 constexpr int kRowsTile = 64;          // rows of a block of the kernel for many
@@ -136,9 +137,9 @@ __device__ __forceinline__ void store_ml(const Kv8AttnArgs& a, int64_t row, int 
 // any kernel's): two dependent loads, one page's arithmetic, the join in LDS.
 template <int D>
 __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a, int chunk, int splits) {
-  constexpr int kRows = 4, kTiles = D / 16;  // tiles of the output's dimensions
+  constexpr int kRows = kStepTile, kTiles = D / 16;  // tiles of the output's dimensions
   const int s = blockIdx.y, hkv = a.cache.hkv, group = a.hq / hkv;
-  const int split = blockIdx.x % splits, h = blockIdx.x / splits;
+  const int split = blockIdx.x % splits, h = blockIdx.x / splits, first = blockIdx.z * kRows;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const int g = lane / 16, col = lane % 16;
   // Page numbers of this wave's next 64 steps, one a lane: read along with the
@@ -152,16 +153,16 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
     if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(a.error, kKv8BadRows);
     return;
   }
-  const int total = span.n * group;  // rows of this group of heads
-  if (total == 0) return;
-  const int pages = (span.context + span.n - 1) / kKv8Page + 1;
+  const int total = min(span.n * group - first, kRows);  // rows of this group of heads, from `first` on
+  if (total <= 0) return;
+  const int last_key = span.context + (first + total - 1) / group, pages = last_key / kKv8Page + 1;
   const int used = splits_used(pages, chunk), end = min(begin + chunk, pages);
   if (split >= used) return;
 
   // This lane's column: digit `digit` of row m.
   const int m = col / 4, digit = col % 4;
   const bool is_row = m < total;
-  const int token = is_row ? m / group : 0, head = h * group + (is_row ? m % group : 0);
+  const int token = is_row ? (first + m) / group : 0, head = h * group + (is_row ? (first + m) % group : 0);
   const int limit = is_row ? span.context + token : -1;  // its last key
   const int64_t row = (static_cast<int64_t>(span.first) + token) * a.hq + head;
 
@@ -274,7 +275,7 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
     const uint32_t key_exps = next_key_exps, value_exps = __builtin_amdgcn_readfirstlane(next_value_exps);
     const bool hidden = next_hidden;
     // Blocks past the last key hold anything: their exponents don't count.
-    const int blocks = hidden ? 0 : min(kKv8Blocks, (span.context + span.n - 1 - p * kKv8Page) / kKv8Block + 1);
+    const int blocks = hidden ? 0 : min(kKv8Blocks, (last_key - p * kKv8Page) / kKv8Block + 1);
     int page_exp = kKv8MinExp - 1;
 #pragma unroll
     for (int b = 0; b < kKv8Blocks; ++b)
@@ -369,7 +370,8 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
       o += f * sh_out[w][mr][dim];
       ll += f * sh_l[w][mr];
     }
-    const int64_t to = (static_cast<int64_t>(span.first) + mr / group) * a.hq + h * group + mr % group;
+    const int64_t to =
+        (static_cast<int64_t>(span.first) + (first + mr) / group) * a.hq + h * group + (first + mr) % group;
     if (used == 1) {
       a.out[to * D + dim] = ll != 0.0f ? o / ll : 0.0f;
     } else {
@@ -789,6 +791,10 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_kernel(Kv8AttnArgs a
 // Splits along the context, sized by the longest one a launch may meet (blocks
 // past a sequence's end leave at once).  Measured in replayed graphs, d 96, two
 // KV heads, us a call:
+//   up to kStepRows rows of a KV head are steps, though the second block of four
+//   reads the pages again (one of eight heads at 32,768 tokens 14.9, 16
+//   sequences of up to 8,000 16.5; as many rows 20.9 and 22.9; 16 heads of 32
+//   sequences of up to 4,000 as steps 34.0, 23.2);
 //   steps of at most kWidePages pages take one block and no join: 9.0 for 32
 //   sequences of 1,000 tokens (10.1 split), while at 2,000 the split wins (8.7,
 //   11.3);
@@ -806,8 +812,8 @@ Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int m
   Kv8AttnPlan p;
   const int64_t most = static_cast<int64_t>(hq / hkv) * max_rows;
   const int64_t pages = (max_tokens + kKv8Page - 1) / kKv8Page;
-  p.tile_rows = most <= 4 ? 4 : kRowsTile;
-  const bool step = p.tile_rows == 4;
+  const bool step = most <= kStepRows;
+  p.tile_rows = step ? kStepTile : kRowsTile;
   const int64_t blocks = (most + p.tile_rows - 1) / p.tile_rows * hkv * seqs;
   const int64_t wanted = step ? kStepBlocks : kRowsBlocks;
   const bool few = step || static_cast<int64_t>(rows) * hq <= kFewRows;
@@ -828,11 +834,13 @@ namespace {
 template <int D>
 void launch_attention_for(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t stream) {
   const int hkv = a.cache.hkv, most = a.hq / hkv * a.max_rows;
-  const dim3 grid(p.splits * ((most + p.tile_rows - 1) / p.tile_rows) * hkv, a.cache.seqs);
-  if (p.tile_rows != 4)
-    kv8_rows_kernel<D><<<grid, kRowsThreads, 0, stream>>>(a, p.chunk_pages, p.splits);
+  const int tiles = (most + p.tile_rows - 1) / p.tile_rows;
+  if (p.tile_rows != kStepTile)
+    kv8_rows_kernel<D><<<dim3(p.splits * tiles * hkv, a.cache.seqs), kRowsThreads, 0, stream>>>(a, p.chunk_pages,
+                                                                                               p.splits);
   else
-    kv8_step_kernel<D><<<grid, kStepThreads, 0, stream>>>(a, p.chunk_pages, p.splits);
+    kv8_step_kernel<D><<<dim3(p.splits * hkv, a.cache.seqs, tiles), kStepThreads, 0, stream>>>(a, p.chunk_pages,
+                                                                                              p.splits);
   if (p.splits > 1 && p.splits <= kFewSplits) {
     const int each = kJoinThreads / (D / 4);
     kv8_combine_few_kernel<<<dim3((a.max_rows * a.hq + each - 1) / each, a.cache.seqs), kJoinThreads, 0, stream>>>(

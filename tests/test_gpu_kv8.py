@@ -253,7 +253,7 @@ def check_attention(mmr, cache, query, rows, context, hq):
 @pytest.mark.parametrize("hq,hkv,d", HEADS + [(12, 4, 96), (16, 1, 64), (3, 3, 128)])
 @pytest.mark.parametrize("rows,context", [
     ([1], [0]), ([1], [1]), ([1], [63]), ([1], [64]), ([1, 1, 1], [15, 777, 200]), ([1], [5000]),
-    ([3, 0, 5], [100, 7, 511]), ([17, 2], [0, 130]), ([64], [0]), ([150], [77])])
+    ([2, 1], [63, 700]), ([3, 0, 5], [100, 7, 511]), ([17, 2], [0, 130]), ([64], [0]), ([150], [77])])
 def test_attention(gpu, hq, hkv, d, rows, context):
     print(f"[case] attention {hq},{hkv},{d} rows {rows} context {context}", flush=True)
     rng = np.random.default_rng(sum(rows) * 17 + sum(context) + d)
@@ -277,7 +277,7 @@ def test_attention_over_many_rows_of_blocks(gpu, rows):
                     hq)
 
 
-@pytest.mark.parametrize("hq,hkv,d", [(4, 1, 32), (4, 4, 64), (8, 2, 96), (6, 3, 128)])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 1, 32), (4, 4, 64), (8, 2, 96), (6, 3, 128), (7, 1, 96)])
 @pytest.mark.parametrize("rows,context", [([1, 1], [20000, 16300]), ([30], [9000])])
 def test_attention_joins_many_splits(gpu, hq, hkv, d, rows, context):
     """As many splits as one join takes, and fewer of the second sequence; the same bits whenever it is called."""
@@ -482,7 +482,7 @@ def test_calls_on_two_streams_at_once(gpu):
         assert (np.abs(r["out"].numpy() - want) <= bound).all()
 
 
-@pytest.mark.parametrize("rows,context", [([1, 1], [100, 2000]), ([40, 90], [3, 600])])
+@pytest.mark.parametrize("rows,context", [([1, 1], [100, 2000]), ([2, 2], [100, 2000]), ([40, 90], [3, 600])])
 def test_out_in_place_of_the_query(gpu, rows, context):
     mmr, rng = gpu, np.random.default_rng(47)
     per = pages_for(rows, context)
