@@ -114,3 +114,56 @@ def test_prompts_and_steps(gpu, shape, group):
             graph.launch()
         mmr.synchronize()
         layer.check(cache, pages, np.arange(seqs + 1), context, seqs)
+
+
+def test_graphs_on_one_workspace(gpu):
+    """Three recorded calls that share a workspace, replayed in changing order on their stream with eager calls between:
+    nothing is kept in it from one call to the next."""
+    mmr, rng = gpu, np.random.default_rng(61)
+    hq, hkv, d, per = 8, 2, 96, 40
+    cache = ref.Cache(rng, 3 * per, 3, per, hkv, d)
+    cache.fill(rng, [2500, 700, 130])
+    pages, stream = cache.upload(mmr), mmr.Stream()
+
+    def upload(a):
+        return mmr.DeviceArray.from_numpy(a)
+
+    def attention(rows, context):
+        n, most = sum(rows), max(rows)
+        offsets = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+        q, out = upload(rng.standard_normal((n, hq * d)).astype(np.float32)), mmr.DeviceArray((n, hq * d), np.float32)
+        arrays = upload(offsets), upload(np.asarray(context, np.int32)), upload(np.zeros(1, np.int32))
+        size = mmr.kv8_attention_workspace_size(hq, hkv, d, 3, n, most, per * ref.PAGE)
+        return size, out, lambda ws, s: mmr.kv8_attention(q, pages, *arrays[:2], n, most, per * ref.PAGE, hq, out, ws,
+                                                          arrays[2], stream=s)
+
+    def matvec(rows, cols, batch):
+        codes, scales = mmr.q4_quantize(rng.standard_normal((rows, cols)).astype(np.float32), 32)
+        w, x = (upload(codes), upload(scales)), upload(rng.standard_normal((batch, cols)).astype(np.float32))
+        y = mmr.DeviceArray((batch, rows), np.float32)
+        return mmr.matvec_q4_workspace_size(cols, batch), y, lambda ws, s: mmr.matvec_q4(
+            *w, 32, rows, cols, x, batch, y, workspace=ws, stream=s)
+
+    calls = [attention([1, 1, 1], [2499, 699, 129]), attention([30, 40, 20], [2470, 660, 110]), matvec(300, 768, 40)]
+    workspace = mmr.DeviceArray(max(c[0] for c in calls), np.uint8)
+    assert min(c[0] for c in calls) > 0
+    mmr.synchronize()
+    want, graphs = [], []
+    for size, out, call in calls:
+        call(workspace, stream)
+        mmr.synchronize()
+        want.append(out.numpy())
+        with mmr.Graph(stream) as graph:
+            call(workspace, stream)
+        graphs.append(graph)
+    for order in ([0, 1, 2], [2, 1, 0], [1, 1, 0, 2], [0, 2, 0, 1], [2, 0, 1]):
+        for _, out, _ in calls:
+            out.zero()
+        workspace.upload(np.full(workspace.shape, 0xFF, np.uint8))
+        mmr.synchronize()
+        for i in order:
+            graphs[i].launch(stream)
+        calls[order[0]][2](workspace, stream)
+        mmr.synchronize()
+        for (_, out, _), a in zip(calls, want):
+            np.testing.assert_array_equal(out.numpy(), a)
