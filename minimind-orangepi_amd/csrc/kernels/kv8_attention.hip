@@ -118,6 +118,19 @@ __device__ __forceinline__ int zero_of_lanes() {
   return zero;
 }
 
+// The largest of a page's first `blocks` exponents.
+__device__ __forceinline__ int largest_exponent(uint32_t exps, int blocks) {
+  int e = kKv8MinExp - 1;
+#pragma unroll
+  for (int b = 0; b < kKv8Blocks; ++b)
+    if (b < blocks) e = max(e, static_cast<int>(static_cast<int8_t>(exps >> (8 * b))));
+  return e;
+}
+// Of the page whose first key is `first`, those whose keys a row with the last key `limit` attends.
+__device__ __forceinline__ int blocks_seen(int limit, int first) {
+  return min(kKv8Blocks, max(0, limit - first + kKv8Block) / kKv8Block);
+}
+
 // Splits of at most `chunk` pages each that a row's `pages` are dealt to, evenly.
 __device__ __forceinline__ int splits_used(int pages, int chunk) { return (pages + chunk - 1) / chunk; }
 
@@ -255,7 +268,7 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
   i32x4 sum[kTiles] = {};        // digits of the output since the last move
   float out[kTiles][4] = {};     // and before it
   float ref = kNoRow, l = 0.0f;  // l: of this lane's keys
-  int held_exp = kKv8MinExp - 1; // of V in sum
+  int held_exp = kKv8MinExp - 1; // of V in sum, for this lane's row
   int since = 0;
 
   auto move = [&](float factor) {  // sum into out, which then scales by factor
@@ -274,12 +287,6 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
   for (int p = from; p < end; p += kStepWaves) {
     const uint32_t key_exps = next_key_exps, value_exps = __builtin_amdgcn_readfirstlane(next_value_exps);
     const bool hidden = next_hidden;
-    // Blocks past the last key hold anything: their exponents don't count.
-    const int blocks = hidden ? 0 : min(kKv8Blocks, (last_key - p * kKv8Page) / kKv8Block + 1);
-    int page_exp = kKv8MinExp - 1;
-#pragma unroll
-    for (int b = 0; b < kKv8Blocks; ++b)
-      if (b < blocks) page_exp = max(page_exp, static_cast<int>(static_cast<int8_t>(value_exps >> (8 * b))));
     const int my_exp = static_cast<int8_t>(value_exps >> (8 * g));
 
     float score[4][4];
@@ -292,13 +299,18 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
     }
     ask();
     ask_keys();
+    // A row's sums are relative to the values that it attends: blocks past its
+    // last key, which hold anything, or what later rows attend, don't count.
+    int page_exp = largest_exponent(value_exps, kKv8Blocks);
     if (hidden) {
       if (lane == 0) atomicOr(a.error, kKv8BadRows);
+      page_exp = kKv8MinExp - 1;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) score[t][i] = -INFINITY;
     } else if (p * kKv8Page + kKv8Page - 1 > span.context) {  // the first token sees keys up to context
+      page_exp = largest_exponent(value_exps, blocks_seen(limit, p * kKv8Page));
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -311,7 +323,7 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, score[t][i]);
 
-    if (__any(top > ref + kStepLead) || page_exp > held_exp || since == kMostPages) {
+    if (__any(top > ref + kStepLead || page_exp > held_exp) || since == kMostPages) {
       const float next = fmaxf(ref, column_max(top));
       if (since > 0) move(__builtin_amdgcn_exp2f(ref - next));  // not before the first page
       ref = next;
@@ -450,7 +462,6 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
   const int wave_first = first + 16 * wave;
   const bool works = wave_first < total;
   const int all_see = span.context + min(wave_first, total - 1) / group;
-  const int wave_last = span.context + (min(wave_first + 16, total) - 1) / group;  // last key of any row
   const int m = wave_first + col, token = m < total ? m / group : 0;
   const int limit = m < total ? span.context + token : -1;  // its last key
   const int64_t row =
@@ -572,11 +583,6 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
     if (hidden && tid == 0) atomicOr(a.error, kKv8BadRows);
     __syncthreads();  // this page is in LDS, and every wave is done with the one before
     if (p + 1 < end) ask(p + 1);
-    const int blocks = hidden ? 0 : min(kKv8Blocks, (wave_last - p * kKv8Page + kKv8Block) / kKv8Block);
-    int page_exp = kKv8MinExp - 1;
-#pragma unroll
-    for (int b = 0; b < kKv8Blocks; ++b)
-      if (b < blocks) page_exp = max(page_exp, static_cast<int>(static_cast<int8_t>(value_exps >> (8 * b))));
     // Two sums at a time: a sum's products wait for each other.
     f32x4 score[4];
 #pragma unroll
@@ -602,7 +608,10 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
     const float key_scale[2] = {ldexpf(1.0f, static_cast<int8_t>(key_exps >> shift)),
                                 ldexpf(1.0f, static_cast<int8_t>(key_exps >> (16 + shift)))};
     float to_log2[2] = {unit * key_scale[0], unit * key_scale[1]};
+    // As for steps: of the blocks that the row attends.
+    int page_exp = largest_exponent(value_exps, kKv8Blocks);
     if (hidden || p * kKv8Page + kKv8Page - 1 > all_see) {
+      page_exp = largest_exponent(value_exps, hidden ? 0 : blocks_seen(limit, p * kKv8Page));
       // Scaled first: a factor may be 0 or, of a block that holds anything, infinite.
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -619,7 +628,7 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
 #pragma unroll
       for (int i = 0; i < 4; ++i) top[t / 2] = fmaxf(top[t / 2], score[t][i]);
     const float page_top = fmaxf(top[0] * to_log2[0], top[1] * to_log2[1]);
-    if (__any(page_top > ref + kRowsLead) || page_exp > held_exp) {
+    if (__any(page_top > ref + kRowsLead || page_exp > held_exp)) {
       const float next = fmaxf(ref, column_max(page_top));
       const int next_exp = max(held_exp, page_exp);
       const float f = __builtin_amdgcn_exp2f(ref - next), down = ldexpf(f, held_exp - next_exp);

@@ -495,3 +495,28 @@ def test_out_in_place_of_the_query(gpu, rows, context):
                       per * 64, 8, both, mmr.DeviceArray(max(size, 1), np.uint8), error)
     want, bound = ref.attention(cache, query, offsets_of(rows), context, 8, query)
     assert (np.abs(both.numpy() - want) <= bound).all()
+
+
+# (query heads, KV heads), rows and context: steps of one and of two blocks, and the kernel for many rows.
+BORDERS = [(2, 2, 2, 15), (2, 2, 4, 30), (2, 2, 3, 62), (4, 2, 3, 47), (2, 1, 4, 126), (4, 1, 9, 60), (6, 2, 20, 700),
+           (1, 1, 40, 8)]
+
+
+@pytest.mark.parametrize("hq,hkv,rows,context", BORDERS)
+@pytest.mark.parametrize("larger", [20, 28, 40])
+def test_attention_rows_before_far_larger_values(gpu, hq, hkv, rows, context, larger):
+    """A later row opens a block whose values are far larger: the rows that do not attend it lose nothing."""
+    print(f"[case] borders {hq},{hkv} rows {rows} context {context} larger {larger}", flush=True)
+    rng = np.random.default_rng(rows * 7 + context + larger)
+    per = pages_for([rows], [context])
+    cache = ref.Cache(rng, per, 1, per, hkv, 64)
+    cache.fill(rng, [rows + context])
+    for block in range(context // ref.BLOCK + 1, (context + rows - 1) // ref.BLOCK + 1):
+        # Each block that the rows open, larger than the one before.
+        cache.value_exps[cache.table[0, block * ref.BLOCK // ref.PAGE], :, block % 4] = (
+            -6 + larger * (block - context // ref.BLOCK))
+    query = rng.standard_normal((rows, hq * 64)).astype(np.float32)
+    got, error = attend(gpu, cache.upload(gpu), cache, query, [0, rows], [context], hq, max_rows=rows)
+    want, bound = ref.attention(cache, query, [0, rows], [context], hq, query)
+    assert error == 0
+    assert (np.abs(got - want) <= bound).all(), float((np.abs(got - want) / np.maximum(bound, 1e-300)).max())
