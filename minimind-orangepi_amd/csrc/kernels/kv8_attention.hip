@@ -172,11 +172,12 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
   const int used = splits_used(pages, chunk), end = min(begin + chunk, pages);
   if (split >= used) return;
 
-  // This lane's column: digit `digit` of row m.
-  const int m = col / 4, digit = col % 4;
-  const bool is_row = m < total;
-  const int token = is_row ? (first + m) / group : 0, head = h * group + (is_row ? (first + m) % group : 0);
-  const int limit = is_row ? span.context + token : -1;  // its last key
+  // This lane's column: digit `digit` of row m.  Columns past the last row are
+  // that row again: another block's row could change while it is read (out in
+  // place of query) and decide when this block's sums are scaled.
+  const int m = col / 4, digit = col % 4, at_row = first + min(m, total - 1);
+  const int token = at_row / group, head = h * group + at_row % group;
+  const int limit = span.context + token;  // its last key
   const int64_t row = (static_cast<int64_t>(span.first) + token) * a.hq + head;
 
   // The operands of the next page, asked for as soon as those of the page at
@@ -462,10 +463,9 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
   const int wave_first = first + 16 * wave;
   const bool works = wave_first < total;
   const int all_see = span.context + min(wave_first, total - 1) / group;
-  const int m = wave_first + col, token = m < total ? m / group : 0;
-  const int limit = m < total ? span.context + token : -1;  // its last key
-  const int64_t row =
-      (static_cast<int64_t>(span.first) + token) * a.hq + h * group + (m < total ? m % group : 0);
+  const int m = min(wave_first + col, total - 1), token = m / group;  // lanes past the last row are that row again
+  const int limit = span.context + token;                             // its last key
+  const int64_t row = (static_cast<int64_t>(span.first) + token) * a.hq + h * group + m % group;
 
   const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
   int numbers = table[min(begin + lane, a.cache.per_seq - 1)];
@@ -679,7 +679,7 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
   }
   l = column_sum(l);
   if (bad) l = __builtin_nanf("");
-  if (m >= total) return;
+  if (wave_first + col >= total) return;
   const float inv = used > 1 ? 1.0f : l != 0.0f ? 1.0f / l : 0.0f;
   float* to = used > 1 ? a.part + (row * splits + split) * D : a.out + row * D;
 #pragma unroll

@@ -520,3 +520,24 @@ def test_attention_rows_before_far_larger_values(gpu, hq, hkv, rows, context, la
     want, bound = ref.attention(cache, query, [0, rows], [context], hq, query)
     assert error == 0
     assert (np.abs(got - want) <= bound).all(), float((np.abs(got - want) / np.maximum(bound, 1e-300)).max())
+
+
+@pytest.mark.parametrize("rows,context", [(2, 300), (2, 1000), (10, 300), (23, 1500)])
+def test_attention_rows_do_not_depend_on_rows_of_other_blocks(gpu, rows, context):
+    """Three heads a KV head: a group's last rows share a block of four or a wave of 16 with places that no row has,
+    and their bits are the same whatever the rows of other blocks ask for."""
+    rng = np.random.default_rng(rows)
+    hkv, d, per = 4, 64, pages_for([rows], [context])
+    cache = ref.Cache(rng, per, 1, per, hkv, d)
+    cache.fill(rng, [rows + context])
+    device = cache.upload(gpu)
+    query = rng.standard_normal((rows, 3 * hkv * d)).astype(np.float32)
+    other = query.copy()
+    other[0] = 60.0 * rng.standard_normal(3 * hkv * d)
+    both = [attend(gpu, device, cache, q, [0, rows], [context], 3 * hkv, max_rows=rows)[0] for q in (query, other)]
+    # [KV head][row (token, head) of the group][d]
+    both = [o.reshape(rows, hkv, 3, d).swapaxes(0, 1).reshape(hkv, rows * 3, d) for o in both]
+    part = 4 if rows * 3 <= 8 else 16
+    assert rows * 3 % part, "places without a row"
+    last = rows * 3 // part * part
+    np.testing.assert_array_equal(both[0][:, last:], both[1][:, last:])
