@@ -334,17 +334,19 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
     // Keys of hidden blocks have p = 0: any finite factor will do.
     const float to_int = ldexpf(1.0f, min(my_exp - held_exp, 0) + kPBits);
     i32x4 pf;
+    float part = 0.0f;  // of the page first: a sum over long contexts is off by its number of terms
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       int u[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float e = __builtin_amdgcn_exp2f(score[t][i] - ref);
-        l += e;
+        part += e;
         u[i] = static_cast<int>(fmaf(e, to_int, 0.5f)) + 0x808080;
       }
       pf[t] = gather_digits(u, digit_select(digit), digit_flip(digit));
     }
+    l += part;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
       sum[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vf[t], pf, sum[t], 0, 0, 0);

@@ -98,3 +98,26 @@ def test_many_rows_of_many_pages_a_split(gpu, per, hot_at):
 
 def test_many_rows_of_many_pages_without_a_split(gpu):
     check(gpu, [64, 128, 129, 0, 63, 100, 65, 127, 126, 64] * 2, 130, 64, 64, 9)
+
+
+# The second: added one by one, 33,408 keys a lane, each fp32 sum from 512 on would lose 0.45 of its step.
+@pytest.mark.parametrize("weight", [2.0 ** -5, 2.0 ** -5 + 0.45 * 2.0 ** -14])
+def test_sums_of_more_pages_than_an_int32_holds(gpu, weight):
+    """Weights of 2^-5 are a digit of -128; with codes of 127, 64 of them a page, an int32 is full after 2,064 pages of
+    a wave. One key of each wave outweighs the others 32 times and has the opposite value."""
+    rng = np.random.default_rng(3)
+    per, hkv, seqs = 16704, 64, 4  # 2,088 pages a wave
+    r = Repeated(gpu, rng, [0] * seqs, per, hkv)
+    c = r.cache
+    r.table[:, :8] = KINDS  # the first page of each wave
+    c.keys[:], c.values[:], c.key_exps[:], c.value_exps[:] = 0, 127, 0, 0
+    c.keys[KINDS, :, 7, 0], c.values[KINDS, :, :, 7] = 64, -127
+    device = gpu.Kv8Pages(*c.upload(gpu).buffers[:4], ints(gpu, r.table), KINDS + 1, seqs, per, hkv, D)
+    query = np.zeros((seqs, hkv * D), np.float32)
+    query[:, ::D] = -np.log(weight) * np.sqrt(D) / 64
+    got, error = attend(gpu, device, c, query, np.arange(seqs + 1), [per * ref.PAGE - 1] * seqs, hkv, max_rows=1)
+    others = (per * ref.PAGE - 8) * weight
+    want = 127 * (others - 8) / (others + 8)
+    assert error == 0
+    # Sums of 2,088 pages a wave one after another, and 64 roundings of the rest.
+    assert (np.abs(got - want) <= 2 * (2088 + 64) * 2.0 ** -24 * 127).all(), float(np.abs(got - want).max() / 127)
