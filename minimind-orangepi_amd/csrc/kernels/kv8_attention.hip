@@ -191,7 +191,7 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
   const int lane_zero = zero_of_lanes();
   auto ask = [&]() {  // addresses and exponents of step ask_at, at most the last
     const int step = min(ask_at, (end - 1 - from) / kStepWaves);
-    if (ask_at > 0 && step % kWave == 0) {
+    if (ask_at == step && step > 0 && step % kWave == 0) {  // not for the last again
       numbers = table[min(from + kStepWaves * (step + lane), a.cache.per_seq - 1)];
       asm volatile("" : "+v"(numbers));  // waited for here, not wherever it is read
     }
