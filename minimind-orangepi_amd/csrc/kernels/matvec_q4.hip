@@ -62,6 +62,12 @@ constexpr int kTwoTiles = 256;
 constexpr int kWideRowsBlocks = 256;
 constexpr int kTilesOfWave = 2;
 
+// Under 2^e >= the largest of 128 columns, the integers are x 2^(30 - e) and 16 q:
+// a product is theirs times 2^(e - 34), of which 2^-32 goes into the sums of a
+// run and the rest, 2^(e - 2), is a normal number for any largest value.  Below
+// 2^-124 e stays: x 2^154 is whole for the least subnormal.
+constexpr int kUnitPower = 2, kLeastPower = -124;
+
 using i32x4 = int __attribute__((ext_vector_type(4)));
 
 // What the launch decides, beside the shape.
@@ -97,14 +103,14 @@ __device__ __forceinline__ Columns load_columns(const MatvecQ4Args& a, const Q4F
 // [rows][16 bytes] (16 rows: in the order of the lanes that read them), half
 // j / 2, part p and bytes 8 (j % 2) + i / 2 (even columns) or + 4 (odd ones)
 // for column 32 j + 8 p + i.  Returns the power of
-// two that the products come in, NaN if a value is not finite.
+// two that run_product's sums come in, NaN if a value is not finite.
 __device__ __forceinline__ float write_digits(const float v[2], int b, int rows, int8_t* to) {
   const int lane = threadIdx.x % kWave;
   const bool bad = __any(!(fabsf(v[0]) < __builtin_inff()) || !(fabsf(v[1]) < __builtin_inff()));
   const float top = group_max<kWave>(fmaxf(fabsf(v[0]), fabsf(v[1])));
   int e = 0;
   (void)frexpf(bad ? 0.0f : top, &e);
-  e = max(e, -90);
+  e = max(e, kLeastPower);
   const int j = lane / 32, p = lane % 32 / 8, i = lane % 8;
   int8_t* at = to + (p * rows + kQ4Batch * b) * 16 + j * 8 + i % 2 * 4 + i / 2;
 #pragma unroll
@@ -114,7 +120,7 @@ __device__ __forceinline__ float write_digits(const float v[2], int b, int rows,
     for (int d = 0; d < 4; ++d)
       at[(k * 4 * rows + d) * 16] = static_cast<int8_t>((n >> (8 * d)) ^ (d < 3 ? 0x80u : 0u));
   }
-  return bad ? __builtin_nanf("") : ldexpf(1.0f, e - 34);  // the weights come as 16 q
+  return bad ? __builtin_nanf("") : ldexpf(1.0f, e - kUnitPower);
 }
 
 // A lane's share of a run of its weight row: 16 bytes of codes, and the scales
@@ -146,8 +152,8 @@ __device__ __forceinline__ Run<kGroup> load_run(const MatvecQ4Args& a, const Q4F
   return r;
 }
 
-// The run's products with the x operand's row of this lane's part: batch row
-// lane / 16, weight row lane % 16.
+// The run's products with the x operand's row of this lane's part, times
+// 2^(kUnitPower - 34): batch row lane / 16, weight row lane % 16.
 template <int kGroup>
 __device__ __forceinline__ float run_product(const Run<kGroup>& r, const i32x4& x0, const i32x4& x1) {
   const uint32_t w[4] = {r.codes.x, r.codes.y, r.codes.z, r.codes.w};
@@ -177,7 +183,7 @@ __device__ __forceinline__ float run_product(const Run<kGroup>& r, const i32x4& 
       join(__builtin_amdgcn_mfma_i32_16x16x64_i8(x1, b1, d0, 0, 0, 0), r.scales[0]);
     }
   }
-  return y;
+  return y * 0x1p-32f;
 }
 
 // Weight (r, c) as the formula has it.

@@ -261,3 +261,15 @@ def test_quantized_weights_round_trip(gpu):
         c.w = gpu.q4_dequantize(c.codes, c.scales, 416, group).astype(np.float64)
         c.dw = gpu.DeviceArray.from_numpy(c.codes), gpu.DeviceArray.from_numpy(c.scales)
         c.check()
+
+
+@pytest.mark.parametrize("rows,batch", [(48, 1), (48, 4), (48, 6), (8230, 2), (8230, 40)])
+@pytest.mark.parametrize("power", [-90, -112, -121, -135])
+def test_x_that_is_tiny_throughout(gpu, rows, batch, power):
+    """As many bits of x as of any other, down to its subnormals. Besides the relative bound, a rounding to a subnormal
+    number is off by half of 2^-149."""
+    c = Call(gpu, np.random.default_rng(23), rows, 640, 64, batch)
+    c.x = np.ldexp(c.x, power).astype(np.float32)
+    got, (want, off) = c.run().numpy(), c.expected()
+    off = off + (640 // 32 + 8) * 2.0 ** -150
+    assert (np.abs(got - want) <= off).all(), float((np.abs(got - want) / off).max())
