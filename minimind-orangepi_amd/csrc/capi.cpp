@@ -1009,6 +1009,8 @@ namespace {
 
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
+constexpr int64_t kKv8MostPages = int64_t{1} << 24;  // of a sequence
+
 void check_kv8_sizes(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs, int64_t rows,
                      int64_t max_rows) {
   require(head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128,
@@ -1030,7 +1032,7 @@ mmr::Kv8Pages kv8_pages(const mmr_kv8_pages* c) {
   require(aligned(c->key_exps, 4) && aligned(c->value_exps, 4) && aligned(c->table, 4),
           "exponents and table must be 4-byte aligned");
   require(c->pages >= 1 && c->pages <= INT32_MAX, "pages out of range");
-  require(c->pages_per_seq >= 1 && c->pages_per_seq <= (int64_t{1} << 24), "pages_per_seq must be in [1, 2^24]");
+  require(c->pages_per_seq >= 1 && c->pages_per_seq <= kKv8MostPages, "pages_per_seq must be in [1, 2^24]");
   mmr::Kv8Pages p;
   p.keys = c->keys;
   p.values = c->values;
@@ -1052,8 +1054,12 @@ mmr::Kv8AttnPlan kv8_plan(int64_t q_heads, int64_t kv_heads, int64_t head_dim, i
                                  max_tokens);
 }
 
+bool q4_in_range(int64_t rows, int64_t cols) {
+  return rows > 0 && cols > 0 && rows <= (1 << 24) && cols <= (1 << 20);
+}
+
 void check_q4_shape(int64_t rows, int64_t cols, int64_t group) {
-  require(rows > 0 && cols > 0 && rows <= (1 << 24) && cols <= (1 << 20), "rows or cols out of range");
+  require(q4_in_range(rows, cols), "rows or cols out of range");
   require(cols % 32 == 0, "cols must be a multiple of 32");
   require(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128");
 }
@@ -1100,7 +1106,7 @@ int mmr_kv8_append(const float* qkv, const float* q_norm, const float* k_norm, f
 size_t mmr_kv8_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
                                         int64_t rows, int64_t max_rows, int64_t max_tokens) {
   if (guarded([&] { check_kv8_sizes(q_heads, kv_heads, head_dim, seqs, rows, max_rows); }) != MMR_OK) return 0;
-  if (max_rows == 0 || max_tokens < 1) return 0;
+  if (max_rows == 0 || max_tokens < 1 || max_tokens > kKv8MostPages * mmr::kKv8Page) return 0;
   return static_cast<size_t>(
              kv8_plan(q_heads, kv_heads, head_dim, seqs, rows, max_rows, max_tokens).partial_floats) *
          sizeof(float);
@@ -1139,7 +1145,7 @@ int mmr_kv8_attention(const float* query, const mmr_kv8_pages* cache, const int3
 }
 
 size_t mmr_q4_code_bytes(int64_t rows, int64_t cols) {
-  return rows > 0 && cols > 0 ? static_cast<size_t>(rows) * static_cast<size_t>(q4_row_bytes(cols)) : 0;
+  return q4_in_range(rows, cols) ? static_cast<size_t>(rows) * static_cast<size_t>(q4_row_bytes(cols)) : 0;
 }
 
 int mmr_q4_quantize(const float* w, int64_t rows, int64_t cols, int64_t group, uint8_t* codes, uint16_t* scales) {

@@ -158,3 +158,18 @@ def test_append_without_a_table_or_rows(mmr):
     with pytest.raises(mmr.InvalidArgument, match="q_heads"):
         mmr.kv8_append(b, b, b, 1e-5, rope, pages(mmr), b, b, 4, 1, 7, b, b)
     assert C.sizeof(mmr._Kv8PagesStruct) == 80
+
+
+def test_sizes_of_what_no_call_takes(mmr):
+    """0 bytes, not the wrapped product."""
+    def attention(max_tokens):
+        return mmr.kv8_attention_workspace_size(8, 2, 96, 1, 1, 1, max_tokens)
+
+    most = 64 << 24  # pages_per_seq is at most 2^24
+    assert attention(most) == attention(most - 63) == 64 * 8 * (96 + 2) * 4
+    for tokens in (most + 1, 1 << 40, 1 << 62, (1 << 63) - 1, 0, -1):
+        assert attention(tokens) == 0, tokens
+    code_bytes = mmr.lib().mmr_q4_code_bytes
+    assert code_bytes(1 << 24, 1 << 20) == 1 << 43
+    for rows, cols in (((1 << 24) + 1, 32), (1, (1 << 20) + 32), (1 << 62, 128), (3, (1 << 63) - 1), (-1, 32)):
+        assert code_bytes(rows, cols) == 0, (rows, cols)
