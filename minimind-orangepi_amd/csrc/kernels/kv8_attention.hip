@@ -118,6 +118,13 @@ __device__ __forceinline__ int zero_of_lanes() {
   return zero;
 }
 
+// Of q.k / sqrt(d), in log2.  Powers of two of the query and of the keys are
+// added before they scale it: either alone may have no fp32 number.
+template <int D>
+__device__ __forceinline__ float score_unit() {
+  return 1.4426950408889634f / sqrtf(static_cast<float>(D));
+}
+
 // The largest of a page's first `blocks` exponents.
 __device__ __forceinline__ int largest_exponent(uint32_t exps, int blocks) {
   int e = kKv8MinExp - 1;
@@ -223,7 +230,7 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
   }
 
   Operand<D> q;
-  float unit;        // of a score's integer, in log2
+  int unit_exp;      // a score's integer has units of 2^unit_exp score_unit<D>(), in log2, before the keys' exponent
   bool bad = false;  // a query that is not finite gives a row of NaN
   {
     constexpr int kQBits = 29;
@@ -262,7 +269,7 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
 #pragma unroll
     for (int c = 0; c < kFull; ++c) q.word[c] = i32x4{w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]};
     if constexpr (kHalf) q.word[kFull] = i32x4{w[4 * kFull], w[4 * kFull + 1], 0, 0};
-    unit = ldexpf(1.4426950408889634f / sqrtf(static_cast<float>(D)), x - kQBits);
+    unit_exp = x - kQBits;
   }
   const float weight = ldexpf(1.0f, 8 * digit);
 
@@ -291,7 +298,7 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
     const int my_exp = static_cast<int8_t>(value_exps >> (8 * g));
 
     float score[4][4];
-    const float to_log2 = unit * ldexpf(1.0f, static_cast<int8_t>(key_exps >> (8 * g)));
+    const float to_log2 = ldexpf(score_unit<D>(), unit_exp + static_cast<int8_t>(key_exps >> (8 * g)));
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const i32x4 acc = multiply<D>(kf[t], q);
@@ -533,7 +540,7 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
   ask(begin);
 
   f16x8 q_hi[kRuns], q_lo[kRuns];
-  float unit;        // of a score, in log2
+  int unit_exp;      // as for steps
   bool bad = false;  // a query that is not finite gives a row of NaN
   {
     float top = 0.0f;
@@ -558,7 +565,7 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
       q_hi[c] = __builtin_bit_cast(f16x8, hi);
       q_lo[c] = __builtin_bit_cast(f16x8, lo);
     }
-    unit = ldexpf(1.4426950408889634f / sqrtf(static_cast<float>(D)), x - 15);
+    unit_exp = x - 15;
   }
 
   f32x4 out[kTiles] = {};
@@ -607,9 +614,8 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
               kf[w][c % kRuns], c < kRuns ? q_lo[c % kRuns] : q_hi[c % kRuns], score[t + w], 0, 0, 0);
     }
     const int shift = 8 * (g / 2);  // of this lane's block of each half page
-    const float key_scale[2] = {ldexpf(1.0f, static_cast<int8_t>(key_exps >> shift)),
-                                ldexpf(1.0f, static_cast<int8_t>(key_exps >> (16 + shift)))};
-    float to_log2[2] = {unit * key_scale[0], unit * key_scale[1]};
+    float to_log2[2] = {ldexpf(score_unit<D>(), unit_exp + static_cast<int8_t>(key_exps >> shift)),
+                        ldexpf(score_unit<D>(), unit_exp + static_cast<int8_t>(key_exps >> (16 + shift)))};
     // As for steps: of the blocks that the row attends.
     int page_exp = largest_exponent(value_exps, kKv8Blocks);
     if (hidden || p * kKv8Page + kKv8Page - 1 > all_see) {

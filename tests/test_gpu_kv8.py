@@ -541,3 +541,17 @@ def test_attention_rows_do_not_depend_on_rows_of_other_blocks(gpu, rows, context
     assert rows * 3 % part, "places without a row"
     last = rows * 3 // part * part
     np.testing.assert_array_equal(both[0][:, last:], both[1][:, last:])
+
+
+@pytest.mark.parametrize("rows", [1, 3, 20])
+@pytest.mark.parametrize("power", [60, 100, 120])
+def test_attention_of_tiny_queries_and_large_keys(gpu, rows, power):
+    """Scores of ordinary size, whatever the sizes of what they are products of; and the other way round."""
+    rng = np.random.default_rng(rows + power)
+    hq, hkv, d, n = 4, 2, 64, 300
+    for sign in (1, -1):
+        cache = ref.Cache(rng, 6, 1, 6, hkv, d)
+        cache.fill(rng, [n + rows])
+        cache.key_exps = np.clip(cache.key_exps + np.int64(sign * power), -126, 122).astype(np.int8)
+        query = np.ldexp(rng.standard_normal((rows, hq * d)), -sign * power).astype(np.float32)
+        check_attention(gpu, cache, query, [rows], [n], hq)
