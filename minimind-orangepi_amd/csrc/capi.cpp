@@ -1005,6 +1005,7 @@ int mmr_prefill_attention(const float* query, const mmr_kv_cache* cache, int64_t
   });
 }
 
+extern "C++" {
 namespace {
 
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
@@ -1073,6 +1074,7 @@ int64_t q4_byte(int64_t c) {
 int64_t q4_row_bytes(int64_t cols) { return (cols + mmr::kQ4Cols - 1) / mmr::kQ4Cols * 64; }
 
 }  // namespace
+}  // extern "C++"
 
 int mmr_kv8_append(const float* qkv, const float* q_norm, const float* k_norm, float eps, const mmr_rope_table* rope,
                    const mmr_kv8_pages* cache, const int32_t* offsets, const int32_t* context, int64_t rows,
