@@ -555,3 +555,31 @@ def test_attention_of_tiny_queries_and_large_keys(gpu, rows, power):
         cache.key_exps = np.clip(cache.key_exps + np.int64(sign * power), -126, 122).astype(np.int8)
         query = np.ldexp(rng.standard_normal((rows, hq * d)), -sign * power).astype(np.float32)
         check_attention(gpu, cache, query, [rows], [n], hq)
+
+
+def test_prompts_and_steps_in_two_calls_on_the_same_arrays(gpu):
+    """Sequences with prompts first: a call for them, and one from the first of the others on, each with max_rows of its
+    own; neither touches the other's rows."""
+    mmr, rng = gpu, np.random.default_rng(57)
+
+    class From:
+        def __init__(self, array, elements):
+            self.ptr, self.nbytes = array.ptr + 4 * elements, array.nbytes - 4 * elements
+
+    hq, hkv, d, rows, context = 8, 2, 96, [70, 33, 1, 1, 2, 1], [5, 0, 400, 15, 700, 64]
+    per, prompts, total = pages_for(rows, context), 2, sum(rows)
+    cache = ref.Cache(rng, 6 * per, 6, per, hkv, d)
+    cache.fill(rng, [a + b for a, b in zip(rows, context)])
+    query = rng.standard_normal((total, hq * d)).astype(np.float32)
+    fill = np.full(query.shape, 7.5, np.float32)
+    device, out, error = cache.upload(mmr), mmr.DeviceArray.from_numpy(fill), ints(mmr, [0])
+    dq, offsets, dcontext = mmr.DeviceArray.from_numpy(query), ints(mmr, offsets_of(rows)), ints(mmr, context)
+    want, bound = ref.attention(cache, query, offsets_of(rows), context, hq, fill)
+    for first, seqs, max_rows in ((0, prompts, 70), (prompts, 6 - prompts, 2)):
+        pages = mmr.Kv8Pages(*device.buffers[:4], From(device.buffers[4], first * per), cache.pages, seqs, per, hkv, d)
+        size = mmr.kv8_attention_workspace_size(hq, hkv, d, seqs, total, max_rows, per * ref.PAGE)
+        mmr.kv8_attention(dq, pages, From(offsets, first), From(dcontext, first), total, max_rows, per * ref.PAGE, hq, out,
+                          mmr.DeviceArray(max(size, 1), np.uint8), error)
+        got, done = out.numpy(), sum(rows[: first + seqs])
+        assert (np.abs(got - want) <= bound)[:done].all() and (got[done:] == 7.5).all()
+    assert int(error.numpy()[0]) == 0
