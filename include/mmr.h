@@ -377,8 +377,11 @@ int mmr_prefill_attention(const float* query, const mmr_kv_cache* cache, int64_t
  * take its positions context[s] .. context[s] + n - 1.  offsets [seqs + 1]
  * and context [seqs] are int32 on the device, so a recorded graph serves
  * every step; rows is what the row buffers hold, max_rows the most that one
- * sequence brings (both size the launch: max_rows x seqs is at most 2^26, and
- * a long prompt is better in a call of its own than among single rows).  Rows
+ * sequence brings (both size the launch, as if every sequence brought that
+ * many: max_rows x seqs is at most 2^26, and a prompt belongs in an attention
+ * call of its own: single rows in a call with it attend their whole context in
+ * one piece, 386 us for 512 rows and 31 single rows over up to 8,192 tokens,
+ * 32 in two calls; the append may take both).  Rows
  * outside [offsets[0], offsets[seqs]) are left as they are.  rows or max_rows
  * of 0 is no work.  As for all op-level calls, the current device is the one
  * that holds the buffers and the stream.
@@ -420,7 +423,7 @@ typedef struct mmr_kv8_pages {
  * a block's rows over several calls rounds its earlier rows again.
  * Values that are not finite don't count in e and are stored as +-127 (an
  * infinity) or 0 (NaN), with the error bit.  qkv and query are 16-byte
- * aligned.  No allocation, no synchronisation, graph-capturable. */
+ * aligned and do not overlap.  No allocation, no synchronisation, graph-capturable. */
 int mmr_kv8_append(const float* qkv, const float* q_norm, const float* k_norm, float eps, const mmr_rope_table* rope,
                    const mmr_kv8_pages* cache, const int32_t* offsets, const int32_t* context, int64_t rows,
                    int64_t max_rows, int64_t q_heads, float* query, int32_t* error, mmr_stream_t stream);
@@ -429,8 +432,13 @@ int mmr_kv8_append(const float* qkv, const float* q_norm, const float* k_norm, f
  * softmax(q.k / sqrt(d)) v per head, GQA mapping kv = h / (Hq/Hkv).  query
  * and out fp32 [rows][q_heads d], 16-byte aligned, q_heads a multiple of
  * kv_heads.  max_tokens bounds context[s] + n over all sequences and sizes
- * the split along the context.  Scores, weights and sums carry 21 bits or
- * more, the sums relative to the largest exponent among a row's values.  A
+ * the split along the context.  Scores are fp32, of a query rounded by up to
+ * 2^-29 of its row's largest value (2^-23 of each value, and 2^-39 of the
+ * largest, where max_rows x q_heads / kv_heads is over 8).  A weight, the largest about 1, times its block's scale is rounded by
+ * up to 2^-29 of the largest scale among the values that the row attends (2^-35,
+ * and 2^-22 of itself, over 8): next to a block with far larger
+ * values, other values lose bits, and all of them where it is 2^28 (2^34)
+ * larger, however little weight it has.  The sums are fp32.  A
  * query row that is not finite gives a row of NaN and no other; out may alias
  * query.  The workspace (mmr_kv8_attention_workspace_size bytes of the same
  * sizes, possibly 0; 16-byte aligned) holds the split partials and is the
@@ -464,8 +472,10 @@ int mmr_q4_dequantize(const uint8_t* codes, const uint16_t* scales, int64_t rows
  * (of each row of x) and epilogues: y and residual fp32 [batch][rows],
  * residual may alias y; MMR_EPI_SWIGLU takes an even number of rows,
  * interleaved gate_0, up_0, ..., and gives y [batch][rows / 2].  codes are 16-byte
- * aligned.  The workspace (mmr_matvec_q4_workspace_size bytes, 0 for few
- * rows of x; 16-byte aligned) is the call's own until it has run.  No
+ * aligned, x and y do not overlap.  x (normalised) is rounded by up to 2^-30 of
+ * the largest of each 128 columns, sums over groups are fp32; a row of x that
+ * is not finite is multiplied as the formula says.  The workspace
+ * (mmr_matvec_q4_workspace_size bytes, 0 for few rows of x; 16-byte aligned) is the call's own until it has run.  No
  * allocation, no synchronisation, graph-capturable. */
 size_t mmr_matvec_q4_workspace_size(int64_t cols, int64_t batch);
 int mmr_matvec_q4(const uint8_t* codes, const uint16_t* scales, int64_t group, int64_t rows, int64_t cols,

@@ -23,12 +23,13 @@
 // holds 16 rows: a block of one head, whose maximum is a wave reduction.  The
 // block's queries are other workgroups', which need nothing but the angles.
 //
-// Measured (8 + 2 + 2 heads): one row of d 96 4.9 us in a replayed graph, 1.6 of
-// them any kernel's there, the rest a chain of three loads, the sine and two
-// reductions; 2,690 rows of d 128 in five sequences 11.0 us, 27.4 MB at 2.5 TB/s:
-// its waves wait for memory 60 % of their time, in one pass each.  Angles of
-// rows 1 to 15 of a block from a table of fixed turns instead of sines of
-// their own changed nothing (12.0 and 12.4 us a launch).
+// Measured in replayed graphs (8 + 2 + 2 heads; medians of graphs of 30 calls
+// over three sets of inputs): one row of d 96 4.9 us, 1.6 of them any kernel's
+// there, the rest a chain of three loads, the sine and two reductions; 2,690
+// rows of d 128 in five sequences 11.5 us, 27.4 MB at 2.4 TB/s: its waves wait
+// on counters 59 % of their time, in one pass each.  Angles of rows 1 to 15 of a
+// block from a table of fixed turns instead of sines of their own changed
+// nothing (12.0 and 12.4 us a launch in a kernel trace).
 #include "device_common.h"
 #include "kv8_common.h"
 

@@ -13,12 +13,15 @@
 // an integer n is the sum of d_k 256^k with d_k in [-128, 127], and the bytes
 // of n + 0x808080 are those digits, the lower three with their top bit
 // flipped.  Products and sums of digits and codes are exact in int32; rounded
-// are q (to 2^-30 of its row's largest value), p (2^-29) and the fp32 sums
-// over pages.  The 16 columns of a product are 4 rows x 4 digits, so K and V
+// are q (by up to 2^-29 of its row's largest value), p times its values' power
+// of two (by 2^-29 of the reference's at the row's largest exponent) and the
+// fp32 sums over pages.  The 16 columns of a product are 4 rows x 4 digits, so K and V
 // are each the operand of one product, and a score is the sum over four lanes.
 //
 // More rows: fp16 matrix cores on codes widened to fp16 (exactly) once per
-// block, with the fp32 operand as two fp16 planes (22 bits).  Per 16 rows this
+// block, with the fp32 operand as two fp16 planes: q is rounded by up to 2^-23
+// of each value, p by 2^-22, but no finer than 2^-39 of the row's largest value
+// and 2^-35 of the reference's at the row's largest exponent.  Per 16 rows this
 // takes as many matrix cycles as digits would (a digit operand multiplies
 // twice the columns, but takes three digits of q and four of p), but none of
 // the adding up and taking apart of digits, which was most of that form's
@@ -30,6 +33,11 @@
 // run of K from part l / 16) a lane keeps its column, and the keys are dealt
 // to the rows of S^T so that the scores that a lane gets are those of the keys
 // whose weights it has to supply: P never leaves the lane.
+//
+// Times in this file are us a call in replayed graphs (medians of graphs of 30
+// calls over three sets of inputs; 1.6 us are any kernel's there), with the
+// join where a call has one.  Sequences of a batch have a quarter to all of the
+// tokens named.
 #include "device_common.h"
 #include "kv8_common.h"
 
@@ -150,11 +158,13 @@ __device__ __forceinline__ void store_ml(const Kv8AttnArgs& a, int64_t row, int 
 }
 
 // Steps: waves take the pages of a split in turn and join their results at the
-// end.  Waves wait for memory half of their time, the vector units are busy 19 %
+// end.  Waves wait on counters 39 % of their time, the vector units are busy 19 %
 // of it: what counts is that a wave always has a page under way.  32 sequences
-// of up to 8,192 tokens, two KV heads of d 96: 72 MB in 18.5 us with the join, 3.9
-// TB/s; one query over 32,768 11.5 us, over 500 7.2 (replayed graph, 1.6 of them
-// any kernel's): two dependent loads, one page's arithmetic, the join in LDS.
+// of up to 8,192 tokens, two KV heads of d 96: 72 MB in 18.8 us, 3.8 TB/s; one
+// query over 32,768 11.6, over 8,192 8.8, over 1,024 8.3, over 500 7.0, over 128
+// 5.3: two dependent loads, a page's arithmetic (two of them one after another
+// from 513 to 1,024 tokens), the join in LDS and, above, the one of the splits.
+// The fp16 cache's attention takes 12.4, 6.9, 6.0, 5.9 and 5.8 there.
 template <int D>
 __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a, int chunk, int splits) {
   constexpr int kRows = kStepTile, kTiles = D / 16;  // tiles of the output's dimensions
@@ -433,13 +443,14 @@ __device__ __forceinline__ void split2_truncated(float x0, float x1, uint32_t& h
 // LDS: the operands of every product, 16 bytes a lane in the order of lanes.
 //
 // Measured: 3,000 rows after 1,111, 8 heads of d 96 over two KV heads, 75 us a
-// call (9 of them the join), 320 TFLOP/s of the formula's products, of which
-// the two planes make twice as many.  Vector units are busy 50 % of the
-// kernel, matrix cores 27 %, LDS 28 %; with the lower planes' products, the
-// exponentials or the widening of pages left out, one at a time, it took 70 to
-// 75 us of 78, so it is none of them but the chain barrier - LDS - products -
-// weights - products with three waves a SIMD.  32 rows a wave (half the LDS
-// reads a row, two waves a SIMD) took as long, blocks of eight waves 101.
+// call (73 to 76 from card to card), 320 TFLOP/s of the formula's products, of which the two planes make
+// twice as many (the fp16 cache's attention: 63.6).  Vector units are busy 50 %
+// of the kernel, matrix cores 27 %, LDS 27 %.  In an earlier state, of 80.2 us a
+// call, the lower planes' products, the exponentials or the widening of pages
+// left out, one at a time, saved 3 to 8 us: it is none of them but the chain
+// barrier - LDS - products - weights - products with three waves a SIMD.  There
+// 32 rows a wave (half the LDS reads a row, two waves a SIMD) took 80.4, blocks
+// of eight waves 101.
 template <int D>
 __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel(Kv8AttnArgs a, int chunk, int splits) {
   constexpr int kTiles = D / 16, kRuns = D / 32;  // tiles of the output, products along D
@@ -553,7 +564,8 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
     bad = column_max(bad ? 1.0f : 0.0f) > 0.0f;
     int x = 0;
     if (top > 0.0f && !bad) (void)frexpf(top, &x);
-    // The largest below 2^15: what is rounded off is under 2^-39 of it.
+    // The largest below 2^15: rounded off is up to 2^-23 of a value or, where its
+    // lower plane is subnormal, 2^-39 of the largest.
 #pragma unroll
     for (int c = 0; c < kRuns; ++c) {
       uint4 hi, lo;
@@ -806,25 +818,34 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_kernel(Kv8AttnArgs a
 }  // namespace
 
 // Splits along the context, sized by the longest one a launch may meet (blocks
-// past a sequence's end leave at once).  Measured in replayed graphs, d 96, two
-// KV heads, us a call:
+// past a sequence's end leave at once).  Measured with d 96 and, where nothing
+// else is said, 8 heads on two KV heads:
 //   up to kStepRows rows of a KV head are steps, though the second block of four
-//   reads the pages again (one of eight heads at 32,768 tokens 14.9, 16
-//   sequences of up to 8,000 16.5; as many rows 20.9 and 22.9; 16 heads of 32
-//   sequences of up to 4,000 as steps 34.0, 23.2);
-//   steps of at most kWidePages pages take one block and no join: 9.0 for 32
-//   sequences of 1,000 tokens (10.1 split), while at 2,000 the split wins (8.7,
-//   11.3);
-//   more take kStepBlocks blocks in all (32 sequences of up to 4,000 tokens
-//   14.2; with 384 blocks 19.6, with 192 15.1) and at most kMostSplits splits
-//   (one sequence of 32,768: 64 splits 13.5, 128 14.5);
+//   reads the pages again (8 heads on one KV head: one query over 32,768 tokens
+//   10.8, 16 over up to 8,000 13.3; as many rows 17.7 and 16.9; 16 heads on two,
+//   32 queries over up to 4,000, 16.3 and 20.4);
+//   steps of at most kWidePages pages take one block and no join, mostly for
+//   batches (32 queries over up to 1,000 tokens 9.1, split from 9 pages on 10.0;
+//   one query over 778 8.1 and 8.2, over 1,000 8.4 and 8.3, over 320 6.5 and, split
+//   from 5 pages on, 8.0; 24 pages of one query without a split 9.7, with it 8.5);
+//   more take kStepBlocks blocks in all (32 queries over up to 4,000 14.1; with
+//   384 blocks 19.2, with 192 15.0) and at most kMostSplits splits, which is what
+//   the join takes (one query over 32,768: 11.5, with 32 splits 12.7);
 //   many rows take kRowsBlocks blocks, whose tiles see different numbers of
-//   keys (3,000 rows after 1,111: 80; with 768 blocks 87, 256 104), but at most
-//   kFewSplits splits, whose join is cheap, unless there are few rows (512 rows
-//   after 2,000: 24 with 8 splits, 32 with 16);
-//   a split has kLeastPages pages (one query at 4,000 tokens 8.8, 5 rows there
-//   10.0; with four 9.1 and 12.5), of many rows kLeastRowsPages, which are more
-//   to join (1,500 rows 24.9; with three 28.4).
+//   keys (3,000 rows after 1,111: 75; with 768 blocks 82, with 256 96), but
+//   at most kFewSplits splits, whose join is cheap, from kFewRows (row, head)
+//   pairs on: 4,096 pairs, 512 rows after 2,000, take 21.6 with 8 splits, 27.9 with
+//   16, 29.8 with 64.  256 pairs, 4 sequences of 8 rows after 13,000, take 16.4
+//   with 64 and 41.8 with 8.  Between, long contexts would gain from more than 8
+//   splits up to some 1,000 pairs (128 rows after 9,000: 32.7, with 64 splits 23.7;
+//   after 2,000: 15.6 and 14.8; 16 sequences of up to 8 rows over up to 13,000:
+//   42.7 and 30.7);
+//   a split has kLeastPages pages (one query over 4,000 tokens 8.6, 5 rows there
+//   9.9; with four 8.9 and 12.5), of many rows kLeastRowsPages, which are more
+//   to join (1,500 rows 24.9; with three 28.2).
+// A launch is sized as if every sequence brought max_rows rows: with a prompt
+// among them, single rows get no splits and a wave each (512 rows and 31 single
+// rows over up to 8,192 tokens 386; apart 13.5 and 18.2).
 Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens) {
   Kv8AttnPlan p;
   const int64_t most = static_cast<int64_t>(hq / hkv) * max_rows;

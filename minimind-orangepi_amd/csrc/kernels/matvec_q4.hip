@@ -10,19 +10,24 @@
 // flipped).  The 16 rows of the x operand are 4 rows of the batch x 4 digits,
 // its product with 16 rows of W leaves the four digits of one (batch row,
 // weight row) in the four registers of one lane, and the sums within a group
-// are exact in int32: the roundings are those of x (2^-31 of the largest of
-// its 128 columns) and of the fp32 sum over groups.
+// are exact in int32: the roundings are those of x (up to 2^-30 of the largest
+// of its 128 columns) and of the fp32 sum over groups.
 //
 // Codes are packed by 128 columns in 64 bytes: word 4 p + j holds columns
 // 32 j + 8 p + 0 .. 7, column 2 i in the low nibble of byte i and 2 i + 1 in
 // the high one.  Part p of a product's K is lanes 16 p .. 16 p + 15, so a lane
 // loads 16 bytes and has a share of every group, whatever the group's size.
 //
-// Measured in replayed graphs, 1.6 us of them any kernel's: 1152 x 768 in groups
-// of 32 for one row 4.1 us (latency), 32768 x 4096 in groups of 128 15.5 us, 69.4
-// MB at 4.5 TB/s, 4096 x 768 for 32 rows 6.4 us (two launches), 16384 x 4096 for 32
-// rows 28.7: there every two tiles of weight rows read all digits of 16 rows of
-// x, 256 KB, from the L2.
+// Times in this file are us a call in replayed graphs (medians of graphs of 30
+// calls over three sets of weights and inputs; 1.6 us are any kernel's there).
+// One row, groups of 32: 1152 x 768 under a norm 4.4, 4096 x 768 with norm and
+// SwiGLU 4.6, of which the kernels of fp16 weights take 2.5 and 2.8: x becomes
+// digits in a chain of load, sum of squares, barrier, maximum, LDS, barrier
+// before the first product.  Where weights count it pays: 32768 x 4096 in groups
+// of 128 16.0, 69.4 MB at 4.3 TB/s (fp16 weights 46.4).  4096 x 768 for 32 rows of x
+// 6.4 (two launches), for 3,000 94, 200 TFLOP/s; 16384 x 4096 for 32 28.4: every
+// two tiles of weight rows read all digits of 16 rows of x, 256 KB there, from
+// the L2.
 #include "device_common.h"
 
 #include <algorithm>
@@ -37,12 +42,12 @@ constexpr int kQ4Tile = 16;        // weight rows of a product
 constexpr int kQ4Batch = 4;        // batch rows of an x operand
 constexpr int kQ4Operands = 2048;  // bytes of the two x operands of a run
 // Runs of all rows of x, up to kQ4Batch rows, that a block itself turns into
-// digits: more of them cost a second launch less (768 x 2048 for 4 rows 9.2 us
-// here and 8.6 in two launches, 4096 x 2048 9.6 and 10.5; replayed graphs).
+// digits: more of them cost a second launch less (768 x 2048 for 4 rows 9.1
+// here and 8.6 in two launches, 4096 x 2048 9.4 and 10.6).
 constexpr int kFusedRuns = 64;
 // Tiles of rows from which blocks take several in turn, so that x is turned
-// into digits once a compute unit (8192 x 4096 in groups of 32: 11.7 us with a
-// tile a block, 9.4; 4096 x 768 with 256 tiles 4.2 and 4.9).
+// into digits once a compute unit (8192 x 4096 in groups of 32: 11.8 with a tile a
+// block, 9.6; 4096 x 768 with 256 tiles 4.2 and 4.9).
 constexpr int kManyRowTiles = 512;
 constexpr int kWideBlocks = 256;    // then: one a compute unit
 constexpr int kManyWaves = 2048;    // and its waves
@@ -52,13 +57,13 @@ constexpr int kCodeBytes = 4096;    // of a chunk of 16 rows
 constexpr int kChunkBytes = kCodeBytes + 512;  // with their scales
 constexpr int kManyTiles = 4;       // x operands of a block whose digits come from the workspace
 // Tiles from which such a block takes two and reads the operands for both
-// (4096 x 768 for 32 rows: 6.8 us with one, 6.4; 768 x 2048 8.4 and 9.9).
+// (4096 x 768 for 32 rows: 6.6 with one, 6.4; 768 x 2048 8.8 and 10.3).
 constexpr int kTwoTiles = 256;
 
 // Blocks of the form whose codes go through LDS, with kTilesOfWave tiles a wave,
 // from which it is taken for many rows of x: one a compute unit (groups of 64,
-// 32 rows: 8192 x 2048, 256 blocks, 11.9 us and 14.5 without; 4096 x 2048, 128
-// blocks, 11.1 and 10.3; 16384 x 4096, 1024 blocks, 28.7 and 39.5).
+// 32 rows: 8192 x 2048, 256 blocks, 12.0 and 14.6 without; 4096 x 2048, 128
+// blocks, 11.0 and 10.5; 16384 x 4096, 1024 blocks, 28.4 and 39.5).
 constexpr int kWideRowsBlocks = 256;
 constexpr int kTilesOfWave = 2;
 
