@@ -15,8 +15,9 @@
 // flipped.  Products and sums of digits and codes are exact in int32; rounded
 // are q (by up to 2^-29 of its row's largest value), p times its values' power
 // of two (by 2^-29 of the reference's at the row's largest exponent) and the
-// fp32 sums over pages.  The 16 columns of a product are 4 rows x 4 digits, so K and V
-// are each the operand of one product, and a score is the sum over four lanes.
+// fp32 sums over pages.  The 16 columns of a product are 4 rows x 4 digits, so K
+// and V are each the operand of one product, and a score is the sum over four
+// lanes.
 //
 // More rows: fp16 matrix cores on codes widened to fp16 (exactly) once per
 // block, with the fp32 operand as two fp16 planes: q is rounded by up to 2^-23
@@ -443,14 +444,14 @@ __device__ __forceinline__ void split2_truncated(float x0, float x1, uint32_t& h
 // LDS: the operands of every product, 16 bytes a lane in the order of lanes.
 //
 // Measured: 3,000 rows after 1,111, 8 heads of d 96 over two KV heads, 75 us a
-// call (73 to 76 from card to card), 320 TFLOP/s of the formula's products, of which the two planes make
-// twice as many (the fp16 cache's attention: 63.6).  Vector units are busy 50 %
-// of the kernel, matrix cores 27 %, LDS 27 %.  In an earlier state, of 80.2 us a
-// call, the lower planes' products, the exponentials or the widening of pages
-// left out, one at a time, saved 3 to 8 us: it is none of them but the chain
-// barrier - LDS - products - weights - products with three waves a SIMD.  There
-// 32 rows a wave (half the LDS reads a row, two waves a SIMD) took 80.4, blocks
-// of eight waves 101.
+// call (73 to 76 from card to card), 320 TFLOP/s of the formula's products, of
+// which the two planes make twice as many (the fp16 cache's attention: 63.6).
+// Vector units are busy 50 % of the kernel, matrix cores 27 %, LDS 27 %.  In an
+// earlier state, whose kernel took 78, it took 70 to 75 with the lower planes'
+// products, the exponentials or the widening of pages left out, one at a time:
+// it is none of them but the chain barrier - LDS - products - weights - products
+// with three waves a SIMD.  32 rows a wave (half the LDS reads a row, two waves
+// a SIMD) took as long there, blocks of eight waves 101.
 template <int D>
 __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel(Kv8AttnArgs a, int chunk, int splits) {
   constexpr int kTiles = D / 16, kRuns = D / 32;  // tiles of the output, products along D

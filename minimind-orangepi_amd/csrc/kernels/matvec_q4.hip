@@ -24,8 +24,8 @@
 // SwiGLU 4.6, of which the kernels of fp16 weights take 2.5 and 2.8: x becomes
 // digits in a chain of load, sum of squares, barrier, maximum, LDS, barrier
 // before the first product.  Where weights count it pays: 32768 x 4096 in groups
-// of 128 16.0, 69.4 MB at 4.3 TB/s (fp16 weights 46.4).  4096 x 768 for 32 rows of x
-// 6.4 (two launches), for 3,000 94, 200 TFLOP/s; 16384 x 4096 for 32 28.4: every
+// of 128 16.0, 69.4 MB at 4.3 TB/s (fp16 weights 46.4).  4096 x 768 for 32 rows of
+// x 6.4 (two launches), for 3,000 94, 200 TFLOP/s; 16384 x 4096 for 32 28.4: every
 // two tiles of weight rows read all digits of 16 rows of x, 256 KB there, from
 // the L2.
 #include "device_common.h"
