@@ -450,6 +450,119 @@ int mmr_kv8_attention(const float* query, const mmr_kv8_pages* cache, const int3
                       int64_t rows, int64_t max_rows, int64_t max_tokens, int64_t q_heads, float* out,
                       void* workspace, size_t workspace_bytes, int32_t* error, mmr_stream_t stream);
 
+/* mmr_kv8_attention with a window: row i of sequence s, at position p =
+ * context[s] + i, attends its keys j <= p with p - j < window (window >= 1:
+ * the row's own key is always one) and those with j < sinks.  Page numbers of
+ * pages that none of the call's rows attends are not read: a sequence that looks
+ * back on `window` keys needs no more pages than those (mmr_kv8_fork frees the
+ * others), and the call takes the time that they take.  Everything else as
+ * there; a row's sums are relative to the values that it attends.  With window
+ * or sinks >= max_tokens it is that call. */
+size_t mmr_kv8_window_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
+                                               int64_t rows, int64_t max_rows, int64_t max_tokens, int64_t sinks,
+                                               int64_t window);
+int mmr_kv8_window_attention(const float* query, const mmr_kv8_pages* cache, const int32_t* offsets,
+                             const int32_t* context, int64_t rows, int64_t max_rows, int64_t max_tokens,
+                             int64_t sinks, int64_t window, int64_t q_heads, float* out, void* workspace,
+                             size_t workspace_bytes, int32_t* error, mmr_stream_t stream);
+
+/* ---- who has which page of the 8-bit cache (no counterpart in the reference,
+ * whose cache holds one sequence) --------------------------------------------
+ * `layers` (host memory, `count` of them) are the caches of a model's layers:
+ * memory of their own, one table and one shape, so that page p holds the same
+ * tokens in each.  users int32 [pages] (device, 16-byte aligned) counts for each
+ * page the table entries that name it, and what else the caller counts (a
+ * prompt's pages kept for later sequences, say); a page without users is free.
+ * Table entries outside [0, pages) hold no page.  A new pool is a table of -1
+ * and users of 0.  pages is at most 2^24, seqs x pages_per_seq at most 2^28.
+ *
+ * mmr_kv8_fork: sequence i becomes the first keep[i] tokens of what sequence
+ * parent[i] was before the call, with room for room[i] more (parent, keep, room
+ * int32 [seqs] on the device; parent -1 is nobody, and keep then counts as 0).
+ * So with
+ *   parent[i] = i, keep = tokens, room = n    a sequence grows by n tokens;
+ *   parent[i] = j                             it goes on as j does (a beam, or a
+ *                                             second answer to a prompt);
+ *   keep less than the tokens                 the last ones are taken back;
+ *   parent[i] = -1, room = n                  what it had is freed, a new one begins;
+ *   parent[i] = -1, room = 0                  it ends.
+ * The table that the layers name is rewritten, users follow.  Pages are shared.
+ * The places keep[i] .. keep[i] + room[i] - 1 are in pages that sequence i alone
+ * names: where its last kept page is partly filled and someone else names it
+ * too, the blocks (of 16 tokens) with kept tokens are copied in every layer to a
+ * new page, whose other blocks stay as they are (of the sequences that would
+ * write to a page that nobody else names, the first keeps it).  New pages are
+ * the lowest free ones, those that this call frees among them, in the order of
+ * the sequences and their pages; entries past a sequence's last page become -1.
+ * With window > 0, the pages behind the window of a row at position keep[i] and
+ * without any of the first `sinks` tokens (see mmr_kv8_window_attention) are let go, too.
+ *
+ * *error (device int32, never cleared here) gets bits: 1 if a parent is outside
+ * [-1, seqs), keep or room are negative or keep + room passes the table row (the
+ * sequence ends, as for parent -1 and room 0), or a partly filled page that is
+ * to be kept has no number (it gets a new page that holds nothing); 4 if there
+ * are no more free pages (entries that got none are -1, and so appending there
+ * is flagged by mmr_kv8_append).  The workspace
+ * (mmr_kv8_fork_workspace_size bytes, 16-byte aligned) is the call's own until
+ * it has run.  No allocation, no synchronisation, graph-capturable. */
+#define MMR_KV8_ERROR_PAGES 4
+size_t mmr_kv8_fork_workspace_size(int64_t seqs, int64_t pages_per_seq, int64_t pages);
+int mmr_kv8_fork(const mmr_kv8_pages* layers, int64_t count, int32_t* users, const int32_t* parent,
+                 const int32_t* keep, const int32_t* room, int64_t sinks, int64_t window, void* workspace,
+                 size_t workspace_bytes, int32_t* error, mmr_stream_t stream);
+/* Moves the pages in use to the numbers 0 .. *live - 1 (*live int32 on the
+ * device: how many there are): those that are there already stay, the k-th of
+ * the others goes to the k-th free one below *live, in every layer, with all of
+ * its tokens.  The rest of the pool is then free, to be given back or put to
+ * other use.  table_out [seqs][pages_per_seq] and users_out [pages] get the
+ * table and the users afterwards (they may be the layers' table and users;
+ * entries that hold no page, or a free one, become -1), moved [pages] each
+ * page's new number, -1 for a free one: for what else names pages.  Pages that
+ * were moved keep their old content until they are used again.  users,
+ * users_out and moved are 16-byte aligned and moved overlaps neither.  Workspace
+ * and capture as above. */
+size_t mmr_kv8_compact_workspace_size(int64_t pages);
+int mmr_kv8_compact(const mmr_kv8_pages* layers, int64_t count, const int32_t* users, int32_t* table_out,
+                    int32_t* users_out, int32_t* moved, int32_t* live, void* workspace, size_t workspace_bytes,
+                    mmr_stream_t stream);
+
+/* ---- beam search: the best continuations (beside mmr_matvec_argmax_f16, which
+ * goes on with the best token; no counterpart in the reference) ---------------
+ * `searches` searches of `beams` beams (1 to 32) each; beam b of search i is row
+ * i * beams + b of every array.  A beam's score is the sum of its tokens' log
+ * probabilities, its length how many they are; one that has produced `eos` has
+ * ended.  From these (`from`) and the logits (fp32 [searches * beams][vocab],
+ * 16-byte aligned) the candidates are, for each beam,
+ *   one that has not ended: every token v, of score s_b + x_v - log sum_u exp
+ *   x_u and length + 1;
+ *   one that has: itself, with eos as its token (its logits are not read),
+ * and of a search's candidates the `beams` of the largest score *
+ * max(length, 1)^-length_power become its beams (`to`, which may be `from`), the
+ * best first: equal ones by the lower beam, the larger logit, the lower token.
+ * parent gets the row that a beam goes on from (what mmr_kv8_fork takes), token
+ * its new token.  Scores are compared in 64 bits (the sum of exponentials is of
+ * 32-bit terms) and rounded once.
+ * Logits of -inf are no candidates, nor is what has a score of -inf in 32 bits;
+ * a beam of score -inf has none (a search begins with one beam of score 0 and the
+ * others at -inf, which makes its first beams differ).  Where there are fewer
+ * candidates than beams, the last beams get parent -1, score -inf, length 0, and
+ * eos as an ended beam (without eos: token 0).  eos is a token, or -1 for none
+ * (ended is then not read, and written as 0).
+ * *error (device int32, never cleared here) gets bit 2 if a score, or a logit
+ * of a beam that has not ended, is NaN or +inf: such a beam has no candidates.
+ * The workspace (mmr_beam_select_workspace_size bytes, 16-byte aligned) is the
+ * call's own until it has run.  No allocation, no synchronisation,
+ * graph-capturable. */
+typedef struct mmr_beams {
+  float* scores;
+  int32_t* lengths;
+  int32_t* ended;
+} mmr_beams;
+size_t mmr_beam_select_workspace_size(int64_t searches, int64_t beams, int64_t vocab);
+int mmr_beam_select(const float* logits, int64_t searches, int64_t beams, int64_t vocab, int32_t eos,
+                    double length_power, const mmr_beams* from, const mmr_beams* to, int32_t* parent, int32_t* token,
+                    void* workspace, size_t workspace_bytes, int32_t* error, mmr_stream_t stream);
+
 /* ---- products with 4-bit weights (no counterpart in the reference, whose
  * projections are fp16: ascend_matmul.cpp:385-410) ---------------------------
  * w[r][c] = scale[r][c / group] * q[r][c], q a whole number in [-8, 7], scale

@@ -1048,11 +1048,112 @@ mmr::Kv8Pages kv8_pages(const mmr_kv8_pages* c) {
   return p;
 }
 
+// What a row looks back on; window 0: on every key.
+struct Kv8Window {
+  int sinks = 0, window = 0;
+};
+
+// No window where every key is within it, or is one of the first.
+Kv8Window kv8_window(int64_t sinks, int64_t window, int64_t max_tokens) {
+  if (window >= max_tokens || sinks >= max_tokens) return {};
+  return {static_cast<int>(sinks), static_cast<int>(window)};
+}
+
+void check_kv8_window(int64_t sinks, int64_t window) {
+  require(sinks >= 0, "sinks must not be negative");
+  require(window >= 1, "window must be at least 1");
+}
+
 mmr::Kv8AttnPlan kv8_plan(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs, int64_t rows,
-                          int64_t max_rows, int64_t max_tokens) {
+                          int64_t max_rows, int64_t max_tokens, const Kv8Window& w) {
   return mmr::kv8_attention_plan(static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(head_dim),
                                  static_cast<int>(seqs), static_cast<int>(rows), static_cast<int>(max_rows),
-                                 max_tokens);
+                                 max_tokens, w.sinks, w.window);
+}
+
+// Bytes of the split partials; 0 for what no call takes.
+size_t kv8_partials(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs, int64_t rows, int64_t max_rows,
+                    int64_t max_tokens, int64_t sinks, int64_t window) {
+  if (guarded([&] { check_kv8_sizes(q_heads, kv_heads, head_dim, seqs, rows, max_rows); }) != MMR_OK) return 0;
+  if (max_rows == 0 || max_tokens < 1 || max_tokens > kKv8MostPages * mmr::kKv8Page) return 0;
+  return static_cast<size_t>(kv8_plan(q_heads, kv_heads, head_dim, seqs, rows, max_rows, max_tokens,
+                                      kv8_window(sinks, window, max_tokens))
+                                 .partial_floats) *
+         sizeof(float);
+}
+
+void kv8_attend(const float* query, const mmr_kv8_pages* cache, const int32_t* offsets, const int32_t* context,
+                int64_t rows, int64_t max_rows, int64_t max_tokens, int64_t sinks, int64_t window, int64_t q_heads,
+                float* out, void* workspace, size_t workspace_bytes, int32_t* error, mmr_stream_t stream) {
+  mmr::Kv8AttnArgs a;
+  a.cache = kv8_pages(cache);
+  check_kv8_sizes(q_heads, cache->kv_heads, cache->head_dim, cache->seqs, rows, max_rows);
+  require(query && offsets && context && out && error, "null argument");
+  require(aligned(query, 16) && aligned(out, 16) && aligned(workspace, 16),
+          "query, out and workspace must be 16-byte aligned");
+  require(max_tokens >= 1 && max_tokens <= cache->pages_per_seq * mmr::kKv8Page,
+          "max_tokens must be in [1, 64 pages_per_seq]");
+  if (max_rows == 0) return;
+  const Kv8Window w = kv8_window(sinks, window, max_tokens);
+  const mmr::Kv8AttnPlan p =
+      kv8_plan(q_heads, cache->kv_heads, cache->head_dim, cache->seqs, rows, max_rows, max_tokens, w);
+  const size_t need = static_cast<size_t>(p.partial_floats) * sizeof(float);
+  require(need == 0 || workspace, "null workspace");
+  require(workspace_bytes >= need, "workspace too small");
+  a.query = query;
+  a.offsets = offsets;
+  a.context = context;
+  a.rows = static_cast<int>(rows);
+  a.max_rows = static_cast<int>(max_rows);
+  a.hq = static_cast<int>(q_heads);
+  a.max_tokens = max_tokens;
+  a.out = out;
+  a.part = static_cast<float*>(workspace);
+  a.error = error;
+  a.sinks = w.sinks;
+  a.window = w.window;
+  hip(mmr::launch_kv8_attention(a, as_stream(stream)), "8-bit cache attention launch");
+}
+
+// The layers of a model: one table and one shape, memory of their own.
+std::vector<mmr::Kv8Layers> kv8_layers(const mmr_kv8_pages* layers, int64_t count) {
+  require(layers, "null layers");
+  require(count >= 1 && count <= 4096, "layers must be 1 to 4096");
+  std::vector<mmr::Kv8Layers> groups((count + mmr::kKv8MostLayers - 1) / mmr::kKv8MostLayers);
+  for (int64_t i = 0; i < count; ++i) {
+    const mmr::Kv8Pages p = kv8_pages(layers + i);
+    check_kv8_sizes(layers[i].kv_heads, layers[i].kv_heads, layers[i].head_dim, layers[i].seqs, 0, 0);
+    require(p.table == layers[0].table && p.pages == layers[0].pages && p.seqs == layers[0].seqs &&
+                p.per_seq == layers[0].pages_per_seq && p.hkv == layers[0].kv_heads && p.d == layers[0].head_dim,
+            "layers must have one table and one shape");
+    mmr::Kv8Layers& g = groups[i / mmr::kKv8MostLayers];
+    g.keys[g.count] = p.keys;
+    g.values[g.count] = p.values;
+    g.key_exps[g.count] = p.key_exps;
+    g.value_exps[g.count] = p.value_exps;
+    g.hkv = p.hkv;
+    g.d = p.d;
+    ++g.count;
+  }
+  return groups;
+}
+
+// Whether page numbers and counts of such a pool are whole numbers of 32 bits.
+bool kv8_pool_in_range(int64_t seqs, int64_t pages_per_seq, int64_t pages) {
+  return seqs >= 1 && seqs <= 65535 && pages_per_seq >= 1 && pages_per_seq <= kKv8MostPages && pages >= 1 &&
+         pages <= kKv8MostPages && seqs * pages_per_seq <= (int64_t{1} << 28);
+}
+
+void check_kv8_pool(const mmr_kv8_pages& c) {
+  require(kv8_pool_in_range(c.seqs, c.pages_per_seq, c.pages),
+          "pages over 2^24, or seqs x pages_per_seq over 2^28");
+}
+
+void check_beams(int64_t searches, int64_t beams, int64_t vocab) {
+  require(searches >= 1 && searches <= 65535, "searches must be in [1, 65535]");
+  require(beams >= 1 && beams <= mmr::kMostBeams, "beams must be in [1, 32]");
+  require(vocab >= 1 && vocab <= (int64_t{1} << 24), "vocab must be in [1, 2^24]");
+  require(searches * beams * ((vocab + 1023) / 1024) <= (int64_t{1} << 26), "too many logits");
 }
 
 bool q4_in_range(int64_t rows, int64_t cols) {
@@ -1107,42 +1208,140 @@ int mmr_kv8_append(const float* qkv, const float* q_norm, const float* k_norm, f
 
 size_t mmr_kv8_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
                                         int64_t rows, int64_t max_rows, int64_t max_tokens) {
-  if (guarded([&] { check_kv8_sizes(q_heads, kv_heads, head_dim, seqs, rows, max_rows); }) != MMR_OK) return 0;
-  if (max_rows == 0 || max_tokens < 1 || max_tokens > kKv8MostPages * mmr::kKv8Page) return 0;
-  return static_cast<size_t>(
-             kv8_plan(q_heads, kv_heads, head_dim, seqs, rows, max_rows, max_tokens).partial_floats) *
-         sizeof(float);
+  return kv8_partials(q_heads, kv_heads, head_dim, seqs, rows, max_rows, max_tokens, 0, max_tokens);
 }
 
 int mmr_kv8_attention(const float* query, const mmr_kv8_pages* cache, const int32_t* offsets, const int32_t* context,
                       int64_t rows, int64_t max_rows, int64_t max_tokens, int64_t q_heads, float* out,
                       void* workspace, size_t workspace_bytes, int32_t* error, mmr_stream_t stream) {
   return guarded([&] {
-    mmr::Kv8AttnArgs a;
-    a.cache = kv8_pages(cache);
-    check_kv8_sizes(q_heads, cache->kv_heads, cache->head_dim, cache->seqs, rows, max_rows);
-    require(query && offsets && context && out && error, "null argument");
-    require(aligned(query, 16) && aligned(out, 16) && aligned(workspace, 16),
-            "query, out and workspace must be 16-byte aligned");
-    require(max_tokens >= 1 && max_tokens <= cache->pages_per_seq * mmr::kKv8Page,
-            "max_tokens must be in [1, 64 pages_per_seq]");
-    if (max_rows == 0) return;
-    const mmr::Kv8AttnPlan p =
-        kv8_plan(q_heads, cache->kv_heads, cache->head_dim, cache->seqs, rows, max_rows, max_tokens);
-    const size_t need = static_cast<size_t>(p.partial_floats) * sizeof(float);
-    require(need == 0 || workspace, "null workspace");
-    require(workspace_bytes >= need, "workspace too small");
-    a.query = query;
-    a.offsets = offsets;
-    a.context = context;
-    a.rows = static_cast<int>(rows);
-    a.max_rows = static_cast<int>(max_rows);
-    a.hq = static_cast<int>(q_heads);
-    a.max_tokens = max_tokens;
-    a.out = out;
-    a.part = static_cast<float*>(workspace);
+    kv8_attend(query, cache, offsets, context, rows, max_rows, max_tokens, 0, max_tokens, q_heads, out, workspace,
+               workspace_bytes, error, stream);
+  });
+}
+
+size_t mmr_kv8_window_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
+                                               int64_t rows, int64_t max_rows, int64_t max_tokens, int64_t sinks,
+                                               int64_t window) {
+  if (guarded([&] { check_kv8_window(sinks, window); }) != MMR_OK) return 0;
+  return kv8_partials(q_heads, kv_heads, head_dim, seqs, rows, max_rows, max_tokens, sinks, window);
+}
+
+int mmr_kv8_window_attention(const float* query, const mmr_kv8_pages* cache, const int32_t* offsets,
+                             const int32_t* context, int64_t rows, int64_t max_rows, int64_t max_tokens,
+                             int64_t sinks, int64_t window, int64_t q_heads, float* out, void* workspace,
+                             size_t workspace_bytes, int32_t* error, mmr_stream_t stream) {
+  return guarded([&] {
+    check_kv8_window(sinks, window);
+    kv8_attend(query, cache, offsets, context, rows, max_rows, max_tokens, sinks, window, q_heads, out, workspace,
+               workspace_bytes, error, stream);
+  });
+}
+
+size_t mmr_kv8_fork_workspace_size(int64_t seqs, int64_t pages_per_seq, int64_t pages) {
+  if (!kv8_pool_in_range(seqs, pages_per_seq, pages)) return 0;
+  return static_cast<size_t>(mmr::kv8_fork_workspace(seqs, pages_per_seq, pages));
+}
+
+int mmr_kv8_fork(const mmr_kv8_pages* layers, int64_t count, int32_t* users, const int32_t* parent,
+                 const int32_t* keep, const int32_t* room, int64_t sinks, int64_t window, void* workspace,
+                 size_t workspace_bytes, int32_t* error, mmr_stream_t stream) {
+  return guarded([&] {
+    const std::vector<mmr::Kv8Layers> groups = kv8_layers(layers, count);
+    check_kv8_pool(layers[0]);
+    require(users && parent && keep && room && error, "null argument");
+    require(aligned(users, 16) && aligned(workspace, 16), "users and workspace must be 16-byte aligned");
+    require(sinks >= 0 && window >= 0, "sinks and window must not be negative");
+    require(workspace, "null workspace");
+    require(workspace_bytes >= mmr_kv8_fork_workspace_size(layers[0].seqs, layers[0].pages_per_seq, layers[0].pages),
+            "workspace too small");
+    mmr::Kv8ForkArgs a;
+    a.table = const_cast<int32_t*>(layers[0].table);
+    a.pages = static_cast<int>(layers[0].pages);
+    a.seqs = static_cast<int>(layers[0].seqs);
+    a.per_seq = static_cast<int>(layers[0].pages_per_seq);
+    a.users = users;
+    a.parent = parent;
+    a.keep = keep;
+    a.room = room;
+    const Kv8Window w = window > 0 ? kv8_window(sinks, window, layers[0].pages_per_seq * mmr::kKv8Page) : Kv8Window{};
+    a.sinks = w.sinks;
+    a.window = w.window;
+    a.workspace = static_cast<int32_t*>(workspace);
     a.error = error;
-    hip(mmr::launch_kv8_attention(a, as_stream(stream)), "8-bit cache attention launch");
+    hip(mmr::launch_kv8_fork(a, groups.data(), static_cast<int>(groups.size()), as_stream(stream)),
+        "8-bit cache fork launch");
+  });
+}
+
+size_t mmr_kv8_compact_workspace_size(int64_t pages) {
+  return kv8_pool_in_range(1, 1, pages) ? static_cast<size_t>(mmr::kv8_compact_workspace(pages)) : 0;
+}
+
+int mmr_kv8_compact(const mmr_kv8_pages* layers, int64_t count, const int32_t* users, int32_t* table_out,
+                    int32_t* users_out, int32_t* moved, int32_t* live, void* workspace, size_t workspace_bytes,
+                    mmr_stream_t stream) {
+  return guarded([&] {
+    const std::vector<mmr::Kv8Layers> groups = kv8_layers(layers, count);
+    check_kv8_pool(layers[0]);
+    require(users && table_out && users_out && moved && live, "null argument");
+    require(aligned(users, 16) && aligned(users_out, 16) && aligned(moved, 16) && aligned(workspace, 16),
+            "users, users_out, moved and workspace must be 16-byte aligned");
+    require(workspace, "null workspace");
+    require(workspace_bytes >= mmr_kv8_compact_workspace_size(layers[0].pages), "workspace too small");
+    mmr::Kv8CompactArgs a;
+    a.table = layers[0].table;
+    a.pages = static_cast<int>(layers[0].pages);
+    a.seqs = static_cast<int>(layers[0].seqs);
+    a.per_seq = static_cast<int>(layers[0].pages_per_seq);
+    a.users = users;
+    a.table_out = table_out;
+    a.users_out = users_out;
+    a.moved = moved;
+    a.live = live;
+    a.workspace = static_cast<int32_t*>(workspace);
+    hip(mmr::launch_kv8_compact(a, groups.data(), static_cast<int>(groups.size()), as_stream(stream)),
+        "8-bit cache compaction launch");
+  });
+}
+
+size_t mmr_beam_select_workspace_size(int64_t searches, int64_t beams, int64_t vocab) {
+  if (guarded([&] { check_beams(searches, beams, vocab); }) != MMR_OK) return 0;
+  return static_cast<size_t>(mmr::beam_select_workspace(static_cast<int>(searches), static_cast<int>(beams),
+                                                        static_cast<int>(vocab)));
+}
+
+int mmr_beam_select(const float* logits, int64_t searches, int64_t beams, int64_t vocab, int32_t eos,
+                    double length_power, const mmr_beams* from, const mmr_beams* to, int32_t* parent, int32_t* token,
+                    void* workspace, size_t workspace_bytes, int32_t* error, mmr_stream_t stream) {
+  return guarded([&] {
+    check_beams(searches, beams, vocab);
+    require(logits && from && to && parent && token && error, "null argument");
+    require(from->scores && from->lengths && from->ended && to->scores && to->lengths && to->ended,
+            "null beams buffer");
+    require(eos >= -1 && eos < vocab, "eos must be -1 or a token");
+    require(length_power >= 0.0 && length_power <= 16.0, "length_power must be in [0, 16]");
+    require(aligned(logits, 16) && aligned(workspace, 16), "logits and workspace must be 16-byte aligned");
+    require(workspace, "null workspace");
+    require(workspace_bytes >= mmr_beam_select_workspace_size(searches, beams, vocab), "workspace too small");
+    mmr::BeamArgs a;
+    a.logits = logits;
+    a.searches = static_cast<int>(searches);
+    a.beams = static_cast<int>(beams);
+    a.vocab = static_cast<int>(vocab);
+    a.eos = eos;
+    a.length_power = length_power;
+    a.scores = from->scores;
+    a.lengths = from->lengths;
+    a.ended = from->ended;
+    a.scores_out = to->scores;
+    a.lengths_out = to->lengths;
+    a.ended_out = to->ended;
+    a.parent = parent;
+    a.token = token;
+    a.workspace = workspace;
+    a.error = error;
+    hip(mmr::launch_beam_select(a, as_stream(stream)), "beam selection launch");
   });
 }
 

@@ -562,7 +562,7 @@ hipError_t measure_launch_floor(int kernels, int blocks, bool load_store, int re
 constexpr int kKv8Page = 64;   // tokens of a page
 constexpr int kKv8Block = 16;  // tokens of a block under one exponent
 constexpr int kKv8MinExp = -126, kKv8MaxExp = 122;
-enum Kv8Error : int { kKv8BadRows = 1, kKv8NotFinite = 2 };  // bits of *error
+enum Kv8Error : int { kKv8BadRows = 1, kKv8NotFinite = 2, kKv8NoPages = 4 };  // bits of *error
 
 struct Kv8Pages {
   int8_t* keys = nullptr;
@@ -592,7 +592,8 @@ struct Kv8AppendArgs {
 };
 hipError_t launch_kv8_append(const Kv8AppendArgs& a, hipStream_t stream);
 
-// Causal attention of the same rows over the cache.
+// Causal attention of the same rows over the cache; with a window, of the last
+// `window` keys and the first `sinks` ones.
 struct Kv8AttnArgs {
   Kv8Pages cache;
   const float* query = nullptr;
@@ -603,6 +604,7 @@ struct Kv8AttnArgs {
   float* out = nullptr;
   float* part = nullptr;  // kv8_attention_plan(...).partial_floats floats
   int32_t* error = nullptr;
+  int sinks = 0, window = 0;  // window 0: every key
 };
 struct Kv8AttnPlan {
   int tile_rows = 0;    // (token, head) rows of one KV group that a block takes
@@ -610,8 +612,70 @@ struct Kv8AttnPlan {
   int splits = 0;
   int64_t partial_floats = 0;  // 0 when one split covers every context
 };
-Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens);
+Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens, int sinks,
+                               int window);
 hipError_t launch_kv8_attention(const Kv8AttnArgs& a, hipStream_t stream);
+
+// -------------------------------------------- pages of the 8-bit cache ----
+// The memory of every layer of a model, whose sequences have one table.
+constexpr int kKv8MostLayers = 64;  // of a launch: their pointers are kernel arguments
+struct Kv8Layers {
+  int8_t* keys[kKv8MostLayers];
+  int8_t* values[kKv8MostLayers];
+  int8_t* key_exps[kKv8MostLayers];
+  int8_t* value_exps[kKv8MostLayers];
+  int count = 0, hkv = 0, d = 0;
+};
+
+// Sequence i becomes the first keep[i] tokens of sequence parent[i] (-1: none)
+// with room for room[i] more; pages are shared, copied, taken and freed.
+struct Kv8ForkArgs {
+  int32_t* table = nullptr;  // [seqs][per_seq]
+  int pages = 0, seqs = 0, per_seq = 0;
+  int32_t* users = nullptr;  // [pages]
+  const int32_t* parent = nullptr;
+  const int32_t* keep = nullptr;
+  const int32_t* room = nullptr;
+  int sinks = 0, window = 0;  // window 0: no page falls behind
+  int32_t* workspace = nullptr;  // kv8_fork_workspace bytes
+  int32_t* error = nullptr;
+};
+int64_t kv8_fork_workspace(int64_t seqs, int64_t per_seq, int64_t pages);
+hipError_t launch_kv8_fork(const Kv8ForkArgs& a, const Kv8Layers* layers, int groups, hipStream_t stream);
+
+// Moves the pages in use to the lowest numbers.
+struct Kv8CompactArgs {
+  const int32_t* table = nullptr;
+  int pages = 0, seqs = 0, per_seq = 0;
+  const int32_t* users = nullptr;
+  int32_t* table_out = nullptr;
+  int32_t* users_out = nullptr;
+  int32_t* moved = nullptr;  // [pages]
+  int32_t* live = nullptr;
+  int32_t* workspace = nullptr;  // kv8_compact_workspace bytes
+};
+int64_t kv8_compact_workspace(int64_t pages);
+hipError_t launch_kv8_compact(const Kv8CompactArgs& a, const Kv8Layers* layers, int groups, hipStream_t stream);
+
+// ------------------------------------------------------- beam search ----
+constexpr int kMostBeams = 32;
+struct BeamArgs {
+  const float* logits = nullptr;  // [searches * beams][vocab]
+  int searches = 0, beams = 0, vocab = 0, eos = -1;
+  double length_power = 0.0;
+  const float* scores = nullptr;
+  const int32_t* lengths = nullptr;
+  const int32_t* ended = nullptr;
+  float* scores_out = nullptr;
+  int32_t* lengths_out = nullptr;
+  int32_t* ended_out = nullptr;
+  int32_t* parent = nullptr;
+  int32_t* token = nullptr;
+  void* workspace = nullptr;  // beam_select_workspace bytes
+  int32_t* error = nullptr;
+};
+int64_t beam_select_workspace(int searches, int beams, int vocab);
+hipError_t launch_beam_select(const BeamArgs& a, hipStream_t stream);
 
 // ------------------------------------------- 4-bit matrix-vector product ----
 // y[b][r] = sum_c scale[r][c / group] * q[r][c] * x[b][c], the prologues and

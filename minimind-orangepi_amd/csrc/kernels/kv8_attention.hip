@@ -147,6 +147,44 @@ __device__ __forceinline__ int blocks_seen(int limit, int first) {
   return min(kKv8Blocks, max(0, limit - first + kKv8Block) / kKv8Block);
 }
 
+// The pages that a block's rows attend, numbered from 0 without a gap.  With a
+// window, those are the pages of the first keys (`sinks`), then those from the
+// window of the block's first row on: `skip` pages between are never read, nor
+// are their numbers.
+template <bool kWindow>
+struct Reach {
+  int early, skip, pages;
+  __device__ __forceinline__ Reach(const Kv8AttnArgs& a, int first_key, int last_key) {
+    pages = last_key / kKv8Page + 1;
+    if constexpr (kWindow) {
+      early = (a.sinks + kKv8Page - 1) / kKv8Page;
+      skip = max(0, max(0, first_key - a.window + 1) / kKv8Page - early);
+      pages -= skip;
+    }
+  }
+  __device__ __forceinline__ int place(int p) const {  // in the sequence
+    if constexpr (kWindow) return p < early ? p : p + skip;
+    return p;
+  }
+};
+// Whether a row with the last key `limit` attends key j, or a key of the block
+// of keys from j on.
+template <bool kWindow>
+__device__ __forceinline__ bool sees(const Kv8AttnArgs& a, int limit, int j) {
+  if constexpr (kWindow) return j <= limit && (j < a.sinks || j > limit - a.window);
+  return j <= limit;
+}
+__device__ __forceinline__ int largest_exponent_seen(const Kv8AttnArgs& a, uint32_t exps, int limit, int first) {
+  int e = kKv8MinExp - 1;
+#pragma unroll
+  for (int b = 0; b < kKv8Blocks; ++b) {
+    const int j = first + kKv8Block * b;
+    if (j <= limit && (j < a.sinks || j + kKv8Block - 1 > limit - a.window))
+      e = max(e, static_cast<int>(static_cast<int8_t>(exps >> (8 * b))));
+  }
+  return e;
+}
+
 // Splits of at most `chunk` pages each that a row's `pages` are dealt to, evenly.
 __device__ __forceinline__ int splits_used(int pages, int chunk) { return (pages + chunk - 1) / chunk; }
 
@@ -166,7 +204,7 @@ __device__ __forceinline__ void store_ml(const Kv8AttnArgs& a, int64_t row, int 
 // 5.3: two dependent loads, a page's arithmetic (two of them one after another
 // from 513 to 1,024 tokens), the join in LDS and, above, the one of the splits.
 // The fp16 cache's attention takes 12.4, 6.9, 6.0, 5.9 and 5.8 there.
-template <int D>
+template <int D, bool kWindow>
 __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a, int chunk, int splits) {
   constexpr int kRows = kStepTile, kTiles = D / 16;  // tiles of the output's dimensions
   const int s = blockIdx.y, hkv = a.cache.hkv, group = a.hq / hkv;
@@ -177,7 +215,8 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
   // offsets, not after them.
   const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
   const int begin = split * chunk, from = begin + wave;
-  int numbers = table[min(from + kStepWaves * lane, a.cache.per_seq - 1)];
+  int numbers = 0;
+  if constexpr (!kWindow) numbers = table[min(from + kStepWaves * lane, a.cache.per_seq - 1)];
   Kv8Span span;
   const bool fine = kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span);
   if (!fine || (span.n > 0 && static_cast<int64_t>(span.context) + span.n > a.max_tokens)) {
@@ -186,9 +225,12 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
   }
   const int total = min(span.n * group - first, kRows);  // rows of this group of heads, from `first` on
   if (total <= 0) return;
-  const int last_key = span.context + (first + total - 1) / group, pages = last_key / kKv8Page + 1;
-  const int used = splits_used(pages, chunk), end = min(begin + chunk, pages);
+  const int first_last = span.context + first / group, last_key = span.context + (first + total - 1) / group;
+  const Reach<kWindow> reach(a, first_last, last_key);
+  const int used = splits_used(reach.pages, chunk), end = min(begin + chunk, reach.pages);
   if (split >= used) return;
+  // Which pages those are follows from the context: their numbers come one load later.
+  if constexpr (kWindow) numbers = table[min(reach.place(from + kStepWaves * lane), a.cache.per_seq - 1)];
 
   // This lane's column: digit `digit` of row m.  Columns past the last row are
   // that row again: another block's row could change while it is read (out in
@@ -210,7 +252,7 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
   auto ask = [&]() {  // addresses and exponents of step ask_at, at most the last
     const int step = min(ask_at, (end - 1 - from) / kStepWaves);
     if (ask_at == step && step > 0 && step % kWave == 0) {  // not for the last again
-      numbers = table[min(from + kStepWaves * (step + lane), a.cache.per_seq - 1)];
+      numbers = table[min(reach.place(from + kStepWaves * (step + lane)), a.cache.per_seq - 1)];
       asm volatile("" : "+v"(numbers));  // waited for here, not wherever it is read
     }
     ++ask_at;
@@ -328,13 +370,20 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) score[t][i] = -INFINITY;
-    } else if (p * kKv8Page + kKv8Page - 1 > span.context) {  // the first token sees keys up to context
-      page_exp = largest_exponent(value_exps, blocks_seen(limit, p * kKv8Page));
+    } else {
+      // The first token sees keys up to context, the last the fewest of those behind it.
+      const int key = reach.place(p) * kKv8Page;
+      bool some = key + kKv8Page - 1 > span.context;
+      if constexpr (kWindow) some = some || (key <= last_key - a.window && key + kKv8Page > a.sinks);
+      if (some) {
+        page_exp = kWindow ? largest_exponent_seen(a, value_exps, limit, key)
+                           : largest_exponent(value_exps, blocks_seen(limit, key));
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (p * kKv8Page + 16 * g + 4 * t + i > limit) score[t][i] = -INFINITY;
+          for (int i = 0; i < 4; ++i)
+            if (!sees<kWindow>(a, limit, key + 16 * g + 4 * t + i)) score[t][i] = -INFINITY;
+      }
     }
     float top = -INFINITY;
 #pragma unroll
@@ -452,7 +501,7 @@ __device__ __forceinline__ void split2_truncated(float x0, float x1, uint32_t& h
 // it is none of them but the chain barrier - LDS - products - weights - products
 // with three waves a SIMD.  32 rows a wave (half the LDS reads a row, two waves
 // a SIMD) took as long there, blocks of eight waves 101.
-template <int D>
+template <int D, bool kWindow>
 __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel(Kv8AttnArgs a, int chunk, int splits) {
   constexpr int kTiles = D / 16, kRuns = D / 32;  // tiles of the output, products along D
   constexpr int kPieces = D / 32;                 // 16-byte pieces of a page that a thread widens
@@ -475,21 +524,23 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
   if (tile < 0) return;
   const int first = tile * kRowsTile;
   const int last_token = (min(first + kRowsTile, total) - 1) / group;
-  const int pages = (span.context + last_token) / kKv8Page + 1;
-  const int used = splits_used(pages, chunk);
+  const Reach<kWindow> reach(a, span.context + first / group, span.context + last_token);
+  const int used = splits_used(reach.pages, chunk);
   if (split >= used) return;
-  const int each = (pages + used - 1) / used, begin = split * each, end = min(begin + each, pages);
+  const int each = (reach.pages + used - 1) / used, begin = split * each, end = min(begin + each, reach.pages);
 
   // This lane's row.
   const int wave_first = first + 16 * wave;
   const bool works = wave_first < total;
   const int all_see = span.context + min(wave_first, total - 1) / group;
+  // Keys up to here are behind the window of the wave's last row.
+  const int some_miss = kWindow ? span.context + min(wave_first + 15, total - 1) / group - a.window : -1;
   const int m = min(wave_first + col, total - 1), token = m / group;  // lanes past the last row are that row again
   const int limit = span.context + token;                             // its last key
   const int64_t row = (static_cast<int64_t>(span.first) + token) * a.hq + h * group + m % group;
 
   const int32_t* table = a.cache.table + static_cast<int64_t>(s) * a.cache.per_seq;
-  int numbers = table[min(begin + lane, a.cache.per_seq - 1)];
+  int numbers = table[min(reach.place(begin + lane), a.cache.per_seq - 1)];
   float v[8 * kRuns];  // of the query, which does not wait for a page's number
 #pragma unroll
   for (int c = 0; c < kRuns; ++c)
@@ -504,7 +555,7 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
   auto ask = [&](int p) {
     const int step = p - begin;
     if (step > 0 && step % kWave == 0) {
-      numbers = table[min(p + lane, a.cache.per_seq - 1)];
+      numbers = table[min(reach.place(p + lane), a.cache.per_seq - 1)];
       asm volatile("" : "+v"(numbers));  // waited for here, not wherever it is read
     }
     const int number = __builtin_amdgcn_readlane(numbers, step % kWave);
@@ -631,14 +682,16 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
                         ldexpf(score_unit<D>(), unit_exp + static_cast<int8_t>(key_exps >> (16 + shift)))};
     // As for steps: of the blocks that the row attends.
     int page_exp = largest_exponent(value_exps, kKv8Blocks);
-    if (hidden || p * kKv8Page + kKv8Page - 1 > all_see) {
-      page_exp = largest_exponent(value_exps, hidden ? 0 : blocks_seen(limit, p * kKv8Page));
+    const int key = reach.place(p) * kKv8Page;
+    if (hidden || key + kKv8Page - 1 > all_see || (kWindow && key <= some_miss && key + kKv8Page > a.sinks)) {
+      page_exp = kWindow ? (hidden ? kKv8MinExp - 1 : largest_exponent_seen(a, value_exps, limit, key))
+                         : largest_exponent(value_exps, hidden ? 0 : blocks_seen(limit, key));
       // Scaled first: a factor may be 0 or, of a block that holds anything, infinite.
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          score[t][i] = hidden || p * kKv8Page + 32 * (t / 2) + 8 * g + 4 * (t % 2) + i > limit
+          score[t][i] = hidden || !sees<kWindow>(a, limit, key + 32 * (t / 2) + 8 * g + 4 * (t % 2) + i)
                             ? -INFINITY
                             : score[t][i] * to_log2[t / 2];
       to_log2[0] = to_log2[1] = 1.0f;
@@ -715,15 +768,17 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
 }
 
 // Splits of row `i` of a sequence's (token, head) rows.
+template <bool kWindow>
 __device__ __forceinline__ int splits_of(const Kv8AttnArgs& a, const Kv8Span& span, int i, int chunk, int tile_rows) {
   const int token = i / a.hq, head = i - token * a.hq, group = a.hq / a.cache.hkv;
   const int m = token * group + head % group;
-  const int tile_end = min((m / tile_rows + 1) * tile_rows, span.n * group);
-  const int pages = (span.context + (tile_end - 1) / group) / kKv8Page + 1;
-  return splits_used(pages, chunk);
+  const int tile_first = m / tile_rows * tile_rows, tile_end = min(tile_first + tile_rows, span.n * group);
+  const Reach<kWindow> reach(a, span.context + tile_first / group, span.context + (tile_end - 1) / group);
+  return splits_used(reach.pages, chunk);
 }
 
 // Joins a few splits of many rows: d / 4 threads a (token, head).
+template <bool kWindow>
 __global__ __launch_bounds__(kJoinThreads) void kv8_combine_few_kernel(Kv8AttnArgs a, int chunk, int splits,
                                                                        int tile_rows) {
   const int s = blockIdx.y, d = a.cache.d, quads = d / 4, each = kJoinThreads / quads;
@@ -732,7 +787,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_few_kernel(Kv8AttnAr
   if (static_cast<int64_t>(span.context) + span.n > a.max_tokens) return;
   const int part = threadIdx.x / quads, quad = threadIdx.x - part * quads, i = blockIdx.x * each + part;
   if (part >= each || i >= span.n * a.hq) return;
-  const int used = splits_of(a, span, i, chunk, tile_rows);
+  const int used = splits_of<kWindow>(a, span, i, chunk, tile_rows);
   if (used == 1) return;
   const int64_t to = static_cast<int64_t>(span.first) * a.hq + i;
   const float2* ml =
@@ -762,7 +817,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_few_kernel(Kv8AttnAr
 // Joins many splits, a block per (token, head): groups of d / 4 threads take
 // splits in turn, four dimensions each, with all loads under way before the
 // first wave, a split a lane, has the weights.
-template <int D>
+template <int D, bool kWindow>
 __global__ __launch_bounds__(kJoinThreads) void kv8_combine_kernel(Kv8AttnArgs a, int chunk, int splits,
                                                                    int tile_rows) {
   constexpr int kQuads = D / 4, kGroups = kJoinThreads / kQuads, kEach = (kMostSplits + kGroups - 1) / kGroups;
@@ -774,7 +829,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_kernel(Kv8AttnArgs a
   if (!kv8_span(a.cache, a.offsets, a.context, s, a.rows, a.max_rows, &span)) return;
   if (static_cast<int64_t>(span.context) + span.n > a.max_tokens) return;
   if (i >= span.n * a.hq) return;
-  const int used = splits_of(a, span, i, chunk, tile_rows);
+  const int used = splits_of<kWindow>(a, span, i, chunk, tile_rows);
   if (used == 1) return;
   const int64_t to = static_cast<int64_t>(span.first) * a.hq + i;
   const float2* ml =
@@ -847,18 +902,28 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_kernel(Kv8AttnArgs a
 // A launch is sized as if every sequence brought max_rows rows: with a prompt
 // among them, single rows get no splits and a wave each (512 rows and 31 single
 // rows over up to 8,192 tokens 386; apart 13.5 and 18.2).
-Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens) {
+Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens, int sinks,
+                               int window) {
   Kv8AttnPlan p;
   const int64_t most = static_cast<int64_t>(hq / hkv) * max_rows;
-  const int64_t pages = (max_tokens + kKv8Page - 1) / kKv8Page;
+  int64_t pages = (max_tokens + kKv8Page - 1) / kKv8Page;
   const bool step = most <= kStepRows;
   p.tile_rows = step ? kStepTile : kRowsTile;
+  bool all_alike = step;  // tiles see like numbers of pages
+  if (window > 0) {
+    // A tile's rows are of up to tile_tokens tokens, and n keys lie in up to (n + 62) / 64 + 1 pages.
+    const int64_t tile_tokens = std::min<int64_t>(max_rows, (p.tile_rows - 1) / (hq / hkv) + 2);
+    const int64_t reach = (static_cast<int64_t>(sinks) + kKv8Page - 1) / kKv8Page +
+                          (static_cast<int64_t>(window) + tile_tokens - 1 + kKv8Page - 2) / kKv8Page + 1;
+    all_alike = all_alike || reach < pages;
+    pages = std::min(pages, reach);
+  }
   const int64_t blocks = (most + p.tile_rows - 1) / p.tile_rows * hkv * seqs;
   const int64_t wanted = step ? kStepBlocks : kRowsBlocks;
   const bool few = step || static_cast<int64_t>(rows) * hq <= kFewRows;
   const int64_t splits = few ? kMostSplits : kFewSplits, least = few ? kLeastPages : kLeastRowsPages;
   // Of a prompt's tiles, the first sees the context and the last all of max_tokens.
-  const int64_t mean = step ? pages : std::max<int64_t>(1, (2 * max_tokens - max_rows) / (2 * kKv8Page));
+  const int64_t mean = all_alike ? pages : std::max<int64_t>(1, (2 * max_tokens - max_rows) / (2 * kKv8Page));
   int64_t chunk = pages;
   if (blocks < wanted && !(step && pages <= kWidePages))
     chunk = std::max<int64_t>({least, (mean * blocks + wanted - 1) / wanted, (pages + splits - 1) / splits});
@@ -870,38 +935,43 @@ Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int m
 
 namespace {
 
-template <int D>
+template <int D, bool kWindow>
 void launch_attention_for(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t stream) {
   const int hkv = a.cache.hkv, most = a.hq / hkv * a.max_rows;
   const int tiles = (most + p.tile_rows - 1) / p.tile_rows;
   if (p.tile_rows != kStepTile)
-    kv8_rows_kernel<D><<<dim3(p.splits * tiles * hkv, a.cache.seqs), kRowsThreads, 0, stream>>>(a, p.chunk_pages,
+    kv8_rows_kernel<D, kWindow><<<dim3(p.splits * tiles * hkv, a.cache.seqs), kRowsThreads, 0, stream>>>(a, p.chunk_pages,
                                                                                                p.splits);
   else
-    kv8_step_kernel<D><<<dim3(p.splits * hkv, a.cache.seqs, tiles), kStepThreads, 0, stream>>>(a, p.chunk_pages,
+    kv8_step_kernel<D, kWindow><<<dim3(p.splits * hkv, a.cache.seqs, tiles), kStepThreads, 0, stream>>>(a, p.chunk_pages,
                                                                                               p.splits);
   if (p.splits > 1 && p.splits <= kFewSplits) {
     const int each = kJoinThreads / (D / 4);
-    kv8_combine_few_kernel<<<dim3((a.max_rows * a.hq + each - 1) / each, a.cache.seqs), kJoinThreads, 0, stream>>>(
+    kv8_combine_few_kernel<kWindow><<<dim3((a.max_rows * a.hq + each - 1) / each, a.cache.seqs), kJoinThreads, 0, stream>>>(
         a, p.chunk_pages, p.splits, p.tile_rows);
   } else if (p.splits > 1)
-    kv8_combine_kernel<D><<<dim3(a.max_rows * a.hq, a.cache.seqs), kJoinThreads, 0, stream>>>(
+    kv8_combine_kernel<D, kWindow><<<dim3(a.max_rows * a.hq, a.cache.seqs), kJoinThreads, 0, stream>>>(
         a, p.chunk_pages, p.splits, p.tile_rows);
+}
+
+template <bool kWindow>
+hipError_t launch_attention(const Kv8AttnArgs& a, hipStream_t stream) {
+  const Kv8AttnPlan p = kv8_attention_plan(a.hq, a.cache.hkv, a.cache.d, a.cache.seqs, a.rows, a.max_rows,
+                                           a.max_tokens, a.sinks, a.window);
+  switch (a.cache.d) {
+    case 32: launch_attention_for<32, kWindow>(a, p, stream); break;
+    case 64: launch_attention_for<64, kWindow>(a, p, stream); break;
+    case 96: launch_attention_for<96, kWindow>(a, p, stream); break;
+    case 128: launch_attention_for<128, kWindow>(a, p, stream); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_kv8_attention(const Kv8AttnArgs& a, hipStream_t stream) {
-  const Kv8AttnPlan p =
-      kv8_attention_plan(a.hq, a.cache.hkv, a.cache.d, a.cache.seqs, a.rows, a.max_rows, a.max_tokens);
-  switch (a.cache.d) {
-    case 32: launch_attention_for<32>(a, p, stream); break;
-    case 64: launch_attention_for<64>(a, p, stream); break;
-    case 96: launch_attention_for<96>(a, p, stream); break;
-    case 128: launch_attention_for<128>(a, p, stream); break;
-    default: return hipErrorInvalidValue;
-  }
-  return hipGetLastError();
+  return a.window > 0 ? launch_attention<true>(a, stream) : launch_attention<false>(a, stream);
 }
 
 }  // namespace mmr

@@ -79,6 +79,10 @@ class _Kv8PagesStruct(C.Structure):
                [(n, C.c_int64) for n in ("pages", "seqs", "pages_per_seq", "kv_heads", "head_dim")]
 
 
+class _BeamsStruct(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("scores", "lengths", "ended")]
+
+
 VP, I64, I32, U64, F32, SZ = C.c_void_p, C.c_int64, C.c_int32, C.c_uint64, C.c_float, C.c_size_t
 P_I32 = C.POINTER(C.c_int32)
 P_F32 = C.POINTER(C.c_float)
@@ -160,6 +164,16 @@ _SIGS = {
     "mmr_kv8_append": ([VP, VP, VP, F32, VP, C.POINTER(_Kv8PagesStruct), VP, VP, I64, I64, I64, VP, VP, VP], C.c_int),
     "mmr_kv8_attention_workspace_size": ([I64] * 7, SZ),
     "mmr_kv8_attention": ([VP, C.POINTER(_Kv8PagesStruct), VP, VP, I64, I64, I64, I64, VP, VP, SZ, VP, VP], C.c_int),
+    "mmr_kv8_window_attention_workspace_size": ([I64] * 9, SZ),
+    "mmr_kv8_window_attention": ([VP, C.POINTER(_Kv8PagesStruct), VP, VP, I64, I64, I64, I64, I64, I64, VP, VP, SZ, VP,
+                                  VP], C.c_int),
+    "mmr_kv8_fork_workspace_size": ([I64] * 3, SZ),
+    "mmr_kv8_fork": ([VP, I64, VP, VP, VP, VP, I64, I64, VP, SZ, VP, VP], C.c_int),
+    "mmr_kv8_compact_workspace_size": ([I64], SZ),
+    "mmr_kv8_compact": ([VP, I64, VP, VP, VP, VP, VP, VP, SZ, VP], C.c_int),
+    "mmr_beam_select_workspace_size": ([I64] * 3, SZ),
+    "mmr_beam_select": ([VP, I64, I64, I64, I32, C.c_double, C.POINTER(_BeamsStruct), C.POINTER(_BeamsStruct), VP, VP,
+                         VP, SZ, VP, VP], C.c_int),
     "mmr_q4_code_bytes": ([I64, I64], SZ),
     "mmr_q4_quantize": ([VP, I64, I64, I64, VP, VP], C.c_int),
     "mmr_q4_dequantize": ([VP, VP, I64, I64, I64, VP], C.c_int),
@@ -617,7 +631,7 @@ def prefill_attention(query, cache: KvCache, start_position, seq_len, q_heads, k
 
 
 KV8_PAGE, KV8_BLOCK = 64, 16
-KV8_ERROR_ROWS, KV8_ERROR_NOT_FINITE = 1, 2
+KV8_ERROR_ROWS, KV8_ERROR_NOT_FINITE, KV8_ERROR_PAGES = 1, 2, 4
 
 
 class Kv8Pages:
@@ -661,6 +675,67 @@ def kv8_attention(query, cache: Kv8Pages, offsets, context, rows: int, max_rows:
     check(_lib.mmr_kv8_attention(query.ptr, cache.ref, offsets.ptr, context.ptr, rows, max_rows, max_tokens, q_heads,
                                  out.ptr, workspace.ptr if workspace else None, workspace.nbytes if workspace else 0,
                                  error.ptr, _s(stream)))
+
+
+def kv8_window_attention_workspace_size(q_heads: int, kv_heads: int, head_dim: int, seqs: int, rows: int,
+                                        max_rows: int, max_tokens: int, sinks: int, window: int) -> int:
+    return int(_lib.mmr_kv8_window_attention_workspace_size(q_heads, kv_heads, head_dim, seqs, rows, max_rows,
+                                                            max_tokens, sinks, window))
+
+
+def kv8_window_attention(query, cache: Kv8Pages, offsets, context, rows: int, max_rows: int, max_tokens: int,
+                         sinks: int, window: int, q_heads: int, out, workspace, error, stream=None) -> None:
+    check(_lib.mmr_kv8_window_attention(query.ptr, cache.ref, offsets.ptr, context.ptr, rows, max_rows, max_tokens,
+                                        sinks, window, q_heads, out.ptr, workspace.ptr if workspace else None,
+                                        workspace.nbytes if workspace else 0, error.ptr, _s(stream)))
+
+
+class Kv8Layers:
+    """The caches of a model's layers (Kv8Pages of one table and one shape, kept alive by this object)."""
+
+    def __init__(self, layers):
+        self.layers = tuple(layers)
+        self.count = len(self.layers)
+        self.structs = (_Kv8PagesStruct * self.count)(*(layer.struct for layer in self.layers))
+        self.ref = C.addressof(self.structs)
+
+
+def kv8_fork_workspace_size(seqs: int, pages_per_seq: int, pages: int) -> int:
+    return int(_lib.mmr_kv8_fork_workspace_size(seqs, pages_per_seq, pages))
+
+
+def kv8_fork(layers: Kv8Layers, users, parent, keep, room, workspace, error, *, sinks: int = 0, window: int = 0,
+             stream=None) -> None:
+    check(_lib.mmr_kv8_fork(layers.ref, layers.count, users.ptr, parent.ptr, keep.ptr, room.ptr, sinks, window,
+                            workspace.ptr, workspace.nbytes, error.ptr, _s(stream)))
+
+
+def kv8_compact_workspace_size(pages: int) -> int:
+    return int(_lib.mmr_kv8_compact_workspace_size(pages))
+
+
+def kv8_compact(layers: Kv8Layers, users, table_out, users_out, moved, live, workspace, stream=None) -> None:
+    check(_lib.mmr_kv8_compact(layers.ref, layers.count, users.ptr, table_out.ptr, users_out.ptr, moved.ptr, live.ptr,
+                               workspace.ptr, workspace.nbytes, _s(stream)))
+
+
+class Beams:
+    """Scores, lengths and ends of the beams of many searches (mmr_beams), in buffers that the caller owns."""
+
+    def __init__(self, scores, lengths, ended):
+        self.buffers = self.scores, self.lengths, self.ended = scores, lengths, ended
+        self.struct = _BeamsStruct(*(b.ptr for b in self.buffers))
+        self.ref = C.byref(self.struct)
+
+
+def beam_select_workspace_size(searches: int, beams: int, vocab: int) -> int:
+    return int(_lib.mmr_beam_select_workspace_size(searches, beams, vocab))
+
+
+def beam_select(logits, searches: int, beams: int, vocab: int, eos: int, length_power: float, before: Beams,
+                after: Beams, parent, token, workspace, error, stream=None) -> None:
+    check(_lib.mmr_beam_select(logits.ptr, searches, beams, vocab, eos, length_power, before.ref, after.ref,
+                               parent.ptr, token.ptr, workspace.ptr, workspace.nbytes, error.ptr, _s(stream)))
 
 
 def q4_quantize(w: np.ndarray, group: int) -> tuple[np.ndarray, np.ndarray]:
