@@ -538,8 +538,8 @@ int mmr_kv8_compact(const mmr_kv8_pages* layers, int64_t count, const int32_t* u
  *   one that has: itself, with eos as its token (its logits are not read),
  * and of a search's candidates the `beams` of the largest score *
  * max(length, 1)^-length_power become its beams (`to`, which may be `from`), the
- * best first: equal ones by the lower beam, the larger logit, the lower token.
- * parent gets the row that a beam goes on from (what mmr_kv8_fork takes), token
+ * best first: equal ones by the lower beam, the larger logit, the lower token
+ * (equal rows of logits have equal sums).  parent gets the row that a beam goes on from (what mmr_kv8_fork takes), token
  * its new token.  Scores are compared in 64 bits (the sum of exponentials is of
  * 32-bit terms) and rounded once.
  * Logits of -inf are no candidates, nor is what has a score of -inf in 32 bits;
@@ -550,8 +550,8 @@ int mmr_kv8_compact(const mmr_kv8_pages* layers, int64_t count, const int32_t* u
  * (ended is then not read, and written as 0).
  * *error (device int32, never cleared here) gets bit 2 if a score, or a logit
  * of a beam that has not ended, is NaN or +inf: such a beam has no candidates.
- * The workspace (mmr_beam_select_workspace_size bytes, 16-byte aligned) is the
- * call's own until it has run.  No allocation, no synchronisation,
+ * The workspace (mmr_beam_select_workspace_size bytes, possibly 0; 16-byte
+ * aligned) is the call's own until it has run.  No allocation, no synchronisation,
  * graph-capturable. */
 typedef struct mmr_beams {
   float* scores;

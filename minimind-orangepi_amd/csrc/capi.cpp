@@ -1322,8 +1322,9 @@ int mmr_beam_select(const float* logits, int64_t searches, int64_t beams, int64_
     require(eos >= -1 && eos < vocab, "eos must be -1 or a token");
     require(length_power >= 0.0 && length_power <= 16.0, "length_power must be in [0, 16]");
     require(aligned(logits, 16) && aligned(workspace, 16), "logits and workspace must be 16-byte aligned");
-    require(workspace, "null workspace");
-    require(workspace_bytes >= mmr_beam_select_workspace_size(searches, beams, vocab), "workspace too small");
+    const size_t need = mmr_beam_select_workspace_size(searches, beams, vocab);
+    require(need == 0 || workspace, "null workspace");
+    require(workspace_bytes >= need, "workspace too small");
     mmr::BeamArgs a;
     a.logits = logits;
     a.searches = static_cast<int>(searches);

@@ -735,7 +735,8 @@ def beam_select_workspace_size(searches: int, beams: int, vocab: int) -> int:
 def beam_select(logits, searches: int, beams: int, vocab: int, eos: int, length_power: float, before: Beams,
                 after: Beams, parent, token, workspace, error, stream=None) -> None:
     check(_lib.mmr_beam_select(logits.ptr, searches, beams, vocab, eos, length_power, before.ref, after.ref,
-                               parent.ptr, token.ptr, workspace.ptr, workspace.nbytes, error.ptr, _s(stream)))
+                               parent.ptr, token.ptr, workspace.ptr if workspace else None,
+                               workspace.nbytes if workspace else 0, error.ptr, _s(stream)))
 
 
 def q4_quantize(w: np.ndarray, group: int) -> tuple[np.ndarray, np.ndarray]:

@@ -104,7 +104,7 @@ def test_compact_refuses(mmr):
 def test_select_refuses(mmr):
     b = At()
     beams = mmr.Beams(b, b, b)
-    good = dict(logits=b, searches=2, beams=4, vocab=100, eos=2, length_power=0.5, before=beams, after=beams, parent=b,
+    good = dict(logits=b, searches=2, beams=4, vocab=50000, eos=2, length_power=0.5, before=beams, after=beams, parent=b,
                 token=b, workspace=b, error=b)
     refused = refuser(mmr, mmr.beam_select, good)
     for name in ("logits", "parent", "token", "error"):
@@ -125,11 +125,11 @@ def test_select_refuses(mmr):
     refused("vocab", vocab=(1 << 24) + 1)
     refused("too many", searches=65535, beams=32, vocab=1 << 20)
     refused("eos", eos=-2)
-    refused("eos", eos=100)
+    refused("eos", eos=50000)
     for power in (-0.5, 17.0, float("nan"), float("inf")):
         refused("length_power", length_power=power)
-    need = mmr.beam_select_workspace_size(2, 4, 100)
-    assert need > 0
+    need = mmr.beam_select_workspace_size(2, 4, 50000)
+    assert need > 0 and mmr.beam_select_workspace_size(2, 4, 100) == 0
     refused("too small", workspace=At(4096, need - 1))
 
 
