@@ -9,11 +9,11 @@
 // logits finds those with the run's sum of exponentials, and what is ranked, in
 // 64 bits, is few.
 //
-// The k largest of many values: the k-th largest of the lanes' own maxima (of
-// groups of lanes, where k is small) is a value that at least k values reach,
-// and few others do; those are gathered in LDS, where each one's place is the
-// number of better ones.  Where more reach it than there is room for (a row of
-// equal logits), the block takes one maximum after another instead.
+// The k largest of many values: of the maxima of at least 2 k groups of them the
+// k-th largest is a limit that at least k values reach, and few others do; those
+// are gathered in LDS, where each one's place is the number of better ones.
+// Where more reach it than there is room for (a row of equal logits), the block
+// takes one maximum after another instead.
 //
 // Two forms, see launch_beam_select: a block a search, or a block a run of a row
 // and a second kernel with a block a search.
@@ -30,29 +30,30 @@ namespace {
 constexpr int kRunThreads = 256, kRunWaves = kRunThreads / kWave;
 constexpr int kRunQuads = 4, kRun = kRunThreads * 4 * kRunQuads;  // columns of a run
 constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / kWave;
-constexpr int kJoinHeld = 4;  // candidates of its first beam that a lane holds
+constexpr int kJoinHeld = 8;  // candidates of its first beam that a lane holds
 constexpr int kOneThreads = 1024, kOneWaves = kOneThreads / kWave;
 constexpr int kOneQuads = 8, kUnit = kWave * 4 * kOneQuads;  // columns of a wave's turn
 constexpr int kMostUnits = 64;                               // turns of a search
-constexpr int kRoom = 512, kPlaceLanes = 8;
+constexpr int kRoom = 512, kFours = 256, kPlaceLanes = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
 
-// The largest x of a run, and the sum of exp(x - top); sum NaN: not all finite.
-struct RunHead {
-  float top, sum;
+// The largest x of a run, the sum of exp(x - top) (NaN: not all finite) and what
+// its kept values reach.
+struct __attribute__((aligned(16))) RunHead {
+  float top, sum, limit;
 };
-// Of a row's run: its head, then `beams` values and columns, in any order (column -1: none).
+// Of a row's run: its head, then values and columns that are, or may be, among
+// its `beams` largest, in any order (column -1: none).
 struct RunLayout {
   RunHead* head;
-  float* value;
-  int* column;
+  float2* kept;
 };
-__host__ __device__ inline RunLayout run_layout(void* workspace, int64_t runs, int beams) {
+__host__ __device__ inline int kept_of(int beams) { return 2 * beams; }
+__host__ __device__ inline RunLayout run_layout(void* workspace, int64_t runs) {
   RunLayout l;
   l.head = static_cast<RunHead*>(workspace);
-  l.value = reinterpret_cast<float*>(l.head + runs);
-  l.column = reinterpret_cast<int*>(l.value + runs * beams);
+  l.kept = reinterpret_cast<float2*>(l.head + runs);
   return l;
 }
 inline int runs_of(int vocab) { return (vocab + kRun - 1) / kRun; }
@@ -63,82 +64,107 @@ inline int units_of(int vocab) { return (vocab + kUnit - 1) / kUnit; }
 struct __attribute__((packed, aligned(4))) Quad {
   float x, y, z, w;
 };
-// Thread t of n holds columns first + 4 (t + n j) + i of a row as v[4 j + i].
+// Thread t of n holds columns first + 4 (t + n j) + i of a row as v[4 j + i]; a
+// branch for all threads, so that no load waits for another.
 template <int kQuads>
 __device__ __forceinline__ void load_columns(const float* x, int vocab, int first, int t, int n, float* v) {
+  if (first + 4 * kQuads * n <= vocab) {
 #pragma unroll
-  for (int j = 0; j < kQuads; ++j) {
-    const int c = first + 4 * (t + n * j);
-    if (c + 4 <= vocab) {
-      const Quad q = *reinterpret_cast<const Quad*>(x + c);
+    for (int j = 0; j < kQuads; ++j) {
+      const Quad q = *reinterpret_cast<const Quad*>(x + first + 4 * (t + n * j));
       v[4 * j] = q.x, v[4 * j + 1] = q.y, v[4 * j + 2] = q.z, v[4 * j + 3] = q.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * j + i] = c + i < vocab ? x[c + i] : -INFINITY;
     }
-  }
-}
-
-// A value that at least k values of the wave's lanes reach, of which `top` is
-// each lane's largest (no number of them being less than k: the least).
-__device__ __forceinline__ float wave_limit(float top, int k) {
-  int above = 0;
-  if (k <= kWave / 8) {  // of 16 groups of four lanes
-    top = fmaxf(top, dpp_move<dpp::kQuadXor1>(top));
-    top = fmaxf(top, dpp_move<dpp::kQuadXor2>(top));
-#pragma unroll
-    for (int i = 0; i < kWave; i += 4) above += read_lane(top, i) > top;
-  } else if (k <= kWave / 4) {  // of 32 pairs
-    top = fmaxf(top, dpp_move<dpp::kQuadXor1>(top));
-#pragma unroll
-    for (int i = 0; i < kWave; i += 2) above += read_lane(top, i) > top;
   } else {
 #pragma unroll
-    for (int i = 0; i < kWave; ++i) above += read_lane(top, i) > top;
+    for (int i = 0; i < 4 * kQuads; ++i) v[i] = x[min(first + 4 * (t + n * (i / 4)) + i % 4, vocab - 1)];
+#pragma unroll
+    for (int i = 0; i < 4 * kQuads; ++i)
+      if (first + 4 * (t + n * (i / 4)) + i % 4 >= vocab) v[i] = -INFINITY;
   }
-  return -group_max<kWave>(above < k ? -top : -INFINITY);
 }
 
-// The wave's largest value (at least the lowest finite number) and the sum of
-// exp(x - that): sums of 16 terms a lane, then over the lanes.  A NaN makes the
-// sum NaN, and so does +inf, from which it is subtracted.
+// The k-th largest of the first n lanes' values, k <= n, where the other lanes
+// have some of those.
+__device__ __forceinline__ float wave_kth(float v, int n, int k) {
+  int above = 0;
+  if (n == kWave) {
+#pragma unroll
+    for (int i = 0; i < kWave; ++i) above += read_lane(v, i) > v;
+  } else {
+    for (int i = 0; i < n; i += 4) {  // n is a multiple of 4
+#pragma unroll
+      for (int m = 0; m < 4; ++m) above += read_lane(v, i + m) > v;
+    }
+  }
+  return -group_max<kWave>(above < k ? -v : -INFINITY);
+}
+// The largest of each 64 / n neighbouring lanes, n being 4, 16 or 64.
+__device__ __forceinline__ float lane_groups_max(float v, int n) {
+  if (n < 64) {
+    v = fmaxf(v, dpp_move<dpp::kQuadXor1>(v));
+    v = fmaxf(v, dpp_move<dpp::kQuadXor2>(v));
+  }
+  if (n < 16) {
+    v = fmaxf(v, dpp_move<dpp::kRowHalfMirror>(v));
+    v = fmaxf(v, dpp_move<dpp::kRowMirror>(v));
+  }
+  return v;
+}
+
+// The wave's sum of exp(x - top), top being no less than any x: sums of 16 terms
+// a lane, then over the lanes.  A NaN makes it NaN, and so does +inf, from which
+// it is subtracted.
 template <int kEach>
-__device__ __forceinline__ RunHead wave_head(const float* v, float top) {
-  RunHead h;
-  h.top = fmaxf(group_max<kWave>(top), -FLT_MAX);
+__device__ __forceinline__ float wave_sum(const float* v, float top) {
   float sum[kEach / 16] = {};
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) sum[i / 16] += __builtin_amdgcn_exp2f((v[i] - h.top) * kLog2e);
+  for (int i = 0; i < kEach; ++i) sum[i / 16] += __builtin_amdgcn_exp2f((v[i] - top) * kLog2e);
 #pragma unroll
   for (int i = 1; i < kEach / 16; ++i) sum[0] += sum[i];
-  h.sum = group_sum<kWave>(sum[0]);
-  return h;
+  return group_sum<kWave>(sum[0]);
 }
 
-// Calls put(place, i) for the values v[i] of the wave's lanes that reach limit,
-// with places of the room that *count counts; most v[i] have none, and are done
-// with after one comparison.
-template <int kEach, typename Put>
-__device__ __forceinline__ void gather(const float* v, float limit, int* count, Put put) {
-  uint64_t hits[kEach];
+// Fours of values in LDS, and what the first of them is the value of.
+struct Fours {
+  float4 x[kFours];
+  int code[kFours], count;
+};
+// Of the lanes' fours (of which most[j] is the largest), those that reach limit;
+// most do not, and are done with after one comparison.
+template <int kQuads, typename Code>
+__device__ __forceinline__ void gather(const float* v, const float* most, float limit, Fours* to, Code code) {
+  uint64_t hits[kQuads];
   int total = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    hits[i] = __ballot(v[i] >= limit);
-    total += __popcll(hits[i]);
+  for (int j = 0; j < kQuads; ++j) {
+    hits[j] = __ballot(most[j] >= limit);
+    total += __popcll(hits[j]);
   }
   if (total == 0) return;
   int base = 0;
-  if (threadIdx.x % kWave == 0) base = atomicAdd(count, total);
+  if (threadIdx.x % kWave == 0) base = atomicAdd(&to->count, total);
   base = __builtin_amdgcn_readfirstlane(base);
 #pragma unroll
-  for (int i = 0; i < kEach; ++i)
-    if (hits[i] != 0) {
-      const int place = base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(hits[i] >> 32),
-                                                         __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hits[i]), 0));
-      if (v[i] >= limit && place < kRoom) put(place, i);
-      base += __popcll(hits[i]);
+  for (int j = 0; j < kQuads; ++j)
+    if (hits[j] != 0) {
+      const int place = base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(hits[j] >> 32),
+                                                         __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hits[j]), 0));
+      if (most[j] >= limit && place < kFours) {
+        to->x[place] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        to->code[place] = code(j);
+      }
+      base += __popcll(hits[j]);
     }
+}
+template <int kQuads>
+__device__ __forceinline__ float largest(const float* v, float* most) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < kQuads; ++j) {
+    most[j] = fmaxf(fmaxf(v[4 * j], v[4 * j + 1]), fmaxf(v[4 * j + 2], v[4 * j + 3]));
+    top = fmaxf(top, most[j]);
+  }
+  return top;
 }
 
 // top + log(sum) to some 2^-25 of 1: the logarithm in 32 bits is of a number near 1.
@@ -167,19 +193,36 @@ __device__ __forceinline__ Candidate no_candidate() { return Candidate{-INFINITY
 
 // Candidates in LDS; what ranks them apart, so that comparing takes one read.
 struct Room {
-  double rank[kRoom];
-  float x[kRoom];
-  int beam[kRoom], token[kRoom];
-  __device__ __forceinline__ Candidate get(int n) const { return Candidate{rank[n], x[n], beam[n], token[n]}; }
+  double rank[kRoom];  // -inf: none
+  float x[kRoom], score[kRoom];
+  int code[kRoom];  // beam * 2^24 + token
+  int count, fine;  // candidates, and those that are some
+  __device__ __forceinline__ Candidate get(int n) const {
+    return Candidate{rank[n], x[n], code[n] >> 24, code[n] & 0xFFFFFF};
+  }
+  // Adds the lanes' candidates that are wanted.
+  __device__ __forceinline__ void add(bool wanted, float value, int c) {
+    const uint64_t lanes = __ballot(wanted);
+    if (lanes == 0) return;
+    int base = 0;
+    if (threadIdx.x % kWave == 0) base = atomicAdd(&count, __popcll(lanes));
+    const int place = __builtin_amdgcn_readfirstlane(base) +
+                      __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
+                                                __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0));
+    if (wanted && place < kRoom) {
+      x[place] = value;
+      code[place] = c;
+    }
+  }
   // The number of better ones than candidate n, by kPlaceLanes lanes together.
-  __device__ __forceinline__ int place(int n, int count) const {
-    const Candidate mine = get(n);
+  __device__ __forceinline__ int place(int n, int all) const {
+    const double mine = rank[n];
     int above = 0;
 #pragma unroll 4
-    for (int j = threadIdx.x % kPlaceLanes; j < count; j += kPlaceLanes) {
+    for (int j = threadIdx.x % kPlaceLanes; j < all; j += kPlaceLanes) {
       const double r = rank[j];
-      above += r > mine.rank;
-      if (r == mine.rank && j != n) above += better(get(j), mine);
+      above += r > mine;
+      if (r == mine && j != n) above += better(get(j), get(n));
     }
     above += dpp_move_int<dpp::kQuadXor1>(above);
     above += dpp_move_int<dpp::kQuadXor2>(above);
@@ -191,25 +234,69 @@ struct Room {
 struct Search {
   double lse[kMostBeams], factor[kMostBeams];
   float score[kMostBeams];
-  int state[kMostBeams];  // 0 no candidates, 1 those of its row, 2 itself
+  int state[kMostBeams];  // 0 no candidates, 1 those of its row, 2 itself, 3 ended without a score
   int length[kMostBeams];
 
-  __device__ __forceinline__ double score_of(int b, float x) const {
-    return state[b] == 2 ? score[b] : score[b] + (static_cast<double>(x) - lse[b]);
+  // Of beam n, as it was: read before the new ones take its place.
+  struct Before {
+    float score;
+    int ended, length;
+  };
+  __device__ __forceinline__ static Before before(const BeamArgs& a, int row) {
+    return Before{a.scores[row], a.eos >= 0 ? a.ended[row] : 0, a.lengths[row]};
   }
-  __device__ __forceinline__ Candidate candidate(int b, float x, int token) const {
-    const double s = score_of(b, x);
-    return static_cast<float>(s) > -INFINITY ? Candidate{s * factor[b], x, b, token} : no_candidate();
+  __device__ __forceinline__ void set(const BeamArgs& a, int n, const Before& was) {
+    const bool done = was.ended != 0;
+    score[n] = was.score;
+    state[n] = fabsf(was.score) < INFINITY ? done ? 2 : 1 : done ? 3 : 0;
+    length[n] = was.length + (done ? 0 : 1);
+    factor[n] = length_factor(a, length[n]);
+    if (!(was.score < INFINITY)) atomicOr(a.error, kKv8NotFinite);
   }
-  __device__ __forceinline__ void store(const BeamArgs& a, int first, int place, const Candidate& c) const {
+  // Of the sum of exp(x - top) over its row.
+  __device__ __forceinline__ void set_sum(const BeamArgs& a, int n, float top, double sum) {
+    lse[n] = log_sum(top, sum);
+    if (!(sum > 0.0)) state[n] = 0;  // not finite, or every token is masked
+    if (!(sum == sum)) atomicOr(a.error, kKv8NotFinite);
+  }
+  __device__ __forceinline__ Candidate candidate(int b, float x, int token, float* score_out) const {
+    const double s = state[b] == 2 ? score[b] : score[b] + (static_cast<double>(x) - lse[b]);
+    *score_out = static_cast<float>(s);
+    return (state[b] == 1 || state[b] == 2) && *score_out > -INFINITY ? Candidate{s * factor[b], x, b, token}
+                                                                      : no_candidate();
+  }
+  __device__ __forceinline__ void store(const BeamArgs& a, int first, int place, const Candidate& c, float s) const {
     const int o = first + place;
     const bool none = c.beam == INT_MAX;
     const int token = none ? max(a.eos, 0) : c.token;
-    a.scores_out[o] = none ? -INFINITY : static_cast<float>(score_of(c.beam, c.x));
+    a.scores_out[o] = none ? -INFINITY : s;
     a.parent[o] = none ? -1 : first + c.beam;
     a.token[o] = token;
     a.lengths_out[o] = none ? 0 : length[c.beam];
     a.ended_out[o] = a.eos >= 0 && token == a.eos;
+  }
+  __device__ __forceinline__ void store(const BeamArgs& a, int first, int place, const Candidate& c) const {
+    float s = 0.0f;
+    if (c.beam != INT_MAX) candidate(c.beam, c.x, c.token, &s);
+    store(a, first, place, c, s);
+  }
+  // Ranks the candidates of the room, and stores the best; the block does so together.
+  template <int kThreads>
+  __device__ __forceinline__ void rank_and_store(const BeamArgs& a, int first, Room* room) const {
+    const int tid = threadIdx.x, count = room->count;
+    for (int n = tid; n < count; n += kThreads) {
+      const int code = room->code[n];
+      const Candidate c = candidate(code >> 24, room->x[n], code & 0xFFFFFF, &room->score[n]);
+      room->rank[n] = c.rank;
+      if (c.beam != INT_MAX) atomicAdd(&room->fine, 1);
+    }
+    __syncthreads();
+    if (tid >= room->fine && tid < a.beams) store(a, first, tid, no_candidate());
+    for (int n = tid / kPlaceLanes; n < count; n += kThreads / kPlaceLanes) {
+      if (!(room->rank[n] > -INFINITY)) continue;
+      const int place = room->place(n, count);
+      if (tid % kPlaceLanes == 0 && place < a.beams) store(a, first, place, room->get(n), room->score[n]);
+    }
   }
 };
 
@@ -233,91 +320,97 @@ __device__ __forceinline__ Candidate block_best(Candidate best, Candidate* wave_
 
 // ------------------------------------------------- a block a search ----
 
-// Waves take (beam, kUnit columns) in turn.
-__global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int units) {
-  constexpr int kEach = 4 * kOneQuads;
+// Waves take (beam, kUnit columns) in turn: the sums first, and the maxima of
+// groups of lanes; those of a beam's turns give its limit, with which the waves
+// gather (from registers, where each has one turn).
+__global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int units, int groups) {
+  constexpr int kOthers = kOneThreads - kWave;
+  static_assert(kMostBeams <= kWave, "a beam a lane of the last wave");
   __shared__ Search search;
   __shared__ Room room;
+  __shared__ Fours fours;
   __shared__ RunHead heads[kMostUnits];
+  __shared__ float maxima[kMostUnits * kWave];
   __shared__ Candidate wave_best[kOneWaves];
-  __shared__ int sh_count, sh_fine;
   const int first = blockIdx.x * a.beams, tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
-  if (tid == 0) sh_count = sh_fine = 0;
-  if (tid < a.beams) {
-    const float score = a.scores[first + tid];
-    const bool done = a.eos >= 0 && a.ended[first + tid] != 0;
-    search.score[tid] = score;
-    search.state[tid] = fabsf(score) < INFINITY ? done ? 2 : 1 : 0;
-    search.length[tid] = a.lengths[first + tid] + (done ? 0 : 1);
-    search.factor[tid] = length_factor(a, search.length[tid]);
-    if (!(score < INFINITY)) atomicOr(a.error, kKv8NotFinite);
-  }
-  __syncthreads();  // the room is empty, and the beams as they were are read
-  for (int u = wave; u < a.beams * units; u += kOneWaves) {
-    const int b = u / units, begin = u % units * kUnit;
-    if (a.eos >= 0 && search.state[b] == 2) {
-      if (u % units == 0 && lane == 0) {
-        const int place = atomicAdd(&sh_count, 1);
-        if (place < kRoom) room.x[place] = 0.0f, room.beam[place] = b, room.token[place] = a.eos;
-      }
-      continue;
+  const int turns = a.beams * units, beam0 = wave / units, unit0 = wave - beam0 * units;
+  float v[4 * kOneQuads], most[kOneQuads];
+  auto ask = [&](int b, int unit) {  // also of a beam that has ended, whose logits then count for nothing
+    load_columns<kOneQuads>(a.logits + static_cast<int64_t>(first + b) * a.vocab, a.vocab, unit * kUnit, lane, kWave, v);
+  };
+  auto every = [&](auto use) {  // of the wave's turns
+    for (int u = wave, b = beam0, unit = unit0; u < turns; u += kOneWaves) {
+      use(u, b, unit);
+      for (unit += kOneWaves; unit >= units; unit -= units) ++b;
     }
-    float v[kEach];
-    load_columns<kOneQuads>(a.logits + static_cast<int64_t>(first + b) * a.vocab, a.vocab, begin, lane, kWave, v);
-    float top = -INFINITY;
+  };
+  if (wave < turns) ask(beam0, unit0);
+  const bool has_beam = tid >= kOthers && tid - kOthers < a.beams;
+  Search::Before was = {};
+  if (has_beam) was = Search::before(a, first + tid - kOthers);
+  if (tid == 0) fours.count = room.count = room.fine = 0;
+  every([&](int u, int b, int unit) {
+    if (u != wave) ask(b, unit);
+    const float top = largest<kOneQuads>(v, most);
+    const float wave_top = fmaxf(group_max<kWave>(top), -FLT_MAX), group_top = lane_groups_max(top, groups);
+    const float sum = wave_sum<4 * kOneQuads>(v, wave_top);
+    if (lane == 0) heads[u] = RunHead{wave_top, sum, 0.0f};
+    if (lane % (kWave / groups) == 0) maxima[u * groups + lane / (kWave / groups)] = group_top;
+  });
+  if (has_beam) search.set(a, tid - kOthers, was);
+  __syncthreads();
+  every([&](int u, int b, int unit) {
+    const int all = units * groups, n = min(all, kWave), state = search.state[b];
+    if (state >= 2) return;
+    if (turns > kOneWaves) {
+      ask(b, unit);
+      largest<kOneQuads>(v, most);
+    }
+    float top = maxima[b * all + min(lane, n - 1)];
+    for (int i = lane + kWave; i < all; i += kWave) top = fmaxf(top, maxima[b * all + i]);
+    const float limit = fmaxf(wave_kth(top, n, a.beams), -FLT_MAX);
+    gather<kOneQuads>(v, most, limit, &fours, [&](int j) { return b << 24 | (unit * kUnit + 4 * (lane + kWave * j)); });
+    if (unit == 0) {
+      const RunHead head = lane < units ? heads[u + lane] : RunHead{-FLT_MAX, 0.0f, 0.0f};
+      const float row_top = group_max<kWave>(head.top);
+      double sum = static_cast<double>(head.sum * __builtin_amdgcn_exp2f((head.top - row_top) * kLog2e));
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) top = fmaxf(top, v[i]);
-    const RunHead head = wave_head<kEach>(v, top);
-    if (lane == 0) heads[u] = head;
-    gather<kEach>(v, fmaxf(wave_limit(top, a.beams), -FLT_MAX), &sh_count, [&](int place, int i) {
-      room.x[place] = v[i];
-      room.beam[place] = b;
-      room.token[place] = begin + 4 * (lane + kWave * (i / 4)) + i % 4;
-    });
-  }
-  __syncthreads();
-  const int count = sh_count;
-  if (tid < a.beams && search.state[tid] != 2) {
-    const RunHead* head = heads + tid * units;
-    float top = -FLT_MAX;
-    for (int u = 0; u < units; ++u) top = fmaxf(top, head[u].top);
-    double sum = 0.0;
-    for (int u = 0; u < units; ++u)
-      sum += static_cast<double>(head[u].sum * __builtin_amdgcn_exp2f((head[u].top - top) * kLog2e));
-    search.lse[tid] = log_sum(top, sum);
-    if (!(sum > 0.0)) search.state[tid] = 0;  // not finite, or every token is masked
-    if (!(sum == sum)) atomicOr(a.error, kKv8NotFinite);
-  }
-  __syncthreads();
-  if (count <= kRoom) {
-    for (int n = tid; n < count; n += kOneThreads) {
-      const int b = room.beam[n];
-      const Candidate c = search.state[b] == 0 ? no_candidate() : search.candidate(b, room.x[n], room.token[n]);
-      room.rank[n] = c.rank;
-      room.beam[n] = c.beam;
-      if (c.beam != INT_MAX) atomicAdd(&sh_fine, 1);
+      for (int step = 1; step < kWave; step *= 2)
+        if (step < units) sum += __shfl_xor(sum, step);
+      if (lane == 0) {
+        heads[u].limit = limit;
+        search.set_sum(a, b, row_top, sum);
+      }
     }
+  });
+  __syncthreads();
+  if (fours.count <= kFours) {
+    // A value a thread; those of beams that have ended by the last wave's other lanes.
+    if (tid < 4 * (fours.count + kWave / 4)) {
+      const int n = tid / 4, code = n < fours.count ? fours.code[n] : 0;
+      const float x = n < fours.count ? reinterpret_cast<const float*>(fours.x)[tid] : -INFINITY;
+      room.add(n < fours.count && x >= heads[(code >> 24) * units].limit, x, code + tid % 4);
+    }
+    if (tid >= kOthers) room.add(has_beam && search.state[tid - kOthers] == 2, 0.0f, (tid - kOthers) << 24 | a.eos);
     __syncthreads();
-    if (tid >= sh_fine && tid < a.beams) search.store(a, first, tid, no_candidate());
-    for (int n = tid / kPlaceLanes; n < count; n += kOneThreads / kPlaceLanes) {
-      const int place = room.place(n, count);
-      if (tid % kPlaceLanes == 0 && place < a.beams && room.beam[n] != INT_MAX)
-        search.store(a, first, place, room.get(n));
+    if (room.count <= kRoom) {
+      search.rank_and_store<kOneThreads>(a, first, &room);
+      return;
     }
-    return;
   }
   Candidate last{INFINITY, INFINITY, -1, -1};
   for (int n = 0; n < a.beams; ++n) {  // each the best that is worse than the last
     Candidate best = no_candidate();
     for (int b = 0; b < a.beams; ++b) {
       const int state = search.state[b];
-      if (state == 0) continue;
+      if (state != 1 && state != 2) continue;
       const float* x = a.logits + static_cast<int64_t>(first + b) * a.vocab;
       for (int t = tid; t < (state == 2 ? 1 : a.vocab); t += kOneThreads) {
         const float value = state == 2 ? 0.0f : x[t];
         if (!(value > -INFINITY)) continue;
-        const Candidate c = search.candidate(b, value, state == 2 ? a.eos : t);
+        float s;
+        const Candidate c = search.candidate(b, value, state == 2 ? a.eos : t, &s);
         if (c.beam != INT_MAX && better(last, c) && better(c, best)) best = c;
       }
     }
@@ -330,10 +423,10 @@ __global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int u
 
 __global__ __launch_bounds__(kRunThreads) void beam_runs_kernel(BeamArgs a, int runs) {
   constexpr int kEach = 4 * kRunQuads;
-  __shared__ float sh_limit[kRunWaves], best_value[kRunWaves];
-  __shared__ RunHead sh_head[kRunWaves];
-  __shared__ int sh_count, best_column[kRunWaves];
-  __shared__ float2 room[kRoom];  // value, column
+  __shared__ float maxima[kWave], sh_sum[kRunWaves], best_value[kRunWaves];
+  __shared__ int best_column[kRunWaves];
+  __shared__ float2 room[kRoom];
+  __shared__ int sh_count;
   const int run = blockIdx.x % runs, row = blockIdx.x / runs, tid = threadIdx.x;
   const int wave = tid / kWave, lane = tid % kWave;
   if (a.eos >= 0 && a.ended[row] != 0) return;  // what it keeps is not used
@@ -341,50 +434,64 @@ __global__ __launch_bounds__(kRunThreads) void beam_runs_kernel(BeamArgs a, int 
   auto column_of = [&](int i) { return run * kRun + 4 * (tid + kRunThreads * (i / 4)) + i % 4; };
   float v[kEach];
   load_columns<kRunQuads>(a.logits + static_cast<int64_t>(row) * a.vocab, a.vocab, run * kRun, tid, kRunThreads, v);
-  float top = -INFINITY;
+  // 16 groups of a block's lanes, or 64.
+  const int groups = a.beams <= 8 ? 4 : 16, all = groups * kRunWaves;
+  float top = v[0];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) top = fmaxf(top, v[i]);
-  const RunHead head = wave_head<kEach>(v, top);
-  const float wave_at_least = wave_limit(top, a.beams);
-  if (lane == 0) {
-    sh_limit[wave] = wave_at_least;
-    sh_head[wave] = head;
-  }
+  for (int i = 1; i < kEach; ++i) top = fmaxf(top, v[i]);
+  const float group_top = lane_groups_max(top, groups);
+  if (lane % (kWave / groups) == 0) maxima[wave * groups + lane / (kWave / groups)] = group_top;
   __syncthreads();
-  float limit = -FLT_MAX;
+  const float group = maxima[lane % all];
+  const float limit = fmaxf(wave_kth(group, all, a.beams), -FLT_MAX);
+  const float block_top = fmaxf(group_max<kWave>(group), -FLT_MAX);
+  const float sum = wave_sum<kEach>(v, block_top);
+  if (lane == 0) sh_sum[wave] = sum;
+  uint64_t hits[kEach];
+  int total = 0;
 #pragma unroll
-  for (int w = 0; w < kRunWaves; ++w) limit = fmaxf(limit, sh_limit[w]);
-  gather<kEach>(v, limit, &sh_count,
-                [&](int place, int i) { room[place] = make_float2(v[i], __int_as_float(column_of(i))); });
-  __syncthreads();
-  const RunLayout to = run_layout(a.workspace, static_cast<int64_t>(runs) * a.searches * a.beams, a.beams);
-  const int64_t at = static_cast<int64_t>(row) * runs + run;
-  float* value = to.value + at * a.beams;
-  int* column = to.column + at * a.beams;
-  if (tid == 0) {
-    float all = sh_head[0].top, s = 0.0f;
-#pragma unroll
-    for (int w = 1; w < kRunWaves; ++w) all = fmaxf(all, sh_head[w].top);
-#pragma unroll
-    for (int w = 0; w < kRunWaves; ++w) s += sh_head[w].sum * __builtin_amdgcn_exp2f((sh_head[w].top - all) * kLog2e);
-    to.head[at] = RunHead{all, s};
+  for (int i = 0; i < kEach; ++i) {
+    hits[i] = __ballot(v[i] >= limit);
+    total += __popcll(hits[i]);
   }
-  const int count = sh_count;
-  if (count <= kRoom) {
-    for (int n = tid; n < max(count, a.beams); n += kRunThreads) {
-      if (n >= count) {
-        column[n] = -1;
-        continue;
+  if (total > 0) {
+    int base = 0;
+    if (lane == 0) base = atomicAdd(&sh_count, total);
+    base = __builtin_amdgcn_readfirstlane(base);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (hits[i] != 0) {
+        const int place = base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(hits[i] >> 32),
+                                                           __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hits[i]), 0));
+        if (v[i] >= limit && place < kRoom) room[place] = make_float2(v[i], __int_as_float(column_of(i)));
+        base += __popcll(hits[i]);
       }
+  }
+  __syncthreads();
+  const RunLayout to = run_layout(a.workspace, static_cast<int64_t>(runs) * a.searches * a.beams);
+  const int64_t at = static_cast<int64_t>(row) * runs + run;
+  const int keep = kept_of(a.beams), count = sh_count;
+  float2* kept = to.kept + at * keep;
+  if (tid == 0) {
+    float s = sh_sum[0];
+#pragma unroll
+    for (int w = 1; w < kRunWaves; ++w) s += sh_sum[w];
+    to.head[at] = RunHead{block_top, s, limit};
+  }
+  const float2 none = make_float2(0.0f, __int_as_float(-1));
+  if (count <= keep) {
+    if (tid < keep) kept[tid] = tid < count ? room[tid] : none;
+    return;
+  }
+  if (tid >= a.beams && tid < keep) kept[tid] = none;
+  if (count <= kRoom) {
+    for (int n = tid; n < count; n += kRunThreads) {
       const float2 mine = room[n];
       int place = 0;
 #pragma unroll 4
       for (int j = 0; j < count; ++j)
         place += argmax_better(room[j].x, __float_as_int(room[j].y), mine.x, __float_as_int(mine.y));
-      if (place < a.beams) {
-        value[place] = mine.x;
-        column[place] = __float_as_int(mine.y);
-      }
+      if (place < a.beams) kept[place] = mine;
     }
     return;
   }
@@ -411,10 +518,7 @@ __global__ __launch_bounds__(kRunThreads) void beam_runs_kernel(BeamArgs a, int 
         bv = best_value[w];
         bc = best_column[w];
       }
-    if (tid == 0) {
-      value[n] = bv;
-      column[n] = bc;
-    }
+    if (tid == 0) kept[n] = make_float2(bv, __int_as_float(bc));
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
       if (column_of(i) == bc) v[i] = -INFINITY;
@@ -427,118 +531,111 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
   __shared__ Search search;
   __shared__ Room room;
   __shared__ Candidate wave_best[kJoinWaves];
-  __shared__ float sh_limit[kJoinWaves];
-  __shared__ int sh_count;
-  const RunLayout from = run_layout(a.workspace, static_cast<int64_t>(runs) * a.searches * a.beams, a.beams);
+  __shared__ float sh_limit[kJoinWaves], row_limit[kMostBeams];
+  const RunLayout from = run_layout(a.workspace, static_cast<int64_t>(runs) * a.searches * a.beams);
   const int first = blockIdx.x * a.beams, tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
-  const int each = runs * a.beams;
-  if (tid == 0) sh_count = 0;
+  const int each = runs * kept_of(a.beams);
+  const bool has_beam = tid < a.beams;
+  Search::Before was = {};
+  if (has_beam) was = Search::before(a, first + tid);
   // Asked for before the sums are known; of a beam that has ended, anything.
-  float held_x[kJoinHeld];
-  int held_token[kJoinHeld];
+  const float2 none = make_float2(0.0f, __int_as_float(-1));
+  float2 held[kJoinHeld];
 #pragma unroll
   for (int i = 0; i < kJoinHeld; ++i) {
     const int n = lane + kWave * i;
-    const bool there = wave < a.beams && n < each;
-    const int64_t at = static_cast<int64_t>(first + wave) * each + n;
-    held_x[i] = there ? from.value[at] : 0.0f;
-    held_token[i] = there ? from.column[at] : -1;
+    held[i] = none;
+    if (wave < a.beams && n < each) held[i] = from.kept[static_cast<int64_t>(first + wave) * each + n];
   }
-  // All that is read of the beams as they were is read before the barriers: the
-  // new ones may take their place.
+  auto head_of = [&](int b) {
+    return lane < runs ? from.head[static_cast<int64_t>(first + b) * runs + lane] : RunHead{-FLT_MAX, 0.0f, -FLT_MAX};
+  };
+  RunHead head = wave < a.beams ? head_of(wave) : RunHead{};
+  if (tid == 0) room.count = room.fine = 0;
+  if (has_beam) search.set(a, tid, was);
+  __syncthreads();
   for (int b = wave; b < a.beams; b += kJoinWaves) {
-    const float score = a.scores[first + b];
-    const bool done = a.eos >= 0 && a.ended[first + b] != 0;
-    const int length = a.lengths[first + b] + (done ? 0 : 1);
-    int state = fabsf(score) < INFINITY ? done ? 2 : 1 : 0;
-    bool bad = !(score < INFINITY);
-    double lse = 0.0;
-    if (!done) {
-      const RunHead* head = from.head + static_cast<int64_t>(first + b) * runs;
-      const RunHead mine = lane < runs ? head[lane] : RunHead{-FLT_MAX, 0.0f};
-      float top = mine.top;
-      for (int r = lane + kWave; r < runs; r += kWave) top = fmaxf(top, head[r].top);
-      top = group_max<kWave>(top);
-      double sum = static_cast<double>(mine.sum * __builtin_amdgcn_exp2f((mine.top - top) * kLog2e));
-      for (int r = lane + kWave; r < runs; r += kWave)
-        sum += static_cast<double>(head[r].sum * __builtin_amdgcn_exp2f((head[r].top - top) * kLog2e));
-#pragma unroll
-      for (int step = 1; step < kWave; step *= 2) sum += __shfl_xor(sum, step);
-      lse = log_sum(top, sum);
-      bad = bad || !(sum == sum);
-      if (!(sum > 0.0)) state = 0;  // not finite, or every token is masked
+    if (search.state[b] >= 2) continue;
+    if (b != wave) head = head_of(b);
+    const RunHead* more = from.head + static_cast<int64_t>(first + b) * runs;
+    float top = head.top, limit = head.limit;
+    for (int r = lane + kWave; r < runs; r += kWave) {
+      top = fmaxf(top, more[r].top);
+      limit = fmaxf(limit, more[r].limit);
     }
+    // What `beams` values of a run reach, or as many runs.
+    limit = fmaxf(group_max<kWave>(limit), wave_kth(lane < runs ? top : -INFINITY, min(kWave, (runs + 3) / 4 * 4), a.beams));
+    top = group_max<kWave>(top);
+    double sum = static_cast<double>(head.sum * __builtin_amdgcn_exp2f((head.top - top) * kLog2e));
+    for (int r = lane + kWave; r < runs; r += kWave)
+      sum += static_cast<double>(more[r].sum * __builtin_amdgcn_exp2f((more[r].top - top) * kLog2e));
+#pragma unroll
+    for (int step = 1; step < kWave; step *= 2) sum += __shfl_xor(sum, step);
     if (lane == 0) {
-      if (bad) atomicOr(a.error, kKv8NotFinite);
-      search.state[b] = state;
-      search.score[b] = score;
-      search.lse[b] = lse;
-      search.length[b] = length;
-      search.factor[b] = length_factor(a, length);
+      row_limit[b] = limit;
+      search.set_sum(a, b, top, sum);
     }
   }
   __syncthreads();
-  auto every = [&](auto use) {  // of this wave's beams
+  auto every = [&](auto use) {  // of this wave's beams, all lanes together: use(whether there is one, x, code)
     for (int b = wave; b < a.beams; b += kJoinWaves) {
       const int state = search.state[b];
-      if (state == 0) continue;
-      if (state == 2) {
-        if (lane == 0) use(search.candidate(b, 0.0f, a.eos));
-        continue;
-      }
-      const int64_t at = static_cast<int64_t>(first + b) * each;
+      if (state == 2) use(lane == 0, 0.0f, b << 24 | a.eos);
+      if (state != 1) continue;
+      const float limit = row_limit[b];  // what `beams` values of the row reach
+      const float2* kept = from.kept + static_cast<int64_t>(first + b) * each;
+      auto one = [&](const float2& k) {
+        const int token = __float_as_int(k.y);
+        use(token >= 0 && k.x >= limit, k.x, b << 24 | token);
+      };
 #pragma unroll
       for (int i = 0; i < kJoinHeld; ++i)
         if (kWave * i < each) {
           const int n = lane + kWave * i;
-          const float x = b == wave ? held_x[i] : n < each ? from.value[at + n] : 0.0f;
-          const int token = b == wave ? held_token[i] : n < each ? from.column[at + n] : -1;
-          if (token >= 0) use(search.candidate(b, x, token));
+          float2 k = held[i];
+          if (b != wave) k = n < each ? kept[n] : none;
+          one(k);
         }
-      for (int n = lane + kWave * kJoinHeld; n < each; n += kWave) {
-        const int token = from.column[at + n];
-        if (token >= 0) use(search.candidate(b, from.value[at + n], token));
-      }
+      for (int i = kWave * kJoinHeld; i < each; i += kWave) one(i + lane < each ? kept[i + lane] : none);
     }
   };
-  // Ranks in 32 bits are in the order of those in 64, or equal: what reaches the
-  // limit in 32 bits is all that may be among the best.
-  float limit = -INFINITY;
-  if (a.beams * each > kWave) {
+  auto candidate = [&](float x, int code) {
+    float score;
+    return search.candidate(code >> 24, x, code & 0xFFFFFF, &score);
+  };
+  every([&](bool is, float x, int code) { room.add(is, x, code); });
+  __syncthreads();
+  if (room.count > kRoom) {
+    // Of many beams.  Ranks in 32 bits are in the order of those in 64, or equal:
+    // what reaches a limit in 32 bits is all that may be among the best.
     float top = -INFINITY;
-    every([&](const Candidate& c) { top = fmaxf(top, static_cast<float>(c.rank)); });
-    const float at_least = wave_limit(top, a.beams);
+    every([&](bool is, float x, int code) {
+      if (is) top = fmaxf(top, static_cast<float>(candidate(x, code).rank));
+    });
+    const float at_least = wave_kth(top, kWave, a.beams);
     if (lane == 0) sh_limit[wave] = at_least;
     __syncthreads();
+    if (tid == 0) room.count = 0;
+    float limit = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kJoinWaves; ++w) limit = fmaxf(limit, sh_limit[w]);
+    __syncthreads();
+    every([&](bool is, float x, int code) {
+      room.add(is && static_cast<float>(candidate(x, code).rank) >= limit, x, code);
+    });
+    __syncthreads();
   }
-  every([&](const Candidate& c) {
-    if (c.beam != INT_MAX && static_cast<float>(c.rank) >= limit) {
-      const int place = atomicAdd(&sh_count, 1);
-      if (place < kRoom) {
-        room.rank[place] = c.rank;
-        room.x[place] = c.x;
-        room.beam[place] = c.beam;
-        room.token[place] = c.token;
-      }
-    }
-  });
-  __syncthreads();
-  const int count = sh_count;
-  if (count <= kRoom) {
-    if (tid >= count && tid < a.beams) search.store(a, first, tid, no_candidate());
-    for (int n = tid / kPlaceLanes; n < count; n += kJoinThreads / kPlaceLanes) {
-      const int place = room.place(n, count);
-      if (tid % kPlaceLanes == 0 && place < a.beams) search.store(a, first, place, room.get(n));
-    }
+  if (room.count <= kRoom) {
+    search.rank_and_store<kJoinThreads>(a, first, &room);
     return;
   }
   Candidate last{INFINITY, INFINITY, -1, -1};
   for (int n = 0; n < a.beams; ++n) {  // each the best that is worse than the last
     Candidate best = no_candidate();
-    every([&](const Candidate& c) {
+    every([&](bool is, float x, int code) {
+      if (!is) return;
+      const Candidate c = candidate(x, code);
       if (c.beam != INT_MAX && better(last, c) && better(c, best)) best = c;
     });
     last = block_best<kJoinWaves>(best, wave_best);
@@ -548,16 +645,21 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
 
 }  // namespace
 
+// Of the lanes of a turn, so that a beam has at least 2 k groups.
+static int one_groups(int units, int beams) {
+  return units * 4 >= 2 * beams ? 4 : units * 16 >= 2 * beams ? 16 : 64;
+}
+
 int64_t beam_select_workspace(int searches, int beams, int vocab) {
   if (beams * units_of(vocab) <= kMostUnits) return 0;
   const int64_t runs = static_cast<int64_t>(runs_of(vocab)) * searches * beams;
-  return runs * static_cast<int64_t>(sizeof(RunHead) + beams * (sizeof(float) + sizeof(int)));
+  return runs * static_cast<int64_t>(sizeof(RunHead) + kept_of(beams) * sizeof(float2));
 }
 
 hipError_t launch_beam_select(const BeamArgs& a, hipStream_t stream) {
   const int runs = runs_of(a.vocab), units = units_of(a.vocab);
   if (beam_select_workspace(a.searches, a.beams, a.vocab) == 0) {
-    beam_one_kernel<<<dim3(a.searches), kOneThreads, 0, stream>>>(a, units);
+    beam_one_kernel<<<dim3(a.searches), kOneThreads, 0, stream>>>(a, units, one_groups(units, a.beams));
   } else {
     beam_runs_kernel<<<dim3(runs * a.searches * a.beams), kRunThreads, 0, stream>>>(a, runs);
     beam_join_kernel<<<dim3(a.searches), kJoinThreads, 0, stream>>>(a, runs);
