@@ -14,15 +14,18 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace mmr {
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kOneThreads = 1024;  // of a block that is alone
-constexpr int kCopyThreads = 256;
-constexpr int kCopyBlocks = 2048;
+constexpr int kOneThreads = 1024;     // of a block that is alone
+constexpr int kHeldSeqs = 2048;       // sequences whose plans the deciding block holds in LDS
+constexpr int kCountEntries = 8192;   // table entries that it counts itself
+constexpr int kHeldPages = 16;        // pages a thread of it holds
+constexpr int kCopyBlocks = 16384;
 
 // ---------------------------------------------------------------- fork ----
 
@@ -47,16 +50,28 @@ struct ForkPlan {
   __device__ __forceinline__ int pages() const { return (keep + room + kKv8Page - 1) / kKv8Page; }
 };
 
+// Of a sequence, while the block decides; in LDS, or in the workspace where there are many.
+struct ForkSeq {
+  int page;          // partly filled, which it will write to, or -1
+  int users;         // of that page
+  int one;           // of the sequences that will write to it, all name the same
+  int first_writer;  // of those that name this sequence, the first, and how many
+  int writers;
+};
+
+// What becomes of a sequence's table row: places from `fresh` to `pages` get new
+// pages, from number `start` of those on.
+struct __attribute__((aligned(16))) ForkRow {
+  int fresh, pages, start;
+};
 struct ForkSpace {
-  int* taken;         // [seqs][per_seq] pages that a sequence takes over, or -1
-  int* claim;         // [pages] one of the sequences that will write to this partly filled page
-  int* first_writer;  // [seqs] of the page that this sequence claims
-  int* writers;       // [seqs]
-  int* copies;        // [seqs] page that the sequence copies its partly filled one from, or -1
-  int* start;         // [seqs + 1] number of the sequence's first new page
-  int* got;           // [min(pages, seqs * per_seq)] the new pages
-  int* copy;          // [seqs][3] source, target, blocks
-  int* counts;        // [2] new pages there were, copies
+  ForkRow* row;   // [seqs]
+  int* taken;     // [seqs][per_seq] pages that a sequence takes over, or -1
+  int* claim;     // [pages] one of the sequences that will write to this partly filled page
+  int* got;       // [min(pages, seqs * per_seq)] the new pages
+  int* copy;      // [seqs][3] source, target, blocks
+  int* counts;    // [2] new pages that there were, copies
+  ForkSeq* seq;   // [seqs] or nothing
 };
 __host__ __device__ inline int64_t fork_layout(ForkSpace* f, int* p, int64_t seqs, int64_t per_seq, int64_t pages) {
   int64_t at = 0;
@@ -65,31 +80,19 @@ __host__ __device__ inline int64_t fork_layout(ForkSpace* f, int* p, int64_t seq
     at += n;
     return mine;
   };
+  f->row = reinterpret_cast<ForkRow*>(take(4 * seqs));
   f->taken = take(seqs * per_seq);
   f->claim = take(pages);
-  f->first_writer = take(seqs);
-  f->writers = take(seqs);
-  f->copies = take(seqs);
-  f->start = take(seqs + 1);
   f->got = take(pages < seqs * per_seq ? pages : seqs * per_seq);
   f->copy = take(3 * seqs);
   f->counts = take(2);
+  f->seq = reinterpret_cast<ForkSeq*>(take(seqs > kHeldSeqs ? 5 * seqs : 0));
   return at;
 }
 
-// Counts: what each sequence takes over, against what it had.
-__global__ __launch_bounds__(kThreads) void kv8_fork_count_kernel(Kv8ForkArgs a) {
-  ForkSpace f;
-  fork_layout(&f, a.workspace, a.seqs, a.per_seq, a.pages);
-  const int tiles = (a.per_seq + kThreads - 1) / kThreads;
-  const int s = blockIdx.x / tiles, place = blockIdx.x % tiles * kThreads + threadIdx.x;
+// What sequence s takes over at a place of its row, against what it had there.
+__device__ __forceinline__ void count_entry(const Kv8ForkArgs& a, const ForkSpace& f, int s, int place) {
   const ForkPlan plan(a, s);
-  if (place >= a.per_seq) return;
-  if (place == 0) {
-    f.first_writer[s] = INT_MAX;
-    f.writers[s] = 0;
-    if (plan.bad) atomicOr(a.error, kKv8BadRows);
-  }
   auto entry = [&](int seq) {
     const int p = a.table[static_cast<int64_t>(seq) * a.per_seq + place];
     return p >= 0 && p < a.pages ? p : -1;
@@ -110,9 +113,17 @@ __global__ __launch_bounds__(kThreads) void kv8_fork_count_kernel(Kv8ForkArgs a)
   }
   if (takes >= 0 && place == plan.full() && plan.partly() && plan.room > 0) f.claim[takes] = s;  // any of them
 }
+__global__ __launch_bounds__(kThreads) void kv8_fork_count_kernel(Kv8ForkArgs a) {
+  ForkSpace f;
+  fork_layout(&f, a.workspace, a.seqs, a.per_seq, a.pages);
+  const int tiles = (a.per_seq + kThreads - 1) / kThreads;
+  const int s = blockIdx.x / tiles, place = blockIdx.x % tiles * kThreads + threadIdx.x;
+  if (place < a.per_seq) count_entry(a, f, s, place);
+}
 
 // Exclusive sum over the block; *total has the sum.  Every thread calls it.
 __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
+  constexpr int kWaves = kOneThreads / kWave;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   int sum = v;
 #pragma unroll
@@ -123,7 +134,8 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
   if (lane == kWave - 1) sh[wave] = sum;
   __syncthreads();
   int before = 0, all = 0;
-  for (int w = 0; w < kOneThreads / kWave; ++w) {
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
     const int n = sh[w];
     if (w < wave) before += n;
     all += n;
@@ -133,64 +145,96 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
   return before + sum - v;
 }
 
-// Decides who copies, and finds the new pages.  One block.
+// Decides who copies, and finds the new pages: one block, a sequence a thread.
+// What it takes is a chain of dependent loads (plans, pages taken, who claims
+// them and their users), so all else is held, or asked for ahead.
+template <bool kCount>
 __global__ __launch_bounds__(kOneThreads) void kv8_fork_decide_kernel(Kv8ForkArgs a) {
   __shared__ int sh[kOneThreads / kWave], sh_copies;
+  __shared__ ForkSeq held[kHeldSeqs];
   ForkSpace f;
   fork_layout(&f, a.workspace, a.seqs, a.per_seq, a.pages);
+  ForkSeq* const seq = a.seqs <= kHeldSeqs ? held : f.seq;
   const int tid = threadIdx.x;
   if (tid == 0) sh_copies = 0;
-  auto partly_filled = [&](const ForkPlan& plan, int s) {
-    return plan.partly() ? f.taken[static_cast<int64_t>(s) * a.per_seq + plan.full()] : -1;
+  for (int s = tid; s < a.seqs; s += kOneThreads) seq[s].first_writer = INT_MAX, seq[s].writers = 0;
+  if constexpr (kCount) {
+    for (int n = tid; n < a.seqs * a.per_seq; n += kOneThreads) {
+      const int s = n / a.per_seq;
+      count_entry(a, f, s, n - s * a.per_seq);
+    }
+  }
+  __syncthreads();
+  // Which pages are free no longer changes: a page that is copied from stays in use.
+  auto ask_users = [&](int p) {
+    if (p + 4 <= a.pages) return *reinterpret_cast<const int4*>(a.users + p);
+    int4 n = make_int4(1, 1, 1, 1);
+    if (p < a.pages) n.x = a.users[p];
+    if (p + 1 < a.pages) n.y = a.users[p + 1];
+    if (p + 2 < a.pages) n.z = a.users[p + 2];
+    return n;
   };
+  int4 users = ask_users(4 * tid);
   // Those who will write to a page agree on one of them, who counts them.
   for (int s = tid; s < a.seqs; s += kOneThreads) {
     const ForkPlan plan(a, s);
-    const int p = partly_filled(plan, s);
+    const int p = plan.partly() ? f.taken[static_cast<int64_t>(s) * a.per_seq + plan.full()] : -1;
+    ForkRow row;
+    row.fresh = plan.full() + (p >= 0);
+    row.pages = plan.pages();
+    row.start = (plan.keep % kKv8Page + kKv8Block - 1) / kKv8Block;  // until it has one: blocks to copy
+    f.row[s] = row;
+    if (plan.bad) atomicOr(a.error, kKv8BadRows);
+    seq[s].page = p >= 0 && plan.room > 0 ? p : -1;
     if (p >= 0 && plan.room > 0) {
       const int one = f.claim[p];
-      atomicMin(f.first_writer + one, s);
-      atomicAdd(f.writers + one, 1);
+      seq[s].users = a.users[p];
+      seq[s].one = one;
+      atomicMin(&seq[one].first_writer, s);
+      atomicAdd(&seq[one].writers, 1);
     }
   }
   __syncthreads();
-  // The first of them keeps the page if nobody else has it.
-  for (int s = tid; s < a.seqs; s += kOneThreads) {
-    const ForkPlan plan(a, s);
-    const int p = partly_filled(plan, s);
-    int from = -1;
-    if (p >= 0 && plan.room > 0) {
-      const int one = f.claim[p];
-      const bool keeps = a.users[p] == f.writers[one] && f.first_writer[one] == s;
-      if (!keeps) from = p;
-    }
-    f.copies[s] = from;
-  }
-  __syncthreads();
+  // The first of them keeps the page if nobody else has it.  Copies are noted with
+  // the number of their new page, which is found after.
   int wanted = 0;
   for (int base = 0; base < a.seqs; base += kOneThreads) {
     const int s = base + tid;
     int mine = 0;
+    ForkRow row = {};
+    bool copies = false;
     if (s < a.seqs) {
-      const ForkPlan plan(a, s);
-      const int from = f.copies[s];
-      if (from >= 0) atomicSub(a.users + from, 1);
-      const int kept = plan.full() + (plan.partly() && partly_filled(plan, s) >= 0 && from < 0 ? 1 : 0);
-      mine = max(0, plan.pages() - kept);
+      row = f.row[s];
+      if (seq[s].page >= 0) {
+        const int one = seq[s].one;
+        copies = seq[s].users != seq[one].writers || seq[one].first_writer != s;
+        if (copies) {
+          atomicSub(a.users + seq[s].page, 1);
+          --row.fresh;
+        }
+      }
+      mine = max(0, row.pages - row.fresh);
     }
     int all;
     const int before = block_scan(mine, sh, &all);
-    if (s < a.seqs) f.start[s] = wanted + before;
+    if (s < a.seqs) {
+      if (copies) {
+        int* c = f.copy + 3 * atomicAdd(&sh_copies, 1);
+        c[0] = seq[s].page;
+        c[1] = wanted + before;
+        c[2] = row.start;
+      }
+      row.start = wanted + before;
+      f.row[s] = row;
+    }
     wanted += all;
   }
-  if (tid == 0) f.start[a.seqs] = wanted;
   // The lowest free pages.
   int got = 0;
   for (int base = 0; base < a.pages && got < wanted; base += 4 * kOneThreads) {
     const int p = base + 4 * tid;
-    int n[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) n[i] = p + i < a.pages ? a.users[p + i] : 1;
+    if (base > 0) users = ask_users(p);
+    const int n[4] = {users.x, users.y, users.z, users.w};
     int mine = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) mine += n[i] <= 0;
@@ -207,17 +251,6 @@ __global__ __launch_bounds__(kOneThreads) void kv8_fork_decide_kernel(Kv8ForkArg
       }
     got = min(got + all, wanted);
   }
-  __syncthreads();
-  for (int s = tid; s < a.seqs; s += kOneThreads) {
-    const int from = f.copies[s], number = f.start[s];
-    if (from < 0 || number >= got) continue;
-    const ForkPlan plan(a, s);
-    int* c = f.copy + 3 * atomicAdd(&sh_copies, 1);
-    c[0] = from;
-    c[1] = f.got[number];
-    c[2] = (plan.keep % kKv8Page + kKv8Block - 1) / kKv8Block;
-  }
-  __syncthreads();
   if (tid == 0) {
     f.counts[0] = got;
     f.counts[1] = sh_copies;
@@ -225,121 +258,194 @@ __global__ __launch_bounds__(kOneThreads) void kv8_fork_decide_kernel(Kv8ForkArg
   }
 }
 
-__global__ __launch_bounds__(kThreads) void kv8_fork_table_kernel(Kv8ForkArgs a) {
+// The keys or values of the blocks [0, kBlocks) of every head of a page; all
+// blocks lie together.
+template <int D, int kBlocks>
+__device__ __forceinline__ void copy_codes(int8_t* base, bool keys, int64_t source, int64_t target, int hkv) {
+  const int pieces = hkv * D * kBlocks;
+  const i32x4* from = reinterpret_cast<const i32x4*>(base + source);
+  i32x4* to = reinterpret_cast<i32x4*>(base + target);
+  for (int n = threadIdx.x; n < pieces; n += kThreads) {
+    // Keys: [head][block][D] pieces of a token; values: [head][D][block].
+    const int at = kBlocks == kKv8Blocks ? n
+                   : keys                ? n / (D * kBlocks) * (kKv8Blocks * D) + n % (D * kBlocks)
+                                         : n / kBlocks * kKv8Blocks + n % kBlocks;
+    __builtin_nontemporal_store(from[at], to + at);
+  }
+}
+template <int D>
+__device__ __forceinline__ void copy_page(const Kv8Layers& l, int layer, bool keys, int from, int to, int blocks) {
+  const int64_t source = kv8_offset(from, 0, l.hkv, D), target = kv8_offset(to, 0, l.hkv, D);
+  int8_t* codes = keys ? l.keys[layer] : l.values[layer];
+  int8_t* exps = keys ? l.key_exps[layer] : l.value_exps[layer];
+  switch (blocks) {
+    case 1: copy_codes<D, 1>(codes, keys, source, target, l.hkv); break;
+    case 2: copy_codes<D, 2>(codes, keys, source, target, l.hkv); break;
+    case 3: copy_codes<D, 3>(codes, keys, source, target, l.hkv); break;
+    default: copy_codes<D, 4>(codes, keys, source, target, l.hkv); break;
+  }
+  static_assert(kKv8Blocks == 4, "a switch over them");
+  const int64_t old = kv8_exp_offset(from, 0, l.hkv), now = kv8_exp_offset(to, 0, l.hkv);
+  for (int n = threadIdx.x; n < l.hkv * kKv8Blocks; n += kThreads)
+    if (n % kKv8Blocks < blocks) exps[now + n] = exps[old + n];
+}
+
+// Table rows of a fork, and the copies of a group of layers: the first `tables`
+// blocks have the rows.
+template <int D>
+__global__ __launch_bounds__(kThreads) void kv8_fork_apply_kernel(Kv8ForkArgs a, Kv8Layers l, int tables) {
   ForkSpace f;
   fork_layout(&f, a.workspace, a.seqs, a.per_seq, a.pages);
-  const int tiles = (a.per_seq + kThreads - 1) / kThreads;
-  const int s = blockIdx.x / tiles, place = blockIdx.x % tiles * kThreads + threadIdx.x;
-  if (place >= a.per_seq) return;
-  const ForkPlan plan(a, s);
-  const int64_t at = static_cast<int64_t>(s) * a.per_seq + place;
-  const int start = f.start[s], end = f.start[s + 1], first_new = plan.pages() - (end - start);
-  int p = f.taken[at];
-  if (place >= first_new && place < plan.pages()) {
-    const int number = start + place - first_new;
-    p = number < f.counts[0] ? f.got[number] : -1;
-  }
-  a.table[at] = p;
-}
-
-// The first `blocks` blocks of a page of one layer, 16 bytes a thread.
-__device__ __forceinline__ void copy_page(const Kv8Layers& l, int layer, int from, int to, int blocks) {
-  const int64_t source = kv8_offset(from, 0, l.hkv, l.d), target = kv8_offset(to, 0, l.hkv, l.d);
-  const int pieces = l.hkv * l.d * blocks;  // of keys, and of values
-  for (int n = threadIdx.x; n < 2 * pieces; n += kCopyThreads) {
-    const bool keys = n < pieces;
-    const int m = keys ? n : n - pieces;
-    int at;
-    if (keys) {
-      const int each = l.d * blocks;  // of a head
-      at = m / each * (kKv8Page * l.d / 16) + m % each;
-    } else {
-      at = m / blocks * (kKv8Page / 16) + m % blocks;
+  if (static_cast<int>(blockIdx.x) < tables) {
+    const int tiles = (a.per_seq + kThreads - 1) / kThreads;
+    const int s = blockIdx.x / tiles, place = blockIdx.x % tiles * kThreads + threadIdx.x;
+    if (place >= a.per_seq) return;
+    const int64_t at = static_cast<int64_t>(s) * a.per_seq + place;
+    const ForkRow row = f.row[s];
+    int p = f.taken[at];
+    if (place >= row.fresh && place < row.pages) {
+      const int number = row.start + place - row.fresh;
+      p = number < f.counts[0] ? f.got[number] : -1;
     }
-    int8_t* base = keys ? l.keys[layer] : l.values[layer];
-    reinterpret_cast<uint4*>(base + target)[at] = reinterpret_cast<const uint4*>(base + source)[at];
+    a.table[at] = p;
+    return;
   }
-  for (int n = threadIdx.x; n < 2 * l.hkv * blocks; n += kCopyThreads) {
-    const int head = n / (2 * blocks), m = n % (2 * blocks);
-    int8_t* base = m < blocks ? l.key_exps[layer] : l.value_exps[layer];
-    base[kv8_exp_offset(to, head, l.hkv) + m % blocks] = base[kv8_exp_offset(from, head, l.hkv) + m % blocks];
-  }
-}
-
-__global__ __launch_bounds__(kCopyThreads) void kv8_copy_kernel(Kv8Layers l, const int* list, const int* count) {
-  const int units = *count * l.count;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const int* c = list + 3 * (u / l.count);
-    copy_page(l, u % l.count, c[0], c[1], c[2]);
+  const int units = f.counts[1] * l.count * 2, got = f.counts[0];
+  for (int u = blockIdx.x - tables; u < units; u += gridDim.x - tables) {
+    const int* c = f.copy + 3 * (u / 2 / l.count);
+    if (c[1] < got) copy_page<D>(l, u / 2 % l.count, u % 2 == 0, c[0], f.got[c[1]], c[2]);
   }
 }
 
 // ------------------------------------------------------------- compact ----
 
 struct CompactSpace {
-  int* copy;    // [pages / 2][3] source, target, blocks
-  int* counts;  // [1] of them
+  int* source;  // [pages / 2] of the k-th move
+  int* target;
+  int* count;
 };
 __host__ __device__ inline int64_t compact_layout(CompactSpace* c, int* p, int64_t pages) {
-  c->copy = p;
-  c->counts = p ? p + 3 * (pages / 2) : nullptr;
-  return 3 * (pages / 2) + 1;
+  c->source = p;
+  c->target = p ? p + pages / 2 : nullptr;
+  c->count = p ? p + 2 * (pages / 2) : nullptr;
+  return 2 * (pages / 2) + 1;
 }
 
-// Pairs the k-th page in use from `live` on with the k-th hole below it.  One block.
+// Pairs the k-th page in use from `live` on with the k-th hole below it.  With
+// the number of pages in use before each page, p is the hole number p - that, or
+// the move number that - (those below live): one sum over the pages.  One block;
+// a thread holds the users of its pages where there are few enough.
 __global__ __launch_bounds__(kOneThreads) void kv8_compact_decide_kernel(Kv8CompactArgs a) {
-  __shared__ int sh[kOneThreads / kWave];
+  __shared__ int sh[kOneThreads / kWave], sh_below;
   CompactSpace c;
   compact_layout(&c, a.workspace, a.pages);
   const int tid = threadIdx.x;
-  int mine = 0, live, unused;
-  for (int p = tid; p < a.pages; p += kOneThreads) mine += a.users[p] > 0;
-  block_scan(mine, sh, &live);
-  int holes = 0, movers = 0;
-  for (int base = 0; base < a.pages; base += kOneThreads) {
-    const int p = base + tid;
-    const int n = p < a.pages ? a.users[p] : 0;
-    const bool hole = p < a.pages && p < live && n <= 0, mover = p >= live && n > 0;
-    const int hole_at = holes + block_scan(hole, sh, &unused);
-    holes += unused;
-    const int mover_at = movers + block_scan(mover, sh, &unused);
-    movers += unused;
-    if (hole) c.copy[3 * hole_at + 1] = p;
-    if (mover) {
-      c.copy[3 * mover_at] = p;
-      c.copy[3 * mover_at + 2] = kKv8Blocks;
+  const int each = ((a.pages + kOneThreads - 1) / kOneThreads + 3) / 4 * 4;  // neighbouring pages of a thread
+  const bool holds = each <= kHeldPages;
+  int held[kHeldPages];
+  const int first = min(static_cast<int64_t>(tid) * each, static_cast<int64_t>(a.pages));
+  const int last = min(static_cast<int64_t>(first) + each, static_cast<int64_t>(a.pages));
+  int mine = 0;
+  if (holds) {
+#pragma unroll
+    for (int i = 0; i < kHeldPages; i += 4) {
+      int4 n = make_int4(0, 0, 0, 0);
+      if (first + i + 4 <= last) {
+        n = *reinterpret_cast<const int4*>(a.users + first + i);
+      } else {
+        if (first + i < last) n.x = a.users[first + i];
+        if (first + i + 1 < last) n.y = a.users[first + i + 1];
+        if (first + i + 2 < last) n.z = a.users[first + i + 2];
+      }
+      held[i] = n.x, held[i + 1] = n.y, held[i + 2] = n.z, held[i + 3] = n.w;
     }
-    if (p < a.pages) {
-      a.moved[p] = n > 0 ? p : -1;
-      if (p < live) a.users_out[p] = max(n, 0);
-    }
+#pragma unroll
+    for (int i = 0; i < kHeldPages; ++i) mine += held[i] > 0;
+  } else {
+    for (int p = first; p < last; ++p) mine += a.users[p] > 0;
   }
+  int live;
+  const int before = block_scan(mine, sh, &live);
+  if (tid == 0) sh_below = live;  // where no page is at `live`: all
   __syncthreads();
-  for (int k = tid; k < movers; k += kOneThreads) {
-    const int from = c.copy[3 * k], to = c.copy[3 * k + 1];
+  auto users_of = [&](auto use) {  // of the thread's pages: use(page, users, pages in use before it)
+    int used = before;
+    if (holds) {
+#pragma unroll
+      for (int i = 0; i < kHeldPages; ++i)
+        if (first + i < last) {
+          use(first + i, held[i], used);
+          used += held[i] > 0;
+        }
+    } else {
+      for (int p = first; p < last; ++p) {
+        const int n = a.users[p];
+        use(p, n, used);
+        used += n > 0;
+      }
+    }
+  };
+  if (first <= live && live < last) users_of([&](int p, int, int used) {
+    if (p == live) sh_below = used;
+  });
+  __syncthreads();
+  const int below = sh_below;
+  // users_out may be users: what is read of a page is read before it is written.
+  users_of([&](int p, int n, int used) {
+    if (p < live && n <= 0) c.target[p - used] = p;
+    if (p >= live && n > 0) c.source[used - below] = p;
+    a.moved[p] = n > 0 ? p : -1;
+    if (p < live) a.users_out[p] = max(n, 0);
+  });
+  __syncthreads();
+  for (int k = tid; k < live - below; k += kOneThreads) {
+    const int from = c.source[k], to = c.target[k];
     a.moved[from] = to;
     a.users_out[to] = a.users[from];
   }
   __syncthreads();
   for (int p = live + tid; p < a.pages; p += kOneThreads) a.users_out[p] = 0;
   if (tid == 0) {
-    *c.counts = movers;
+    *c.count = live - below;
     *a.live = live;
   }
 }
 
-__global__ __launch_bounds__(kThreads) void kv8_compact_table_kernel(Kv8CompactArgs a) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (at >= static_cast<int64_t>(a.seqs) * a.per_seq) return;
-  const int p = a.table[at];
-  a.table_out[at] = p >= 0 && p < a.pages ? a.moved[p] : -1;
+// The table, and the moves of a group of layers.
+template <int D>
+__global__ __launch_bounds__(kThreads) void kv8_compact_apply_kernel(Kv8CompactArgs a, Kv8Layers l, int tables) {
+  if (static_cast<int>(blockIdx.x) < tables) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (at >= static_cast<int64_t>(a.seqs) * a.per_seq) return;
+    const int p = a.table[at];
+    a.table_out[at] = p >= 0 && p < a.pages ? a.moved[p] : -1;
+    return;
+  }
+  CompactSpace c;
+  compact_layout(&c, a.workspace, a.pages);
+  const int units = *c.count * l.count * 2;
+  for (int u = blockIdx.x - tables; u < units; u += gridDim.x - tables) {
+    const int k = u / 2 / l.count;
+    copy_page<D>(l, u / 2 % l.count, u % 2 == 0, c.source[k], c.target[k], kKv8Blocks);
+  }
 }
 
-hipError_t launch_copies(const Kv8Layers* layers, int groups, const int* list, const int* count, int64_t most,
-                         hipStream_t stream) {
+// Calls launch(D, layers, table blocks, all blocks) for each group of layers; the
+// first has the table's blocks.
+template <typename Launch>
+hipError_t launch_groups(const Kv8Layers* layers, int groups, int64_t table_blocks, int64_t most_copies,
+                         Launch launch) {
   for (int g = 0; g < groups; ++g) {
-    const int64_t blocks = std::min<int64_t>(kCopyBlocks, most * layers[g].count);
-    if (blocks > 0) kv8_copy_kernel<<<dim3(blocks), kCopyThreads, 0, stream>>>(layers[g], list, count);
+    const int tables = static_cast<int>(g == 0 ? table_blocks : 0);
+    const int blocks = tables + static_cast<int>(std::min<int64_t>(kCopyBlocks, most_copies * layers[g].count * 2));
+    if (blocks == 0) continue;
+    switch (layers[g].d) {
+      case 32: launch(std::integral_constant<int, 32>(), layers[g], tables, blocks); break;
+      case 64: launch(std::integral_constant<int, 64>(), layers[g], tables, blocks); break;
+      case 96: launch(std::integral_constant<int, 96>(), layers[g], tables, blocks); break;
+      case 128: launch(std::integral_constant<int, 128>(), layers[g], tables, blocks); break;
+      default: return hipErrorInvalidValue;
+    }
   }
   return hipGetLastError();
 }
@@ -352,13 +458,16 @@ int64_t kv8_fork_workspace(int64_t seqs, int64_t per_seq, int64_t pages) {
 }
 
 hipError_t launch_kv8_fork(const Kv8ForkArgs& a, const Kv8Layers* layers, int groups, hipStream_t stream) {
-  ForkSpace f;
-  fork_layout(&f, a.workspace, a.seqs, a.per_seq, a.pages);
   const int blocks = a.seqs * ((a.per_seq + kThreads - 1) / kThreads);
-  kv8_fork_count_kernel<<<dim3(blocks), kThreads, 0, stream>>>(a);
-  kv8_fork_decide_kernel<<<dim3(1), kOneThreads, 0, stream>>>(a);
-  kv8_fork_table_kernel<<<dim3(blocks), kThreads, 0, stream>>>(a);
-  return launch_copies(layers, groups, f.copy, f.counts + 1, a.seqs, stream);
+  if (static_cast<int64_t>(a.seqs) * a.per_seq <= kCountEntries) {
+    kv8_fork_decide_kernel<true><<<dim3(1), kOneThreads, 0, stream>>>(a);
+  } else {
+    kv8_fork_count_kernel<<<dim3(blocks), kThreads, 0, stream>>>(a);
+    kv8_fork_decide_kernel<false><<<dim3(1), kOneThreads, 0, stream>>>(a);
+  }
+  return launch_groups(layers, groups, blocks, a.seqs, [&](auto d, const Kv8Layers& l, int tables, int all) {
+    kv8_fork_apply_kernel<decltype(d)::value><<<dim3(all), kThreads, 0, stream>>>(a, l, tables);
+  });
 }
 
 int64_t kv8_compact_workspace(int64_t pages) {
@@ -367,12 +476,12 @@ int64_t kv8_compact_workspace(int64_t pages) {
 }
 
 hipError_t launch_kv8_compact(const Kv8CompactArgs& a, const Kv8Layers* layers, int groups, hipStream_t stream) {
-  CompactSpace c;
-  compact_layout(&c, a.workspace, a.pages);
   kv8_compact_decide_kernel<<<dim3(1), kOneThreads, 0, stream>>>(a);
   const int64_t entries = static_cast<int64_t>(a.seqs) * a.per_seq;
-  kv8_compact_table_kernel<<<dim3((entries + kThreads - 1) / kThreads), kThreads, 0, stream>>>(a);
-  return launch_copies(layers, groups, c.copy, c.counts, a.pages / 2, stream);
+  return launch_groups(layers, groups, (entries + kThreads - 1) / kThreads, a.pages / 2,
+                       [&](auto d, const Kv8Layers& l, int tables, int all) {
+                         kv8_compact_apply_kernel<decltype(d)::value><<<dim3(all), kThreads, 0, stream>>>(a, l, tables);
+                       });
 }
 
 }  // namespace mmr
