@@ -24,7 +24,7 @@ constexpr int kThreads = 256;
 constexpr int kOneThreads = 1024;     // of a block that is alone
 constexpr int kHeldSeqs = 2048;       // sequences whose plans the deciding block holds in LDS
 constexpr int kCountEntries = 8192;   // table entries that it counts itself
-constexpr int kHeldPages = 16;        // pages a thread of it holds
+constexpr int kHeldPages = 16;        // pages that a thread of a compacting block holds
 constexpr int kCopyBlocks = 16384;
 
 // ---------------------------------------------------------------- fork ----
@@ -334,21 +334,24 @@ __host__ __device__ inline int64_t compact_layout(CompactSpace* c, int* p, int64
 // Pairs the k-th page in use from `live` on with the k-th hole below it.  With
 // the number of pages in use before each page, p is the hole number p - that, or
 // the move number that - (those below live): one sum over the pages.  One block;
-// a thread holds the users of its pages where there are few enough.
+// kHolds: few enough pages that threads hold their users, and LDS the holes.
+template <bool kHolds>
 __global__ __launch_bounds__(kOneThreads) void kv8_compact_decide_kernel(Kv8CompactArgs a) {
   __shared__ int sh[kOneThreads / kWave], sh_below;
+  __shared__ int holes[kHolds ? kOneThreads * kHeldPages / 2 : 1], movers[kHolds ? kOneThreads * kHeldPages / 2 : 1];
   CompactSpace c;
   compact_layout(&c, a.workspace, a.pages);
   const int tid = threadIdx.x;
   const int each = ((a.pages + kOneThreads - 1) / kOneThreads + 3) / 4 * 4;  // neighbouring pages of a thread
-  const bool holds = each <= kHeldPages;
   int held[kHeldPages];
   const int first = min(static_cast<int64_t>(tid) * each, static_cast<int64_t>(a.pages));
   const int last = min(static_cast<int64_t>(first) + each, static_cast<int64_t>(a.pages));
   int mine = 0;
-  if (holds) {
+  if constexpr (kHolds) {
 #pragma unroll
     for (int i = 0; i < kHeldPages; i += 4) {
+      held[i] = held[i + 1] = held[i + 2] = held[i + 3] = 0;
+      if (i >= each) continue;
       int4 n = make_int4(0, 0, 0, 0);
       if (first + i + 4 <= last) {
         n = *reinterpret_cast<const int4*>(a.users + first + i);
@@ -366,17 +369,19 @@ __global__ __launch_bounds__(kOneThreads) void kv8_compact_decide_kernel(Kv8Comp
   }
   int live;
   const int before = block_scan(mine, sh, &live);
-  if (tid == 0) sh_below = live;  // where no page is at `live`: all
-  __syncthreads();
-  auto users_of = [&](auto use) {  // of the thread's pages: use(page, users, pages in use before it)
+  auto pages_of = [&](auto use) {  // of the thread: use(page, users, pages in use before it)
     int used = before;
-    if (holds) {
+    if constexpr (kHolds) {
 #pragma unroll
-      for (int i = 0; i < kHeldPages; ++i)
-        if (first + i < last) {
-          use(first + i, held[i], used);
-          used += held[i] > 0;
-        }
+      for (int i = 0; i < kHeldPages; i += 4) {
+        if (i >= each) continue;  // of all threads
+#pragma unroll
+        for (int m = i; m < i + 4; ++m)
+          if (first + m < last) {
+            use(first + m, held[m], used);
+            used += held[m] > 0;
+          }
+      }
     } else {
       for (int p = first; p < last; ++p) {
         const int n = a.users[p];
@@ -385,26 +390,68 @@ __global__ __launch_bounds__(kOneThreads) void kv8_compact_decide_kernel(Kv8Comp
       }
     }
   };
-  if (first <= live && live < last) users_of([&](int p, int, int used) {
+  if (tid == 0 && live == a.pages) sh_below = live;
+  if (first <= live && live < last) pages_of([&](int p, int, int used) {
     if (p == live) sh_below = used;
   });
   __syncthreads();
   const int below = sh_below;
-  // users_out may be users: what is read of a page is read before it is written.
-  users_of([&](int p, int n, int used) {
-    if (p < live && n <= 0) c.target[p - used] = p;
-    if (p >= live && n > 0) c.source[used - below] = p;
-    a.moved[p] = n > 0 ? p : -1;
-    if (p < live) a.users_out[p] = max(n, 0);
-  });
-  __syncthreads();
-  for (int k = tid; k < live - below; k += kOneThreads) {
-    const int from = c.source[k], to = c.target[k];
-    a.moved[from] = to;
-    a.users_out[to] = a.users[from];
+  if constexpr (kHolds) {
+    pages_of([&](int p, int n, int used) {
+      if (p < live && n <= 0) holes[p - used] = p;
+      if (p >= live && n > 0) movers[used - below] = n;
+    });
+    __syncthreads();  // and nothing of users is read after
+    // Four pages a store: one at a time, stores take most of the time.
+    int used = before;
+#pragma unroll
+    for (int i = 0; i < kHeldPages; i += 4) {
+      if (i >= each) continue;
+      int to[4], n[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const int p = first + i + m;
+        n[m] = held[i + m];
+        to[m] = n[m] > 0 ? p : -1;
+        if (p < last && p < live && n[m] <= 0) n[m] = movers[p - used];
+        else if (p < last && p >= live && n[m] > 0) {
+          const int k = used - below;
+          to[m] = holes[k];
+          c.source[k] = p;
+          c.target[k] = to[m];
+        }
+        if (p >= live) n[m] = 0;
+        used += held[i + m] > 0;
+      }
+      if (first + i + 4 <= last) {
+        *reinterpret_cast<int4*>(a.moved + first + i) = make_int4(to[0], to[1], to[2], to[3]);
+        *reinterpret_cast<int4*>(a.users_out + first + i) = make_int4(n[0], n[1], n[2], n[3]);
+      } else {
+#pragma unroll
+        for (int m = 0; m < 3; ++m)
+          if (first + i + m < last) {
+            a.moved[first + i + m] = to[m];
+            a.users_out[first + i + m] = n[m];
+          }
+      }
+    }
+  } else {
+    // users_out may be users: what is read of a page is read before it is written.
+    pages_of([&](int p, int n, int used) {
+      if (p < live && n <= 0) c.target[p - used] = p;
+      if (p >= live && n > 0) c.source[used - below] = p;
+      a.moved[p] = n > 0 ? p : -1;
+      if (p < live) a.users_out[p] = max(n, 0);
+    });
+    __syncthreads();
+    for (int k = tid; k < live - below; k += kOneThreads) {
+      const int from = c.source[k], to = c.target[k];
+      a.moved[from] = to;
+      a.users_out[to] = a.users[from];
+    }
+    __syncthreads();
+    for (int p = live + tid; p < a.pages; p += kOneThreads) a.users_out[p] = 0;
   }
-  __syncthreads();
-  for (int p = live + tid; p < a.pages; p += kOneThreads) a.users_out[p] = 0;
   if (tid == 0) {
     *c.count = live - below;
     *a.live = live;
@@ -476,7 +523,10 @@ int64_t kv8_compact_workspace(int64_t pages) {
 }
 
 hipError_t launch_kv8_compact(const Kv8CompactArgs& a, const Kv8Layers* layers, int groups, hipStream_t stream) {
-  kv8_compact_decide_kernel<<<dim3(1), kOneThreads, 0, stream>>>(a);
+  if (a.pages <= kOneThreads * kHeldPages)
+    kv8_compact_decide_kernel<true><<<dim3(1), kOneThreads, 0, stream>>>(a);
+  else
+    kv8_compact_decide_kernel<false><<<dim3(1), kOneThreads, 0, stream>>>(a);
   const int64_t entries = static_cast<int64_t>(a.seqs) * a.per_seq;
   return launch_groups(layers, groups, (entries + kThreads - 1) / kThreads, a.pages / 2,
                        [&](auto d, const Kv8Layers& l, int tables, int all) {
