@@ -121,16 +121,26 @@ __global__ __launch_bounds__(kThreads) void kv8_fork_count_kernel(Kv8ForkArgs a)
   if (place < a.per_seq) count_entry(a, f, s, place);
 }
 
+// v and the sum of those lanes before it: shifts within rows of 16 lanes, then
+// the last lane of a row (and of two) handed to those after it.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int lane_before(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v += lane_before<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v += lane_before<0x112, 0xF>(v);
+  v += lane_before<0x114, 0xF>(v);
+  v += lane_before<0x118, 0xF>(v);
+  v += lane_before<0x142, 0xA>(v);  // row_bcast 15 to the second and fourth row
+  return v + lane_before<0x143, 0xC>(v);  // row_bcast 31 to the third and fourth
+}
+
 // Exclusive sum over the block; *total has the sum.  Every thread calls it.
 __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
   constexpr int kWaves = kOneThreads / kWave;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  int sum = v;
-#pragma unroll
-  for (int step = 1; step < kWave; step *= 2) {
-    const int other = __shfl_up(sum, step);
-    if (lane >= step) sum += other;
-  }
+  const int sum = wave_scan(v);
   if (lane == kWave - 1) sh[wave] = sum;
   __syncthreads();
   int before = 0, all = 0;
@@ -176,6 +186,7 @@ __global__ __launch_bounds__(kOneThreads) void kv8_fork_decide_kernel(Kv8ForkArg
   };
   int4 users = ask_users(4 * tid);
   // Those who will write to a page agree on one of them, who counts them.
+  ForkRow first_row = {};  // of sequence tid
   for (int s = tid; s < a.seqs; s += kOneThreads) {
     const ForkPlan plan(a, s);
     const int p = plan.partly() ? f.taken[static_cast<int64_t>(s) * a.per_seq + plan.full()] : -1;
@@ -183,7 +194,8 @@ __global__ __launch_bounds__(kOneThreads) void kv8_fork_decide_kernel(Kv8ForkArg
     row.fresh = plan.full() + (p >= 0);
     row.pages = plan.pages();
     row.start = (plan.keep % kKv8Page + kKv8Block - 1) / kKv8Block;  // until it has one: blocks to copy
-    f.row[s] = row;
+    if (s == tid) first_row = row;
+    else f.row[s] = row;
     if (plan.bad) atomicOr(a.error, kKv8BadRows);
     seq[s].page = p >= 0 && plan.room > 0 ? p : -1;
     if (p >= 0 && plan.room > 0) {
@@ -204,7 +216,7 @@ __global__ __launch_bounds__(kOneThreads) void kv8_fork_decide_kernel(Kv8ForkArg
     ForkRow row = {};
     bool copies = false;
     if (s < a.seqs) {
-      row = f.row[s];
+      row = base == 0 ? first_row : f.row[s];
       if (seq[s].page >= 0) {
         const int one = seq[s].one;
         copies = seq[s].users != seq[one].writers || seq[one].first_writer != s;
