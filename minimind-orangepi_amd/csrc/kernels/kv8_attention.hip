@@ -62,6 +62,7 @@ constexpr int kPBits = 28;              // p of steps in units of 2^-28: at most
 // See kv8_attention_plan.
 constexpr int kLeastPages = 2, kLeastRowsPages = 4, kWidePages = 16;
 constexpr int kStepBlocks = 256, kRowsBlocks = 1280, kFewRows = 256;
+constexpr int kWindowBlocks = 64, kWindowPages = 40, kComputeUnits = 256;
 constexpr int kMostSplits = 64;         // a lane of a wave each in the join
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 using f32x4 = float __attribute__((ext_vector_type(4)));
@@ -873,6 +874,37 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_kernel(Kv8AttnArgs a
 
 }  // namespace
 
+// With a window, all tiles of many rows see the same few pages, and the best
+// number of splits is that of the shortest estimate: the pages of a split, times
+// what a page takes with so many blocks on a compute unit, and for more than one
+// split the join and its bytes.  us a page with d 96 (d 128): 1.73 (1.9) for one
+// block, 2.2 (2.6) for two, 2.95 for three, then 1.02 (1.3) a block; a join 5.5
+// and 0.8 a split of 1,000 rows of 8 heads.  Measured (5,000 rows, window 1,500,
+// d 96): one split 77.5, two 82.9, four 90.8; 3,000 rows 57.1, 49.8, 54.7; 1,000
+// rows 42.9, 31.1, 27.8 (with the rule below 85.5, 54.3, 30.5).
+static int64_t window_split_pages(int64_t pages, int64_t blocks, int d, int64_t row_heads, int64_t most) {
+  const bool two = d > 96;  // blocks of many rows on a compute unit at once, else three
+  const double unit = two ? 1.0 : 0.35 + 0.65 * d / 96;
+  double best = 0.0;
+  int64_t best_each = pages;
+  for (int64_t s = 1; s <= most; ++s) {
+    const int64_t each = (pages + s - 1) / s;
+    if (s > 1 && each < kLeastPages) break;
+    const double on_unit = static_cast<double>(blocks * s) / kComputeUnits;
+    double page = two ? 1.3 * on_unit : 1.02 * on_unit;
+    if (on_unit <= 1.0) page = two ? 1.9 : 1.73;
+    else if (on_unit <= 2.0) page = two ? 2.6 : 2.2;
+    else if (on_unit <= 3.0 && !two) page = 2.95;
+    double us = each * page * unit;
+    if (s > 1) us += 5.5 + 0.0001 * static_cast<double>(s * row_heads) * d / 96;
+    if (s == 1 || us < best) {
+      best = us;
+      best_each = each;
+    }
+  }
+  return best_each;
+}
+
 // Splits along the context, sized by the longest one a launch may meet (blocks
 // past a sequence's end leave at once).  Measured with d 96 and, where nothing
 // else is said, 8 heads on two KV heads:
@@ -902,6 +934,11 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_combine_kernel(Kv8AttnArgs a
 // A launch is sized as if every sequence brought max_rows rows: with a prompt
 // among them, single rows get no splits and a wave each (512 rows and 31 single
 // rows over up to 8,192 tokens 386; apart 13.5 and 18.2).
+//
+// With a window, steps of kWindowBlocks blocks or more stay whole up to
+// kWindowPages pages: 64 queries over 2,048 keys 14.1 and, in two splits, 16.2,
+// over 1,000 10.8 and 13.9, over 4,000 25.4 and 22.9; 16 over 2,048 12.9 and, in
+// nine, 11.6.
 Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens, int sinks,
                                int window) {
   Kv8AttnPlan p;
@@ -909,13 +946,11 @@ Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int m
   int64_t pages = (max_tokens + kKv8Page - 1) / kKv8Page;
   const bool step = most <= kStepRows;
   p.tile_rows = step ? kStepTile : kRowsTile;
-  bool all_alike = step;  // tiles see like numbers of pages
   if (window > 0) {
     // A tile's rows are of up to tile_tokens tokens, and n keys lie in up to (n + 62) / 64 + 1 pages.
     const int64_t tile_tokens = std::min<int64_t>(max_rows, (p.tile_rows - 1) / (hq / hkv) + 2);
     const int64_t reach = (static_cast<int64_t>(sinks) + kKv8Page - 1) / kKv8Page +
                           (static_cast<int64_t>(window) + tile_tokens - 1 + kKv8Page - 2) / kKv8Page + 1;
-    all_alike = all_alike || reach < pages;
     pages = std::min(pages, reach);
   }
   const int64_t blocks = (most + p.tile_rows - 1) / p.tile_rows * hkv * seqs;
@@ -923,9 +958,11 @@ Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int m
   const bool few = step || static_cast<int64_t>(rows) * hq <= kFewRows;
   const int64_t splits = few ? kMostSplits : kFewSplits, least = few ? kLeastPages : kLeastRowsPages;
   // Of a prompt's tiles, the first sees the context and the last all of max_tokens.
-  const int64_t mean = all_alike ? pages : std::max<int64_t>(1, (2 * max_tokens - max_rows) / (2 * kKv8Page));
+  const int64_t mean = step ? pages : std::max<int64_t>(1, (2 * max_tokens - max_rows) / (2 * kKv8Page));
   int64_t chunk = pages;
-  if (blocks < wanted && !(step && pages <= kWidePages))
+  if (window > 0 && !step)
+    chunk = window_split_pages(pages, blocks, d, static_cast<int64_t>(rows) * hq, splits);
+  else if (blocks < wanted && !(step && pages <= (window > 0 && blocks >= kWindowBlocks ? kWindowPages : kWidePages)))
     chunk = std::max<int64_t>({least, (mean * blocks + wanted - 1) / wanted, (pages + splits - 1) / splits});
   p.chunk_pages = static_cast<int>(chunk);
   p.splits = static_cast<int>((pages + chunk - 1) / chunk);
