@@ -32,9 +32,10 @@ constexpr int kRunQuads = 4, kRun = kRunThreads * 4 * kRunQuads;  // columns of 
 constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / kWave;
 constexpr int kJoinHeld = 8;  // candidates of its first beam that a lane holds
 constexpr int kOneThreads = 1024, kOneWaves = kOneThreads / kWave;
-constexpr int kOneQuads = 8, kUnit = kWave * 4 * kOneQuads;  // columns of a wave's turn
-constexpr int kMostUnits = 64;                               // turns of a search
-constexpr int kRoom = 512, kFours = 256, kPlaceLanes = 8;
+constexpr int kOneQuads = 8, kUnit = kWave * 4 * kOneQuads;  // columns of one of its waves
+constexpr int kRoom = 512, kFours = 512, kPlaceLanes = 8;
+constexpr int kFewCandidates = 64;  // that are placed without a limit
+static_assert(kRoom <= kJoinThreads && kRoom <= kOneThreads, "a candidate a thread");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
 
@@ -81,6 +82,12 @@ __device__ __forceinline__ void load_columns(const float* x, int vocab, int firs
     for (int i = 0; i < 4 * kQuads; ++i)
       if (first + 4 * (t + n * (i / 4)) + i % 4 >= vocab) v[i] = -INFINITY;
   }
+}
+
+// How many of these lanes come before this one.
+__device__ __forceinline__ int lanes_before(uint64_t lanes) {
+  return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
+                                   __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0));
 }
 
 // The k-th largest of the first n lanes' values, k <= n, where the other lanes
@@ -147,8 +154,7 @@ __device__ __forceinline__ void gather(const float* v, const float* most, float 
 #pragma unroll
   for (int j = 0; j < kQuads; ++j)
     if (hits[j] != 0) {
-      const int place = base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(hits[j] >> 32),
-                                                         __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hits[j]), 0));
+      const int place = base + lanes_before(hits[j]);
       if (most[j] >= limit && place < kFours) {
         to->x[place] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
         to->code[place] = code(j);
@@ -193,12 +199,16 @@ __device__ __forceinline__ Candidate no_candidate() { return Candidate{-INFINITY
 
 // Candidates in LDS; what ranks them apart, so that comparing takes one read.
 struct Room {
-  double rank[kRoom];  // -inf: none
-  float x[kRoom], score[kRoom];
+  float x[kRoom];
   int code[kRoom];  // beam * 2^24 + token
-  int count, fine;  // candidates, and those that are some
+  int count;
+  // Of those that are placed:
+  double rank[kRoom];
+  float chosen_x[kRoom], score[kRoom];
+  int chosen_code[kRoom], chosen;
+  float limit[kOneWaves];
   __device__ __forceinline__ Candidate get(int n) const {
-    return Candidate{rank[n], x[n], code[n] >> 24, code[n] & 0xFFFFFF};
+    return Candidate{rank[n], chosen_x[n], chosen_code[n] >> 24, chosen_code[n] & 0xFFFFFF};
   }
   // Adds the lanes' candidates that are wanted.
   __device__ __forceinline__ void add(bool wanted, float value, int c) {
@@ -206,9 +216,7 @@ struct Room {
     if (lanes == 0) return;
     int base = 0;
     if (threadIdx.x % kWave == 0) base = atomicAdd(&count, __popcll(lanes));
-    const int place = __builtin_amdgcn_readfirstlane(base) +
-                      __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
-                                                __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0));
+    const int place = __builtin_amdgcn_readfirstlane(base) + lanes_before(lanes);
     if (wanted && place < kRoom) {
       x[place] = value;
       code[place] = c;
@@ -280,21 +288,45 @@ struct Search {
     if (c.beam != INT_MAX) candidate(c.beam, c.x, c.token, &s);
     store(a, first, place, c, s);
   }
-  // Ranks the candidates of the room, and stores the best; the block does so together.
+  // Ranks the candidates of the room, and stores the best; the block does so
+  // together.  Ranks in 32 bits are in the order of those in 64, or equal: what
+  // reaches a limit in 32 bits is all that may be among the best.
   template <int kThreads>
   __device__ __forceinline__ void rank_and_store(const BeamArgs& a, int first, Room* room) const {
-    const int tid = threadIdx.x, count = room->count;
-    for (int n = tid; n < count; n += kThreads) {
-      const int code = room->code[n];
-      const Candidate c = candidate(code >> 24, room->x[n], code & 0xFFFFFF, &room->score[n]);
-      room->rank[n] = c.rank;
-      if (c.beam != INT_MAX) atomicAdd(&room->fine, 1);
+    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, count = room->count;
+    Candidate mine = no_candidate();
+    float s = 0.0f, limit = -INFINITY;
+    if (tid < count) {
+      const int code = room->code[tid];
+      mine = candidate(code >> 24, room->x[tid], code & 0xFFFFFF, &s);
+    }
+    const float rank = static_cast<float>(mine.rank);
+    if (count > kFewCandidates) {
+      if (wave * kWave < count) {
+        const float at_least = wave_kth(rank, kWave, a.beams);
+        if (lane == 0) room->limit[wave] = at_least;
+      }
+      __syncthreads();
+      for (int w = 0; w * kWave < count; ++w) limit = fmaxf(limit, room->limit[w]);
+    }
+    const bool wanted = mine.beam != INT_MAX && rank >= limit;
+    const uint64_t lanes = __ballot(wanted);
+    if (lanes != 0) {
+      int base = 0;
+      if (lane == 0) base = atomicAdd(&room->chosen, __popcll(lanes));
+      const int n = __builtin_amdgcn_readfirstlane(base) + lanes_before(lanes);
+      if (wanted) {
+        room->rank[n] = mine.rank;
+        room->score[n] = s;
+        room->chosen_x[n] = mine.x;
+        room->chosen_code[n] = mine.beam << 24 | mine.token;
+      }
     }
     __syncthreads();
-    if (tid >= room->fine && tid < a.beams) store(a, first, tid, no_candidate());
-    for (int n = tid / kPlaceLanes; n < count; n += kThreads / kPlaceLanes) {
-      if (!(room->rank[n] > -INFINITY)) continue;
-      const int place = room->place(n, count);
+    const int chosen = room->chosen;
+    if (tid >= chosen && tid < a.beams) store(a, first, tid, no_candidate());
+    for (int n = tid / kPlaceLanes; n < chosen; n += kThreads / kPlaceLanes) {
+      const int place = room->place(n, chosen);
       if (tid % kPlaceLanes == 0 && place < a.beams) store(a, first, place, room->get(n), room->score[n]);
     }
   }
@@ -320,77 +352,61 @@ __device__ __forceinline__ Candidate block_best(Candidate best, Candidate* wave_
 
 // ------------------------------------------------- a block a search ----
 
-// Waves take (beam, kUnit columns) in turn: the sums first, and the maxima of
-// groups of lanes; those of a beam's turns give its limit, with which the waves
-// gather (from registers, where each has one turn).
+// A wave takes kUnit columns of a beam: the sum first, and the maxima of groups
+// of lanes; those of a beam's waves give its limit, with which they gather.
 __global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int units, int groups) {
   constexpr int kOthers = kOneThreads - kWave;
-  static_assert(kMostBeams <= kWave, "a beam a lane of the last wave");
   __shared__ Search search;
   __shared__ Room room;
   __shared__ Fours fours;
-  __shared__ RunHead heads[kMostUnits];
-  __shared__ float maxima[kMostUnits * kWave];
+  __shared__ RunHead heads[kOneWaves];
+  __shared__ float maxima[kOneWaves * kWave];
   __shared__ Candidate wave_best[kOneWaves];
   const int first = blockIdx.x * a.beams, tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
-  const int turns = a.beams * units, beam0 = wave / units, unit0 = wave - beam0 * units;
+  const int b = wave / units, unit = wave - b * units;
+  const bool works = b < a.beams;
   float v[4 * kOneQuads], most[kOneQuads];
-  auto ask = [&](int b, int unit) {  // also of a beam that has ended, whose logits then count for nothing
+  if (works)  // also of a beam that has ended, whose logits then count for nothing
     load_columns<kOneQuads>(a.logits + static_cast<int64_t>(first + b) * a.vocab, a.vocab, unit * kUnit, lane, kWave, v);
-  };
-  auto every = [&](auto use) {  // of the wave's turns
-    for (int u = wave, b = beam0, unit = unit0; u < turns; u += kOneWaves) {
-      use(u, b, unit);
-      for (unit += kOneWaves; unit >= units; unit -= units) ++b;
-    }
-  };
-  if (wave < turns) ask(beam0, unit0);
   const bool has_beam = tid >= kOthers && tid - kOthers < a.beams;
   Search::Before was = {};
   if (has_beam) was = Search::before(a, first + tid - kOthers);
-  if (tid == 0) fours.count = room.count = room.fine = 0;
-  every([&](int u, int b, int unit) {
-    if (u != wave) ask(b, unit);
+  if (tid == 0) fours.count = room.count = room.chosen = 0;
+  if (works) {
     const float top = largest<kOneQuads>(v, most);
     const float wave_top = fmaxf(group_max<kWave>(top), -FLT_MAX), group_top = lane_groups_max(top, groups);
     const float sum = wave_sum<4 * kOneQuads>(v, wave_top);
-    if (lane == 0) heads[u] = RunHead{wave_top, sum, 0.0f};
-    if (lane % (kWave / groups) == 0) maxima[u * groups + lane / (kWave / groups)] = group_top;
-  });
+    if (lane == 0) heads[wave] = RunHead{wave_top, sum, 0.0f};
+    if (lane % (kWave / groups) == 0) maxima[wave * groups + lane / (kWave / groups)] = group_top;
+  }
   if (has_beam) search.set(a, tid - kOthers, was);
   __syncthreads();
-  every([&](int u, int b, int unit) {
-    const int all = units * groups, n = min(all, kWave), state = search.state[b];
-    if (state >= 2) return;
-    if (turns > kOneWaves) {
-      ask(b, unit);
-      largest<kOneQuads>(v, most);
-    }
+  if (works && search.state[b] < 2) {
+    const int all = units * groups, n = min(all, kWave);
     float top = maxima[b * all + min(lane, n - 1)];
     for (int i = lane + kWave; i < all; i += kWave) top = fmaxf(top, maxima[b * all + i]);
     const float limit = fmaxf(wave_kth(top, n, a.beams), -FLT_MAX);
     gather<kOneQuads>(v, most, limit, &fours, [&](int j) { return b << 24 | (unit * kUnit + 4 * (lane + kWave * j)); });
     if (unit == 0) {
-      const RunHead head = lane < units ? heads[u + lane] : RunHead{-FLT_MAX, 0.0f, 0.0f};
+      const RunHead head = lane < units ? heads[wave + lane] : RunHead{-FLT_MAX, 0.0f, 0.0f};
       const float row_top = group_max<kWave>(head.top);
       double sum = static_cast<double>(head.sum * __builtin_amdgcn_exp2f((head.top - row_top) * kLog2e));
 #pragma unroll
-      for (int step = 1; step < kWave; step *= 2)
+      for (int step = 1; step < kOneWaves; step *= 2)
         if (step < units) sum += __shfl_xor(sum, step);
       if (lane == 0) {
-        heads[u].limit = limit;
+        heads[wave].limit = limit;
         search.set_sum(a, b, row_top, sum);
       }
     }
-  });
+  }
   __syncthreads();
   if (fours.count <= kFours) {
-    // A value a thread; those of beams that have ended by the last wave's other lanes.
-    if (tid < 4 * (fours.count + kWave / 4)) {
-      const int n = tid / 4, code = n < fours.count ? fours.code[n] : 0;
-      const float x = n < fours.count ? reinterpret_cast<const float*>(fours.x)[tid] : -INFINITY;
-      room.add(n < fours.count && x >= heads[(code >> 24) * units].limit, x, code + tid % 4);
+    for (int base = wave * kWave; base < 4 * fours.count; base += kOneThreads) {  // a value a lane
+      const int n = (base + lane) / 4, code = n < fours.count ? fours.code[n] : 0;
+      const float x = n < fours.count ? reinterpret_cast<const float*>(fours.x)[base + lane] : -INFINITY;
+      room.add(n < fours.count && x >= heads[(code >> 24) * units].limit, x, code + lane % 4);
     }
     if (tid >= kOthers) room.add(has_beam && search.state[tid - kOthers] == 2, 0.0f, (tid - kOthers) << 24 | a.eos);
     __syncthreads();
@@ -461,8 +477,7 @@ __global__ __launch_bounds__(kRunThreads) void beam_runs_kernel(BeamArgs a, int 
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
       if (hits[i] != 0) {
-        const int place = base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(hits[i] >> 32),
-                                                           __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hits[i]), 0));
+        const int place = base + lanes_before(hits[i]);
         if (v[i] >= limit && place < kRoom) room[place] = make_float2(v[i], __int_as_float(column_of(i)));
         base += __popcll(hits[i]);
       }
@@ -552,7 +567,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
     return lane < runs ? from.head[static_cast<int64_t>(first + b) * runs + lane] : RunHead{-FLT_MAX, 0.0f, -FLT_MAX};
   };
   RunHead head = wave < a.beams ? head_of(wave) : RunHead{};
-  if (tid == 0) room.count = room.fine = 0;
+  if (tid == 0) room.count = room.chosen = 0;
   if (has_beam) search.set(a, tid, was);
   __syncthreads();
   for (int b = wave; b < a.beams; b += kJoinWaves) {
@@ -645,13 +660,13 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
 
 }  // namespace
 
-// Of the lanes of a turn, so that a beam has at least 2 k groups.
+// Of a wave's lanes, so that a beam has at least 2 k groups.
 static int one_groups(int units, int beams) {
   return units * 4 >= 2 * beams ? 4 : units * 16 >= 2 * beams ? 16 : 64;
 }
 
 int64_t beam_select_workspace(int searches, int beams, int vocab) {
-  if (beams * units_of(vocab) <= kMostUnits) return 0;
+  if (beams * units_of(vocab) <= kOneWaves) return 0;
   const int64_t runs = static_cast<int64_t>(runs_of(vocab)) * searches * beams;
   return runs * static_cast<int64_t>(sizeof(RunHead) + kept_of(beams) * sizeof(float2));
 }

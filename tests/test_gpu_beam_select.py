@@ -71,7 +71,10 @@ def logits_of(rng, rows, vocab):
 
 SIZES = [(1, 1, 1), (1, 4, 6400), (3, 5, 257), (2, 32, 33), (1, 32, 5), (2, 32, 1), (2, 8, 100003), (1, 3, 4096),
          (1, 3, 4097), (4, 16, 12289), (1, 1, 6400), (5, 2, 63), (1, 32, 20000), (300, 2, 700), (2, 7, 16385),
-         (1, 2, 1023), (1, 2, 1025)]
+         (1, 2, 1023), (1, 2, 1025),
+         # On both sides of what one block takes: 16 waves of 2,048 columns each.
+         (2, 16, 2048), (2, 16, 2049), (1, 8, 4096), (1, 8, 4097), (3, 5, 6144), (3, 5, 6145), (2, 4, 8192), (1, 4, 8193),
+         (2, 1, 32768), (1, 1, 32769), (1, 16, 6400), (1, 31, 6400), (1, 16, 100)]
 
 
 @pytest.mark.parametrize("searches,beams,vocab", SIZES)
