@@ -158,14 +158,15 @@ def compact(pool):
 
 
 def select(logits, beams, eos, power, scores, lengths, ended):
-    """The candidates chosen: (scores in 64 bits, lengths, ended, parent, token), the error bits, and the least gap of
-    rank between one that was chosen and the next, of another beam and not of equal rank."""
+    """The candidates chosen: (scores in 64 bits, lengths, ended, parent, token), the error bits, and what scores may be
+    off by without another choice: of one that was chosen and the next (of another beam and not of equal rank), the gap
+    of their ranks over what an error of 1 of both scores makes of it."""
     rows, vocab = logits.shape
     out = [np.full(rows, -np.inf), np.zeros(rows, np.int32), np.full(rows, int(eos >= 0), np.int32),
            np.full(rows, -1, np.int32), np.full(rows, max(eos, 0), np.int32)]
     error, gap = 0, np.inf
     for first in range(0, rows, beams):
-        rank, score, row, token, x = [], [], [], [], []
+        rank, score, row, token, x, factor = [], [], [], [], [], {}
         for b in range(first, first + beams):
             done = eos >= 0 and ended[b] != 0
             length = max(int(lengths[b]) + (0 if done else 1), 1)
@@ -184,7 +185,8 @@ def select(logits, beams, eos, power, scores, lengths, ended):
                 t = np.arange(vocab)
             with np.errstate(over="ignore"):
                 fine = s.astype(np.float32) > -np.inf
-            rank.append(s[fine] * float(length) ** -power)
+            factor[b] = float(length) ** -power
+            rank.append(s[fine] * factor[b])
             score.append(s[fine]), token.append(t[fine]), x.append(values[fine])
             row.append(np.full(fine.sum(), b))
         if not rank:
@@ -193,7 +195,7 @@ def select(logits, beams, eos, power, scores, lengths, ended):
         order = np.lexsort((token, -x, row, -rank))[: beams + 1]
         for a, b in zip(order[:-1], order[1:]):
             if row[a] != row[b] and rank[a] != rank[b]:
-                gap = min(gap, rank[a] - rank[b])
+                gap = min(gap, (rank[a] - rank[b]) / (factor[row[a]] + factor[row[b]]))
         order = order[:beams]
         to = slice(first, first + len(order))
         out[0][to], out[3][to], out[4][to] = score[order], row[order], token[order]
