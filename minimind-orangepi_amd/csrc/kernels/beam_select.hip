@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <climits>
+#include <type_traits>
 
 namespace mmr {
 
@@ -103,6 +104,16 @@ __device__ __forceinline__ float wave_kth(float v, int n, int k) {
       for (int m = 0; m < 4; ++m) above += read_lane(v, i + m) > v;
     }
   }
+  return -group_max<kWave>(above < k ? -v : -INFINITY);
+}
+// As few groups of lanes as k allows: of 16, 2 k groups or more.
+__device__ __forceinline__ float wave_kth_of_groups(float v, int k) {
+  if (k > kWave / 8) return wave_kth(v, kWave, k);
+  v = fmaxf(v, dpp_move<dpp::kQuadXor1>(v));
+  v = fmaxf(v, dpp_move<dpp::kQuadXor2>(v));
+  int above = 0;
+#pragma unroll
+  for (int i = 0; i < kWave; i += 4) above += read_lane(v, i) > v;
   return -group_max<kWave>(above < k ? -v : -INFINITY);
 }
 // The largest of each 64 / n neighbouring lanes, n being 4, 16 or 64.
@@ -210,18 +221,32 @@ struct Room {
   __device__ __forceinline__ Candidate get(int n) const {
     return Candidate{rank[n], chosen_x[n], chosen_code[n] >> 24, chosen_code[n] & 0xFFFFFF};
   }
-  // Adds the lanes' candidates that are wanted.
-  __device__ __forceinline__ void add(bool wanted, float value, int c) {
-    const uint64_t lanes = __ballot(wanted);
-    if (lanes == 0) return;
+  // Adds of kEach values of each lane those that are wanted, at once: an atomic
+  // takes as long for one as for many.
+  template <int kEach>
+  __device__ __forceinline__ void add(const bool* wanted, const float* value, const int* c) {
+    uint64_t lanes[kEach];
+    int total = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      lanes[i] = __ballot(wanted[i]);
+      total += __popcll(lanes[i]);
+    }
+    if (total == 0) return;
     int base = 0;
-    if (threadIdx.x % kWave == 0) base = atomicAdd(&count, __popcll(lanes));
-    const int place = __builtin_amdgcn_readfirstlane(base) + lanes_before(lanes);
-    if (wanted && place < kRoom) {
-      x[place] = value;
-      code[place] = c;
+    if (threadIdx.x % kWave == 0) base = atomicAdd(&count, total);
+    base = __builtin_amdgcn_readfirstlane(base);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int place = base + lanes_before(lanes[i]);
+      if (wanted[i] && place < kRoom) {
+        x[place] = value[i];
+        code[place] = c[i];
+      }
+      base += __popcll(lanes[i]);
     }
   }
+  __device__ __forceinline__ void add(bool wanted, float value, int c) { add<1>(&wanted, &value, &c); }
   // The number of better ones than candidate n, by kPlaceLanes lanes together.
   __device__ __forceinline__ int place(int n, int all) const {
     const double mine = rank[n];
@@ -303,7 +328,7 @@ struct Search {
     const float rank = static_cast<float>(mine.rank);
     if (count > kFewCandidates) {
       if (wave * kWave < count) {
-        const float at_least = wave_kth(rank, kWave, a.beams);
+        const float at_least = wave_kth_of_groups(rank, a.beams);
         if (lane == 0) room->limit[wave] = at_least;
       }
       __syncthreads();
@@ -555,14 +580,14 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
   Search::Before was = {};
   if (has_beam) was = Search::before(a, first + tid);
   // Asked for before the sums are known; of a beam that has ended, anything.
-  const float2 none = make_float2(0.0f, __int_as_float(-1));
-  float2 held[kJoinHeld];
+  float2 held[kJoinHeld] = {};
+  auto ask = [&](int b) {
+    const float2* kept = from.kept + static_cast<int64_t>(first + b) * each;
 #pragma unroll
-  for (int i = 0; i < kJoinHeld; ++i) {
-    const int n = lane + kWave * i;
-    held[i] = none;
-    if (wave < a.beams && n < each) held[i] = from.kept[static_cast<int64_t>(first + wave) * each + n];
-  }
+    for (int i = 0; i < kJoinHeld; ++i)
+      if (kWave * i < each) held[i] = kept[min(lane + kWave * i, each - 1)];
+  };
+  if (wave < a.beams) ask(wave);
   auto head_of = [&](int b) {
     return lane < runs ? from.head[static_cast<int64_t>(first + b) * runs + lane] : RunHead{-FLT_MAX, 0.0f, -FLT_MAX};
   };
@@ -593,40 +618,54 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
     }
   }
   __syncthreads();
-  auto every = [&](auto use) {  // of this wave's beams, all lanes together: use(whether there is one, x, code)
+  // Of this wave's beams, all lanes together: use<n>(whether there is one, x, code), n of each.
+  auto every = [&](auto use) {
     for (int b = wave; b < a.beams; b += kJoinWaves) {
       const int state = search.state[b];
-      if (state == 2) use(lane == 0, 0.0f, b << 24 | a.eos);
+      bool is[kJoinHeld];
+      float x[kJoinHeld];
+      int code[kJoinHeld];
+      if (state == 2) {
+        is[0] = lane == 0, x[0] = 0.0f, code[0] = b << 24 | a.eos;
+        use(std::integral_constant<int, 1>(), is, x, code);
+      }
       if (state != 1) continue;
       const float limit = row_limit[b];  // what `beams` values of the row reach
-      const float2* kept = from.kept + static_cast<int64_t>(first + b) * each;
-      auto one = [&](const float2& k) {
+      if (a.beams > kJoinWaves) ask(b);
+      auto one = [&](int i, const float2& k, bool there) {
         const int token = __float_as_int(k.y);
-        use(token >= 0 && k.x >= limit, k.x, b << 24 | token);
+        is[i] = there && token >= 0 && k.x >= limit;
+        x[i] = k.x;
+        code[i] = b << 24 | token;
       };
+      one(0, held[0], lane < each);
+      if (each <= kWave) {
+        use(std::integral_constant<int, 1>(), is, x, code);
+        continue;
+      }
 #pragma unroll
-      for (int i = 0; i < kJoinHeld; ++i)
-        if (kWave * i < each) {
-          const int n = lane + kWave * i;
-          float2 k = held[i];
-          if (b != wave) k = n < each ? kept[n] : none;
-          one(k);
-        }
-      for (int i = kWave * kJoinHeld; i < each; i += kWave) one(i + lane < each ? kept[i + lane] : none);
+      for (int i = 1; i < kJoinHeld; ++i) one(i, held[i], lane + kWave * i < each);
+      use(std::integral_constant<int, kJoinHeld>(), is, x, code);
+      const float2* kept = from.kept + static_cast<int64_t>(first + b) * each;
+      for (int n = lane + kWave * kJoinHeld; n - lane < each; n += kWave) {
+        one(0, kept[min(n, each - 1)], n < each);
+        use(std::integral_constant<int, 1>(), is, x, code);
+      }
     }
   };
   auto candidate = [&](float x, int code) {
     float score;
     return search.candidate(code >> 24, x, code & 0xFFFFFF, &score);
   };
-  every([&](bool is, float x, int code) { room.add(is, x, code); });
+  every([&](auto n, const bool* is, const float* x, const int* code) { room.add<decltype(n)::value>(is, x, code); });
   __syncthreads();
   if (room.count > kRoom) {
     // Of many beams.  Ranks in 32 bits are in the order of those in 64, or equal:
     // what reaches a limit in 32 bits is all that may be among the best.
     float top = -INFINITY;
-    every([&](bool is, float x, int code) {
-      if (is) top = fmaxf(top, static_cast<float>(candidate(x, code).rank));
+    every([&](auto n, const bool* is, const float* x, const int* code) {
+      for (int i = 0; i < decltype(n)::value; ++i)
+        if (is[i]) top = fmaxf(top, static_cast<float>(candidate(x[i], code[i]).rank));
     });
     const float at_least = wave_kth(top, kWave, a.beams);
     if (lane == 0) sh_limit[wave] = at_least;
@@ -636,8 +675,9 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
 #pragma unroll
     for (int w = 0; w < kJoinWaves; ++w) limit = fmaxf(limit, sh_limit[w]);
     __syncthreads();
-    every([&](bool is, float x, int code) {
-      room.add(is && static_cast<float>(candidate(x, code).rank) >= limit, x, code);
+    every([&](auto n, const bool* is, const float* x, const int* code) {
+      for (int i = 0; i < decltype(n)::value; ++i)
+        room.add(is[i] && static_cast<float>(candidate(x[i], code[i]).rank) >= limit, x[i], code[i]);
     });
     __syncthreads();
   }
@@ -648,10 +688,12 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
   Candidate last{INFINITY, INFINITY, -1, -1};
   for (int n = 0; n < a.beams; ++n) {  // each the best that is worse than the last
     Candidate best = no_candidate();
-    every([&](bool is, float x, int code) {
-      if (!is) return;
-      const Candidate c = candidate(x, code);
-      if (c.beam != INT_MAX && better(last, c) && better(c, best)) best = c;
+    every([&](auto n, const bool* is, const float* x, const int* code) {
+      for (int i = 0; i < decltype(n)::value; ++i) {
+        if (!is[i]) continue;
+        const Candidate c = candidate(x[i], code[i]);
+        if (c.beam != INT_MAX && better(last, c) && better(c, best)) best = c;
+      }
     });
     last = block_best<kJoinWaves>(best, wave_best);
     if (tid == 0) search.store(a, first, n, last);
