@@ -172,7 +172,7 @@ struct Reach {
 // of keys from j on.
 template <bool kWindow>
 __device__ __forceinline__ bool sees(const Kv8AttnArgs& a, int limit, int j) {
-  if constexpr (kWindow) return j <= limit && (j < a.sinks || j > limit - a.window);
+  if constexpr (kWindow) return (j <= limit) & ((j < a.sinks) | (j > limit - a.window));  // no branches
   return j <= limit;
 }
 __device__ __forceinline__ int largest_exponent_seen(const Kv8AttnArgs& a, uint32_t exps, int limit, int first) {
@@ -180,8 +180,8 @@ __device__ __forceinline__ int largest_exponent_seen(const Kv8AttnArgs& a, uint3
 #pragma unroll
   for (int b = 0; b < kKv8Blocks; ++b) {
     const int j = first + kKv8Block * b;
-    if (j <= limit && (j < a.sinks || j + kKv8Block - 1 > limit - a.window))
-      e = max(e, static_cast<int>(static_cast<int8_t>(exps >> (8 * b))));
+    const bool seen = (j <= limit) & ((j < a.sinks) | (j + kKv8Block - 1 > limit - a.window));
+    e = max(e, seen ? static_cast<int>(static_cast<int8_t>(exps >> (8 * b))) : kKv8MinExp - 1);
   }
   return e;
 }
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(kStepThreads, 2) void kv8_step_kernel(Kv8AttnArgs a
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (!sees<kWindow>(a, limit, key + 16 * g + 4 * t + i)) score[t][i] = -INFINITY;
+            score[t][i] = sees<kWindow>(a, limit, key + 16 * g + 4 * t + i) ? score[t][i] : -INFINITY;
       }
     }
     float top = -INFINITY;
@@ -691,10 +691,13 @@ __global__ __launch_bounds__(kRowsThreads, D <= 96 ? 3 : 2) void kv8_rows_kernel
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          score[t][i] = hidden || !sees<kWindow>(a, limit, key + 32 * (t / 2) + 8 * g + 4 * (t % 2) + i)
-                            ? -INFINITY
-                            : score[t][i] * to_log2[t / 2];
+        for (int i = 0; i < 4; ++i) {
+          const int j = key + 32 * (t / 2) + 8 * g + 4 * (t % 2) + i;
+          bool drop;
+          if constexpr (kWindow) drop = hidden | !sees<kWindow>(a, limit, j);
+          else drop = hidden || !sees<kWindow>(a, limit, j);
+          score[t][i] = drop ? -INFINITY : score[t][i] * to_log2[t / 2];
+        }
       to_log2[0] = to_log2[1] = 1.0f;
     }
     float top[2] = {-INFINITY, -INFINITY};
