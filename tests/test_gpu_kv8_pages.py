@@ -161,6 +161,23 @@ def test_many_sequences_and_pages(gpu, seqs, per, pages):
         tokens = keep + room
 
 
+@pytest.mark.parametrize("pages,free", [(16384, 0.1), (16385, 0.1), (18000, 0.001), (19001, 0.3), (20480, 1.0)])
+def test_free_pages_of_large_pools(gpu, pages, free):
+    """Free pages far apart among those that the caller keeps, more and fewer than are wanted."""
+    rng = np.random.default_rng(pages)
+    seqs, per = 6, 40
+    pool = paging.Pool(rng, 1, pages, seqs, per, 1, 32)
+    pool.users[:] = rng.random(pages) >= free
+    pool.users[-1] = 0  # the last page is the last to be taken
+    step = Forks(gpu, pool)
+    wanted = [64 * per, 1, 0, 64 * per, 640, 65]
+    error = step([-1] * seqs, [0] * seqs, wanted)
+    assert (error == 0) == ((pool.users == 0).any() or free > 0.01)
+    tokens = [n if (pool.table[s, : -(-n // 64)] >= 0).all() else 0 for s, n in enumerate(wanted)]
+    step([5, 5, 1, -1, 4, 0], [tokens[5], tokens[5] // 2, tokens[1], 0, tokens[4], tokens[0]], [1, 70, 3, 0, 64, 0])
+    step([-1] * seqs, [0] * seqs, [64 * per] * seqs)
+
+
 def test_windows_free_pages(gpu):
     """A chat grows far past its window on a pool of little more pages than that."""
     rng = np.random.default_rng(9)
@@ -204,8 +221,10 @@ def test_compact(gpu, layers, heads, d, pages, seqs, tokens):
                 setattr(pool, n, a)
 
 
-@pytest.mark.parametrize("pages,part", [(20000, 0.5), (5000, 0.02), (5000, 0.97), (4097, 1.0), (9000, 0.0)])
-def test_compact_many_pages(gpu, pages, part):
+@pytest.mark.parametrize("alias", [True, False])
+@pytest.mark.parametrize("pages,part", [(20000, 0.5), (5000, 0.02), (5000, 0.97), (4097, 1.0), (9000, 0.0), (16384, 0.6),
+                                        (16385, 0.6), (17000, 1.0), (17408, 0.0), (18433, 0.9999), (16400, 0.0001)])
+def test_compact_many_pages(gpu, pages, part, alias):
     mmr, rng = gpu, np.random.default_rng(pages)
     pool = paging.Pool(rng, 1, pages, 10, pages // 10 + 1, 1, 32)
     used = rng.permutation(pages)[: int(pages * part)]
@@ -214,9 +233,14 @@ def test_compact_many_pages(gpu, pages, part):
     pool.users[used] = rng.integers(1, 4, used.size)  # the caller's own among them
     layer_refs, table, users = pool.upload(mmr)
     moved, live = ints(mmr, [77] * pages), ints(mmr, [0])
-    workspace = mmr.DeviceArray(mmr.kv8_compact_workspace_size(pages), np.uint8)
-    mmr.kv8_compact(layer_refs, users, table, users, moved, live, workspace)
+    workspace = mmr.DeviceArray.from_numpy(np.full(mmr.kv8_compact_workspace_size(pages), 0xA5, np.uint8))
+    was_users, source = pool.users.copy(), users
+    if not alias:
+        table, users = ints(mmr, pool.table * 0 + 99), ints(mmr, pool.users * 0 + 99)
+    mmr.kv8_compact(layer_refs, source, table, users, moved, live, workspace)
     mmr.synchronize()
+    if not alias:
+        np.testing.assert_array_equal(source.numpy(), was_users)
     want_moved, want_live = paging.compact(pool)
     assert int(live.numpy()[0]) == want_live
     np.testing.assert_array_equal(moved.numpy(), want_moved)
