@@ -52,7 +52,7 @@ class Select:
             np.testing.assert_array_equal(g[:rows], w, err_msg=name)
         none = want[3] < 0
         assert (got[0][:rows][none] == -np.inf).all()
-        off = np.abs(got[0][:rows].astype(np.float64) - want[0])[~none]
+        off = np.abs(got[0][:rows][~none].astype(np.float64) - want[0][~none])
         assert (off <= LSE + 2.0 ** -24 * np.abs(want[0][~none])).all(), off.max()
         for g in got:
             assert (g[rows:] == (7.5 if g.dtype == np.float32 else 77)).all()
