@@ -493,7 +493,8 @@ int mmr_kv8_window_attention(const float* query, const mmr_kv8_pages* cache, con
  * new page, whose other blocks stay as they are (of the sequences that would
  * write to a page that nobody else names, the first keeps it).  New pages are
  * the lowest free ones, those that this call frees among them, in the order of
- * the sequences and their pages; entries past a sequence's last page become -1.
+ * the sequences and their pages; entries past a sequence's last page become -1,
+ * and full pages that the parent has no number for stay without one.
  * With window > 0, the pages behind the window of a row at position keep[i] and
  * without any of the first `sinks` tokens (see mmr_kv8_window_attention) are let go, too.
  *

@@ -418,7 +418,9 @@ __global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int u
     float top = maxima[b * all + min(lane, n - 1)];
     for (int i = lane + kWave; i < all; i += kWave) top = fmaxf(top, maxima[b * all + i]);
     const float limit = fmaxf(wave_kth(top, n, a.beams), -FLT_MAX);
-    gather<kOneQuads>(v, most, limit, &fours, [&](int j) { return b << 24 | (unit * kUnit + 4 * (lane + kWave * j)); });
+    if (search.state[b] == 1)  // or 0 by now, where the row turns out to have no candidates
+      gather<kOneQuads>(v, most, limit, &fours,
+                        [&](int j) { return b << 24 | (unit * kUnit + 4 * (lane + kWave * j)); });
     if (unit == 0) {
       const RunHead head = lane < units ? heads[wave + lane] : RunHead{-FLT_MAX, 0.0f, 0.0f};
       const float row_top = group_max<kWave>(head.top);

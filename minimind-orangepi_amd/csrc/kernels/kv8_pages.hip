@@ -267,13 +267,15 @@ __global__ __launch_bounds__(kOneThreads) void kv8_fork_decide_kernel(Kv8ForkArg
     }
     wanted += all;
   }
-  // The lowest free pages: of pages p .. p + 3 with these users, numbers from `at` on.
+  // The lowest free pages: of pages p .. p + 3 with these users, numbers from `at`
+  // on (no more than there are pages, whatever the users say).
+  const int most = min(wanted, a.pages);
   auto give = [&](int p, const int4& n, int at) {
     const int of[4] = {n.x, n.y, n.z, n.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (of[i] <= 0) {
-        if (at < wanted) {
+        if (at < most) {
           f.got[at] = p + i;
           a.users[p + i] = 1;
         }
@@ -297,7 +299,7 @@ __global__ __launch_bounds__(kOneThreads) void kv8_fork_decide_kernel(Kv8ForkArg
       if (tid == 0) sh_list = 0;
       int all;
       const int before = block_scan(mine, sh, &all);
-      if (mine > 0 && got + before < wanted) {
+      if (mine > 0 && got + before < most) {
         const int n = atomicAdd(&sh_list, 1);
         list[n] = make_int2(c, got + before);
       }

@@ -181,6 +181,34 @@ def test_in_place_and_always_the_same(gpu):
                 np.testing.assert_array_equal(g[:rows], w)
 
 
+def test_largest_sizes(gpu):
+    """Tokens of 24 bits, and as many searches as there may be."""
+    rng = np.random.default_rng(9)
+    logits = rng.standard_normal((2, 1 << 24)).astype(np.float32)
+    logits[0, [(1 << 24) - 1, 5]], logits[1, [0, (1 << 24) - 2]] = [9.0, 8.5], [8.75, 9.25]
+    call = Select(gpu, logits, 2, (1 << 24) - 1, 0.6, [-3.0, -2.5], [4, 4], [0, 0])
+    call.run()
+    call.check()
+    logits = rng.standard_normal((65535, 3)).astype(np.float32)
+    call = Select(gpu, logits, 1, 1, 1.0, *beams_of(rng, 65535))
+    call.run()
+    call.check()
+
+
+def test_searches_on_two_streams(gpu):
+    mmr, rng = gpu, np.random.default_rng(10)
+    streams, calls = [mmr.Stream(), mmr.Stream()], []
+    for searches, beams, vocab in ((40, 4, 6400), (20, 8, 30000)):
+        calls.append(Select(mmr, logits_of(rng, searches * beams, vocab), beams, 2, 0.6, *beams_of(rng, searches * beams)))
+    mmr.synchronize()
+    for _ in range(20):
+        for call, stream in zip(calls, streams):
+            call.run(stream=stream)
+    mmr.synchronize()
+    for call in calls:
+        call.check()
+
+
 def test_recorded_calls_share_a_workspace(gpu):
     mmr, rng, stream = gpu, np.random.default_rng(7), gpu.Stream()
     calls = []

@@ -41,7 +41,7 @@ class Forks:
             self.pool.assert_pages_equal()
 
 
-SHAPES = [(1, 1, 32), (3, 2, 96), (2, 4, 64), (2, 1, 128), (70, 1, 32)]  # layers, KV heads, head dimension
+SHAPES = [(1, 1, 32), (3, 2, 96), (2, 4, 64), (2, 1, 128), (70, 1, 32), (1, 64, 32), (1, 21, 64)]  # layers, KV heads, head dimension
 
 
 @pytest.mark.parametrize("layers,heads,d", SHAPES)
@@ -106,6 +106,55 @@ def test_pages_kept_by_the_caller(gpu):
     assert pool.table[0, 0] == kept[0] and pool.table[0, 1] != kept[1]
     step([-1, -1], [0, 0], [0, 256])
     assert (pool.users[kept] == 1).all() and not set(kept) & set(pool.table[1])
+
+
+def test_a_page_twice_in_a_row(gpu):
+    """A row that names a page at two places counts it twice, and copies it before it writes to it."""
+    rng = np.random.default_rng(16)
+    pool = paging.Pool(rng, 2, 9, 3, 4, 1, 64)
+    pool.table[0, :3], pool.table[1, :2] = [5, 2, 5], [7, 7]
+    pool.users[[5, 2, 7]] = 2, 1, 2
+    step = Forks(gpu, pool)
+    step([0, 1, 0], [130, 128, 70], [1, 0, 64])
+    assert pool.table[0, 2] not in (5, 2) and pool.users[5] == 2
+    step([0, 0, 1], [131, 131, 100], [1, 1, 1])
+    step([-1, 1, 1], [0, 50, 50], [0, 2, 2])
+
+
+def test_most_sequences(gpu):
+    rng = np.random.default_rng(17)
+    pool = paging.Pool(rng, 1, 3000, 65535, 1, 1, 32)
+    step = Forks(gpu, pool)
+    room = np.zeros(65535, int)
+    room[rng.permutation(65535)[:2500]] = 40
+    step([-1] * 65535, np.zeros(65535, int), room)
+    holders = np.flatnonzero(pool.table[:, 0] >= 0)
+    parent = np.full(65535, -1)
+    parent[holders] = rng.permutation(holders)
+    parent[rng.permutation(65535)[:300]] = holders[0]
+    keep = np.where(parent >= 0, 40, 0)
+    step(parent, keep, np.where(parent >= 0, rng.integers(0, 2, 65535), 0))
+
+
+def test_pools_on_two_streams(gpu):
+    """Calls of two pools that run at the same time, each on its stream and workspace."""
+    mmr, rng = gpu, np.random.default_rng(18)
+    forks, streams, plans = [], [mmr.Stream(), mmr.Stream()], []
+    for seqs in (16, 24):
+        pool = paging.Pool(rng, 3, 200, seqs, 6, 2, 64)
+        pool.fill(rng, [100] * seqs, 0.3)
+        forks.append(Forks(mmr, pool))
+        plan = rng.integers(0, seqs, seqs), np.full(seqs, 100), np.full(seqs, 30)
+        plans.append((plan, [ints(mmr, a) for a in plan]))
+    mmr.synchronize()
+    for _ in range(20):
+        for f, (_, device), stream in zip(forks, plans, streams):
+            mmr.kv8_fork(f.layers, f.users, *device, f.workspace, f.error, stream=stream)
+    mmr.synchronize()
+    for f, (plan, _) in zip(forks, plans):
+        for _ in range(20):
+            paging.fork(f.pool, *plan)
+        f.check()
 
 
 def test_no_more_pages(gpu):

@@ -217,3 +217,38 @@ def test_window_in_place_and_always_the_same(gpu):
                                      error)
             mmr.synchronize()
             np.testing.assert_array_equal(both.numpy(), first)
+
+
+def test_recorded_windows_share_a_workspace(gpu):
+    """Recorded calls of several forms on one workspace, replayed in changing order with eager calls between."""
+    mmr, rng, stream = gpu, np.random.default_rng(39), gpu.Stream()
+    hq, hkv, d, per = 8, 2, 96, 60
+    cache = ref.Cache(rng, 3 * per, 3, per, hkv, d)
+    cache.fill(rng, [3800, 700, 130])
+    device, calls = cache.upload(mmr), []
+    for rows, context, sinks, window in (([1, 1, 1], [3799, 699, 129], 4, 3000), ([30, 40, 20], [3770, 660, 110], 70, 600),
+                                         ([1, 0, 5], [3799, 5, 100], 0, 2900)):
+        n, offsets = sum(rows), offsets_of(rows)
+        query = rng.standard_normal((n, hq * d)).astype(np.float32)
+        args = [mmr.DeviceArray.from_numpy(query), device, ints(mmr, offsets), ints(mmr, context), n, max(rows), per * 64,
+                sinks, window, hq, mmr.DeviceArray((n, hq * d), np.float32)]
+        size = mmr.kv8_window_attention_workspace_size(hq, hkv, d, 3, n, max(rows), per * 64, sinks, window)
+        calls.append((args, size, check(mmr, cache, query, rows, context, hq, sinks, window, device)))
+    workspace, error, graphs = mmr.DeviceArray(max(c[1] for c in calls), np.uint8), ints(mmr, [0]), []
+    assert min(c[1] for c in calls) > 0
+    for args, _, _ in calls:
+        with mmr.Graph(stream) as graph:
+            mmr.kv8_window_attention(*args, workspace, error, stream=stream)
+        graphs.append(graph)
+    for order in ([0, 1, 2], [2, 1, 0], [1, 1, 0, 2], [0, 2, 0, 1]):
+        for args, _, _ in calls:
+            args[-1].zero()
+        workspace.upload(np.full(workspace.shape, 0xFF, np.uint8))
+        mmr.synchronize()
+        for i in order:
+            graphs[i].launch(stream)
+        mmr.kv8_window_attention(*calls[order[0]][0], workspace, error, stream=stream)
+        mmr.synchronize()
+        for args, _, want in calls:
+            np.testing.assert_array_equal(args[-1].numpy(), want)
+    assert int(error.numpy()[0]) == 0
