@@ -62,7 +62,7 @@ constexpr int kPBits = 28;              // p of steps in units of 2^-28: at most
 // See kv8_attention_plan.
 constexpr int kLeastPages = 2, kLeastRowsPages = 4, kWidePages = 16;
 constexpr int kStepBlocks = 256, kRowsBlocks = 1280, kFewRows = 256;
-constexpr int kWindowBlocks = 64, kWindowPages = 40, kComputeUnits = 256;
+constexpr int kWindowBlocks = 64, kWindowPages = 40, kWindowWide = 20, kComputeUnits = 256;
 constexpr int kMostSplits = 64;         // a lane of a wave each in the join
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 using f32x4 = float __attribute__((ext_vector_type(4)));
@@ -154,7 +154,7 @@ __device__ __forceinline__ int blocks_seen(int limit, int first) {
 // are their numbers.
 // Finding them takes a load more than without a window (the page numbers follow
 // from the context).  us: one query at 32,000 tokens that looks back on 300 keys
-// 7.2, on 1,000 8.8, on 16,000 9.6; 64 queries on 2,048 keys 14.0 (51 MB, 3.6
+// 7.2, on 1,000 9.0, on 16,000 9.6; 64 queries on 2,048 keys 14.0 (51 MB, 3.6
 // TB/s), 128 22.5 (4.5 TB/s); 5 rows of 16 sequences on 500 keys, d 64, 9.2; 5,000
 // rows on 1,500 keys 75 (without a window 150).
 template <bool kWindow>
@@ -946,7 +946,9 @@ static int64_t window_split_pages(int64_t pages, int64_t blocks, int d, int64_t 
 // With a window, steps of kWindowBlocks blocks or more stay whole up to
 // kWindowPages pages: 64 queries over 2,048 keys 14.1 and, in two splits, 16.2,
 // over 1,000 10.8 and 13.9, over 4,000 25.4 and 22.9; 16 over 2,048 12.9 and, in
-// nine, 11.6.
+// nine, 11.6.  Fewer blocks stay whole up to kWindowWide pages: one query over
+// 1,000 9.0 and, in nine splits, 8.8, but in calls that are not recorded, where
+// the join is a launch more, 9.0 and 10.4; over 1,500 10.4 and 8.9.
 Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens, int sinks,
                                int window) {
   Kv8AttnPlan p;
@@ -967,10 +969,11 @@ Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int m
   const int64_t splits = few ? kMostSplits : kFewSplits, least = few ? kLeastPages : kLeastRowsPages;
   // Of a prompt's tiles, the first sees the context and the last all of max_tokens.
   const int64_t mean = step ? pages : std::max<int64_t>(1, (2 * max_tokens - max_rows) / (2 * kKv8Page));
+  const int whole = window == 0 ? kWidePages : blocks >= kWindowBlocks ? kWindowPages : kWindowWide;  // of steps
   int64_t chunk = pages;
   if (window > 0 && !step)
     chunk = window_split_pages(pages, blocks, d, static_cast<int64_t>(rows) * hq, splits);
-  else if (blocks < wanted && !(step && pages <= (window > 0 && blocks >= kWindowBlocks ? kWindowPages : kWidePages)))
+  else if (blocks < wanted && !(step && pages <= whole))
     chunk = std::max<int64_t>({least, (mean * blocks + wanted - 1) / wanted, (pages + splits - 1) / splits});
   p.chunk_pages = static_cast<int>(chunk);
   p.splits = static_cast<int>((pages + chunk - 1) / chunk);
