@@ -286,7 +286,6 @@ struct Search {
     score[n] = was.score;
     state[n] = fabsf(was.score) < INFINITY ? done ? 2 : 1 : done ? 3 : 0;
     length[n] = was.length + (done ? 0 : 1);
-    factor[n] = length_factor(a, length[n]);
     if (!(was.score < INFINITY)) atomicOr(a.error, kKv8NotFinite);
   }
   // Of the sum of exp(x - top) over its row.
@@ -413,6 +412,8 @@ __global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int u
   }
   if (has_beam) search.set(a, tid - kOthers, was);
   __syncthreads();
+  // Of a beam's waves, the first has its sum to do, so another has this.
+  if (works && unit == min(1, units - 1) && lane == 0) search.factor[b] = length_factor(a, search.length[b]);
   if (works && search.state[b] < 2) {
     const int all = units * groups, n = min(all, kWave);
     float top = maxima[b * all + min(lane, n - 1)];
@@ -607,7 +608,10 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
   };
   RunHead head = wave < a.beams ? head_of(wave) : RunHead{};
   if (tid == 0) room.count = room.chosen = 0;
-  if (has_beam) search.set(a, tid, was);
+  if (has_beam) {
+    search.set(a, tid, was);
+    search.factor[tid] = length_factor(a, search.length[tid]);
+  }
   __syncthreads();
   for (int b = wave; b < a.beams; b += kJoinWaves) {
     if (search.state[b] >= 2) continue;

@@ -116,17 +116,17 @@ struct ForkPlan {
 
 // Of a sequence, while the block decides; in LDS, or in the workspace where there are many.
 struct ForkSeq {
-  int page;          // partly filled, which it will write to, or -1
-  int users;         // of that page
+  int page, users;   // that it will write to, and its users
   int one;           // of the sequences that will write to it, all name the same
   int first_writer;  // of those that name this sequence, the first, and how many
   int writers;
 };
 
 // What becomes of a sequence's table row: places from `fresh` to `pages` get new
-// pages, from number `start` of those on.
+// pages, from number `start` of those on (before that is known: the blocks that a
+// copy would have).  `page` is a partly filled one that it will write to, or -1.
 struct __attribute__((aligned(16))) ForkRow {
-  int fresh, pages, start;
+  int fresh, pages, start, page;
 };
 struct ForkSpace {
   ForkRow* row;   // [seqs]
@@ -177,7 +177,13 @@ __device__ __forceinline__ void count_entry(const Kv8ForkArgs& a, const ForkSpac
     if (had >= 0) atomicSub(a.users + had, 1);
     if (takes >= 0) atomicAdd(a.users + takes, 1);
   }
-  if (takes >= 0 && place == plan.full() && plan.partly() && plan.room > 0) f.claim[takes] = s;  // any of them
+  if (place == 0 && plan.bad) atomicOr(a.error, kKv8BadRows);
+  if (place == (plan.partly() ? plan.full() : 0)) {
+    const bool partly = plan.partly() && takes >= 0, writes = partly && plan.room > 0;
+    f.row[s] = ForkRow{plan.full() + partly, plan.pages(), (plan.keep % kKv8Page + kKv8Block - 1) / kKv8Block,
+                       writes ? takes : -1};
+    if (writes) f.claim[takes] = s;  // any of them
+  }
 }
 __global__ __launch_bounds__(kThreads) void kv8_fork_count_kernel(Kv8ForkArgs a) {
   ForkSpace f;
@@ -188,8 +194,8 @@ __global__ __launch_bounds__(kThreads) void kv8_fork_count_kernel(Kv8ForkArgs a)
 }
 
 // Decides who copies, and finds the new pages: one block, a sequence a thread.
-// What it takes (4.5 of 7.8 for four beams of 777 tokens) is a chain of dependent
-// loads (plans, pages taken, who claims them and their users) and two sums over
+// What it takes (4.2 of 7.8 for four beams of 777 tokens) is a chain of dependent
+// loads (rows, who claims their pages and those pages' users) and two sums over
 // the block, so all else is held, or asked for ahead.
 template <bool kCount>
 __global__ __launch_bounds__(kOneThreads) void kv8_fork_decide_kernel(Kv8ForkArgs a) {
@@ -214,19 +220,12 @@ __global__ __launch_bounds__(kOneThreads) void kv8_fork_decide_kernel(Kv8ForkArg
   // Those who will write to a page agree on one of them, who counts them.
   ForkRow first_row = {};  // of sequence tid
   for (int s = tid; s < a.seqs; s += kOneThreads) {
-    const ForkPlan plan(a, s);
-    const int p = plan.partly() ? f.taken[static_cast<int64_t>(s) * a.per_seq + plan.full()] : -1;
-    ForkRow row;
-    row.fresh = plan.full() + (p >= 0);
-    row.pages = plan.pages();
-    row.start = (plan.keep % kKv8Page + kKv8Block - 1) / kKv8Block;  // until it has one: blocks to copy
+    const ForkRow row = f.row[s];
     if (s == tid) first_row = row;
-    else f.row[s] = row;
-    if (plan.bad) atomicOr(a.error, kKv8BadRows);
-    seq[s].page = p >= 0 && plan.room > 0 ? p : -1;
-    if (p >= 0 && plan.room > 0) {
-      const int one = f.claim[p];
-      seq[s].users = a.users[p];
+    seq[s].page = row.page;
+    if (row.page >= 0) {
+      const int one = f.claim[row.page];
+      seq[s].users = a.users[row.page];
       seq[s].one = one;
       atomicMin(&seq[one].first_writer, s);
       atomicAdd(&seq[one].writers, 1);
