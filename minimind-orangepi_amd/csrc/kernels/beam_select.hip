@@ -38,7 +38,7 @@ constexpr int kJoinHeld = 8;  // candidates of its first beam that a lane holds
 constexpr int kOneThreads = 1024, kOneWaves = kOneThreads / kWave;
 constexpr int kOneQuads = 8, kUnit = kWave * 4 * kOneQuads;  // columns of one of its waves
 constexpr int kRoom = 512, kFours = 512, kPlaceLanes = 8;
-constexpr int kFewCandidates = 64;  // that are placed without a limit
+constexpr int kFewCandidates = 64;  // that are all placed
 static_assert(kRoom <= kJoinThreads && kRoom <= kOneThreads, "a candidate a thread");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
@@ -213,16 +213,17 @@ __device__ __forceinline__ Candidate no_candidate() { return Candidate{-INFINITY
 
 // Candidates in LDS; what ranks them apart, so that comparing takes one read.
 struct Room {
+  // To be ranked:
   float x[kRoom];
   int code[kRoom];  // beam * 2^24 + token
   int count;
-  // Of those that are placed:
+  // Ranked:
   double rank[kRoom];
-  float chosen_x[kRoom], score[kRoom];
-  int chosen_code[kRoom], chosen;
+  float ranked_x[kRoom], score[kRoom];
+  int ranked_code[kRoom], ranked;
   float limit[kOneWaves];
   __device__ __forceinline__ Candidate get(int n) const {
-    return Candidate{rank[n], chosen_x[n], chosen_code[n] >> 24, chosen_code[n] & 0xFFFFFF};
+    return Candidate{rank[n], ranked_x[n], ranked_code[n] >> 24, ranked_code[n] & 0xFFFFFF};
   }
   // Adds of kEach values of each lane those that are wanted, at once: an atomic
   // takes as long for one as for many.
@@ -250,6 +251,21 @@ struct Room {
     }
   }
   __device__ __forceinline__ void add(bool wanted, float value, int c) { add<1>(&wanted, &value, &c); }
+  // Adds the lanes' candidates, where they are some.
+  __device__ __forceinline__ void add_ranked(const Candidate& c, float s) {
+    const bool wanted = c.beam != INT_MAX;
+    const uint64_t lanes = __ballot(wanted);
+    if (lanes == 0) return;
+    int base = 0;
+    if (threadIdx.x % kWave == 0) base = atomicAdd(&ranked, __popcll(lanes));
+    const int n = __builtin_amdgcn_readfirstlane(base) + lanes_before(lanes);
+    if (wanted && n < kRoom) {
+      rank[n] = c.rank;
+      score[n] = s;
+      ranked_x[n] = c.x;
+      ranked_code[n] = c.beam << 24 | c.token;
+    }
+  }
   // The number of better ones than candidate n, by kPlaceLanes lanes together.
   __device__ __forceinline__ int place(int n, int all) const {
     const double mine = rank[n];
@@ -315,49 +331,32 @@ struct Search {
     if (c.beam != INT_MAX) candidate(c.beam, c.x, c.token, &s);
     store(a, first, place, c, s);
   }
-  // Ranks the candidates of the room, and stores the best; the block does so
-  // together.  Ranks in 32 bits are in the order of those in 64, or equal: what
-  // reaches a limit in 32 bits is all that may be among the best.
+  // Stores the best of the room's ranked candidates.
   template <int kThreads>
-  __device__ __forceinline__ void rank_and_store(const BeamArgs& a, int first, Room* room) const {
-    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, count = room->count;
-    Candidate mine = no_candidate();
-    float s = 0.0f, limit = -INFINITY;
-    if (tid < count) {
-      const int code = room->code[tid];
-      mine = candidate(code >> 24, room->x[tid], code & 0xFFFFFF, &s);
-    }
-    const float rank = static_cast<float>(mine.rank);
-    if (count > kFewCandidates) {
-      if (wave * kWave < count) {
-        const float at_least = wave_kth_of_groups(rank, a.beams);
-        if (lane == 0) room->limit[wave] = at_least;
-      }
-      __syncthreads();
-      for (int w = 0; w * kWave < count; ++w) limit = fmaxf(limit, room->limit[w]);
-    }
-    const bool wanted = mine.beam != INT_MAX && rank >= limit;
-    const uint64_t lanes = __ballot(wanted);
-    if (lanes != 0) {
-      int base = 0;
-      if (lane == 0) base = atomicAdd(&room->chosen, __popcll(lanes));
-      const int n = __builtin_amdgcn_readfirstlane(base) + lanes_before(lanes);
-      if (wanted) {
-        room->rank[n] = mine.rank;
-        room->score[n] = s;
-        room->chosen_x[n] = mine.x;
-        room->chosen_code[n] = mine.beam << 24 | mine.token;
-      }
-    }
-    __syncthreads();
-    const int chosen = room->chosen;
-    if (tid >= chosen && tid < a.beams) store(a, first, tid, no_candidate());
-    for (int n = tid / kPlaceLanes; n < chosen; n += kThreads / kPlaceLanes) {
-      const int place = room->place(n, chosen);
+  __device__ __forceinline__ void place_and_store(const BeamArgs& a, int first, const Room* room) const {
+    const int tid = threadIdx.x, count = room->ranked;
+    if (tid >= count && tid < a.beams) store(a, first, tid, no_candidate());
+    for (int n = tid / kPlaceLanes; n < count; n += kThreads / kPlaceLanes) {
+      const int place = room->place(n, count);
       if (tid % kPlaceLanes == 0 && place < a.beams) store(a, first, place, room->get(n), room->score[n]);
     }
   }
 };
+
+// Of `count` ranks, a thread each, a limit that the best reach: 32 bits are in
+// the order of 64, or equal, so that what reaches it in 32 is all that may be
+// among them.  The block finds it together.
+__device__ __forceinline__ float rank_limit(float rank, int count, int beams, float* limits) {
+  const int wave = threadIdx.x / kWave;
+  if (wave * kWave < count) {
+    const float at_least = wave_kth_of_groups(rank, beams);
+    if (threadIdx.x % kWave == 0) limits[wave] = at_least;
+  }
+  __syncthreads();
+  float limit = -INFINITY;
+  for (int w = 0; w * kWave < count; ++w) limit = fmaxf(limit, limits[w]);
+  return limit;
+}
 
 // The best of the block's candidates, in every thread.
 template <int kWaves>
@@ -381,7 +380,7 @@ __device__ __forceinline__ Candidate block_best(Candidate best, Candidate* wave_
 
 // A wave takes kUnit columns of a beam: the sum first, and the maxima of groups
 // of lanes; those of a beam's waves give its limit, with which they gather.
-// One search of 4 beams of 6,400 logits 7.9, of which the exponentials of four
+// One search of 4 beams of 6,400 logits 7.7, of which the exponentials of four
 // waves a SIMD are 1.1, the memory 1.2, and the chain limit - gather - rank -
 // place, with a barrier between each two, most of the rest.
 __global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int units, int groups) {
@@ -402,7 +401,7 @@ __global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int u
   const bool has_beam = tid >= kOthers && tid - kOthers < a.beams;
   Search::Before was = {};
   if (has_beam) was = Search::before(a, first + tid - kOthers);
-  if (tid == 0) fours.count = room.count = room.chosen = 0;
+  if (tid == 0) fours.count = room.ranked = 0;
   if (works) {
     const float top = largest<kOneQuads>(v, most);
     const float wave_top = fmaxf(group_max<kWave>(top), -FLT_MAX), group_top = lane_groups_max(top, groups);
@@ -437,15 +436,37 @@ __global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int u
   }
   __syncthreads();
   if (fours.count <= kFours) {
-    for (int base = wave * kWave; base < 4 * fours.count; base += kOneThreads) {  // a value a lane
-      const int n = (base + lane) / 4, code = n < fours.count ? fours.code[n] : 0;
-      const float x = n < fours.count ? reinterpret_cast<const float*>(fours.x)[base + lane] : -INFINITY;
-      room.add(n < fours.count && x >= heads[(code >> 24) * units].limit, x, code + lane % 4);
+    const int values = 4 * fours.count;
+    for (int base = wave * kWave; base < values; base += kOneThreads) {  // a value a lane
+      const int at = min(base + lane, values - 1), code = fours.code[at / 4];
+      const float x = reinterpret_cast<const float*>(fours.x)[at];
+      float score = 0.0f;
+      Candidate c = no_candidate();
+      if (base + lane < values && x >= heads[(code >> 24) * units].limit)
+        c = search.candidate(code >> 24, x, (code & 0xFFFFFF) + at % 4, &score);
+      room.add_ranked(c, score);
     }
-    if (tid >= kOthers) room.add(has_beam && search.state[tid - kOthers] == 2, 0.0f, (tid - kOthers) << 24 | a.eos);
+    if (tid >= kOthers) {
+      float score = 0.0f;
+      Candidate c = no_candidate();
+      if (has_beam && search.state[tid - kOthers] == 2) c = search.candidate(tid - kOthers, 0.0f, a.eos, &score);
+      room.add_ranked(c, score);
+    }
     __syncthreads();
-    if (room.count <= kRoom) {
-      search.rank_and_store<kOneThreads>(a, first, &room);
+    const int count = room.ranked;
+    if (count <= kRoom) {
+      if (count > kFewCandidates) {  // only those that reach a limit
+        Candidate c = no_candidate();
+        float score = 0.0f;
+        if (tid < count) c = room.get(tid), score = room.score[tid];
+        const float limit = rank_limit(static_cast<float>(c.rank), count, a.beams, room.limit);
+        if (static_cast<float>(c.rank) < limit) c = no_candidate();
+        if (tid == 0) room.ranked = 0;
+        __syncthreads();
+        room.add_ranked(c, score);
+        __syncthreads();
+      }
+      search.place_and_store<kOneThreads>(a, first, &room);
       return;
     }
   }
@@ -607,7 +628,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
     return lane < runs ? from.head[static_cast<int64_t>(first + b) * runs + lane] : RunHead{-FLT_MAX, 0.0f, -FLT_MAX};
   };
   RunHead head = wave < a.beams ? head_of(wave) : RunHead{};
-  if (tid == 0) room.count = room.chosen = 0;
+  if (tid == 0) room.count = room.ranked = 0;
   if (has_beam) {
     search.set(a, tid, was);
     search.factor[tid] = length_factor(a, search.length[tid]);
@@ -700,7 +721,18 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
     __syncthreads();
   }
   if (room.count <= kRoom) {
-    search.rank_and_store<kJoinThreads>(a, first, &room);
+    float score = 0.0f;
+    Candidate c = no_candidate();
+    if (tid < room.count) {
+      const int code = room.code[tid];
+      c = search.candidate(code >> 24, room.x[tid], code & 0xFFFFFF, &score);
+    }
+    if (room.count > kFewCandidates &&
+        static_cast<float>(c.rank) < rank_limit(static_cast<float>(c.rank), room.count, a.beams, room.limit))
+      c = no_candidate();
+    room.add_ranked(c, score);
+    __syncthreads();
+    search.place_and_store<kJoinThreads>(a, first, &room);
     return;
   }
   Candidate last{INFINITY, INFINITY, -1, -1};
@@ -732,9 +764,9 @@ int64_t beam_select_workspace(int searches, int beams, int vocab) {
 }
 
 // One block a search as long as a wave has one turn: 32 searches of 4 beams of
-// 6,400 logits 8.7 and, in two kernels, 9.4, 128 searches 9.7 and 11.8, one search
-// 7.9 and 8.2.  With two turns or more two kernels are faster (8 beams 10.0,
-// in one block 15.9; 4 beams of 32,000 logits 8.7 and 22.9).
+// 6,400 logits 8.4 and, in two kernels, 9.4, 128 searches 9.4 and 11.8, one search
+// 7.7 and 8.2.  With two turns or more two kernels are faster (8 beams 10.2,
+// in one block 15.9; 4 beams of 32,000 logits 8.8 and 22.9).
 hipError_t launch_beam_select(const BeamArgs& a, hipStream_t stream) {
   const int runs = runs_of(a.vocab), units = units_of(a.vocab);
   if (beam_select_workspace(a.searches, a.beams, a.vocab) == 0) {
