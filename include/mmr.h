@@ -478,8 +478,8 @@ int mmr_kv8_window_attention(const float* query, const mmr_kv8_pages* cache, con
  *
  * mmr_kv8_fork: sequence i becomes the first keep[i] tokens of what sequence
  * parent[i] was before the call, with room for room[i] more (parent, keep, room
- * int32 [seqs] on the device; parent -1 is nobody, and keep then counts as 0).
- * So with
+ * int32 [seqs] on the device; parent -1 is nobody, and keep then counts as 0,
+ * whatever it is: the tokens that the row had before, say).  So with
  *   parent[i] = i, keep = tokens, room = n    a sequence grows by n tokens;
  *   parent[i] = j                             it goes on as j does (a beam, or a
  *                                             second answer to a prompt);

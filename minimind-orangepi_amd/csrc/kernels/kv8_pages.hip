@@ -101,12 +101,13 @@ struct ForkPlan {
     parent = a.parent[s];
     keep = a.keep[s];
     room = a.room[s];
-    bad = parent < -1 || parent >= a.seqs || keep < 0 || room < 0 ||
-          static_cast<int64_t>(keep) + room > static_cast<int64_t>(a.per_seq) * kKv8Page;
-    if (bad) room = 0;
-    if (bad || parent < 0) {
+    if (parent == -1) keep = 0;  // of nobody, whatever it says
+    // No branches: the three loads are under way together.
+    bad = (parent < -1) | (parent >= a.seqs) | (keep < 0) | (room < 0) |
+          (static_cast<int64_t>(keep) + room > static_cast<int64_t>(a.per_seq) * kKv8Page);
+    if (bad) {
       parent = -1;
-      keep = 0;
+      keep = room = 0;
     }
   }
   __device__ __forceinline__ int full() const { return keep / kKv8Page; }       // pages that are full of kept tokens
