@@ -540,9 +540,10 @@ int mmr_kv8_compact(const mmr_kv8_pages* layers, int64_t count, const int32_t* u
  * and of a search's candidates the `beams` of the largest score *
  * max(length, 1)^-length_power become its beams (`to`, which may be `from`), the
  * best first: equal ones by the lower beam, the larger logit, the lower token
- * (equal rows of logits have equal sums).  parent gets the row that a beam goes on from (what mmr_kv8_fork takes), token
- * its new token.  Scores are compared in 64 bits (the sum of exponentials is of
- * 32-bit terms) and rounded once.
+ * (equal rows of logits have equal sums).  parent gets the row that a beam goes
+ * on from (what mmr_kv8_fork takes), token its new token.  Scores are compared in
+ * 64 bits (the sum of exponentials is of 32-bit terms, its logarithm of 64 bits)
+ * and rounded once.
  * Logits of -inf are no candidates, nor is what has a score of -inf in 32 bits;
  * a beam of score -inf has none (a search begins with one beam of score 0 and the
  * others at -inf, which makes its first beams differ).  Where there are fewer
