@@ -548,8 +548,10 @@ int mmr_kv8_compact(const mmr_kv8_pages* layers, int64_t count, const int32_t* u
  * a beam of score -inf has none (a search begins with one beam of score 0 and the
  * others at -inf, which makes its first beams differ).  Where there are fewer
  * candidates than beams, the last beams get parent -1, score -inf, length 0, and
- * eos as an ended beam (without eos: token 0).  eos is a token, or -1 for none
- * (ended is then not read, and written as 0).
+ * eos as an ended beam (without eos: token 0).  To mmr_kv8_fork such a row is a
+ * sequence that begins anew, so until a later call gives it a parent again it has
+ * no tokens: context 0 for mmr_kv8_append and the attention, whatever it was.
+ * eos is a token, or -1 for none (ended is then not read, and written as 0).
  * *error (device int32, never cleared here) gets bit 2 if a score, or a logit
  * of a beam that has not ended, is NaN or +inf: such a beam has no candidates.
  * The workspace (mmr_beam_select_workspace_size bytes, possibly 0; 16-byte
