@@ -503,9 +503,16 @@ int mmr_kv8_window_attention(const float* query, const mmr_kv8_pages* cache, con
  * sequence ends, as for parent -1 and room 0), or a partly filled page that is
  * to be kept has no number (it gets a new page that holds nothing); 4 if there
  * are no more free pages (entries that got none are -1, and so appending there
- * is flagged by mmr_kv8_append).  The workspace
- * (mmr_kv8_fork_workspace_size bytes, 16-byte aligned) is the call's own until
- * it has run.  No allocation, no synchronisation, graph-capturable. */
+ * is flagged by mmr_kv8_append).  A partly filled page that was to be copied and
+ * got no page is gone from its sequence with up to 63 kept tokens: it belongs to
+ * the others who name it, and must not be written to.  To free pages and try again,
+ * put back table and users as they were before the call (a copy of the caller's):
+ * the tokens that the call was to keep are all still there, those that it let
+ * go may have been written over.
+ *
+ * The workspace (mmr_kv8_fork_workspace_size bytes, 16-byte aligned) is the
+ * call's own until it has run.  No allocation, no synchronisation,
+ * graph-capturable. */
 #define MMR_KV8_ERROR_PAGES 4
 size_t mmr_kv8_fork_workspace_size(int64_t seqs, int64_t pages_per_seq, int64_t pages);
 int mmr_kv8_fork(const mmr_kv8_pages* layers, int64_t count, int32_t* users, const int32_t* parent,
