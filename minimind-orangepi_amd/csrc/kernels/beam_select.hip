@@ -411,7 +411,8 @@ __global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int u
   const bool works = b < a.beams;
   float v[4 * kOneQuads], most[kOneQuads];
   if (works)  // also of a beam that has ended, whose logits then count for nothing
-    load_columns<kOneQuads>(a.logits + static_cast<int64_t>(first + b) * a.vocab, a.vocab, unit * kUnit, lane, kWave, v);
+    load_columns<kOneQuads>(a.logits + static_cast<int64_t>(first + b) * a.vocab, a.vocab, unit * kUnit, lane, kWave,
+                            v);
   const bool has_beam = tid >= kOthers && tid - kOthers < a.beams;
   Search::Before was = {};
   if (has_beam) was = Search::before(a, first + tid - kOthers);
@@ -428,10 +429,8 @@ __global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int u
   // Of a beam's waves, the first has its sum to do, so another has this.
   if (works && unit == min(1, units - 1) && lane == 0) search.factor[b] = length_factor(a, search.length[b]);
   if (works && search.state[b] < 2) {
-    const int all = units * groups, n = min(all, kWave);
-    float top = maxima[b * all + min(lane, n - 1)];
-    for (int i = lane + kWave; i < all; i += kWave) top = fmaxf(top, maxima[b * all + i]);
-    const float limit = fmaxf(wave_kth(top, n, a.beams), -FLT_MAX);
+    const int all = units * groups;  // at most a wave's lanes, see one_groups
+    const float limit = fmaxf(wave_kth(maxima[b * all + min(lane, all - 1)], all, a.beams), -FLT_MAX);
     if (search.state[b] == 1)  // or 0 by now, where the row turns out to have no candidates
       gather<kOneQuads>(v, most, limit, &fours,
                         [&](int j) { return b << 24 | (unit * kUnit + 4 * (lane + kWave * j)); });
@@ -658,7 +657,8 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
       limit = fmaxf(limit, more[r].limit);
     }
     // What `beams` values of a run reach, or as many runs.
-    limit = fmaxf(group_max<kWave>(limit), wave_kth(lane < runs ? top : -INFINITY, min(kWave, (runs + 3) / 4 * 4), a.beams));
+    limit = fmaxf(group_max<kWave>(limit),
+                  wave_kth(lane < runs ? top : -INFINITY, min(kWave, (runs + 3) / 4 * 4), a.beams));
     top = group_max<kWave>(top);
     double sum = static_cast<double>(head.sum * __builtin_amdgcn_exp2f((head.top - top) * kLog2e));
     for (int r = lane + kWave; r < runs; r += kWave)
@@ -766,7 +766,9 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a, int
 
 }  // namespace
 
-// Of a wave's lanes, so that a beam has at least 2 k groups.
+// Of a wave's lanes, so that a beam has at least 2 k groups; and at most 64, as
+// beams x units is at most 16: 4 each of up to 16 waves, 16 where units < beams / 2
+// (of up to 2), 64 where units < beams / 8 (of one).
 static int one_groups(int units, int beams) {
   return units * 4 >= 2 * beams ? 4 : units * 16 >= 2 * beams ? 16 : 64;
 }
