@@ -434,16 +434,16 @@ int mmr_kv8_append(const float* qkv, const float* q_norm, const float* k_norm, f
  * kv_heads.  max_tokens bounds context[s] + n over all sequences and sizes
  * the split along the context.  Scores are fp32, of a query rounded by up to
  * 2^-29 of its row's largest value (2^-23 of each value, and 2^-39 of the
- * largest, where max_rows x q_heads / kv_heads is over 8).  A weight, the largest about 1, times its block's scale is rounded by
- * up to 2^-29 of the largest scale among the values that the row attends (2^-35,
- * and 2^-22 of itself, over 8): next to a block with far larger
- * values, other values lose bits, and all of them where it is 2^28 (2^34)
- * larger, however little weight it has.  The sums are fp32.  A
- * query row that is not finite gives a row of NaN and no other; out may alias
- * query.  The workspace (mmr_kv8_attention_workspace_size bytes of the same
- * sizes, possibly 0; 16-byte aligned) holds the split partials and is the
- * call's own until it has run; it keeps nothing between calls.  No allocation,
- * no synchronisation, graph-capturable. */
+ * largest, where max_rows x q_heads / kv_heads is over 8).  A weight, the
+ * largest about 1, times its block's scale is rounded by up to 2^-29 of the
+ * largest scale among the values that the row attends (2^-35, and 2^-22 of
+ * itself, over 8): next to a block with far larger values, other values lose
+ * bits, and all of them where it is 2^28 (2^34) larger, however little weight it
+ * has.  The sums are fp32.  A query row that is not finite gives a row of NaN and
+ * no other; out may alias query.  The workspace (mmr_kv8_attention_workspace_size
+ * bytes of the same sizes, possibly 0; 16-byte aligned) holds the split partials
+ * and is the call's own until it has run; it keeps nothing between calls.  No
+ * allocation, no synchronisation, graph-capturable. */
 size_t mmr_kv8_attention_workspace_size(int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs,
                                         int64_t rows, int64_t max_rows, int64_t max_tokens);
 int mmr_kv8_attention(const float* query, const mmr_kv8_pages* cache, const int32_t* offsets, const int32_t* context,
@@ -496,7 +496,12 @@ int mmr_kv8_window_attention(const float* query, const mmr_kv8_pages* cache, con
  * the sequences and their pages; entries past a sequence's last page become -1,
  * and full pages that the parent has no number for stay without one.
  * With window > 0, the pages behind the window of a row at position keep[i] and
- * without any of the first `sinks` tokens (see mmr_kv8_window_attention) are let go, too.
+ * without any of the first `sinks` tokens (see mmr_kv8_window_attention) are let
+ * go, too.
+ * Tokens that are taken back leave their mark on the last block of 16: it keeps
+ * the exponent that they gave it, and kept tokens in it the rounding to that one
+ * (see mmr_kv8_append), so cached values there, and what is appended to the block,
+ * are as if the dropped tokens had been kept.
  *
  * *error (device int32, never cleared here) gets bits: 1 if a parent is outside
  * [-1, seqs), keep or room are negative or keep + room passes the table row (the

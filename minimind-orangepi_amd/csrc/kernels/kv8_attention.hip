@@ -987,19 +987,21 @@ template <int D, bool kWindow>
 void launch_attention_for(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t stream) {
   const int hkv = a.cache.hkv, most = a.hq / hkv * a.max_rows;
   const int tiles = (most + p.tile_rows - 1) / p.tile_rows;
-  if (p.tile_rows != kStepTile)
-    kv8_rows_kernel<D, kWindow><<<dim3(p.splits * tiles * hkv, a.cache.seqs), kRowsThreads, 0, stream>>>(a, p.chunk_pages,
-                                                                                               p.splits);
-  else
-    kv8_step_kernel<D, kWindow><<<dim3(p.splits * hkv, a.cache.seqs, tiles), kStepThreads, 0, stream>>>(a, p.chunk_pages,
-                                                                                              p.splits);
+  if (p.tile_rows != kStepTile) {
+    const dim3 grid(p.splits * tiles * hkv, a.cache.seqs);
+    kv8_rows_kernel<D, kWindow><<<grid, kRowsThreads, 0, stream>>>(a, p.chunk_pages, p.splits);
+  } else {
+    const dim3 grid(p.splits * hkv, a.cache.seqs, tiles);
+    kv8_step_kernel<D, kWindow><<<grid, kStepThreads, 0, stream>>>(a, p.chunk_pages, p.splits);
+  }
   if (p.splits > 1 && p.splits <= kFewSplits) {
     const int each = kJoinThreads / (D / 4);
-    kv8_combine_few_kernel<kWindow><<<dim3((a.max_rows * a.hq + each - 1) / each, a.cache.seqs), kJoinThreads, 0, stream>>>(
-        a, p.chunk_pages, p.splits, p.tile_rows);
-  } else if (p.splits > 1)
-    kv8_combine_kernel<D, kWindow><<<dim3(a.max_rows * a.hq, a.cache.seqs), kJoinThreads, 0, stream>>>(
-        a, p.chunk_pages, p.splits, p.tile_rows);
+    const dim3 grid((a.max_rows * a.hq + each - 1) / each, a.cache.seqs);
+    kv8_combine_few_kernel<kWindow><<<grid, kJoinThreads, 0, stream>>>(a, p.chunk_pages, p.splits, p.tile_rows);
+  } else if (p.splits > 1) {
+    const dim3 grid(a.max_rows * a.hq, a.cache.seqs);
+    kv8_combine_kernel<D, kWindow><<<grid, kJoinThreads, 0, stream>>>(a, p.chunk_pages, p.splits, p.tile_rows);
+  }
 }
 
 template <bool kWindow>

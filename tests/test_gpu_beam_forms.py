@@ -20,8 +20,8 @@ def select(mmr, logits, beams, *rest, fill=0xFF):
     return call
 
 
-# Scores are checked with the bound of test_gpu_beam_select, whose entropy of 11.5 holds here, too: the logits' exponentials
-# are far from alike (0.7 in a row of 300,001).
+# Scores are checked with the bound of test_gpu_beam_select, whose entropy of 11.5 holds here, too: the logits'
+# exponentials are far from alike (0.7 in a row of 300,001).
 # Some of a row's runs of 4,096 columns are masked as a whole, with few tokens left.
 @pytest.mark.parametrize("mask", [-np.inf, LOWEST, -1e30])
 @pytest.mark.parametrize("left", [0, 1, 3, 40])

@@ -10,8 +10,8 @@ pytestmark = pytest.mark.gpu
 
 
 # Beams whose scores differ by less than 32 bits tell of their logarithms.  A row has n zeros among -inf: its terms and
-# sum are whole numbers, so a token's score is s - log n, in 64 bits off by some 2^-49.  The scores are chosen so that two
-# beams are 2^-42 to 2^-30 apart.
+# sum are whole numbers, so a token's score is s - log n, in 64 bits off by some 2^-49.  The scores are chosen so that
+# two beams are 2^-42 to 2^-30 apart.
 def close_pair(rng, vocab):
     while True:
         a, b = (int(n) for n in rng.integers(vocab // 2, vocab + 1, 2))

@@ -1,5 +1,6 @@
-"""Beam search whose masks leave fewer continuations than beams: steps with beams of no parent, which are empty sequences
-until a later step gives them one again, over a decoder on the 8-bit paged cache, eagerly and from recorded graphs."""
+"""Beam search whose masks leave fewer continuations than beams: steps with beams of no parent, which are empty
+sequences until a later step gives them one again, over a decoder on the 8-bit paged cache, eagerly and from recorded
+graphs."""
 from __future__ import annotations
 
 import numpy as np
@@ -74,8 +75,8 @@ class Server:
             self.select, self.go_on = ((lambda graph=graph: graph.launch(self.stream)) for graph in graphs)
 
     def fork(self):
-        self.mmr.kv8_fork(self.refs, self.users, self.parent, self.keep, self.room, self.fork_ws, self.error, sinks=SINKS,
-                          window=WINDOW, stream=self.stream)
+        self.mmr.kv8_fork(self.refs, self.users, self.parent, self.keep, self.room, self.fork_ws, self.error,
+                          sinks=SINKS, window=WINDOW, stream=self.stream)
 
     def run_layers(self, n, most, offsets):
         for layer, pages in zip(self.layers, self.refs.layers):
@@ -86,8 +87,8 @@ class Server:
                            prologue=self.mmr.PRO_RMSNORM, workspace=self.head_ws, stream=self.stream)
 
     def run_select(self):
-        self.mmr.beam_select(self.logits, len(self.prompts), BEAMS, VOCAB, EOS, 0.6, self.beams, self.beams, self.parent,
-                             self.token, self.select_ws, self.error, stream=self.stream)
+        self.mmr.beam_select(self.logits, len(self.prompts), BEAMS, VOCAB, EOS, 0.6, self.beams, self.beams,
+                             self.parent, self.token, self.select_ws, self.error, stream=self.stream)
 
     def run_step(self):
         self.fork()

@@ -1,5 +1,5 @@
-"""Forks whose plans leave something open: sequences without a parent that had tokens, counts beside the plans in memory,
-pools that run out, and searches that run out of candidates."""
+"""Forks whose plans leave something open: sequences without a parent that had tokens, pools that run out, and counts
+beside the plans in memory."""
 from __future__ import annotations
 
 import numpy as np
@@ -74,15 +74,15 @@ class Part:
 
 @pytest.mark.parametrize("seqs,per", [(4, 5), (4, 400)])  # counted by the deciding block, and by a kernel of its own
 def test_plans_counts_and_table_side_by_side(gpu, seqs, per):
-    """What a call reads once and what it counts in, in the same lines of memory: counts are read as they were counted."""
+    """What a call reads once and what it counts in, in the same lines of memory: counts are read as counted."""
     mmr, rng = gpu, np.random.default_rng(24)
     pool = paging.Pool(rng, 1, 24, seqs, per, 1, 32)
     pool.fill(rng, [200, 130, 64, 31], 0.5)
     _, table, users = pool.upload(mmr)
     plans = [([1, 1, 0, 3], [70, 130, 200, 31], [1, 1, 60, 2]), ([2, 0, -1, 2], [100, 5, 9, 260], [30, 1, 90, 0]),
              ([0, 0, 0, 0], [120] * 4, [5, 0, 9, 1]), ([-1, 1, 3, 0], [120, 120, 0, 125], [0, 10, 0, 3])]
-    words = np.concatenate([np.zeros(3 * seqs, np.int32), pool.users, [0, 0, 0, 0], pool.table.reshape(-1)]).astype(np.int32)
-    memory = mmr.DeviceArray.from_numpy(words)
+    words = np.concatenate([np.zeros(3 * seqs), pool.users, [0, 0, 0, 0], pool.table.reshape(-1)])
+    memory = ints(mmr, words)
     at = 3 * seqs
     parent, keep, room = (Part(memory, i * seqs) for i in range(3))
     users, error, table = Part(memory, at), Part(memory, at + 24), Part(memory, at + 28)
