@@ -556,11 +556,13 @@ int mmr_kv8_compact(const mmr_kv8_pages* layers, int64_t count, const int32_t* u
  * on from (what mmr_kv8_fork takes), token its new token.  Scores are compared in
  * 64 bits (the sum of exponentials is of 32-bit terms, its logarithm of 64 bits)
  * and rounded once.
- * Logits of -inf are no candidates, nor is what has a score of -inf in 32 bits;
- * a beam of score -inf has none (a search begins with one beam of score 0 and the
- * others at -inf, which makes its first beams differ).  Where there are fewer
- * candidates than beams, the last beams get parent -1, score -inf, length 0, and
- * eos as an ended beam (without eos: token 0).  To mmr_kv8_fork such a row is a
+ * Logits of -inf are no candidates (masked by a finite lowest value they are, and
+ * where that leaves fewer tokens than beams a call takes up to some ten times as
+ * long), nor is what has a score of -inf in 32 bits; a beam of score -inf has none
+ * (a search begins with one beam of score 0 and the others at -inf, which makes
+ * its first beams differ).  Where there are fewer candidates than beams, the last
+ * beams get parent -1, score -inf, length 0, and eos as an ended beam (without
+ * eos: token 0).  To mmr_kv8_fork such a row is a
  * sequence that begins anew, so until a later call gives it a parent again it has
  * no tokens: context 0 for mmr_kv8_append and the attention, whatever it was.
  * eos is a token, or -1 for none (ended is then not read, and written as 0).

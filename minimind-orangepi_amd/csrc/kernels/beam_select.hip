@@ -12,8 +12,10 @@
 // The k largest of many values: of the maxima of at least 2 k groups of them the
 // k-th largest is a limit that at least k values reach, and few others do; those
 // are gathered in LDS, where each one's place is the number of better ones.
-// Where more reach it than there is room for (a row of equal logits), the block
-// takes one maximum after another instead.
+// Where more reach it than there is room for, the block takes one maximum after
+// another instead: a row of equal logits, or of a finite lowest value as a mask that
+// leaves fewer tokens than beams (one search of 4 beams of 6,400 logits with one left
+// 81, masked by -inf 7.6; 16 of 8 beams of 100,003 with 100 left 53 and 18.5).
 //
 // Two forms, see launch_beam_select: a block a search, or a block a run of a row
 // and a second kernel with a block a search.
@@ -505,7 +507,7 @@ __global__ __launch_bounds__(kOneThreads) void beam_one_kernel(BeamArgs a, int u
 
 // ------------------------------------- a block a run, then a block a search ----
 
-// Of 128 rows of 100,003 logits (51 MB) this kernel takes 12.5 of 19.8: 4.1 TB/s.
+// Of 128 rows of 100,003 logits (51 MB) this kernel takes 12.5 of 20.0: 4.1 TB/s.
 // Vector instructions bound it, which is why the limit is of 16 groups of a
 // block's lanes where that is enough, sums are against the block's maximum, and
 // values are kept as they come (they took 38 with a limit of each thread's
@@ -780,9 +782,9 @@ int64_t beam_select_workspace(int searches, int beams, int vocab) {
 }
 
 // One block a search as long as a wave has one turn: 32 searches of 4 beams of
-// 6,400 logits 8.4 and, in two kernels, 9.4, 128 searches 9.4 and 11.8, one search
-// 7.7 and 8.2.  With two turns or more two kernels are faster (8 beams 10.2,
-// in one block 15.9; 4 beams of 32,000 logits 8.8 and 22.9).
+// 6,400 logits 8.4 and, in two kernels, 9.3, 128 searches 9.3 and 11.8, one search
+// 7.9 and 8.4.  With two turns or more two kernels are faster (8 beams 10.1,
+// in one block 15.9; 4 beams of 32,000 logits 8.7 and 22.9).
 hipError_t launch_beam_select(const BeamArgs& a, hipStream_t stream) {
   const int runs = runs_of(a.vocab), units = units_of(a.vocab);
   if (beam_select_workspace(a.searches, a.beams, a.vocab) == 0) {

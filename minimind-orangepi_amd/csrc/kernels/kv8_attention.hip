@@ -946,9 +946,15 @@ static int64_t window_split_pages(int64_t pages, int64_t blocks, int d, int64_t 
 // With a window, steps of kWindowBlocks blocks or more stay whole up to
 // kWindowPages pages: 64 queries over 2,048 keys 14.1 and, in two splits, 16.2,
 // over 1,000 10.8 and 13.9, over 4,000 25.4 and 22.9; 16 over 2,048 12.9 and, in
-// nine, 11.6.  Fewer blocks stay whole up to kWindowWide pages: one query over
-// 1,000 9.0 and, in nine splits, 8.8, but in calls that are not recorded, where
-// the join is a launch more, 9.0 and 10.4; over 1,500 10.4 and 8.9.
+// nine, 11.6.  Fewer blocks stay whole up to kWindowWide pages, from which on splits
+// are faster in replayed graphs; in calls that are not recorded the join is a launch
+// more, which costs 1 to 3.  Whole and split, of 2 / 8 / 32 / 62 blocks (sequences x KV
+// heads):
+//   12 pages  7.5 8.5 / 7.6 8.8 / 7.8 9.1 / 8.3 9.9
+//   16 pages  8.7 8.6 / 8.8 8.9 / 9.0 9.3 / 9.8 10.6
+//   20 pages  9.0 8.8 / 9.2 9.2 / 9.6 9.8 / 10.3 12.0 (not recorded 8.9 10.5 / 9.2 10.4 / 9.6
+//             10.5 / 10.0 11.9)
+//   24 pages  10.1 8.9 / 10.2 9.0 / 10.8 10.0 / 11.5 12.5
 Kv8AttnPlan kv8_attention_plan(int hq, int hkv, int d, int seqs, int rows, int max_rows, int64_t max_tokens, int sinks,
                                int window) {
   Kv8AttnPlan p;

@@ -195,7 +195,7 @@ __global__ __launch_bounds__(kThreads) void kv8_fork_count_kernel(Kv8ForkArgs a)
 }
 
 // Decides who copies, and finds the new pages: one block, a sequence a thread.
-// What it takes (4.2 of 7.8 for four beams of 777 tokens) is a chain of dependent
+// What it takes (4.1 of 7.7 for four beams of 777 tokens) is a chain of dependent
 // loads (rows, who claims their pages and those pages' users) and two sums over
 // the block, so all else is held, or asked for ahead.
 template <bool kCount>
@@ -614,8 +614,11 @@ int64_t kv8_fork_workspace(int64_t seqs, int64_t per_seq, int64_t pages) {
 // The deciding block counts the entries of small tables itself: 1,120 entries 9.6
 // and, by a kernel of many blocks, 10.4; 2,240 both 12.4; 4,480 13.5 and 11.0.
 // Up to kOnePages it looks for free pages from the first on; in larger pools a
-// kernel counts those in use by chunks first, which one block would take longer
-// for (a compaction of 20,000 pages, two layers: 73 and 99).
+// kernel counts those in use by chunks first, so that the time no longer grows with
+// the number of the first free page.  64 sequences that take a page each, the last
+// free ones: 16,384 pages 9.7 by one block; 20,000 pages 11.8 and, by one block,
+// 10.6; 65,536 11.5 and 18.2; 262,144 11.4 and 50.5.  Where the first pages are free
+// the two kernels more cost 3 (11.0 and 7.8).
 hipError_t launch_kv8_fork(const Kv8ForkArgs& a, const Kv8Layers* layers, int groups, hipStream_t stream) {
   const int blocks = a.seqs * ((a.per_seq + kThreads - 1) / kThreads);
   if (static_cast<int64_t>(a.seqs) * a.per_seq <= kCountEntries && a.pages <= kOnePages) {
