@@ -541,11 +541,12 @@ int mmr_kv8_compact(const mmr_kv8_pages* layers, int64_t count, const int32_t* u
 
 /* ---- beam search: the best continuations (beside mmr_matvec_argmax_f16, which
  * goes on with the best token; no counterpart in the reference) ---------------
- * `searches` searches of `beams` beams (1 to 32) each; beam b of search i is row
- * i * beams + b of every array.  A beam's score is the sum of its tokens' log
- * probabilities, its length how many they are; one that has produced `eos` has
- * ended.  From these (`from`) and the logits (fp32 [searches * beams][vocab],
- * 16-byte aligned) the candidates are, for each beam,
+ * `searches` searches (up to 65,535) of `beams` beams (1 to 32) each over a
+ * vocabulary of up to 2^24, with searches x beams x ceil(vocab / 4096) below 2^24;
+ * beam b of search i is row i * beams + b of every array.  A beam's score is the
+ * sum of its tokens' log probabilities, its length how many they are; one that has
+ * produced `eos` has ended.  From these (`from`) and the logits (fp32
+ * [searches * beams][vocab], 16-byte aligned) the candidates are, for each beam,
  *   one that has not ended: every token v, of score s_b + x_v - log sum_u exp
  *   x_u and length + 1;
  *   one that has: itself, with eos as its token (its logits are not read),

@@ -1153,7 +1153,7 @@ void check_beams(int64_t searches, int64_t beams, int64_t vocab) {
   require(searches >= 1 && searches <= 65535, "searches must be in [1, 65535]");
   require(beams >= 1 && beams <= mmr::kMostBeams, "beams must be in [1, 32]");
   require(vocab >= 1 && vocab <= (int64_t{1} << 24), "vocab must be in [1, 2^24]");
-  require(searches * beams * ((vocab + 1023) / 1024) <= (int64_t{1} << 26), "too many logits");
+  require(mmr::beam_select_in_range(searches * beams, vocab), "too many logits");
 }
 
 bool q4_in_range(int64_t rows, int64_t cols) {

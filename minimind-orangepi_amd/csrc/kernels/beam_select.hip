@@ -775,6 +775,11 @@ static int one_groups(int units, int beams) {
   return units * 4 >= 2 * beams ? 4 : units * 16 >= 2 * beams ? 16 : 64;
 }
 
+// A block a run of every row, and fewer than 2^32 threads in a launch.
+bool beam_select_in_range(int64_t rows, int64_t vocab) {
+  return rows * ((vocab + kRun - 1) / kRun) * kRunThreads < int64_t{1} << 32;
+}
+
 int64_t beam_select_workspace(int searches, int beams, int vocab) {
   if (beams * units_of(vocab) <= kOneWaves) return 0;
   const int64_t runs = static_cast<int64_t>(runs_of(vocab)) * searches * beams;

@@ -674,6 +674,8 @@ struct BeamArgs {
   void* workspace = nullptr;  // beam_select_workspace bytes
   int32_t* error = nullptr;
 };
+// Whether a launch has the blocks for so many rows.
+bool beam_select_in_range(int64_t rows, int64_t vocab);
 int64_t beam_select_workspace(int searches, int beams, int vocab);
 hipError_t launch_beam_select(const BeamArgs& a, hipStream_t stream);
 
